@@ -638,6 +638,191 @@ typedef struct wl_attn_taps_out {
 } wl_attn_taps_out;
 wl_status   wl_attn_taps(wl_attn* a, wl_attn_taps_out* out);
 
+/* ---- a paged cache of latent rows, and trees of drafted tokens over it -----
+ * wl_run_attention's cache is one context per wl_attn, in a row, one new
+ * position per call. A serving loop holds many requests in pages of one cache
+ * and verifies several drafted tokens of each at once. No counterpart in the
+ * reference (one sequence, no drafts). Per step:
+ *
+ *   wl_paged_map             the step's block tables, cache slots, positions
+ *                            and ancestor masks, from the requests' lengths
+ *   per layer:
+ *   wl_paged_write           the new tokens' cache rows (wl_run_attention's
+ *                            prep stage) and their heads' rotary queries
+ *   wl_paged_tree_attention  the new tokens' attention over the cache
+ *
+ * These calls have no context: every buffer is the caller's, named by an
+ * argument block that may be kept and used again (a program keeps one per
+ * layer, its buffers staying where they are). Lengths stay on the device, no
+ * call waits for the device, allocates, or reads anything back, and all of
+ * them can be captured into a HIP graph. They run on the device of `stream`
+ * (NULL: the current device's null stream). Calls on different streams may
+ * run at the same time if none of their outputs, scratch among them, is used
+ * by another. Buffers of one call must not overlap except where stated.
+ *
+ * What is wrong on the host's side of a call (a null pointer, a size or
+ * alignment) returns WL_ERR_INVALID before anything is enqueued, with a
+ * message in wl_paged_last_error() (this thread's last). What only the device
+ * can see (lengths, pages, trees) sets WL_PAGED_E_* bits in the block's
+ * d_status word (one uint32_t, bits are added, never cleared; may be NULL),
+ * with the outcome stated at each call; nothing out of range is ever read or
+ * written. */
+#define WL_TYPE_F32  0
+#define WL_TYPE_BF16 1
+#define WL_PAGED_MAX_REQ   4096  /* requests in one call */
+#define WL_TREE_MAX_NODES  64    /* drafted tokens of one request in one call */
+#define WL_PAGED_E_LEN   1u      /* a length, a page count or a token range that cannot be */
+#define WL_PAGED_E_SPACE 2u      /* more pages asked for than are free */
+#define WL_PAGED_E_PAGE  4u      /* a page or a stack outside the cache */
+#define WL_PAGED_E_TREE  8u      /* a parent that is no earlier node, or too many nodes */
+#define WL_PAGED_E_SLOT  16u     /* a slot or a source row outside its buffer */
+const char* wl_paged_last_error(void);
+
+/* One layer's cache: n_pages pages of page_size rows (a power of two, at most
+ * 1024; n_pages * page_size < 2^31), row_stride elements from row to row (>=
+ * kv_lora_rank + qk_rope, a multiple of 8), 16-byte aligned. A row holds the
+ * normalised compressed key/value (kv_lora_rank values: a multiple of 8, at
+ * most 512) and behind it the rotated key (qk_rope: a multiple of 8, 8 to 64).
+ * dtype: WL_TYPE_F32, the precision of wl_run_attention's caches, or
+ * WL_TYPE_BF16, half the bytes. A slot is page * page_size + row. */
+typedef struct wl_paged_cache {
+    void*    d_rows;
+    uint32_t dtype;
+    uint32_t n_pages, page_size;
+    uint32_t kv_lora_rank, qk_rope;
+    uint32_t row_stride;
+} wl_paged_cache;
+
+/* The page map of a step of n_req requests. Request r holds d_len[r] tokens in
+ * the cache and d_have[r] pages (d_table[r][0, d_have[r]), at least as many as
+ * its tokens fill), and adds d_add[r] tokens. Afterwards it holds exactly the
+ * pages that d_len + d_add tokens fill: pages it no longer needs (drafts that
+ * were turned down; all of them for an ended request, d_len = d_add = 0) go
+ * onto the stack of free pages d_free[0, *d_n_free), in request order; then
+ * new ones are taken from its top, in request order, and written behind its
+ * table row's entries. Entries behind a row's pages stay as they were, and so
+ * does the stack below and above what is pushed.
+ *   d_have_out[r]    pages held (not d_have itself)
+ *   *d_n_free_out    pages left on the stack (not d_n_free itself)
+ *   d_cu[r]          sum of d_add before r; d_cu[n_req] the step's tokens
+ *   per token t = d_cu[r] + i (arrays of max_tokens, the rest as it was):
+ *   d_slot[t]        where its row goes
+ *   d_pos[t]         its position: d_len[r] + i, or in a tree d_len[r] + the
+ *                    number of its ancestors (may be NULL)
+ *   d_mask[t]        bit j: node j of its request is itself or an ancestor
+ *                    (may be NULL). A request then adds at most
+ *                    WL_TREE_MAX_NODES tokens.
+ * d_parent[t] is the node (an earlier one of the request) that drafted token t
+ * follows, -1 the request's last token; d_parent NULL: each token follows the
+ * one before it. A parent that is neither sets E_TREE and counts as -1.
+ * E_LEN, E_SPACE, E_PAGE (*d_n_free, or what would be pushed, does not fit the
+ * stack of n_pages entries) or too many nodes (E_TREE): the step is refused as
+ * a whole: d_have_out and *d_n_free_out are what came in, d_cu is all 0, every
+ * d_slot is -1, nothing else is written. A page outside the cache, in a table
+ * or on the stack: E_PAGE, its tokens' slots are -1. n_req * max_pages < 2^31. */
+typedef struct wl_page_map {
+    uint32_t n_req, page_size, n_pages;
+    uint32_t max_pages;      /* entries per row of d_table */
+    uint32_t max_tokens;
+    const int32_t* d_len;    /* [n_req] */
+    const int32_t* d_add;    /* [n_req] */
+    const int32_t* d_have;   /* [n_req] */
+    int32_t* d_free;         /* [n_pages] */
+    const int32_t* d_n_free; /* [1] */
+    const int32_t* d_parent; /* [max_tokens] or NULL */
+    int32_t* d_table;        /* [n_req][max_pages] */
+    int32_t* d_have_out;     /* [n_req] */
+    int32_t* d_n_free_out;   /* [1] */
+    int32_t* d_cu;           /* [n_req + 1] */
+    int32_t* d_slot;         /* [max_tokens] */
+    int32_t* d_pos;          /* [max_tokens] or NULL */
+    uint64_t* d_mask;        /* [max_tokens] or NULL */
+    uint32_t* d_status;
+} wl_page_map;
+wl_status wl_paged_map(const wl_page_map* m, void* stream);
+
+/* Writes the cache rows of n_tokens tokens: row d_slot[t] = RMSNorm(kv[0,
+ * kv_lora_rank)) * d_norm_w | RoPE(kv[kv_lora_rank, + qk_rope), d_pos[t]), kv
+ * the kv_a_proj output d_kv[t] (the norm's epsilon `eps`, pairs of neighbours
+ * rotated and the halves held apart, as wl_run_attention writes its rows).
+ * With n_heads > 0 also d_q_rope_out[t][h] = RoPE(d_q_rope[t][h], d_pos[t])
+ * for every head's rotary query (d_q_rope_out may be d_q_rope itself). dtype:
+ * the type of d_kv, d_q_rope and d_q_rope_out; strides in elements from token
+ * to token, multiples of 8; 16-byte aligned. Angles are computed in 64 bits,
+ * everything else in 32, rounded once. A slot of -1 is passed over (as is its
+ * token's row; its rotary queries are written). d_src (may be NULL): token t's
+ * kv row is d_kv[d_src[t]], of n_kv rows: after a verification the accepted
+ * nodes' rows are written again, at their final slots, from the same
+ * projections. A slot or source row outside its buffer: E_SLOT, passed over; a
+ * negative position: E_LEN, passed over and its queries not written. Slots are
+ * distinct: where two tokens have the same one, its row is made of parts of
+ * either. */
+typedef struct wl_row_write {
+    wl_paged_cache cache;
+    uint32_t dtype, n_tokens, n_heads;
+    float    eps, rope_theta;
+    const void* d_kv;
+    uint64_t kv_stride;
+    const uint16_t* d_norm_w;  /* [kv_lora_rank] bf16 */
+    const int32_t* d_pos;      /* [n_tokens] */
+    const int32_t* d_slot;     /* [n_tokens] */
+    const int32_t* d_src;      /* [n_tokens] or NULL */
+    uint32_t n_kv;             /* rows of d_kv (with d_src) */
+    const void* d_q_rope;      /* [n_tokens][n_heads][qk_rope] */
+    uint64_t q_stride;
+    void* d_q_rope_out;
+    uint64_t q_out_stride;
+    uint32_t* d_status;
+} wl_row_write;
+wl_status wl_paged_write(const wl_row_write* w, void* stream);
+
+/* Attention of the tokens of n_req requests over the paged cache, in the
+ * absorbed form: token t's head h has the query d_q_lat[t][h] (kv_lora_rank
+ * values, the query taken through the key half of kv_b_proj) and
+ * d_q_rope[t][h] (qk_rope, rotated), and
+ *   d_out[t][h] = sum_k softmax_k(scale * (q_lat . c_k + q_rope . r_k)) c_k
+ * over the keys k that t sees, c_k | r_k the cache row of token k of its
+ * request: every k < d_len[r], and of the request's tokens of this call (rows
+ * d_len[r] + j, node j = token d_cu[r] + j, written before) those whose bit j
+ * is set in d_mask[t]; d_mask NULL: j <= t - d_cu[r]. A token that sees no key
+ * gets zeros. Keys that a token does not see count for nothing, whatever
+ * their rows hold; a NaN or an infinity in a row reaches the tokens that see
+ * it. d_len, d_cu, d_mask and d_table are wl_paged_map's.
+ * dtype: the type of queries and output; WL_TYPE_BF16 needs a BF16 cache.
+ * Products are exact in f32 sums for 32-bit queries (and caches: three bf16
+ * parts a value); in a BF16 output's call the softmax weights are rounded to
+ * bf16 once. Strides in elements from token to token, multiples of 8; heads
+ * lie next to each other, at most 1024; 16-byte aligned. A request has at most
+ * WL_TREE_MAX_NODES tokens (E_TREE). Tokens that no request holds stay as they
+ * were. A request with an impossible length or more keys than its table row
+ * has entries for (E_LEN), too many tokens (E_TREE) or a page outside the cache
+ * (E_PAGE) gets NaN in all its rows; a token range outside [0, n_tokens)
+ * (E_LEN) is left out.
+ * Long contexts are split over the chip and joined through d_scratch,
+ * wl_paged_tree_scratch(a) bytes (0 if `a` is invalid; it depends on the
+ * shapes, not on lengths), 16-byte aligned; it holds nothing between calls. */
+typedef struct wl_tree_attn {
+    wl_paged_cache cache;
+    uint32_t dtype, n_req, n_tokens, n_heads;
+    uint32_t max_pages;        /* entries per row of d_table */
+    float    scale;
+    const void* d_q_lat;       /* [n_tokens][n_heads][kv_lora_rank] */
+    uint64_t q_lat_stride;
+    const void* d_q_rope;      /* [n_tokens][n_heads][qk_rope] */
+    uint64_t q_rope_stride;
+    void* d_out;               /* [n_tokens][n_heads][kv_lora_rank] */
+    uint64_t out_stride;
+    const int32_t* d_table;    /* [n_req][max_pages] */
+    const int32_t* d_len;      /* [n_req] */
+    const int32_t* d_cu;       /* [n_req + 1] */
+    const uint64_t* d_mask;    /* [n_tokens] or NULL */
+    void* d_scratch;
+    size_t scratch_bytes;
+    uint32_t* d_status;
+} wl_tree_attn;
+size_t    wl_paged_tree_scratch(const wl_tree_attn* a);
+wl_status wl_paged_tree_attention(const wl_tree_attn* a, void* stream);
+
 /* ---- single-expert building blocks ---------------------------------------
  * y[N] = W . x for MXFP4 W ([N,K/2] packed nibbles + [N,K/32] E8M0 scales) and
  * f32 x [K]. Replaces launch_dequant_matvec_mxfp4 (src/glm_kernels.cuh:104-110).

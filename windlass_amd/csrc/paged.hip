@@ -1,0 +1,377 @@
+// paged.hip — the page map of a step (wl_paged_map) and the write of its
+// latent cache rows (wl_paged_write).
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "dev_common.h"
+#include "paged.h"
+
+namespace wl {
+namespace paged {
+namespace {
+
+WL_DEV void set_status(uint32_t* status, uint32_t bits) {
+    if (status && bits) __hip_atomic_fetch_or(status, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// ---- the page map ---------------------------------------------------------
+// One launch. With n = len, a = add, h = have of a request and w = ceil((n +
+// a) / ps) the pages it needs, the step is three exclusive sums over the
+// requests: of a (the tokens' ranges), of max(0, h - w) (where a request's
+// surplus pages go on the stack) and of max(0, w - h) (which pages from the
+// top it takes: the k-th of them all is stack[F - 1 - k], F = n_free + the
+// surplus). Every work-group computes all three for itself from the lengths
+// (12 bytes a request), so nothing is handed from one to another and the
+// outputs are written in the same launch: the k-th page, when it is one that
+// this step pushes, is looked up in the table it comes from, not on the stack.
+// In a call with trees a wave takes a request, lane i its node i; otherwise a
+// thread takes a token and finds its request by bisection.
+struct Sums {
+    uint64_t tok;
+    uint32_t back, take;
+};
+WL_DEV Sums operator+(const Sums& a, const Sums& b) { return Sums{a.tok + b.tok, a.back + b.back, a.take + b.take}; }
+WL_DEV Sums shfl_up(const Sums& s, uint32_t o) {
+    Sums r;
+    r.tok = (uint64_t)__shfl_up((unsigned long long)s.tok, o, 64);
+    r.back = __shfl_up(s.back, o, 64);
+    r.take = __shfl_up(s.take, o, 64);
+    return r;
+}
+
+template <uint32_t THREADS, uint32_t RPT>
+__global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
+    constexpr uint32_t CAP = THREADS * RPT, NW = THREADS / 64;
+    __shared__ uint32_t cu[CAP + 1], back[CAP + 1], take[CAP + 1], need[CAP], have[CAP], len[CAP];
+    __shared__ Sums wsum[NW];
+    __shared__ uint32_t err;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = tid >> 6, R = m.n_req;
+    const uint32_t psh = 31u - (uint32_t)__clz((int)m.page_size), pmask = m.page_size - 1u;
+    const bool trees = m.d_parent || m.d_mask;
+    if (tid == 0) err = 0;
+    __syncthreads();
+    // thread tid's requests are [RPT tid, RPT tid + RPT)
+    Sums own[RPT], mine{0, 0, 0};
+    uint32_t bad = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < RPT; i++) {
+        const uint32_t r = tid * RPT + i;
+        own[i] = Sums{0, 0, 0};
+        if (r < R) {
+            const int32_t n = m.d_len[r], a = m.d_add[r], h = m.d_have[r];
+            const uint64_t w = n < 0 || a < 0 ? 0 : ((uint64_t)n + (uint64_t)a + pmask) >> psh;
+            const uint64_t filled = n < 0 ? 0 : ((uint64_t)n + pmask) >> psh;
+            // an ended request (n = 0) may hold any number of pages
+            if (n < 0 || a < 0 || h < 0 || (uint32_t)h > m.max_pages || w > m.max_pages || (uint64_t)(uint32_t)h < filled) {
+                bad |= WL_PAGED_E_LEN;
+            } else {
+                if (trees && a > WL_TREE_MAX_NODES) bad |= WL_PAGED_E_TREE;
+                own[i].tok = (uint64_t)a;
+                own[i].back = (uint32_t)h > (uint32_t)w ? (uint32_t)h - (uint32_t)w : 0u;
+                own[i].take = (uint32_t)w > (uint32_t)h ? (uint32_t)w - (uint32_t)h : 0u;
+                need[r] = (uint32_t)w;
+                have[r] = (uint32_t)h;
+                len[r] = (uint32_t)n;
+            }
+        }
+        mine = mine + own[i];
+    }
+    if (bad) atomicOr(&err, bad);
+    Sums inc = mine;
+    for (uint32_t o = 1; o < 64; o <<= 1) {
+        const Sums v = shfl_up(inc, o);
+        if (lane >= o) inc = inc + v;
+    }
+    if (lane == 63) wsum[wv] = inc;
+    __syncthreads();
+    Sums at{inc.tok - mine.tok, inc.back - mine.back, inc.take - mine.take}, all{0, 0, 0};
+#pragma unroll
+    for (uint32_t w = 0; w < NW; w++) {
+        if (w < wv) at = at + wsum[w];
+        all = all + wsum[w];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < RPT; i++) {
+        const uint32_t r = tid * RPT + i;
+        cu[r] = (uint32_t)at.tok;  // wraps only in a refused step
+        back[r] = at.back;
+        take[r] = at.take;
+        at = at + own[i];
+    }
+    if (tid == THREADS - 1) {
+        cu[CAP] = (uint32_t)at.tok;
+        back[CAP] = at.back;
+        take[CAP] = at.take;
+    }
+    const int32_t nf = *m.d_n_free;
+    uint32_t refuse = err;  // set before the barrier above
+    if (all.tok > m.max_tokens) refuse |= WL_PAGED_E_LEN;
+    if (nf < 0 || (uint32_t)nf > m.n_pages || (uint64_t)(uint32_t)nf + all.back > m.n_pages) refuse |= WL_PAGED_E_PAGE;
+    else if (all.take > (uint32_t)nf + all.back) refuse |= WL_PAGED_E_SPACE;
+    __syncthreads();
+    const uint32_t gt = blockIdx.x * THREADS + tid, gn = gridDim.x * THREADS;
+    if (refuse) {
+        for (uint32_t r = gt; r < R; r += gn) m.d_have_out[r] = m.d_have[r];
+        for (uint32_t r = gt; r <= R; r += gn) m.d_cu[r] = 0;
+        for (uint32_t t = gt; t < m.max_tokens; t += gn) m.d_slot[t] = -1;
+        if (gt == 0) {
+            *m.d_n_free_out = nf;
+            set_status(m.d_status, refuse);
+        }
+        return;
+    }
+    const uint32_t F = (uint32_t)nf + all.back, total = (uint32_t)all.tok;
+    for (uint32_t r = gt; r < R; r += gn) m.d_have_out[r] = (int32_t)need[r];
+    for (uint32_t r = gt; r <= R; r += gn) m.d_cu[r] = (int32_t)cu[r];
+    if (gt == 0) *m.d_n_free_out = (int32_t)(F - all.take);
+    // the last r with base[r] <= x: the owner of element x (empty ranges before it share its base)
+    auto owner = [&](const uint32_t* base, uint32_t x) {
+        uint32_t lo = 0, hi = R;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (base[mid] <= x) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    auto pushed = [&](uint32_t j) {  // the j-th page that this step pushes
+        const uint32_t r = owner(back, j);
+        return m.d_table[(size_t)r * m.max_pages + need[r] + (j - back[r])];
+    };
+    for (uint32_t j = gt; j < all.back; j += gn) m.d_free[(uint32_t)nf + j] = pushed(j);
+    uint32_t flaw = 0;
+    // token i of request r: its slot; the first token of a new page writes the table's entry
+    auto place = [&](uint32_t r, uint32_t i, uint32_t t) {
+        const uint32_t row = len[r] + i, k = row >> psh;
+        int32_t page;
+        if (k < have[r]) {
+            page = m.d_table[(size_t)r * m.max_pages + k];
+        } else {
+            const uint32_t s = F - 1u - (take[r] + (k - have[r]));
+            page = s >= (uint32_t)nf ? pushed(s - (uint32_t)nf) : m.d_free[s];
+            if ((row & pmask) == 0) m.d_table[(size_t)r * m.max_pages + k] = page;
+        }
+        const bool ok = page >= 0 && (uint32_t)page < m.n_pages;
+        if (!ok) flaw |= WL_PAGED_E_PAGE;
+        m.d_slot[t] = ok ? (int32_t)(((uint32_t)page << psh) + (row & pmask)) : -1;
+    };
+    if (trees) {
+        for (uint32_t r = blockIdx.x * NW + wv; r < R; r += gridDim.x * NW) {
+            const uint32_t t0 = cu[r], a = cu[r + 1] - t0, i = lane;
+            const uint32_t t = t0 + (i < a ? i : 0u);
+            int32_t up = (int32_t)i - 1;
+            if (m.d_parent && i < a) {
+                up = m.d_parent[t];
+                if (up < -1 || up >= (int32_t)i) {
+                    flaw |= WL_PAGED_E_TREE;
+                    up = -1;
+                }
+            }
+            // pointer doubling: after step s the mask covers 2^s generations
+            uint64_t bits = 1ull << i;
+            uint32_t depth = up >= 0 ? 1u : 0u;
+#pragma unroll
+            for (int s = 0; s < 6; s++) {
+                const int from = up >= 0 ? up : 0;
+                const uint64_t b = (uint64_t)__shfl((unsigned long long)bits, from, 64);
+                const uint32_t d = __shfl(depth, from, 64);
+                const int32_t u = __shfl(up, from, 64);
+                if (up >= 0) {
+                    bits |= b;
+                    depth += d;
+                    up = u;
+                }
+            }
+            if (i < a) {
+                place(r, i, t);
+                if (m.d_mask) m.d_mask[t] = bits;
+                if (m.d_pos) m.d_pos[t] = (int32_t)(len[r] + depth);
+            }
+        }
+    } else {
+        for (uint32_t t = gt; t < total; t += gn) {
+            const uint32_t r = owner(cu, t), i = t - cu[r];
+            place(r, i, t);
+            if (m.d_pos) m.d_pos[t] = (int32_t)(len[r] + i);
+        }
+    }
+    set_status(m.d_status, flaw);
+}
+
+// ---- the write of cache rows ------------------------------------------------
+// A wave holds a token's row in registers: lane l the values [8 l, 8 l + 8) of
+// the compressed part (one pass: square sum over the wave, scale, store) and,
+// in lanes below RP / 8, 4 pairs of the rotary part. Lane i < RP / 2 computes
+// the angle of pair i: pos * theta^(-2 i / RP) in 64 bits, less its whole
+// turns, then sine and cosine of the rest in f32 with the rest's own rounding
+// added to first order; the other lanes take the pairs' values by permutes.
+struct RowWrite {
+    wl_row_write w;
+    double inv[kMaxRope / 2];  // theta^(-2 i / qk_rope)
+    uint32_t wpt;              // waves per token
+};
+
+WL_DEV void sincos_of(double ang, float& s, float& c) {
+    const double turns = rint(ang * 0.15915494309189533577);        // 1 / (2 pi)
+    double x = fma(-turns, 6.283185307179586232, ang);              // 2 pi, its leading 53 bits
+    x = fma(-turns, 2.4492935982947064e-16, x);                     // and the rest
+    const float h = (float)x, d = (float)(x - (double)h);
+    float s0, c0;
+    sincosf(h, &s0, &c0);
+    s = s0 + d * c0;
+    c = c0 - d * s0;
+}
+
+template <bool BF>
+WL_DEV void load8(const void* p, size_t i, float* v) {
+    if (BF) {
+        const u32x4 x = gld16((const uint16_t*)p + i);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            v[2 * k] = __uint_as_float(x[k] << 16);
+            v[2 * k + 1] = __uint_as_float(x[k] & 0xFFFF0000u);
+        }
+    } else {
+        const u32x4 a = gld16((const float*)p + i), b = gld16((const float*)p + i + 4);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            v[k] = __uint_as_float(a[k]);
+            v[4 + k] = __uint_as_float(b[k]);
+        }
+    }
+}
+WL_DEV uint32_t pack2(float a, float b) {
+    bf16x2 r;
+    r[0] = (__bf16)a;  // round to nearest even
+    r[1] = (__bf16)b;
+    return __builtin_bit_cast(uint32_t, r);
+}
+template <int N>
+WL_DEV void store_n(void* p, size_t i, const float* v, bool bf) {
+    if (bf) {
+#pragma unroll
+        for (int k = 0; k < N; k += 4) {
+            typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+            const u32x2 x = {pack2(v[k], v[k + 1]), pack2(v[k + 2], v[k + 3])};
+            gst((u32x2*)((uint16_t*)p + i + k), x);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k += 4) gst((f32x4*)((float*)p + i + k), f32x4{v[k], v[k + 1], v[k + 2], v[k + 3]});
+    }
+}
+
+template <bool BF>
+__global__ __launch_bounds__(256) void row_write_kernel(RowWrite a) {
+    const wl_row_write& w = a.w;
+    const uint32_t lane = threadIdx.x & 63u, wave = blockIdx.x * 4u + (threadIdx.x >> 6);
+    const uint32_t t = wave / a.wpt, part = wave % a.wpt;
+    if (t >= w.n_tokens) return;
+    const uint32_t L = w.cache.kv_lora_rank, RP = w.cache.qk_rope, HP = RP / 2;
+    const int32_t pos = w.d_pos[t];
+    const bool cbf = w.cache.dtype == WL_TYPE_BF16;
+    if (pos < 0) {
+        if (lane == 0 && part == 0) set_status(w.d_status, WL_PAGED_E_LEN);
+        return;
+    }
+    float sn = 0.f, cs = 0.f;
+    if (lane < HP) sincos_of((double)pos * a.inv[lane], sn, cs);
+    // this lane's 4 pairs: chunk c of the RP / 8 chunks of a rotary vector, of vector vl of the wave's vpw
+    const uint32_t cph = RP / 8, vpw = 64 / cph, c = lane % cph, vl = lane / cph;
+    float s4[4], c4[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        s4[k] = __shfl(sn, 4 * c + k, 64);
+        c4[k] = __shfl(cs, 4 * c + k, 64);
+    }
+    auto turn = [&](const float* v, float* lo, float* hi) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            lo[k] = v[2 * k] * c4[k] - v[2 * k + 1] * s4[k];
+            hi[k] = v[2 * k + 1] * c4[k] + v[2 * k] * s4[k];
+        }
+    };
+    if (part == 0) {
+        const int32_t slot = w.d_slot[t], src = w.d_src ? w.d_src[t] : (int32_t)t;
+        const uint32_t rows = w.cache.n_pages * w.cache.page_size;
+        const bool bad = slot < -1 || (slot >= 0 && (uint32_t)slot >= rows) || (w.d_src && (src < 0 || (uint32_t)src >= w.n_kv));
+        if (bad && lane == 0) set_status(w.d_status, WL_PAGED_E_SLOT);
+        if (!bad && slot >= 0) {
+            const size_t in = (size_t)src * w.kv_stride, out = (size_t)slot * w.cache.row_stride;
+            const uint32_t i = 8 * lane;
+            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, r[8], g[8];
+            if (i < L) {
+                load8<BF>(w.d_kv, in + i, v);
+                load8<true>(w.d_norm_w, i, g);
+            }
+            if (lane < cph) load8<BF>(w.d_kv, in + L + i, r);
+            float ss = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) ss += v[k] * v[k];
+            for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+            const float rs = 1.0f / sqrtf(ss / (float)L + w.eps);
+            if (i < L) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = g[k] * (v[k] * rs);
+                store_n<8>(w.cache.d_rows, out + i, v, cbf);
+            }
+            if (lane < cph) {
+                float lo[4], hi[4];
+                turn(r, lo, hi);
+                store_n<4>(w.cache.d_rows, out + L + 4 * c, lo, cbf);
+                store_n<4>(w.cache.d_rows, out + L + HP + 4 * c, hi, cbf);
+            }
+        }
+    }
+    // a wave's heads come vpw at a time; a vector is read whole before any of
+    // it is written (its lanes are one wave's), so the output may be the input
+    for (uint32_t h0 = part * vpw; h0 < w.n_heads; h0 += a.wpt * vpw) {
+        const uint32_t h = h0 + vl;
+        const bool ok = vl < vpw && h < w.n_heads;
+        float v[8], lo[4], hi[4];
+        if (ok) load8<BF>(w.d_q_rope, (size_t)t * w.q_stride + (size_t)h * RP + 8 * c, v);
+        __builtin_amdgcn_wave_barrier();
+        if (ok) {
+            turn(v, lo, hi);
+            const size_t out = (size_t)t * w.q_out_stride + (size_t)h * RP + 4 * c;
+            store_n<4>(w.d_q_rope_out, out, lo, BF);
+            store_n<4>(w.d_q_rope_out, out + HP, hi, BF);
+        }
+    }
+}
+
+}  // namespace
+
+int launch_map(const wl_page_map& m, void* stream) {
+    const bool trees = m.d_parent || m.d_mask;
+    // a wave per request or a thread per token, four rounds of them at the
+    // least, and no more work-groups than the chip has places for
+    const uint32_t R = m.n_req;
+    auto grid = [&](uint32_t threads) {
+        const uint64_t work = trees ? (uint64_t)R * 64u : m.max_tokens;
+        const uint64_t g = (work + threads - 1) / threads;
+        return dim3((uint32_t)(g < 1 ? 1 : g > 512 ? 512 : g));
+    };
+    hipStream_t st = (hipStream_t)stream;
+    if (R <= 256) hipLaunchKernelGGL((page_map_kernel<256, 1>), grid(256), dim3(256), 0, st, m);
+    else if (R <= 1024) hipLaunchKernelGGL((page_map_kernel<1024, 1>), grid(1024), dim3(1024), 0, st, m);
+    else hipLaunchKernelGGL((page_map_kernel<1024, 4>), grid(1024), dim3(1024), 0, st, m);
+    return (int)hipGetLastError();
+}
+
+int launch_write(const wl_row_write& w, void* stream) {
+    RowWrite a{};
+    a.w = w;
+    for (uint32_t i = 0; i < w.cache.qk_rope / 2; i++)
+        a.inv[i] = 1.0 / std::pow((double)w.rope_theta, (double)(2 * i) / (double)w.cache.qk_rope);
+    a.wpt = w.n_tokens >= 1024 ? 1 : 4;
+    const uint32_t wgs = (uint32_t)(((uint64_t)w.n_tokens * a.wpt + 3) / 4);
+    hipStream_t st = (hipStream_t)stream;
+    if (w.dtype == WL_TYPE_BF16) hipLaunchKernelGGL(row_write_kernel<true>, dim3(wgs), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(row_write_kernel<false>, dim3(wgs), dim3(256), 0, st, a);
+    return (int)hipGetLastError();
+}
+
+}  // namespace paged
+}  // namespace wl
