@@ -748,7 +748,7 @@ wl_status wl_paged_map(const wl_page_map* m, void* stream);
  * With n_heads > 0 also d_q_rope_out[t][h] = RoPE(d_q_rope[t][h], d_pos[t])
  * for every head's rotary query (d_q_rope_out may be d_q_rope itself). dtype:
  * the type of d_kv, d_q_rope and d_q_rope_out; strides in elements from token
- * to token, multiples of 8; 16-byte aligned. Angles are computed in 64 bits,
+ * to token, multiples of 8 up to 2^22; 16-byte aligned. Angles are computed in 64 bits,
  * everything else in 32, rounded once. A slot of -1 is passed over (as is its
  * token's row; its rotary queries are written). d_src (may be NULL): token t's
  * kv row is d_kv[d_src[t]], of n_kv rows: after a verification the accepted
@@ -791,8 +791,8 @@ wl_status wl_paged_write(const wl_row_write* w, void* stream);
  * dtype: the type of queries and output; WL_TYPE_BF16 needs a BF16 cache.
  * Products are exact in f32 sums for 32-bit queries (and caches: three bf16
  * parts a value); in a BF16 output's call the softmax weights are rounded to
- * bf16 once. Strides in elements from token to token, multiples of 8; heads
- * lie next to each other, at most 1024; 16-byte aligned. A request has at most
+ * bf16 once. Strides in elements from token to token, multiples of 8 up to
+ * 2^22; heads lie next to each other, at most 1024; 16-byte aligned. A request has at most
  * WL_TREE_MAX_NODES tokens (E_TREE). Tokens that no request holds stay as they
  * were. A request with an impossible length or more keys than its table row
  * has entries for (E_LEN), too many tokens (E_TREE) or a page outside the cache

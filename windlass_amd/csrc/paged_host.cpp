@@ -48,8 +48,8 @@ wl_status check_cache(const wl_paged_cache& c) {
 // A [tokens][width] array with `stride` elements from token to token.
 wl_status check_rows(const void* p, uint64_t stride, uint64_t width, const char* what) {
     if (!p || !aligned(p, 16)) return fail(WL_ERR_INVALID, "%s must be 16-byte aligned and not null", what);
-    if (stride % 8 || stride < width || stride > (1ull << 32))
-        return fail(WL_ERR_INVALID, "%s: a stride of %llu elements (a multiple of 8, at least %llu)", what,
+    if (stride % 8 || stride < width || stride > (1u << 22))
+        return fail(WL_ERR_INVALID, "%s: a stride of %llu elements (a multiple of 8, %llu to 2^22)", what,
                     (unsigned long long)stride, (unsigned long long)width);
     return WL_OK;
 }
