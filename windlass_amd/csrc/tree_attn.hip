@@ -24,7 +24,7 @@ struct Tree {
     float scale2;      // scale * log2(e): scores in powers of two
     float* part;       // [2 kGrid][rows][cols] unnormalised sums of split tiles
     float* part_ml;    // [2 kGrid][rows][2] their maxima and weight sums
-    uint32_t* desc;    // [kGrid][4] split tiles: {request + 1, row tile, last work-group, -}
+    uint32_t* desc;    // [2 kGrid][4] split tiles: {request + 1, row tile, first and last work-group}
 };
 
 // ---- the work and its split --------------------------------------------------
@@ -149,36 +149,37 @@ WL_DEV constexpr uint32_t swz8(uint32_t row) { return (row & 2u) | ((row & 8u) >
 // ROWS = 16 MT RG rows (node, head) against 64 keys at a time, RG groups of four
 // waves with 16 MT rows each.
 //   S^T[keys][rows] = K Q^T: wave (ks, kh) of a group takes keys [32 ks, + 32)
-//           and half kh of the columns, whose part of the queries it holds in
-//           registers (2 LC + 1 steps of 32 columns, MT row tiles) through the
-//           whole walk; it hands the sums of one 16-key tile to the wave of the
+//           and half kh of the columns (of the latent and of the rotary ones),
+//           whose part of the queries it holds in registers (2 LC + 1 steps of
+//           32 columns, MT row tiles) through the whole walk; it hands the sums of one 16-key tile to the wave of the
 //           other half and takes those of its own, 16 (2 ks + kh), from it;
 //   P = 2^(S - m) in bf16, through LDS, to all waves of the group;
 //   O^T[cols][rows] += V^T P^T: wave w owns columns [32 LC w, + 32 LC); the key
 //           rows are read again, transposed (ds_read_b64_tr_b16).
-// m is a reference, not the maximum: weights may exceed 1 and lose nothing by
-// it (bf16 and f32 keep their relative precision), so it stays as it is until
-// a score passes it by kSlack powers of two, and only then (and in the first
-// tile) the waves exchange their maxima and rescale. A tile costs three barriers.
+// m is a reference, not the maximum: that of the walk's first tile. Weights may
+// exceed 1 and lose nothing by it (bf16 and f32 keep their relative precision);
+// only where a score passes it by kSlack powers of two the walk is done again,
+// after one over the scores alone for the true maxima. So nothing is rescaled,
+// and a tile costs three barriers.
 // Key rows come into LDS by DMA (16 bytes a lane), a tile ahead, a wave for a
 // row, its address in scalars: rows behind the last key and columns behind the
 // row's are read as zeros by the resource's bounds. The rotary parts have one
 // buffer, filled again as soon as the scores are there.
-constexpr float kSlack = 24.f;
+constexpr float kSlack = 64.f;  // a weight at most 2^64, 2^31 of them 2^95
 
 template <int MT, int RG, int LC>
 __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t min_per) {
-    constexpr uint32_t ROWS = 16 * MT * RG, PITCH = 256 * LC, NS = 2 * LC + 1, CT = 2 * LC, DR = 16 / RG;
+    constexpr uint32_t ROWS = 16 * MT * RG, PITCH = 256 * LC, NL = 2 * LC, NS = NL + 1, CT = 2 * LC, DR = 16 / RG;
     __shared__ __align__(1024) uint8_t lat0[kKT * PITCH], lat1[kKT * PITCH];
     __shared__ __align__(1024) uint8_t rot[kKT * 128];
     // a slot per wave, written by the other half's wave (partial scores) and,
-    // once it has read them, by itself: its weights [ROWS of the group][16 keys],
-    // its rows' maxima, and whether a score passed the reference
-    constexpr uint32_t SLOT = 1024 * MT, MAXIMA = 512 * MT, PASSED = MAXIMA + 64 * MT;
+    // once it has read them, by itself: its weights [rows of the group][16 keys]
+    // and its rows' maxima
+    constexpr uint32_t SLOT = 1024 * MT, MAXIMA = 512 * MT;
     __shared__ __align__(1024) uint8_t xbuf[4 * RG * SLOT];
     __shared__ uint64_t seen[ROWS];
     __shared__ float wsum[4][ROWS];
-    __shared__ uint32_t bad_page;
+    __shared__ uint32_t bad_page, again;
     __shared__ uint64_t tmp[4 * RG + 2];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uni(tid >> 6), n = lane & 15u, g = lane >> 4;
     const uint32_t wv = wave & 3u, kh = wave & 1u, r0 = 16u * MT * (wave >> 2);
@@ -187,11 +188,10 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
     const uint8_t* slots = xbuf + (wave & ~3u) * SLOT;  // the group's
     const uint32_t c = (blockIdx.x % 8u) * (kGrid / 8u) + blockIdx.x / 8u;
     const uint32_t H = p.a.n_heads, L = p.a.cache.kv_lora_rank, RP = p.a.cache.qk_rope;
-    if (tid == 0) bad_page = 0;
+    if (tid == 0) bad_page = again = 0;
     const Place f = find_place<ROWS, 256 * RG>(p, c, min_per, tmp);
-    uint32_t* desc = p.desc + 4 * c;
     const uint64_t u1 = f.u0 + f.per < f.total ? f.u0 + f.per : f.total;
-    if (tid == 0) desc[0] = 0;
+    if (tid < 2) p.desc[4 * (2 * c + tid)] = 0;
     if (f.u0 >= u1) return;
 
     uint64_t u = f.u0, base = f.base;
@@ -210,15 +210,21 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
 
         f32x4 acc[MT][CT];
         float m[MT], l[MT];
+        auto clear = [&]() {
 #pragma unroll
-        for (int i = 0; i < MT; i++) {
-            m[i] = kNone;
-            l[i] = 0.f;
+            for (int i = 0; i < MT; i++) {
+                l[i] = 0.f;
 #pragma unroll
-            for (uint32_t j = 0; j < CT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+                for (uint32_t j = 0; j < CT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        };
         bool bad = false;
-        if (!q.flaw) {
+        if (q.flaw) {
+            clear();
+#pragma unroll
+            for (int i = 0; i < MT; i++) m[i] = kNone;
+        } else {
+            int32_t page = 0;
             // the page of key 64 t + lane
             auto page_of = [&](uint32_t t) {
                 const uint32_t key = t * kKT + lane;
@@ -259,10 +265,6 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
                                                      WL_LDS(rot + (DR * wave + 8u * j) * 128u), 16u, 0, 0);
                 }
             };
-            int32_t page = page_of(kt0);
-            issue(lat0, kt0, page);
-            issue_rot();
-            page = page_of(kt0 + 1);
             // the queries, in the operand's layout: lane (row n, k group g)
             bf16x8 qf[MT][NS];
             const rsrc_t ql = make_rsrc((const uint16_t*)p.a.d_q_lat + q.t0 * p.a.q_lat_stride,
@@ -277,9 +279,8 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
                 const uint32_t vr = live ? 2u * (node * (uint32_t)p.a.q_rope_stride + h * RP + 8u * g) : kOOB;
 #pragma unroll
                 for (uint32_t s = 0; s < NS; s++) {
-                    const uint32_t st = kh * NS + s;  // of the 4 LC + 2 steps
-                    const bool lat = st < 4 * LC;
-                    const uint32_t o = 64u * (lat ? st : st - 4 * LC);
+                    const bool lat = s < NL;
+                    const uint32_t o = 64u * (lat ? kh * NL + s : kh);
                     u32x4 x = lat ? bld16(ql, vl + o, 0) : bld16(qr, vr + o, 0);
                     if (o / 2u + 8u * g >= (lat ? L : RP)) x = u32x4{0u, 0u, 0u, 0u};
                     qf[i][s] = as_bf16x8(x);
@@ -289,17 +290,10 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
                     seen[lr] = p.a.d_mask ? p.a.d_mask[q.t0 + nd] : (2ull << nd) - 1ull;
                 }
             }
-            auto step = [&](uint8_t* lat, uint8_t* nlat, uint32_t t) {
-                uint32_t lane = tid & 63u;
-                asm volatile("" : "+v"(lane));  // addresses are worked out per tile, not held in registers
+            // the scores of tile t for this wave's 16 keys (row n, keys 4 g + j of them) in
+            // powers of two; `between` runs once the rotary buffer is free
+            auto scores = [&](uint8_t* lat, uint32_t t, uint32_t lane, f32x4* sc, auto between) {
                 const uint32_t n = lane & 15u, g = lane >> 4;
-                vm_drain();
-                lds_barrier();
-                const bool more = t + 1 < kt1;
-                if (more) {
-                    issue(nlat, t + 1, page);
-                    page = page_of(t + 2);
-                }
                 // this half's part of the scores of keys 32 ks + 16 k + ...: chunk 4 st + g of a
                 // row lies at (64 st) ^ (16 (g ^ swz))
                 f32x4 pa[2][MT];
@@ -308,28 +302,20 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
                 const uint32_t key0 = 32u * (wv >> 1) + n;
                 const uint32_t ko = key0 * PITCH, kx = 16u * (g ^ swz(n));
                 const uint32_t ro = key0 * 128u + 16u * (g ^ swz8(n));
-                auto lread = [&](uint32_t s, uint32_t k) {
-                    return *(const u32x4*)(lat + ko + ((64u * (kh * NS + s)) ^ kx) + 16u * k * PITCH);
+                auto kread = [&](uint32_t s, uint32_t k) {
+                    return s < NL ? *(const u32x4*)(lat + ko + ((64u * (kh * NL + s)) ^ kx) + 16u * k * PITCH)
+                                  : *(const u32x4*)(rot + (ro ^ (64u * kh)) + 2048u * k);
                 };
-                auto rread = [&](uint32_t s, uint32_t k) { return *(const u32x4*)(rot + (ro ^ (64u * s)) + 2048u * k); };
-                {  // the reads of a step ahead of its products; the last two steps are rotary ones in half 1
+                {  // the reads of a step ahead of its products
                     u32x4 kf[2][2];
-                    kf[0][0] = lread(0, 0);
-                    kf[0][1] = lread(0, 1);
+                    kf[0][0] = kread(0, 0);
+                    kf[0][1] = kread(0, 1);
 #pragma unroll
                     for (uint32_t s = 0; s < NS; s++) {
                         const uint32_t b = s & 1u;
-                        if (s + 1 < NS - 2) {
-                            kf[b ^ 1u][0] = lread(s + 1, 0);
-                            kf[b ^ 1u][1] = lread(s + 1, 1);
-                        } else if (s + 1 < NS) {
-                            if (kh) {
-                                kf[b ^ 1u][0] = rread(s + 3 - NS, 0);
-                                kf[b ^ 1u][1] = rread(s + 3 - NS, 1);
-                            } else {
-                                kf[b ^ 1u][0] = lread(s + 1, 0);
-                                kf[b ^ 1u][1] = lread(s + 1, 1);
-                            }
+                        if (s + 1 < NS) {
+                            kf[b ^ 1u][0] = kread(s + 1, 0);
+                            kf[b ^ 1u][1] = kread(s + 1, 1);
                         }
 #pragma unroll
                         for (uint32_t k = 0; k < 2; k++)
@@ -338,14 +324,13 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-                f32x4 sc[MT];
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
                     *(f32x4*)(slot_other + 1024u * i + 16u * lane) = kh ? pa[0][i] : pa[1][i];
                     sc[i] = kh ? pa[1][i] : pa[0][i];
                 }
                 lds_barrier();
-                if (more) issue_rot();
+                between();
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
                     const f32x4 o = *(const f32x4*)(slot_own + 1024u * i + 16u * lane);
@@ -370,60 +355,70 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
                             }
                         }
                     }
-                    nf |= __shfl_xor(nf, 16, 64);
-                    nf |= __shfl_xor(nf, 32, 64);
+                    uint64_t fl = __ballot(nf != 0);  // lane 16 g + n: key n
+                    fl |= fl >> 32;
+                    const uint32_t flawed = (uint32_t)(fl | (fl >> 16));
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const uint32_t key = t * kKT + 16u * wv + 4u * g + j;
-                        const bool nan = __shfl(nf, 4u * g + j, 64) != 0;
-                        const uint32_t b = key - q.len;  // the node, where key >= len
+                        const uint32_t kj = 4u * g + j, key = t * kKT + 16u * wv + kj;
+                        const float nan = (flawed >> kj) & 1u ? __builtin_nanf("") : 0.f;
 #pragma unroll
                         for (int i = 0; i < MT; i++) {
-                            const bool vis = key < q.len || (key < q.keys && ((seen[r0 + 16u * i + n] >> (b & 63u)) & 1u));
-                            sc[i][j] = !vis ? -INFINITY : nan ? __builtin_nanf("") : sc[i][j];
+                            const uint32_t bit = (uint32_t)(seen[r0 + 16u * i + n] >> ((key - q.len) & 63u)) & (key < q.keys ? 1u : 0u);
+                            sc[i][j] = (bit | (key < q.len ? 1u : 0u)) ? sc[i][j] + nan : -INFINITY;
                         }
                     }
                 }
-                float psum[MT];
-                for (;;) {
-                    bool pass = false;
+            };
+            // m = the largest of m and what the group's waves have in x (a row's lanes differ in g)
+            auto share_maxima = [&](float* x) {
 #pragma unroll
-                    for (int i = 0; i < MT; i++) {
-                        float e[4];
+                for (int i = 0; i < MT; i++) {
+                    x[i] = fmaxf(x[i], __shfl_xor(x[i], 16, 64));
+                    x[i] = fmaxf(x[i], __shfl_xor(x[i], 32, 64));
+                    if (g == 0) *(float*)(slot_own + MAXIMA + 4u * (16u * i + n)) = x[i];
+                }
+                lds_barrier();
 #pragma unroll
-                        for (int j = 0; j < 4; j++) e[j] = exp2_(sc[i][j] - m[i]);
-                        psum[i] = (e[0] + e[1]) + (e[2] + e[3]);
-                        *(u32x2*)(slot_own + (16u * i + n) * 32u + 8u * g) = u32x2{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
-                        pass |= fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])) > m[i] + kSlack;
-                    }
-                    const uint32_t passed = __ballot(pass) != 0;
-                    if (lane == 0) *(uint32_t*)(slot_own + PASSED) = passed;
-                    lds_barrier();
-                    if (!__ballot(*(const uint32_t*)(xbuf + (lane % (4u * RG)) * SLOT + PASSED) != 0)) break;
+                for (int i = 0; i < MT; i++) {
+                    m[i] = kNone;
 #pragma unroll
-                    for (int i = 0; i < MT; i++) {
-                        float x = fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3]));
-                        x = fmaxf(x, __shfl_xor(x, 16, 64));
-                        x = fmaxf(x, __shfl_xor(x, 32, 64));
-                        if (g == 0) *(float*)(slot_own + MAXIMA + 4u * (16u * i + n)) = x;
-                    }
-                    lds_barrier();
+                    for (uint32_t w = 0; w < 4; w++) m[i] = fmaxf(m[i], *(const float*)(slots + w * SLOT + MAXIMA + 4u * (16u * i + n)));
+                }
+            };
+            bool pass = false;
+            uint32_t first = kt0;  // the tile that sets the reference
+            auto step = [&](uint8_t* lat, uint8_t* nlat, uint32_t t) {
+                uint32_t lane = tid & 63u;
+                asm volatile("" : "+v"(lane));  // addresses are worked out per tile, not held in registers
+                const uint32_t n = lane & 15u, g = lane >> 4;
+                vm_drain();
+                lds_barrier();
+                const bool more = t + 1 < kt1;
+                if (more) {
+                    issue(nlat, t + 1, page);
+                    page = page_of(t + 2);
+                }
+                f32x4 sc[MT];
+                scores(lat, t, lane, sc, [&]() {
+                    if (more) issue_rot();
+                });
+                if (t == first) {
+                    float x[MT];
 #pragma unroll
-                    for (int i = 0; i < MT; i++) {
-                        float mn = m[i];
-#pragma unroll
-                        for (uint32_t w = 0; w < 4; w++) mn = fmaxf(mn, *(const float*)(slots + w * SLOT + MAXIMA + 4u * (16u * i + n)));
-                        const float al = exp2_(m[i] - mn);
-                        m[i] = mn;
-                        l[i] *= al;
-#pragma unroll
-                        for (uint32_t ct = 0; ct < CT; ct++)
-#pragma unroll
-                            for (int j = 0; j < 4; j++) acc[i][ct][j] *= al;
-                    }
+                    for (int i = 0; i < MT; i++) x[i] = fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3]));
+                    share_maxima(x);
                 }
 #pragma unroll
-                for (int i = 0; i < MT; i++) l[i] += psum[i];
+                for (int i = 0; i < MT; i++) {
+                    float e[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) e[j] = exp2_(sc[i][j] - m[i]);
+                    l[i] += (e[0] + e[1]) + (e[2] + e[3]);
+                    *(u32x2*)(slot_own + (16u * i + n) * 32u + 8u * g) = u32x2{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
+                    pass |= fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])) > m[i] + kSlack;
+                }
+                lds_barrier();
                 // O^T += V^T P^T
                 const uint32_t vq = (lane & 15u) >> 2, vb = (lane & 3u) >> 1;
                 const uint32_t vo = (8u * g + vq) * PITCH + 16u * ((4u * LC * wv + vb) ^ swz((8u * g + vq) & 15u)) + 8u * (lane & 1u);
@@ -459,9 +454,40 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
-            for (uint32_t t = kt0; t < kt1; t += 2) {
-                step(lat0, lat1, t);
-                if (t + 1 < kt1) step(lat1, lat0, t + 1);
+            for (;;) {
+                clear();
+                issue(lat0, kt0, page_of(kt0));
+                issue_rot();
+                page = page_of(kt0 + 1);
+                for (uint32_t t = kt0; t < kt1; t += 2) {
+                    step(lat0, lat1, t);
+                    if (t + 1 < kt1) step(lat1, lat0, t + 1);
+                }
+                if (first != kt0) break;
+                if (__ballot(pass) && lane == 0) again = 1u;
+                lds_barrier();
+                const bool redo = again != 0;
+                lds_barrier();
+                if (!redo) break;
+                if (tid == 0) again = 0u;
+                float x[MT];
+#pragma unroll
+                for (int i = 0; i < MT; i++) x[i] = kNone;
+                for (uint32_t t = kt0; t < kt1; t++) {
+                    issue(lat0, t, page_of(t));
+                    issue_rot();
+                    vm_drain();
+                    lds_barrier();
+                    f32x4 sc[MT];
+                    scores(lat0, t, lane, sc, [] {});
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+                        x[i] = fmaxf(x[i], fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])));
+                    lds_barrier();
+                }
+                share_maxima(x);
+                lds_barrier();
+                first = ~0u;
             }
         }
         // the weight sums over the waves' keys; flaws
@@ -508,11 +534,13 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
                 }
             }
         }
-        if (!whole && kt0 == 0 && tid == 0) {  // the rest of this row tile is with the next work-groups
-            const uint64_t end = base + (uint64_t)(rt + 1) * q.nkt;
+        if (!whole && tid == (kt0 == 0 ? 1u : 0u)) {  // the thread that cleared it
+            const uint64_t start = base + (uint64_t)rt * q.nkt;
+            uint32_t* desc = p.desc + 4 * slot;
             desc[0] = r + 1u;
             desc[1] = rt;
-            desc[2] = (uint32_t)((end - 1) / f.per);
+            desc[2] = (uint32_t)(start / f.per);
+            desc[3] = (uint32_t)((start + q.nkt - 1) / f.per);
         }
         __syncthreads();
         if (tid == 0) bad_page = 0u;
@@ -520,39 +548,40 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
     }
 }
 
-// Joins the parts of split row tiles: work-group (c, j) the rows [16 j, + 16) of
-// the tile whose first part is work-group c's last; a wave takes a row, lane the
-// columns 4 lane + 256 k. out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,
-// in the parts' order.
+// Joins the parts of split row tiles: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s
+// - M) l_s. Each work-group that a tile's keys were spread over joins its share
+// of the tile's rows, so the parts are read by as many work-groups as wrote
+// them. Work-group (c, k): slot 2 c + k's tile. A row's parts are summed by the
+// four waves in turn (wave w parts w, w + 4, ...), lane the columns 4 lane + 256 j,
+// and the four sums in order.
 template <int ROWS, int LC, bool OBF>
 __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
     constexpr uint32_t COLS = 128 * LC, NV = (COLS + 255) / 256;
-    const uint32_t c = blockIdx.x, lane = threadIdx.x & 63u, wv = threadIdx.x >> 6;
-    const uint32_t* desc = p.desc + 4 * c;
+    __shared__ f32x4 sums[4][NV][64];
+    __shared__ float wsum[4];
+    const uint32_t c = blockIdx.x, lane = threadIdx.x & 63u, wv = uni(threadIdx.x >> 6);
+    const uint32_t* desc = p.desc + 4 * (2 * c + blockIdx.y);
     if (desc[0] == 0) return;
     uint32_t status = 0;
     const Req q = request<ROWS>(p, desc[0] - 1u, status);
-    const uint32_t rt = desc[1], c1 = desc[2], H = p.a.n_heads, L = p.a.cache.kv_lora_rank;
+    const uint32_t rt = desc[1], c0 = desc[2], S = desc[3] - c0 + 1u, H = p.a.n_heads, L = p.a.cache.kv_lora_rank;
     const uint32_t all = q.nodes * H - rt * ROWS, rows = all < ROWS ? all : ROWS;
-    for (uint32_t lr = 16u * blockIdx.y + wv; lr < 16u * blockIdx.y + 16u && lr < rows; lr += 4) {
-        // part s: slot 2 c + 1 for s = 0, else 2 (c + s)
-        const uint32_t S = c1 - c + 1u;
+    for (uint32_t lr = rows * (c - c0) / S; lr < rows * (c - c0 + 1u) / S; lr++) {
+        // part s: slot 2 c0 + 1 for s = 0, else 2 (c0 + s)
+        auto at = [&](uint32_t s) { return (size_t)(s == 0 ? 2u * c0 + 1u : 2u * (c0 + s)) * ROWS + lr; };
         float M = kNone;
-        for (uint32_t s = lane; s < S; s += 64) {
-            const uint32_t slot = s == 0 ? 2u * c + 1u : 2u * (c + s);
-            M = fmaxf(M, p.part_ml[2u * (slot * ROWS + lr)]);
-        }
+        for (uint32_t s = lane; s < S; s += 64) M = fmaxf(M, p.part_ml[2 * at(s)]);
         for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
         f32x4 y[NV];
 #pragma unroll
         for (uint32_t k = 0; k < NV; k++) y[k] = f32x4{0.f, 0.f, 0.f, 0.f};
         float sum = 0.f;
 #pragma unroll 4
-        for (uint32_t s = 0; s < S; s++) {
-            const uint32_t slot = s == 0 ? 2u * c + 1u : 2u * (c + s);
-            const float w = exp2_(p.part_ml[2u * (slot * ROWS + lr)] - M);
-            sum += w * p.part_ml[2u * (slot * ROWS + lr) + 1u];
-            const float* o = p.part + ((size_t)slot * ROWS + lr) * COLS + 4u * lane;
+        for (uint32_t s = wv; s < S; s += 4) {
+            const float* ml = p.part_ml + 2 * at(s);
+            const float w = exp2_(ml[0] - M);
+            sum += w * ml[1];
+            const float* o = p.part + at(s) * COLS + 4u * lane;
 #pragma unroll
             for (uint32_t k = 0; k < NV; k++) {
                 if (4u * lane + 256u * k < COLS) {
@@ -562,21 +591,25 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
                 }
             }
         }
-        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-        const uint32_t row = rt * ROWS + lr, node = row / H, h = row - node * H;
-        const size_t at = (size_t)(q.t0 + node) * p.a.out_stride + (size_t)h * L;
 #pragma unroll
-        for (uint32_t k = 0; k < NV; k++) {
-            const uint32_t col = 4u * lane + 256u * k;
+        for (uint32_t k = 0; k < NV; k++) sums[wv][k][lane] = y[k];
+        if (lane == 0) wsum[wv] = sum;
+        __syncthreads();
+        if (wv < NV) {
+            const float total = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
+            const float inv = total == 0.f ? 0.f : 1.0f / total;
+            f32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                v[j] = ((sums[0][wv][lane][j] + sums[1][wv][lane][j]) + (sums[2][wv][lane][j] + sums[3][wv][lane][j])) * inv;
+            const uint32_t row = rt * ROWS + lr, node = row / H, h = row - node * H, col = 4u * lane + 256u * wv;
+            const size_t o = (size_t)(q.t0 + node) * p.a.out_stride + (size_t)h * L + col;
             if (col < L) {
-                const f32x4 v = y[k];
-                if (OBF)
-                    gst((u32x2*)((uint16_t*)p.a.d_out + at + col),
-                        u32x2{pack_bf16(v[0] * inv, v[1] * inv), pack_bf16(v[2] * inv, v[3] * inv)});
-                else
-                    gst((f32x4*)((float*)p.a.d_out + at + col), f32x4{v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv});
+                if (OBF) gst((u32x2*)((uint16_t*)p.a.d_out + o), u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])});
+                else gst((f32x4*)((float*)p.a.d_out + o), v);
             }
         }
+        __syncthreads();
     }
 }
 template <bool BF>
@@ -666,7 +699,7 @@ uint32_t row_class(const wl_tree_attn& a) {  // rows of a work-group's block
 
 size_t tree_scratch(const wl_tree_attn& a) {
     const size_t rows = 2 * kGrid * 64;
-    return rows * (128 * lat_class(a) + 2) * 4 + kGrid * 16;
+    return rows * (128 * lat_class(a) + 2) * 4 + 2 * kGrid * 16;
 }
 
 template <int MT, int RG, int LC>
@@ -675,7 +708,7 @@ int run_bf16(const Tree& p, hipStream_t st) {
     hipLaunchKernelGGL((tree_bf16_kernel<MT, RG, LC>), dim3(kGrid), dim3(256 * RG), 0, st, p, 1u);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL((tree_join_kernel<ROWS, LC, true>), dim3(kGrid, ROWS / 16), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((tree_join_kernel<ROWS, LC, true>), dim3(kGrid, 2), dim3(256), 0, st, p);
     return (int)hipGetLastError();
 }
 
