@@ -9,7 +9,7 @@ namespace wl {
 namespace paged {
 namespace {
 
-constexpr uint32_t kKT = 64;    // keys of a tile
+constexpr uint32_t kKT = 32;    // keys of a tile
 constexpr uint32_t kGrid = 256; // work-groups of a launch: one per CU (LDS and registers allow one)
 constexpr float kNone = -3.0e38f;  // the running maximum of a row that has seen no key
 
@@ -24,18 +24,21 @@ struct Tree {
     float scale2;      // scale * log2(e): scores in powers of two
     float* part;       // [2 kGrid][rows][cols] unnormalised sums of split tiles
     float* part_ml;    // [2 kGrid][rows][2] their maxima and weight sums
-    uint32_t* desc;    // [2 kGrid][4] split tiles: {request + 1, row tile, first and last work-group}
+    uint32_t* desc;    // [2 kGrid][8] the parts' row tiles: {request + 1, row tile, base, per}, the last two 64-bit
 };
 
 // ---- the work and its split --------------------------------------------------
 // A request's rows (node, head) come in tiles of ROWS, its keys in tiles of
-// kKT; a unit is one of each. The units of all requests, row tile by row tile,
-// stand in one row, and work-group c takes [c per, c per + per) of them, so
-// every work-group has the same number of key tiles to go through, whatever
-// the requests' lengths. A row tile that falls into one work-group is finished
-// there; one that is split leaves its parts in the scratch for the second
-// launch. Work-group b runs on XCD b % 8: c = (b % 8)(G / 8) + b / 8, so the
-// row tiles of a request that run at the same time share one XCD's L2.
+// kKT; a unit is one of each. The units of all requests stand in one row, and
+// work-group c takes [c per, c per + per) of them, so every work-group has the
+// same number of key tiles to go through, whatever the requests' lengths. A
+// request's keys are cut into chunks of at least `per` tiles (one chunk, if they
+// are fewer); its units come chunk by chunk, in a chunk row tile by row tile:
+// the row tiles that run at the same time are at the same keys, which the L2 of
+// their XCD then holds once for all of them. (Work-group b runs on XCD b % 8:
+// c = (b % 8)(G / 8) + b / 8.) A row tile that one work-group has whole is
+// finished there; the others leave their parts in the scratch for the second
+// launch, at most two per work-group: its first walk's and its last one's.
 struct Req {
     uint32_t t0, nodes, len, keys, nrt, nkt, flaw;  // flaw: WL_PAGED_E_* (its rows get NaN)
 };
@@ -118,7 +121,9 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
     return f;
 }
 
-__device__ const uint32_t g_zero[4] = {0u, 0u, 0u, 0u};
+// Chunk j of a request's nc: key tiles [chunk_at(j), chunk_at(j + 1)), each at least `per` if nc > 1.
+WL_DEV uint32_t chunks(const Req& q, uint64_t per) { return per > q.nkt ? 1u : q.nkt / (uint32_t)per; }
+WL_DEV uint32_t chunk_at(const Req& q, uint32_t nc, uint32_t j) { return (uint32_t)((uint64_t)j * q.nkt / nc); }
 
 WL_DEV uint32_t pack_bf16(float a, float b) {
     bf16x2 r;
@@ -146,52 +151,65 @@ WL_DEV constexpr uint32_t swz(uint32_t row) { return ((row & 3u) << 1) | (row & 
 WL_DEV constexpr uint32_t swz8(uint32_t row) { return (row & 2u) | ((row & 8u) >> 1); }
 
 // ---- 16-bit queries and cache --------------------------------------------------
-// ROWS = 16 MT RG rows (node, head) against 64 keys at a time, RG groups of four
-// waves with 16 MT rows each.
-//   S^T[keys][rows] = K Q^T: wave (ks, kh) of a group takes keys [32 ks, + 32)
-//           and half kh of the columns (of the latent and of the rotary ones),
-//           whose part of the queries it holds in registers (2 LC + 1 steps of
-//           32 columns, MT row tiles) through the whole walk; it hands the sums of one 16-key tile to the wave of the
-//           other half and takes those of its own, 16 (2 ks + kh), from it;
-//   P = 2^(S - m) in bf16, through LDS, to all waves of the group;
-//   O^T[cols][rows] += V^T P^T: wave w owns columns [32 LC w, + 32 LC); the key
-//           rows are read again, transposed (ds_read_b64_tr_b16).
+// ROWS = 8 NW rows (node, head) against 32 keys at a time, NW waves.
+//   S^T[keys][rows] = K Q^T: wave w takes row tile w / 2 and 16-key tile w % 2;
+//           its 16 rows' queries stay in its registers through the whole walk
+//           (4 LC + 2 steps of 32 columns);
+//   P = 2^(S - m) in bf16, through LDS, to the four waves of the rows' group;
+//   O^T[cols][rows] += V^T P^T: a group of four waves has 32 rows, its wave w % 4
+//           the columns [32 LC (w % 4), + 32 LC); the key rows are read again,
+//           transposed (ds_read_b64_tr_b16).
 // m is a reference, not the maximum: that of the walk's first tile. Weights may
 // exceed 1 and lose nothing by it (bf16 and f32 keep their relative precision);
 // only where a score passes it by kSlack powers of two the walk is done again,
-// after one over the scores alone for the true maxima. So nothing is rescaled,
-// and a tile costs three barriers.
-// Key rows come into LDS by DMA (16 bytes a lane), a tile ahead, a wave for a
-// row, its address in scalars: rows behind the last key and columns behind the
-// row's are read as zeros by the resource's bounds. The rotary parts have one
-// buffer, filled again as soon as the scores are there.
+// after one over the scores alone for the true maxima. So nothing is rescaled.
+// Key rows come into a ring of four tiles in LDS by DMA (16 bytes a lane), up to
+// three tiles ahead, a wave for a row, its address in scalars: rows behind the
+// last key and columns behind the row's are read as zeros by the resource's
+// bounds. One barrier a tile: before it a wave has written its weights of tile t
+// (two buffers in turn) and waited for its rows of tile t + 1; behind it tile t
+// - 1's place is free for tile t + 3, called for between tile t's products.
 constexpr float kSlack = 64.f;  // a weight at most 2^64, 2^31 of them 2^95
 
-template <int MT, int RG, int LC>
-__global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t min_per) {
-    constexpr uint32_t ROWS = 16 * MT * RG, PITCH = 256 * LC, NL = 2 * LC, NS = NL + 1, CT = 2 * LC, DR = 16 / RG;
-    __shared__ __align__(1024) uint8_t lat0[kKT * PITCH], lat1[kKT * PITCH];
-    __shared__ __align__(1024) uint8_t rot[kKT * 128];
-    // a slot per wave, written by the other half's wave (partial scores) and,
-    // once it has read them, by itself: its weights [rows of the group][16 keys]
-    // and its rows' maxima
-    constexpr uint32_t SLOT = 1024 * MT, MAXIMA = 512 * MT;
-    __shared__ __align__(1024) uint8_t xbuf[4 * RG * SLOT];
+// s_waitcnt vmcnt(N): all but the last N memory operations of this wave are done.
+template <uint32_t N>
+WL_DEV void vm_wait() {
+    static_assert(N < 64u, "vmcnt is 6 bits");
+    __builtin_amdgcn_s_waitcnt((N & 15u) | ((N >> 4) << 14) | 0x0F70u);
+}
+
+// A barrier that orders LDS accesses of the waves' instructions only: DMA into
+// LDS goes on across it (a release fence would wait for that too).
+WL_DEV void ring_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
+template <int NW, int LC>
+__global__ __launch_bounds__(64 * NW) void tree_bf16_kernel(Tree p, uint32_t min_per) {
+    constexpr uint32_t ROWS = 8 * NW, PITCH = 256 * LC, NL = 4 * LC, NS = NL + 2, CT = 2 * LC, DR = 32 / NW;
+    // the ring: separate objects, so that the compiler's own waits for DMA-written LDS stay per tile
+    __shared__ __align__(1024) uint8_t ring0[kKT * (PITCH + 128)], ring1[kKT * (PITCH + 128)], ring2[kKT * (PITCH + 128)],
+        ring3[kKT * (PITCH + 128)];
+    constexpr uint32_t ROT = kKT * PITCH;  // the rotary parts' place behind the latent ones
+    __shared__ __align__(1024) uint8_t pb0[ROWS * 64], pb1[ROWS * 64];  // weights [row][32 keys]
+    __shared__ float rowred[2][ROWS];                                   // per 16-key tile
     __shared__ uint64_t seen[ROWS];
-    __shared__ float wsum[4][ROWS];
     __shared__ uint32_t bad_page, again;
-    __shared__ uint64_t tmp[4 * RG + 2];
+    __shared__ uint64_t tmp[NW + 2];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uni(tid >> 6), n = lane & 15u, g = lane >> 4;
-    const uint32_t wv = wave & 3u, kh = wave & 1u, r0 = 16u * MT * (wave >> 2);
-    uint8_t* slot_own = xbuf + wave * SLOT;
-    uint8_t* slot_other = xbuf + (wave ^ 1u) * SLOT;
-    const uint8_t* slots = xbuf + (wave & ~3u) * SLOT;  // the group's
+    const uint32_t sr = 8u * (wave & ~1u), sk = 16u * (wave & 1u);  // first row and key of this wave's scores
+    const uint32_t pr = 32u * (wave >> 2), wv = wave & 3u;          // first row of its sums, and its columns
     const uint32_t c = (blockIdx.x % 8u) * (kGrid / 8u) + blockIdx.x / 8u;
     const uint32_t H = p.a.n_heads, L = p.a.cache.kv_lora_rank, RP = p.a.cache.qk_rope;
     if (tid == 0) bad_page = again = 0;
-    const Place f = find_place<ROWS, 256 * RG>(p, c, min_per, tmp);
+    const Place f = find_place<ROWS, 64 * NW>(p, c, min_per, tmp);
     const uint64_t u1 = f.u0 + f.per < f.total ? f.u0 + f.per : f.total;
-    if (tid < 2) p.desc[4 * (2 * c + tid)] = 0;
+    if (tid < 2) p.desc[8 * (2 * c + tid)] = 0;
     if (f.u0 >= u1) return;
 
     uint64_t u = f.u0, base = f.base;
@@ -202,314 +220,276 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
             base += (uint64_t)q.nrt * q.nkt;
             q = request<ROWS>(p, ++r, status);
         }
-        const uint32_t rt = uni((uint32_t)((u - base) / q.nkt)), kt0 = uni((uint32_t)((u - base) % q.nkt));
-        const uint32_t kt1 = uni((uint32_t)(u1 - u < q.nkt - kt0 ? kt0 + (u1 - u) : q.nkt));
+        const uint64_t o = u - base;
+        const uint32_t nc = uni(chunks(q, f.per)), j = uni((uint32_t)((((o / q.nrt) + 1) * nc - 1) / q.nkt));
+        const uint32_t ka = uni(chunk_at(q, nc, j)), kb = uni(chunk_at(q, nc, j + 1));
+        const uint64_t oj = o - (uint64_t)q.nrt * ka;
+        const uint32_t rt = uni((uint32_t)(oj / (kb - ka))), kt0 = uni(ka + (uint32_t)(oj % (kb - ka)));
+        const uint32_t kt1 = uni(u1 - u < kb - kt0 ? kt0 + (uint32_t)(u1 - u) : kb);
+        const uint32_t slot = 2u * c + (u == f.u0 ? 0u : 1u);
         u += kt1 - kt0;
         const uint32_t rows = uni(q.nodes * H - rt * ROWS < ROWS ? q.nodes * H - rt * ROWS : ROWS);
         const int32_t* table = p.a.d_table + (size_t)r * p.a.max_pages;
 
-        f32x4 acc[MT][CT];
-        float m[MT], l[MT];
+        f32x4 acc[2][CT];
+        float m = kNone, l = 0.f;  // of row sr + n: the reference, this lane's part of the weights' sum
         auto clear = [&]() {
+            l = 0.f;
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
-                l[i] = 0.f;
+            for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (uint32_t j = 0; j < CT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
+                for (uint32_t k = 0; k < CT; k++) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
         };
         bool bad = false;
         if (q.flaw) {
             clear();
-#pragma unroll
-            for (int i = 0; i < MT; i++) m[i] = kNone;
         } else {
-            int32_t page = 0;
-            // the page of key 64 t + lane
+            // the page of key kKT t + lane % kKT; behind the last key the last one's
             auto page_of = [&](uint32_t t) {
-                const uint32_t key = t * kKT + lane;
-                return key < q.keys ? table[key >> p.psh] : -1;
+                const uint32_t key = t * kKT + (lane & (kKT - 1u));
+                return table[(key < q.keys ? key : q.keys - 1u) >> p.psh];
             };
-            uint32_t ri_rot = 0, nb_rot = 0;
-            auto issue = [&](uint8_t* lat, uint32_t t, int32_t page) {
-                const uint32_t key = t * kKT + lane;
-                const bool ok = key < q.keys && page >= 0 && (uint32_t)page < p.a.cache.n_pages;
-                bad |= key < q.keys && !ok;
-                const uint32_t ri = ok ? ((uint32_t)page << p.psh) + (key & (p.a.cache.page_size - 1u)) : 0u;
-                const uint32_t nb = ok ? 2u * L : 0u;  // a row that is not there is read as zeros
-                const uint64_t sb = 2ull * p.a.cache.row_stride;
-                uint32_t lx = lane * 16u;
-                asm volatile("" : "+v"(lx));  // the offsets are worked out per tile, not held
-                const uint32_t d0 = DR * wave;
-#pragma unroll
-                for (uint32_t i = 0; i < DR; i++) {
-                    const uint32_t row = __builtin_amdgcn_readlane(ri, d0 + i);
-                    const rsrc_t rs = make_rsrc((const uint8_t*)p.a.cache.d_rows + row * sb, __builtin_amdgcn_readlane(nb, d0 + i));
-                    if (LC == 4 || lane < 16 * LC)
-                        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, WL_LDS(lat + (d0 + i) * PITCH), 16u,
-                                                                 lx ^ (16u * swz((d0 + i) & 15u)), 0u, 0, 0);
-                }
-                ri_rot = ri;
-                nb_rot = nb;
+            // the rows of tile t and whether they are there (read as zeros, if not), lane's key;
+            // tiles behind the walk's last are called for too, as zeros, so that a wave's
+            // memory operations can be counted
+            uint32_t ri = 0, nb = 0;
+            auto find_rows = [&](uint32_t t, int32_t page) {
+                const uint32_t key = t * kKT + (lane & (kKT - 1u));
+                const bool in = t < kt1 && key < q.keys, ok = in & (page >= 0) & ((uint32_t)page < p.a.cache.n_pages);
+                bad |= in && !ok;
+                ri = ok ? ((uint32_t)page << p.psh) + (key & (p.a.cache.page_size - 1u)) : 0u;
+                nb = ok ? 1u : 0u;
             };
-            auto issue_rot = [&]() {
-#pragma unroll
-                for (uint32_t j = 0; j < DR / 8; j++) {
-                    const uint32_t kr = DR * wave + 8u * j + (lane >> 3);
-                    const uint32_t row = __shfl(ri_rot, kr, 64), there = __shfl(nb_rot, kr, 64);
-                    const uint32_t ch = (lane & 7u) ^ swz8(kr & 15u);
-                    const uint8_t* src = there && 8u * ch < RP ? (const uint8_t*)p.a.cache.d_rows +
-                                                                     row * (2ull * p.a.cache.row_stride) + 2u * L + 16u * ch
-                                                               : (const uint8_t*)g_zero;
-                    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)src,
-                                                     WL_LDS(rot + (DR * wave + 8u * j) * 128u), 16u, 0, 0);
-                }
+            auto issue_row = [&](uint8_t* lat, uint32_t i) {  // the wave's i-th row
+                const uint32_t kr = DR * wave + i, there = __builtin_amdgcn_readlane(nb, kr);
+                const uint8_t* row = (const uint8_t*)p.a.cache.d_rows +
+                                     __builtin_amdgcn_readlane(ri, kr) * (2ull * p.a.cache.row_stride);
+                const rsrc_t rl = make_rsrc(row, there ? 2u * L : 0u), rr = make_rsrc(row + 2u * L, there ? 2u * RP : 0u);
+                if (LC == 4 || lane < 16 * LC)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, WL_LDS(lat + kr * PITCH), 16u,
+                                                             16u * (lane ^ swz(kr & 15u)), 0u, 0, 0);
+                if (lane < 8)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, WL_LDS(lat + ROT + kr * 128u), 16u, 16u * (lane ^ swz8(kr & 15u)),
+                                                             0u, 0, 0);
             };
-            // the queries, in the operand's layout: lane (row n, k group g)
-            bf16x8 qf[MT][NS];
-            const rsrc_t ql = make_rsrc((const uint16_t*)p.a.d_q_lat + q.t0 * p.a.q_lat_stride,
-                                        2u * ((q.nodes - 1u) * (uint32_t)p.a.q_lat_stride + H * L));
-            const rsrc_t qr = make_rsrc((const uint16_t*)p.a.d_q_rope + q.t0 * p.a.q_rope_stride,
-                                        2u * ((q.nodes - 1u) * (uint32_t)p.a.q_rope_stride + H * RP));
+            auto issue_tile = [&](uint8_t* lat, uint32_t t, int32_t page) {
+                find_rows(t, page);
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
-                const uint32_t lr = r0 + 16u * i + n, row = rt * ROWS + lr, node = row / H, h = row - node * H;
+                for (uint32_t i = 0; i < DR; i++) issue_row(lat, i);
+            };
+            // the queries of rows sr + n, in the operand's layout: lane (row n, k group g)
+            bf16x8 qf[NS];
+            {
+                const rsrc_t ql = make_rsrc((const uint16_t*)p.a.d_q_lat + q.t0 * p.a.q_lat_stride,
+                                            2u * ((q.nodes - 1u) * (uint32_t)p.a.q_lat_stride + H * L));
+                const rsrc_t qr = make_rsrc((const uint16_t*)p.a.d_q_rope + q.t0 * p.a.q_rope_stride,
+                                            2u * ((q.nodes - 1u) * (uint32_t)p.a.q_rope_stride + H * RP));
+                const uint32_t lr = sr + n, row = rt * ROWS + lr, node = row / H, h = row - node * H;
                 const bool live = lr < rows;
                 const uint32_t vl = live ? 2u * (node * (uint32_t)p.a.q_lat_stride + h * L + 8u * g) : kOOB;
                 const uint32_t vr = live ? 2u * (node * (uint32_t)p.a.q_rope_stride + h * RP + 8u * g) : kOOB;
 #pragma unroll
                 for (uint32_t s = 0; s < NS; s++) {
-                    const bool lat = s < NL;
-                    const uint32_t o = 64u * (lat ? kh * NL + s : kh);
-                    u32x4 x = lat ? bld16(ql, vl + o, 0) : bld16(qr, vr + o, 0);
-                    if (o / 2u + 8u * g >= (lat ? L : RP)) x = u32x4{0u, 0u, 0u, 0u};
-                    qf[i][s] = as_bf16x8(x);
+                    u32x4 x = s < NL ? bld16(ql, vl + 64u * s, 0) : bld16(qr, vr + 64u * (s - NL), 0);
+                    if (32u * (s < NL ? s : s - NL) + 8u * g >= (s < NL ? L : RP)) x = u32x4{0u, 0u, 0u, 0u};
+                    qf[s] = as_bf16x8(x);
                 }
-                if (wv == 0 && g == 0) {
+                if (sk == 0 && g == 0) {
                     const uint32_t nd = live ? node : 0u;
                     seen[lr] = p.a.d_mask ? p.a.d_mask[q.t0 + nd] : (2ull << nd) - 1ull;
                 }
             }
-            // the scores of tile t for this wave's 16 keys (row n, keys 4 g + j of them) in
-            // powers of two; `between` runs once the rotary buffer is free
-            auto scores = [&](uint8_t* lat, uint32_t t, uint32_t lane, f32x4* sc, auto between) {
+            auto has_nodes = [&](uint32_t t) { return (t + 1) * kKT > q.len; };  // tree nodes, or the end, in tile t
+            // the scores of row sr + n with keys sk + 4 g + j of tile t, in powers of two
+            auto scores = [&](const uint8_t* lat, uint32_t t, uint32_t lane) {
                 const uint32_t n = lane & 15u, g = lane >> 4;
-                // this half's part of the scores of keys 32 ks + 16 k + ...: chunk 4 st + g of a
-                // row lies at (64 st) ^ (16 (g ^ swz))
-                f32x4 pa[2][MT];
-#pragma unroll
-                for (int i = 0; i < MT; i++) pa[0][i] = pa[1][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-                const uint32_t key0 = 32u * (wv >> 1) + n;
-                const uint32_t ko = key0 * PITCH, kx = 16u * (g ^ swz(n));
-                const uint32_t ro = key0 * 128u + 16u * (g ^ swz8(n));
-                auto kread = [&](uint32_t s, uint32_t k) {
-                    return s < NL ? *(const u32x4*)(lat + ko + ((64u * (kh * NL + s)) ^ kx) + 16u * k * PITCH)
-                                  : *(const u32x4*)(rot + (ro ^ (64u * kh)) + 2048u * k);
+                // chunk 4 s + g of a row lies at (64 s) ^ (16 (g ^ swz))
+                const uint32_t ko = (sk + n) * PITCH, kx = 16u * (g ^ swz(n));
+                const uint32_t ro = (sk + n) * 128u + 16u * (g ^ swz8(n));
+                auto kread = [&](uint32_t s) {
+                    return s < NL ? *(const u32x4*)(lat + ko + (kx ^ (64u * (s & 3u))) + 256u * (s >> 2))
+                                  : *(const u32x4*)(lat + ROT + (ro ^ (64u * (s - NL))));
                 };
-                {  // the reads of a step ahead of its products
-                    u32x4 kf[2][2];
-                    kf[0][0] = kread(0, 0);
-                    kf[0][1] = kread(0, 1);
+                f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+                constexpr uint32_t KG = 2;  // reads a group of steps ahead of their products
+                u32x4 kf[2][KG];
 #pragma unroll
-                    for (uint32_t s = 0; s < NS; s++) {
-                        const uint32_t b = s & 1u;
-                        if (s + 1 < NS) {
-                            kf[b ^ 1u][0] = kread(s + 1, 0);
-                            kf[b ^ 1u][1] = kread(s + 1, 1);
-                        }
+                for (uint32_t k = 0; k < KG; k++) kf[0][k] = kread(k);
 #pragma unroll
-                        for (uint32_t k = 0; k < 2; k++)
+                for (uint32_t s = 0; s < NS; s += KG) {
+                    const uint32_t b = (s / KG) & 1u;
+                    if (s + KG < NS) {
 #pragma unroll
-                            for (int i = 0; i < MT; i++) pa[k][i] = mma(as_bf16x8(kf[b][k]), qf[i][s], pa[k][i]);
-                        __builtin_amdgcn_sched_barrier(0);
+                        for (uint32_t k = 0; k < KG; k++) kf[b ^ 1u][k] = kread(s + KG + k);
                     }
+                    s0 = mma(as_bf16x8(kf[b][0]), qf[s], s0);
+                    s1 = mma(as_bf16x8(kf[b][1]), qf[s + 1], s1);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                f32x4 sc;
 #pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    *(f32x4*)(slot_other + 1024u * i + 16u * lane) = kh ? pa[0][i] : pa[1][i];
-                    sc[i] = kh ? pa[1][i] : pa[0][i];
-                }
-                lds_barrier();
-                between();
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    const f32x4 o = *(const f32x4*)(slot_own + 1024u * i + 16u * lane);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) sc[i][j] = (kh ? o[j] + sc[i][j] : sc[i][j] + o[j]) * p.scale2;
-                }
-                if ((t + 1) * kKT > q.len) {  // tree nodes, or the end, in this tile
+                for (int j = 0; j < 4; j++) sc[j] = (s0[j] + s1[j]) * p.scale2;
+                if (has_nodes(t)) {
                     // a row that some nodes may not see must not reach them through
-                    // 0 x inf: its non-finite chunks are cleared (every score is
-                    // there), and its scores are NaN for those that see it. The
-                    // rotary part only enters scores.
-                    const uint32_t mykey = t * kKT + 16u * wv + n;
+                    // 0 x inf: where its latent part is not finite, its scores are NaN
+                    // for those that see it, and the part is cleared before the sums
+                    // (clear_flawed). The rotary part only enters scores.
                     uint32_t nf = 0;
-                    if (mykey >= q.len) {
-                        uint8_t* row = lat + (16u * wv + n) * PITCH + 16u * g;
+                    if (t * kKT + sk + n >= q.len) {
 #pragma unroll 1
-                        for (uint32_t s = 0; s < 4 * LC; s++) {
-                            u32x4* x = (u32x4*)(row + 64u * s);
-                            if (has_nonfinite(*x)) {
-                                nf = 1;
-                                *x = u32x4{0u, 0u, 0u, 0u};
-                            }
-                        }
+                        for (uint32_t s = 0; s < NL; s++) nf |= has_nonfinite(*(const u32x4*)(lat + ko + 16u * g + 64u * s)) ? 1u : 0u;
                     }
                     uint64_t fl = __ballot(nf != 0);  // lane 16 g + n: key n
                     fl |= fl >> 32;
                     const uint32_t flawed = (uint32_t)(fl | (fl >> 16));
+                    const uint64_t bits = seen[sr + n];
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const uint32_t kj = 4u * g + j, key = t * kKT + 16u * wv + kj;
+                        const uint32_t kj = 4u * g + j, key = t * kKT + sk + kj;
+                        const uint32_t bit = (uint32_t)(bits >> ((key - q.len) & 63u)) & (key < q.keys ? 1u : 0u);
                         const float nan = (flawed >> kj) & 1u ? __builtin_nanf("") : 0.f;
-#pragma unroll
-                        for (int i = 0; i < MT; i++) {
-                            const uint32_t bit = (uint32_t)(seen[r0 + 16u * i + n] >> ((key - q.len) & 63u)) & (key < q.keys ? 1u : 0u);
-                            sc[i][j] = (bit | (key < q.len ? 1u : 0u)) ? sc[i][j] + nan : -INFINITY;
-                        }
+                        sc[j] = (bit | (key < q.len ? 1u : 0u)) ? sc[j] + nan : -INFINITY;
+                    }
+                }
+                return sc;
+            };
+            auto clear_flawed = [&](uint8_t* lat, uint32_t t) {
+                if (wave < 2 && t * kKT + sk + n >= q.len) {
+#pragma unroll 1
+                    for (uint32_t s = 0; s < NL; s++) {
+                        u32x4* x = (u32x4*)(lat + (sk + n) * PITCH + 16u * g + 64u * s);
+                        if (has_nonfinite(*x)) *x = u32x4{0u, 0u, 0u, 0u};
                     }
                 }
             };
-            // m = the largest of m and what the group's waves have in x (a row's lanes differ in g)
-            auto share_maxima = [&](float* x) {
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    x[i] = fmaxf(x[i], __shfl_xor(x[i], 16, 64));
-                    x[i] = fmaxf(x[i], __shfl_xor(x[i], 32, 64));
-                    if (g == 0) *(float*)(slot_own + MAXIMA + 4u * (16u * i + n)) = x[i];
-                }
-                lds_barrier();
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    m[i] = kNone;
-#pragma unroll
-                    for (uint32_t w = 0; w < 4; w++) m[i] = fmaxf(m[i], *(const float*)(slots + w * SLOT + MAXIMA + 4u * (16u * i + n)));
-                }
+            // m = the largest of x over the row's lanes and its two waves
+            auto share_maxima = [&](float x) {
+                x = fmaxf(x, __shfl_xor(x, 16, 64));
+                x = fmaxf(x, __shfl_xor(x, 32, 64));
+                if (g == 0) rowred[wave & 1u][sr + n] = x;
+                ring_barrier();
+                m = fmaxf(kNone, fmaxf(rowred[0][sr + n], rowred[1][sr + n]));
             };
+            int32_t page = 0, page2 = 0;  // of tiles t + 3 and t + 4
             bool pass = false;
             uint32_t first = kt0;  // the tile that sets the reference
-            auto step = [&](uint8_t* lat, uint8_t* nlat, uint32_t t) {
+            auto step = [&](uint8_t* lat, uint8_t* pb, uint8_t* nlat, uint32_t t) {
                 uint32_t lane = tid & 63u;
                 asm volatile("" : "+v"(lane));  // addresses are worked out per tile, not held in registers
                 const uint32_t n = lane & 15u, g = lane >> 4;
-                vm_drain();
-                lds_barrier();
-                const bool more = t + 1 < kt1;
-                if (more) {
-                    issue(nlat, t + 1, page);
-                    page = page_of(t + 2);
-                }
-                f32x4 sc[MT];
-                scores(lat, t, lane, sc, [&]() {
-                    if (more) issue_rot();
-                });
-                if (t == first) {
-                    float x[MT];
+                const f32x4 sc = scores(lat, t, lane);
+                const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+                if (t == first) share_maxima(top);
+                float e[4];
 #pragma unroll
-                    for (int i = 0; i < MT; i++) x[i] = fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3]));
-                    share_maxima(x);
+                for (int k = 0; k < 4; k++) e[k] = exp2_(sc[k] - m);
+                l += (e[0] + e[1]) + (e[2] + e[3]);
+                pass |= top > m + kSlack;
+                *(u32x2*)(pb + (sr + n) * 64u + 16u * ((sk / 8u + (g >> 1)) ^ ((n & 8u) >> 2)) + 8u * (g & 1u)) =
+                    u32x2{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
+                vm_wait<2 * DR + 1>();  // tile t + 1 is there; t + 2 and a page may be on the way
+                ring_barrier();
+                if (has_nodes(t)) {
+                    clear_flawed(lat, t);
+                    ring_barrier();
                 }
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    float e[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) e[j] = exp2_(sc[i][j] - m[i]);
-                    l[i] += (e[0] + e[1]) + (e[2] + e[3]);
-                    *(u32x2*)(slot_own + (16u * i + n) * 32u + 8u * g) = u32x2{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
-                    pass |= fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])) > m[i] + kSlack;
-                }
-                lds_barrier();
-                // O^T += V^T P^T
+                find_rows(t + 3, page);
+                page = page2;
+                page2 = page_of(t + 5);
                 const uint32_t vq = (lane & 15u) >> 2, vb = (lane & 3u) >> 1;
                 const uint32_t vo = (8u * g + vq) * PITCH + 16u * ((4u * LC * wv + vb) ^ swz((8u * g + vq) & 15u)) + 8u * (lane & 1u);
-                auto vfrag = [&](uint32_t i) {  // columns 16 (i % CT) of the wave's, keys 32 (i / CT) + 8 g + [0, 8)
-                    const uint8_t* pa = lat + (vo ^ (32u * (i % CT))) + 32u * PITCH * (i / CT);
+                auto vfrag = [&](uint32_t k) {  // columns 16 k of the wave's, keys 8 g + [0, 8)
+                    const uint8_t* pa = lat + (vo ^ (32u * k));
                     typedef __attribute__((address_space(3))) s16x4 l_s16x4;
                     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa));
                     const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa + 4 * PITCH));
                     const u32x2 xx = __builtin_bit_cast(u32x2, x), yy = __builtin_bit_cast(u32x2, y);
                     return u32x4{xx[0], xx[1], yy[0], yy[1]};
                 };
-                constexpr uint32_t VG = 2, NV = 2 * CT;
+                constexpr uint32_t VG = 2;
                 u32x4 vf[2][VG];
-                bf16x8 pf[MT];
+                bf16x8 pf[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    pf[i] = as_bf16x8(*(const u32x4*)(pb + (pr + 16u * i + n) * 64u + 16u * (g ^ ((n & 8u) >> 2))));
 #pragma unroll
                 for (uint32_t k = 0; k < VG; k++) vf[0][k] = vfrag(k);
 #pragma unroll
-                for (uint32_t v = 0; v < NV; v += VG) {
-                    const uint32_t b = (v / VG) & 1u, kk = v / CT;
-                    if (v % CT == 0) {
-#pragma unroll
-                        for (int i = 0; i < MT; i++)
-                            pf[i] = as_bf16x8(*(const u32x4*)(slots + (2u * kk + (g >> 1)) * SLOT + (16u * i + n) * 32u + 16u * (g & 1u)));
-                    }
-                    if (v + VG < NV) {
+                for (uint32_t v = 0; v < CT; v += VG) {
+                    const uint32_t b = (v / VG) & 1u;
+                    if (v + VG < CT) {
 #pragma unroll
                         for (uint32_t k = 0; k < VG; k++) vf[b ^ 1u][k] = vfrag(v + VG + k);
                     }
 #pragma unroll
                     for (uint32_t k = 0; k < VG; k++)
 #pragma unroll
-                        for (int i = 0; i < MT; i++) acc[i][(v + k) % CT] = mma(as_bf16x8(vf[b][k]), pf[i], acc[i][(v + k) % CT]);
+                        for (int i = 0; i < 2; i++) acc[i][v + k] = mma(as_bf16x8(vf[b][k]), pf[i], acc[i][v + k]);
+                    constexpr uint32_t PER = (DR * VG + CT - 1) / CT;
+#pragma unroll
+                    for (uint32_t i = v / VG * PER; i < v / VG * PER + PER && i < DR; i++) issue_row(nlat, i);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
             for (;;) {
                 clear();
-                issue(lat0, kt0, page_of(kt0));
-                issue_rot();
-                page = page_of(kt0 + 1);
-                for (uint32_t t = kt0; t < kt1; t += 2) {
-                    step(lat0, lat1, t);
-                    if (t + 1 < kt1) step(lat1, lat0, t + 1);
+                const int32_t pg0 = page_of(kt0), pg1 = page_of(kt0 + 1), pg2 = page_of(kt0 + 2);
+                issue_tile(ring0, kt0, pg0);
+                issue_tile(ring1, kt0 + 1, pg1);
+                page = page_of(kt0 + 3);
+                page2 = page_of(kt0 + 4);
+                issue_tile(ring2, kt0 + 2, pg2);
+                vm_wait<4 * DR + 2>();
+                ring_barrier();
+                for (uint32_t t = kt0;;) {
+                    step(ring0, pb0, ring3, t);
+                    if (++t >= kt1) break;
+                    step(ring1, pb1, ring0, t);
+                    if (++t >= kt1) break;
+                    step(ring2, pb0, ring1, t);
+                    if (++t >= kt1) break;
+                    step(ring3, pb1, ring2, t);
+                    if (++t >= kt1) break;
                 }
+                vm_wait<0>();
                 if (first != kt0) break;
                 if (__ballot(pass) && lane == 0) again = 1u;
-                lds_barrier();
+                ring_barrier();
                 const bool redo = again != 0;
-                lds_barrier();
+                ring_barrier();
                 if (!redo) break;
                 if (tid == 0) again = 0u;
-                float x[MT];
-#pragma unroll
-                for (int i = 0; i < MT; i++) x[i] = kNone;
+                float x = kNone;
                 for (uint32_t t = kt0; t < kt1; t++) {
-                    issue(lat0, t, page_of(t));
-                    issue_rot();
-                    vm_drain();
-                    lds_barrier();
-                    f32x4 sc[MT];
-                    scores(lat0, t, lane, sc, [] {});
-#pragma unroll
-                    for (int i = 0; i < MT; i++)
-                        x[i] = fmaxf(x[i], fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3])));
-                    lds_barrier();
+                    issue_tile(ring0, t, page_of(t));
+                    vm_wait<0>();
+                    ring_barrier();
+                    const f32x4 sc = scores(ring0, t, lane);
+                    x = fmaxf(x, fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
+                    ring_barrier();
                 }
                 share_maxima(x);
-                lds_barrier();
+                ring_barrier();
                 first = ~0u;
             }
         }
-        // the weight sums over the waves' keys; flaws
+        // the weights' sums over the row's lanes and waves; flaws
         if (__ballot(bad) && lane == 0) {
             bad_page = 1u;
             if (p.a.d_status)
                 __hip_atomic_fetch_or(p.a.d_status, WL_PAGED_E_PAGE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
-            l[i] += __shfl_xor(l[i], 16, 64);
-            l[i] += __shfl_xor(l[i], 32, 64);
-            if (g == 0) wsum[wv][r0 + 16u * i + n] = l[i];
-        }
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (g == 0) rowred[wave & 1u][sr + n] = l;
+        const bool whole = kt1 - kt0 == q.nkt;
+        if (!whole && sk == 0 && g == 0) p.part_ml[2u * (slot * ROWS + sr + n)] = m;
         __syncthreads();
         const bool nan = bad_page != 0 || q.flaw;
-        const bool whole = kt0 == 0 && kt1 == q.nkt;
-        const uint32_t slot = 2u * c + (kt0 == 0 ? 1u : 0u);
 #pragma unroll
-        for (int i = 0; i < MT; i++) {
-            const uint32_t lr = r0 + 16u * i + n;
-            float sum = (wsum[0][lr] + wsum[1][lr]) + (wsum[2][lr] + wsum[3][lr]);
+        for (int i = 0; i < 2; i++) {
+            const uint32_t lr = pr + 16u * i + n;
+            float sum = rowred[0][lr] + rowred[1][lr];
             if (nan) sum = __builtin_nanf("");
             if (lr < rows) {
                 if (whole) {
@@ -517,30 +497,26 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
                     uint16_t* o = (uint16_t*)p.a.d_out + (size_t)(q.t0 + node) * p.a.out_stride + (size_t)h * L;
                     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
-                    for (uint32_t ct = 0; ct < CT; ct++) {
-                        const uint32_t col = 32u * LC * wv + 16u * ct + 4u * g;
-                        const f32x4 y = acc[i][ct];
+                    for (uint32_t k = 0; k < CT; k++) {
+                        const uint32_t col = 32u * LC * wv + 16u * k + 4u * g;
+                        const f32x4 y = acc[i][k];
                         if (col < L)
                             gst((u32x2*)(o + col), u32x2{pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv)});
                     }
                 } else {
                     float* o = p.part + ((size_t)slot * ROWS + lr) * (128u * LC);
 #pragma unroll
-                    for (uint32_t ct = 0; ct < CT; ct++) gst((f32x4*)(o + 32u * LC * wv + 16u * ct + 4u * g), acc[i][ct]);
-                    if (wv == 0 && g == 0) {
-                        p.part_ml[2u * (slot * ROWS + lr)] = m[i];
-                        p.part_ml[2u * (slot * ROWS + lr) + 1u] = sum;
-                    }
+                    for (uint32_t k = 0; k < CT; k++) gst((f32x4*)(o + 32u * LC * wv + 16u * k + 4u * g), acc[i][k]);
+                    if (wv == 0 && g == 0) p.part_ml[2u * (slot * ROWS + lr) + 1u] = sum;
                 }
             }
         }
-        if (!whole && tid == (kt0 == 0 ? 1u : 0u)) {  // the thread that cleared it
-            const uint64_t start = base + (uint64_t)rt * q.nkt;
-            uint32_t* desc = p.desc + 4 * slot;
+        if (!whole && tid == (slot & 1u)) {  // the thread that cleared it
+            uint32_t* desc = p.desc + 8 * slot;
             desc[0] = r + 1u;
             desc[1] = rt;
-            desc[2] = (uint32_t)(start / f.per);
-            desc[3] = (uint32_t)((start + q.nkt - 1) / f.per);
+            *(uint64_t*)(desc + 2) = base;
+            *(uint64_t*)(desc + 4) = f.per;
         }
         __syncthreads();
         if (tid == 0) bad_page = 0u;
@@ -549,26 +525,59 @@ __global__ __launch_bounds__(256 * RG) void tree_bf16_kernel(Tree p, uint32_t mi
 }
 
 // Joins the parts of split row tiles: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s
-// - M) l_s. Each work-group that a tile's keys were spread over joins its share
-// of the tile's rows, so the parts are read by as many work-groups as wrote
-// them. Work-group (c, k): slot 2 c + k's tile. A row's parts are summed by the
-// four waves in turn (wave w parts w, w + 4, ...), lane the columns 4 lane + 256 j,
-// and the four sums in order.
+// - M) l_s. Each part's writer (slot blockIdx.x) has four work-groups here that
+// join its share of the tile's rows, so the parts are read by as many CUs as
+// wrote them. The tile's parts are listed first, a thread per chunk of its keys.
+// Of few parts a wave joins a row by itself; many are dealt out to the four
+// waves and their sums added in order. Lane: columns 4 lane + 256 k.
+constexpr uint32_t kJoinZ = 4, kManyParts = 16;
 template <int ROWS, int LC, bool OBF>
 __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
     constexpr uint32_t COLS = 128 * LC, NV = (COLS + 255) / 256;
     __shared__ f32x4 sums[4][NV][64];
     __shared__ float wsum[4];
-    const uint32_t c = blockIdx.x, lane = threadIdx.x & 63u, wv = uni(threadIdx.x >> 6);
-    const uint32_t* desc = p.desc + 4 * (2 * c + blockIdx.y);
+    __shared__ uint32_t count[4], list[2 * kGrid];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = uni(tid >> 6), mine = blockIdx.x;
+    const uint32_t* desc = p.desc + 8 * mine;
     if (desc[0] == 0) return;
     uint32_t status = 0;
     const Req q = request<ROWS>(p, desc[0] - 1u, status);
-    const uint32_t rt = desc[1], c0 = desc[2], S = desc[3] - c0 + 1u, H = p.a.n_heads, L = p.a.cache.kv_lora_rank;
+    const uint32_t rt = desc[1], H = p.a.n_heads, L = p.a.cache.kv_lora_rank;
+    const uint64_t base = *(const uint64_t*)(desc + 2), per = *(const uint64_t*)(desc + 4);
+    {
+        const uint32_t nc = chunks(q, per);
+        uint64_t start = 0;
+        uint32_t w0 = 0, nw = 0;
+        if (tid < nc) {
+            const uint32_t ka = chunk_at(q, nc, tid), kb = chunk_at(q, nc, tid + 1);
+            start = base + (uint64_t)q.nrt * ka + (uint64_t)rt * (kb - ka);
+            w0 = (uint32_t)(start / per);
+            nw = (uint32_t)((start + (kb - ka) - 1) / per) - w0 + 1u;
+        }
+        uint32_t inc = nw;
+        for (uint32_t o = 1; o < 64; o <<= 1) {
+            const uint32_t v = __shfl_up(inc, o, 64);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 63) count[wv] = inc;
+        __syncthreads();
+        uint32_t at = inc - nw;
+        for (uint32_t w = 0; w < wv; w++) at += count[w];
+        for (uint32_t i = 0; i < nw; i++)  // a work-group's first walk has its even slot
+            list[at + i] = 2u * (w0 + i) + (start <= (w0 + i) * per ? 0u : 1u);
+        __syncthreads();
+    }
+    const uint32_t S = count[0] + count[1] + count[2] + count[3];
+    uint32_t idx = 0;
+    for (uint32_t s = lane; s < S; s += 64)
+        if (list[s] == mine) idx = s + 1u;
+    for (int o = 32; o > 0; o >>= 1) idx |= __shfl_xor(idx, o, 64);
+    idx = uni(idx) - 1u;
     const uint32_t all = q.nodes * H - rt * ROWS, rows = all < ROWS ? all : ROWS;
-    for (uint32_t lr = rows * (c - c0) / S; lr < rows * (c - c0 + 1u) / S; lr++) {
-        // part s: slot 2 c0 + 1 for s = 0, else 2 (c0 + s)
-        auto at = [&](uint32_t s) { return (size_t)(s == 0 ? 2u * c0 + 1u : 2u * (c0 + s)) * ROWS + lr; };
+    const bool many = S >= kManyParts;
+    const uint32_t r0 = rows * idx / S, r1 = rows * (idx + 1u) / S;
+    for (uint32_t lr = r0 + (many ? blockIdx.y : 4u * blockIdx.y + wv); lr < r1; lr += many ? kJoinZ : 4u * kJoinZ) {
+        auto at = [&](uint32_t s) { return (size_t)list[s] * ROWS + lr; };
         float M = kNone;
         for (uint32_t s = lane; s < S; s += 64) M = fmaxf(M, p.part_ml[2 * at(s)]);
         for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
@@ -577,7 +586,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
         for (uint32_t k = 0; k < NV; k++) y[k] = f32x4{0.f, 0.f, 0.f, 0.f};
         float sum = 0.f;
 #pragma unroll 4
-        for (uint32_t s = wv; s < S; s += 4) {
+        for (uint32_t s = many ? wv : 0u; s < S; s += many ? 4u : 1u) {
             const float* ml = p.part_ml + 2 * at(s);
             const float w = exp2_(ml[0] - M);
             sum += w * ml[1];
@@ -591,23 +600,34 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
                 }
             }
         }
+        const uint32_t row = rt * ROWS + lr, node = row / H, h = row - node * H;
+        const size_t out = (size_t)(q.t0 + node) * p.a.out_stride + (size_t)h * L;
+        auto put = [&](f32x4 v, float total, uint32_t k) {
+            const float inv = total == 0.f ? 0.f : 1.0f / total;
+            const uint32_t col = 4u * lane + 256u * k;
+            if (col < L) {
+                if (OBF)
+                    gst((u32x2*)((uint16_t*)p.a.d_out + out + col),
+                        u32x2{pack_bf16(v[0] * inv, v[1] * inv), pack_bf16(v[2] * inv, v[3] * inv)});
+                else
+                    gst((f32x4*)((float*)p.a.d_out + out + col), f32x4{v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv});
+            }
+        };
+        if (!many) {
+#pragma unroll
+            for (uint32_t k = 0; k < NV; k++) put(y[k], sum, k);
+            continue;
+        }
 #pragma unroll
         for (uint32_t k = 0; k < NV; k++) sums[wv][k][lane] = y[k];
         if (lane == 0) wsum[wv] = sum;
         __syncthreads();
         if (wv < NV) {
-            const float total = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
-            const float inv = total == 0.f ? 0.f : 1.0f / total;
             f32x4 v;
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                v[j] = ((sums[0][wv][lane][j] + sums[1][wv][lane][j]) + (sums[2][wv][lane][j] + sums[3][wv][lane][j])) * inv;
-            const uint32_t row = rt * ROWS + lr, node = row / H, h = row - node * H, col = 4u * lane + 256u * wv;
-            const size_t o = (size_t)(q.t0 + node) * p.a.out_stride + (size_t)h * L + col;
-            if (col < L) {
-                if (OBF) gst((u32x2*)((uint16_t*)p.a.d_out + o), u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])});
-                else gst((f32x4*)((float*)p.a.d_out + o), v);
-            }
+                v[j] = (sums[0][wv][lane][j] + sums[1][wv][lane][j]) + (sums[2][wv][lane][j] + sums[3][wv][lane][j]);
+            put(v, (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]), wv);
         }
         __syncthreads();
     }
@@ -694,21 +714,20 @@ uint32_t lat_class(const wl_tree_attn& a) {  // 128-column blocks of a row's lat
 }
 uint32_t row_class(const wl_tree_attn& a) {  // rows of a work-group's block
     const uint64_t rows = (uint64_t)a.n_heads * (a.n_req ? (a.n_tokens + a.n_req - 1) / a.n_req : 1);
-    return rows > 32 ? 64 : rows > 16 ? 32 : 16;
+    return rows > 32 ? 64 : 32;
 }
 
 size_t tree_scratch(const wl_tree_attn& a) {
     const size_t rows = 2 * kGrid * 64;
-    return rows * (128 * lat_class(a) + 2) * 4 + 2 * kGrid * 16;
+    return rows * (128 * lat_class(a) + 2) * 4 + 2 * kGrid * 32;
 }
 
-template <int MT, int RG, int LC>
+template <int NW, int LC>
 int run_bf16(const Tree& p, hipStream_t st) {
-    constexpr int ROWS = 16 * MT * RG;
-    hipLaunchKernelGGL((tree_bf16_kernel<MT, RG, LC>), dim3(kGrid), dim3(256 * RG), 0, st, p, 1u);
+    hipLaunchKernelGGL((tree_bf16_kernel<NW, LC>), dim3(kGrid), dim3(64 * NW), 0, st, p, 1u);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL((tree_join_kernel<ROWS, LC, true>), dim3(kGrid, 2), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((tree_join_kernel<8 * NW, LC, true>), dim3(2 * kGrid, kJoinZ), dim3(256), 0, st, p);
     return (int)hipGetLastError();
 }
 
@@ -723,9 +742,8 @@ int launch_tree(const wl_tree_attn& a, void* stream) {
     p.part_ml = p.part + (size_t)2 * kGrid * 64 * 128 * lc;
     p.desc = (uint32_t*)(p.part_ml + (size_t)2 * kGrid * 64 * 2);
     if (a.dtype == WL_TYPE_BF16) {
-        if (rows == 64) return lc == 4 ? run_bf16<2, 2, 4>(p, st) : lc == 2 ? run_bf16<2, 2, 2>(p, st) : run_bf16<2, 2, 1>(p, st);
-        if (rows == 32) return lc == 4 ? run_bf16<1, 2, 4>(p, st) : lc == 2 ? run_bf16<1, 2, 2>(p, st) : run_bf16<1, 2, 1>(p, st);
-        return lc == 4 ? run_bf16<1, 1, 4>(p, st) : lc == 2 ? run_bf16<1, 1, 2>(p, st) : run_bf16<1, 1, 1>(p, st);
+        if (rows == 64) return lc == 4 ? run_bf16<8, 4>(p, st) : lc == 2 ? run_bf16<8, 2>(p, st) : run_bf16<8, 1>(p, st);
+        return lc == 4 ? run_bf16<4, 4>(p, st) : lc == 2 ? run_bf16<4, 2>(p, st) : run_bf16<4, 1>(p, st);
     }
     const dim3 g(a.n_req, (a.n_heads + 3) / 4, 8);
     if (a.cache.dtype == WL_TYPE_BF16) hipLaunchKernelGGL((tree_attn_kernel<false, true>), g, dim3(256), 0, st, a);
