@@ -678,7 +678,7 @@ wl_status   wl_attn_taps(wl_attn* a, wl_attn_taps_out* out);
 #define WL_PAGED_E_SLOT  16u     /* a slot or a source row outside its buffer */
 const char* wl_paged_last_error(void);
 
-/* One layer's cache: n_pages pages of page_size rows (a power of two, at most
+/* One layer's cache: n_pages pages of page_size rows (a power of two, 8 to
  * 1024; n_pages * page_size < 2^31), row_stride elements from row to row (>=
  * kv_lora_rank + qk_rope, a multiple of 8), 16-byte aligned. A row holds the
  * normalised compressed key/value (kv_lora_rank values: a multiple of 8, at

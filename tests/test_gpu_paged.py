@@ -53,7 +53,7 @@ def check_step(m, s, extra=0):
 
 
 @pytest.mark.parametrize("trees", [False, True])
-@pytest.mark.parametrize("R,ps,max_add,max_len", [(1, 1, 1, 0), (1, 16, 64, 40), (3, 1, 5, 9), (37, 16, 64, 300),
+@pytest.mark.parametrize("R,ps,max_add,max_len", [(1, 8, 1, 0), (1, 16, 64, 40), (3, 8, 5, 9), (37, 16, 64, 300),
                                                   (256, 64, 64, 2000), (257, 32, 33, 500), (1024, 8, 9, 200),
                                                   (1025, 16, 17, 100), (4096, 128, 6, 700)])
 def test_map(gpu, R, ps, max_add, max_len, trees):
@@ -88,7 +88,7 @@ def test_map_no_requests(gpu):
 def test_map_takes_pages_it_pushes(gpu):
     """An empty stack: the growing request's pages are the ended ones', the last pushed first."""
     table = np.array([[3, 1, 2, -1], [0, -1, -1, -1], [5, 4, -1, -1]], np.int32)
-    s = dict(ps=4, n_pages=6, max_pages=4, lens=[0, 3, 0], adds=[0, 12, 0], have=[3, 1, 2], free=np.full(6, -5, np.int32),
+    s = dict(ps=8, n_pages=6, max_pages=4, lens=[0, 7, 0], adds=[0, 24, 0], have=[3, 1, 2], free=np.full(6, -5, np.int32),
              n_free=0, table=table, parent=None)
     m = P.Map(**s)
     paged.page_map(m.args)
@@ -97,12 +97,12 @@ def test_map_takes_pages_it_pushes(gpu):
     assert m.get("table")[1].tolist() == [0, 4, 5, 2]
 
 
-REFUSED = [("negative length", dict(lens=[5, -1, 0]), paged.E_LEN),
-           ("negative addition", dict(adds=[2, -2, 1]), paged.E_LEN),
+REFUSED = [("negative length", dict(lens=[10, -1, 0]), paged.E_LEN),
+           ("negative addition", dict(adds=[4, -2, 1]), paged.E_LEN),
            ("pages missing for the tokens held", dict(have=[1, 0, 0]), paged.E_LEN),
            ("more pages than the table's row", dict(have=[1, 9, 0]), paged.E_LEN),
-           ("a request longer than its row", dict(adds=[2, 2 ** 31 - 1, 1]), paged.E_LEN),
-           ("more tokens than the arrays hold", dict(max_tokens=4), paged.E_LEN),
+           ("a request longer than its row", dict(adds=[4, 2 ** 31 - 1, 1]), paged.E_LEN),
+           ("more tokens than the arrays hold", dict(max_tokens=14), paged.E_LEN),
            ("a stack above the cache", dict(n_free=9), paged.E_PAGE),
            ("a stack below nothing", dict(n_free=-1), paged.E_PAGE),
            ("too few pages", dict(n_free=1), paged.E_SPACE)]
@@ -111,10 +111,10 @@ REFUSED = [("negative length", dict(lens=[5, -1, 0]), paged.E_LEN),
 @pytest.mark.parametrize("what,change,bit", REFUSED, ids=[x[0] for x in REFUSED])
 def test_map_refused_on_the_device(gpu, what, change, bit):
     table = np.array([[3, 1, -1], [0, -1, -1], [-1, -1, -1]], np.int32)
-    s = dict(ps=4, n_pages=8, max_pages=3, lens=[5, 4, 0], adds=[2, 5, 1], have=[2, 1, 0],
+    s = dict(ps=8, n_pages=8, max_pages=3, lens=[10, 8, 0], adds=[4, 10, 1], have=[2, 1, 0],
              free=np.array([2, 4, 5, 6, 7, -5, -5, -5], np.int32), n_free=5, table=table, parent=None)
     s = {**s, **change}
-    m = P.Map(**{"max_tokens": 8, **s})
+    m = P.Map(**{"max_tokens": 15, **s})
     paged.page_map(m.args)
     hip.synchronize()
     assert m.get("status")[0] == bit
@@ -141,13 +141,13 @@ def test_map_too_large_trees_and_wrong_parents(gpu):
 
 
 def test_map_pages_outside_the_cache(gpu):
-    s = dict(ps=4, n_pages=6, max_pages=3, lens=[2, 3], adds=[1, 3], have=[1, 1], n_free=2, parent=None,
+    s = dict(ps=8, n_pages=6, max_pages=3, lens=[6, 7], adds=[1, 3], have=[1, 1], n_free=2, parent=None,
              free=np.array([99, -3, 0, 0, 0, 0], np.int32), table=np.array([[6, -1, -1], [1, -1, -1]], np.int32))
     m = P.Map(**s)
     paged.page_map(m.args)
     hip.synchronize()
     assert m.get("status")[0] == paged.E_PAGE
-    assert m.get("slot").tolist() == [-1, 7, -1, -1]  # a held page, a held one, and a taken one
+    assert m.get("slot").tolist() == [-1, 15, -1, -1]  # a held page, a held one, and a taken one
 
 
 # ---- the write ----------------------------------------------------------------
@@ -220,7 +220,7 @@ class Write:
 
 
 @pytest.mark.parametrize("x,cache", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("bf16", "f32")])
-@pytest.mark.parametrize("T,L,RP,H,ps,pad", [(1, 512, 64, 64, 64, 0), (1, 8, 8, 0, 1, 8), (7, 96, 24, 5, 16, 16),
+@pytest.mark.parametrize("T,L,RP,H,ps,pad", [(1, 512, 64, 64, 64, 0), (1, 8, 8, 0, 8, 8), (7, 96, 24, 5, 16, 16),
                                              (333, 256, 32, 20, 32, 8), (1030, 504, 56, 3, 8, 0)])
 def test_write(gpu, T, L, RP, H, ps, pad, x, cache):
     w = Write(T + L, T, x, cache, L, RP, H, ps, pad)
@@ -370,8 +370,8 @@ def random_trees(rng, adds):
 
 
 TYPES = [("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32")]
-SHAPES = [(512, 64, 64, 64), (512, 64, 16, 16), (256, 32, 20, 32), (128, 64, 128, 64), (96, 8, 1, 1), (200, 40, 7, 8),
-          (512, 64, 33, 1024), (8, 8, 3, 2)]
+SHAPES = [(512, 64, 64, 64), (512, 64, 16, 16), (256, 32, 20, 32), (128, 64, 128, 64), (96, 8, 1, 8), (200, 40, 7, 8),
+          (512, 64, 33, 1024), (8, 8, 3, 8)]
 
 
 @pytest.mark.parametrize("q,cache", TYPES)

@@ -49,7 +49,7 @@ def refused(call, args):
 
 
 @pytest.mark.parametrize("change", [
-    dict(n_req=4097), dict(page_size=0), dict(page_size=24), dict(page_size=2048), dict(n_pages=0), dict(n_pages=1 << 27),
+    dict(n_req=4097), dict(page_size=0), dict(page_size=4), dict(page_size=24), dict(page_size=2048), dict(n_pages=0), dict(n_pages=1 << 27),
     dict(max_pages=0), dict(max_pages=1 << 29), dict(max_tokens=1 << 30), dict(d_len=None), dict(d_free=None),
     dict(d_n_free=None), dict(d_table=None), dict(d_cu=None), dict(d_slot=None), dict(d_len=at(0) + 2), dict(d_mask=at(12) + 4),
     dict(d_have_out=at(2)), dict(d_n_free_out=at(4)), dict(d_slot=at(5)), dict(d_pos=at(10) + 196), dict(d_table=at(3) + 396)],
@@ -58,7 +58,7 @@ def test_map_refuses(change):
     refused(paged.page_map, a_map(**change))
 
 
-CACHES = [dict(d_rows=None), dict(d_rows=at(20) + 8), dict(dtype=2), dict(n_pages=0), dict(n_pages=1 << 27), dict(page_size=48),
+CACHES = [dict(d_rows=None), dict(d_rows=at(20) + 8), dict(dtype=2), dict(n_pages=0), dict(n_pages=1 << 27), dict(page_size=48), dict(page_size=4),
           dict(kv_lora_rank=0), dict(kv_lora_rank=516), dict(kv_lora_rank=520, row_stride=640), dict(qk_rope=4),
           dict(qk_rope=72, row_stride=640), dict(qk_rope=0), dict(row_stride=568), dict(row_stride=580)]
 

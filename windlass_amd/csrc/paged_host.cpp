@@ -23,7 +23,7 @@ wl_status fail(wl_status s, const char* fmt, ...) {
 }
 
 bool aligned(const void* p, size_t a) { return (uintptr_t)p % a == 0; }
-bool pow2_page(uint32_t ps) { return ps >= 1 && ps <= 1024 && (ps & (ps - 1)) == 0; }
+bool pow2_page(uint32_t ps) { return ps >= 8 && ps <= 1024 && (ps & (ps - 1)) == 0; }
 bool overlap(const void* a, size_t na, const void* b, size_t nb) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
     return a && b && na && nb && x < y + nb && y < x + na;
@@ -33,7 +33,7 @@ size_t esize(uint32_t t) { return t == WL_TYPE_F32 ? 4 : 2; }
 wl_status check_cache(const wl_paged_cache& c) {
     if (!c.d_rows || !aligned(c.d_rows, 16)) return fail(WL_ERR_INVALID, "the cache must be 16-byte aligned and not null");
     if (c.dtype > WL_TYPE_BF16) return fail(WL_ERR_INVALID, "cache type %u", c.dtype);
-    if (!pow2_page(c.page_size)) return fail(WL_ERR_INVALID, "page_size %u: a power of two, 1 to 1024", c.page_size);
+    if (!pow2_page(c.page_size)) return fail(WL_ERR_INVALID, "page_size %u: a power of two, 8 to 1024", c.page_size);
     if (c.n_pages == 0 || (uint64_t)c.n_pages * c.page_size >= (1ull << 31))
         return fail(WL_ERR_INVALID, "n_pages x page_size must be in [1, 2^31)");
     if (c.kv_lora_rank == 0 || c.kv_lora_rank % 8 || c.kv_lora_rank > 512)
@@ -103,7 +103,7 @@ const char* wl_paged_last_error(void) { return t_err; }
 wl_status wl_paged_map(const wl_page_map* m, void* stream) {
     if (!m) return fail(WL_ERR_INVALID, "the argument block is null");
     if (m->n_req > WL_PAGED_MAX_REQ) return fail(WL_ERR_INVALID, "n_req %u exceeds %u", m->n_req, WL_PAGED_MAX_REQ);
-    if (!pow2_page(m->page_size)) return fail(WL_ERR_INVALID, "page_size %u: a power of two, 1 to 1024", m->page_size);
+    if (!pow2_page(m->page_size)) return fail(WL_ERR_INVALID, "page_size %u: a power of two, 8 to 1024", m->page_size);
     if (m->n_pages == 0 || (uint64_t)m->n_pages * m->page_size >= (1ull << 31))
         return fail(WL_ERR_INVALID, "n_pages x page_size must be in [1, 2^31)");
     if (m->max_pages == 0 || (uint64_t)(m->n_req ? m->n_req : 1) * m->max_pages >= (1ull << 31) ||

@@ -2,6 +2,8 @@
 // latent rows (wl_paged_tree_attention).
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "dev_common.h"
 #include "paged.h"
 
@@ -63,23 +65,30 @@ WL_DEV Req request(const Tree& p, uint32_t r, uint32_t& status) {
     return q;
 }
 
-// The launch's units, and the request (and its first unit) that unit u0 = c per
+// a / b, in 32 bits where both fit (64-bit quotients take some hundred instructions).
+WL_DEV uint64_t div64(uint64_t a, uint64_t b) {
+    return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// The launch's units, and the request (with its first unit) that unit u0 = c per
 // falls into. Each thread sums the requests of its share; tmp: a word per wave, and two.
 struct Place {
     uint64_t total, per, u0, base;
     uint32_t r;
+    Req q;
 };
 template <uint32_t ROWS, uint32_t THREADS>
-WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* tmp) {
+WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* tmp, Req* found) {
     constexpr uint32_t NW = THREADS / 64;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = tid >> 6, R = p.a.n_req;
     const uint32_t share = (R + THREADS - 1u) / THREADS;
     uint64_t mine = 0;
     uint32_t status = 0;
+    Req q{};
     for (uint32_t i = 0; i < share; i++) {
         const uint32_t r = tid * share + i;
         if (r < R) {
-            const Req q = request<ROWS>(p, r, status);
+            q = request<ROWS>(p, r, status);
             mine += (uint64_t)q.nrt * q.nkt;
         }
     }
@@ -102,28 +111,29 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
     uint64_t at = inc - mine;
     for (uint32_t w = 0; w < wv; w++) at += tmp[w];
     if (f.u0 >= at && f.u0 < at + mine) {  // one thread at most
-        for (uint32_t i = 0; i < share; i++) {
-            const uint32_t r = tid * share + i;
-            const Req q = request<ROWS>(p, r, status);
-            const uint64_t n = (uint64_t)q.nrt * q.nkt;
-            if (f.u0 < at + n) {
-                tmp[NW] = at;
-                tmp[NW + 1] = r;
-                break;
+        uint32_t r = tid * share;
+        if (share > 1) {
+            for (;; r++) {
+                q = request<ROWS>(p, r, status);
+                const uint64_t n = (uint64_t)q.nrt * q.nkt;
+                if (f.u0 < at + n) break;
+                at += n;
             }
-            at += n;
         }
+        tmp[NW] = at;
+        tmp[NW + 1] = r;
+        *found = q;
     }
     __syncthreads();
     f.base = tmp[NW];
     f.r = uni((uint32_t)tmp[NW + 1]);
-    __syncthreads();
+    f.q = Req{uni(found->t0), uni(found->nodes), uni(found->len), uni(found->keys), uni(found->nrt), uni(found->nkt), uni(found->flaw)};
     return f;
 }
 
 // Chunk j of a request's nc: key tiles [chunk_at(j), chunk_at(j + 1)), each at least `per` if nc > 1.
 WL_DEV uint32_t chunks(const Req& q, uint64_t per) { return per > q.nkt ? 1u : q.nkt / (uint32_t)per; }
-WL_DEV uint32_t chunk_at(const Req& q, uint32_t nc, uint32_t j) { return (uint32_t)((uint64_t)j * q.nkt / nc); }
+WL_DEV uint32_t chunk_at(const Req& q, uint32_t nc, uint32_t j) { return (uint32_t)div64((uint64_t)j * q.nkt, nc); }
 
 WL_DEV uint32_t pack_bf16(float a, float b) {
     bf16x2 r;
@@ -151,24 +161,25 @@ WL_DEV constexpr uint32_t swz(uint32_t row) { return ((row & 3u) << 1) | (row & 
 WL_DEV constexpr uint32_t swz8(uint32_t row) { return (row & 2u) | ((row & 8u) >> 1); }
 
 // ---- 16-bit queries and cache --------------------------------------------------
-// ROWS = 8 NW rows (node, head) against 32 keys at a time, NW waves.
+// ROWS = 32 GR rows (node, head) against 32 keys at a time, GR groups of four
+// waves with 32 rows each. In a group
 //   S^T[keys][rows] = K Q^T: wave w takes row tile w / 2 and 16-key tile w % 2;
 //           its 16 rows' queries stay in its registers through the whole walk
 //           (4 LC + 2 steps of 32 columns);
-//   P = 2^(S - m) in bf16, through LDS, to the four waves of the rows' group;
-//   O^T[cols][rows] += V^T P^T: a group of four waves has 32 rows, its wave w % 4
-//           the columns [32 LC (w % 4), + 32 LC); the key rows are read again,
-//           transposed (ds_read_b64_tr_b16).
+//   P = 2^(S - m) in bf16, through LDS, to the group's waves;
+//   O^T[cols][rows] += V^T P^T: wave w has columns [32 LC w, + 32 LC); the key
+//           rows are read again, transposed (ds_read_b64_tr_b16).
+// One barrier a tile: between two of them a wave makes the weights of tile t and
+// sums tile t - 1, group 0 the sums first, group 1 the weights first. A SIMD has
+// one wave of either group, so one's products fill the other's waits.
 // m is a reference, not the maximum: that of the walk's first tile. Weights may
 // exceed 1 and lose nothing by it (bf16 and f32 keep their relative precision);
 // only where a score passes it by kSlack powers of two the walk is done again,
 // after one over the scores alone for the true maxima. So nothing is rescaled.
-// Key rows come into a ring of four tiles in LDS by DMA (16 bytes a lane), up to
-// three tiles ahead, a wave for a row, its address in scalars: rows behind the
-// last key and columns behind the row's are read as zeros by the resource's
-// bounds. One barrier a tile: before it a wave has written its weights of tile t
-// (two buffers in turn) and waited for its rows of tile t + 1; behind it tile t
-// - 1's place is free for tile t + 3, called for between tile t's products.
+// Key rows come into a ring of four tiles in LDS by DMA (16 bytes a lane): rows
+// behind the last key and columns behind the row's are read as zeros by the
+// resource's bounds. While tiles t - 1 and t are worked on, tile t + 2 is called
+// for between products; before the barrier each wave waits for its rows of t + 1.
 constexpr float kSlack = 64.f;  // a weight at most 2^64, 2^31 of them 2^95
 
 // s_waitcnt vmcnt(N): all but the last N memory operations of this wave are done.
@@ -177,9 +188,8 @@ WL_DEV void vm_wait() {
     static_assert(N < 64u, "vmcnt is 6 bits");
     __builtin_amdgcn_s_waitcnt((N & 15u) | ((N >> 4) << 14) | 0x0F70u);
 }
-
 // A barrier that orders LDS accesses of the waves' instructions only: DMA into
-// LDS goes on across it (a release fence would wait for that too).
+// LDS, loads and stores go on across it (a release fence would wait for them).
 WL_DEV void ring_barrier() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -189,42 +199,44 @@ WL_DEV void ring_barrier() {
     asm volatile("" ::: "memory");
 }
 
-template <int NW, int LC>
-__global__ __launch_bounds__(64 * NW) void tree_bf16_kernel(Tree p, uint32_t min_per) {
-    constexpr uint32_t ROWS = 8 * NW, PITCH = 256 * LC, NL = 4 * LC, NS = NL + 2, CT = 2 * LC, DR = 32 / NW;
+template <int GR, int LC>
+__global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t min_per) {
+    constexpr uint32_t NW = 4 * GR, ROWS = 32 * GR, PITCH = 256 * LC, NL = 4 * LC, NS = NL + 2, CT = 2 * LC, DR = 32 / NW;
     // the ring: separate objects, so that the compiler's own waits for DMA-written LDS stay per tile
     __shared__ __align__(1024) uint8_t ring0[kKT * (PITCH + 128)], ring1[kKT * (PITCH + 128)], ring2[kKT * (PITCH + 128)],
         ring3[kKT * (PITCH + 128)];
     constexpr uint32_t ROT = kKT * PITCH;  // the rotary parts' place behind the latent ones
-    __shared__ __align__(1024) uint8_t pb0[ROWS * 64], pb1[ROWS * 64];  // weights [row][32 keys]
+    __shared__ __align__(1024) uint8_t pb0[ROWS * 64], pb1[ROWS * 64];  // weights [row][32 keys], of tiles in turn
     __shared__ float rowred[2][ROWS];                                   // per 16-key tile
     __shared__ uint64_t seen[ROWS];
+    __shared__ uint32_t flaws[kKT / 4];  // a byte per key of a tile with nodes: its row is not finite
     __shared__ uint32_t bad_page, again;
     __shared__ uint64_t tmp[NW + 2];
+    __shared__ Req found;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uni(tid >> 6), n = lane & 15u, g = lane >> 4;
     const uint32_t sr = 8u * (wave & ~1u), sk = 16u * (wave & 1u);  // first row and key of this wave's scores
     const uint32_t pr = 32u * (wave >> 2), wv = wave & 3u;          // first row of its sums, and its columns
     const uint32_t c = (blockIdx.x % 8u) * (kGrid / 8u) + blockIdx.x / 8u;
     const uint32_t H = p.a.n_heads, L = p.a.cache.kv_lora_rank, RP = p.a.cache.qk_rope;
     if (tid == 0) bad_page = again = 0;
-    const Place f = find_place<ROWS, 64 * NW>(p, c, min_per, tmp);
+    const Place f = find_place<ROWS, 64 * NW>(p, c, min_per, tmp, &found);
     const uint64_t u1 = f.u0 + f.per < f.total ? f.u0 + f.per : f.total;
     if (tid < 2) p.desc[8 * (2 * c + tid)] = 0;
     if (f.u0 >= u1) return;
 
     uint64_t u = f.u0, base = f.base;
     uint32_t r = f.r, status = 0;
-    Req q = request<ROWS>(p, r, status);
+    Req q = f.q;
     while (u < u1) {
         while (u >= base + (uint64_t)q.nrt * q.nkt) {  // the next request that has units
             base += (uint64_t)q.nrt * q.nkt;
             q = request<ROWS>(p, ++r, status);
         }
         const uint64_t o = u - base;
-        const uint32_t nc = uni(chunks(q, f.per)), j = uni((uint32_t)((((o / q.nrt) + 1) * nc - 1) / q.nkt));
+        const uint32_t nc = uni(chunks(q, f.per)), j = uni((uint32_t)div64((div64(o, q.nrt) + 1) * nc - 1, q.nkt));
         const uint32_t ka = uni(chunk_at(q, nc, j)), kb = uni(chunk_at(q, nc, j + 1));
         const uint64_t oj = o - (uint64_t)q.nrt * ka;
-        const uint32_t rt = uni((uint32_t)(oj / (kb - ka))), kt0 = uni(ka + (uint32_t)(oj % (kb - ka)));
+        const uint32_t rt = uni((uint32_t)div64(oj, kb - ka)), kt0 = uni(ka + (uint32_t)(oj - (uint64_t)rt * (kb - ka)));
         const uint32_t kt1 = uni(u1 - u < kb - kt0 ? kt0 + (uint32_t)(u1 - u) : kb);
         const uint32_t slot = 2u * c + (u == f.u0 ? 0u : 1u);
         u += kt1 - kt0;
@@ -244,39 +256,46 @@ __global__ __launch_bounds__(64 * NW) void tree_bf16_kernel(Tree p, uint32_t min
         if (q.flaw) {
             clear();
         } else {
-            // the page of key kKT t + lane % kKT; behind the last key the last one's
+            // A wave's DR rows of a tile lie in one page (pages have at least 8 rows).
+            // Its page in tile t; behind the last key, the last key's
             auto page_of = [&](uint32_t t) {
-                const uint32_t key = t * kKT + (lane & (kKT - 1u));
+                const uint32_t key = t * kKT + DR * wave;
                 return table[(key < q.keys ? key : q.keys - 1u) >> p.psh];
             };
-            // the rows of tile t and whether they are there (read as zeros, if not), lane's key;
-            // tiles behind the walk's last are called for too, as zeros, so that a wave's
-            // memory operations can be counted
-            uint32_t ri = 0, nb = 0;
-            auto find_rows = [&](uint32_t t, int32_t page) {
-                const uint32_t key = t * kKT + (lane & (kKT - 1u));
-                const bool in = t < kt1 && key < q.keys, ok = in & (page >= 0) & ((uint32_t)page < p.a.cache.n_pages);
-                bad |= in && !ok;
-                ri = ok ? ((uint32_t)page << p.psh) + (key & (p.a.cache.page_size - 1u)) : 0u;
-                nb = ok ? 1u : 0u;
+            // The wave's rows of tile t: one resource, whose bounds make zeros of rows
+            // behind the last key. Tiles behind the walk's last are called for too, as
+            // zeros, so that a wave's memory operations can be counted.
+            const uint32_t stride = 2u * p.a.cache.row_stride;
+            rsrc_t rs;
+            auto find_rows = [&](uint32_t t, int32_t page_v) {
+                const int32_t page = (int32_t)uni((uint32_t)page_v);
+                const uint32_t key = t * kKT + DR * wave;
+                const uint32_t left = t < kt1 && key < q.keys ? (q.keys - key < DR ? q.keys - key : DR) : 0u;
+                const bool ok = page >= 0 && (uint32_t)page < p.a.cache.n_pages;
+                bad |= left && !ok;
+                const uint32_t row = ok ? ((uint32_t)page << p.psh) + (key & (p.a.cache.page_size - 1u)) : 0u;
+                rs = make_rsrc((const uint8_t*)p.a.cache.d_rows + (uint64_t)row * stride,
+                               ok && left ? (left - 1u) * stride + 2u * (L + RP) : 0u);
             };
-            auto issue_row = [&](uint8_t* lat, uint32_t i) {  // the wave's i-th row
-                const uint32_t kr = DR * wave + i, there = __builtin_amdgcn_readlane(nb, kr);
-                const uint8_t* row = (const uint8_t*)p.a.cache.d_rows +
-                                     __builtin_amdgcn_readlane(ri, kr) * (2ull * p.a.cache.row_stride);
-                const rsrc_t rl = make_rsrc(row, there ? 2u * L : 0u), rr = make_rsrc(row + 2u * L, there ? 2u * RP : 0u);
+            auto issue_row = [&](uint8_t* lat, uint32_t i, uint32_t lane) {  // the latent part of the wave's i-th row
+                const uint32_t ch = lane ^ swz((DR * wave + i) & 15u);
+                const uint32_t vo = 8u * ch < L ? i * stride + 16u * ch : kOOB;
                 if (LC == 4 || lane < 16 * LC)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, WL_LDS(lat + kr * PITCH), 16u,
-                                                             16u * (lane ^ swz(kr & 15u)), 0u, 0, 0);
-                if (lane < 8)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, WL_LDS(lat + ROT + kr * 128u), 16u, 16u * (lane ^ swz8(kr & 15u)),
-                                                             0u, 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, WL_LDS(lat + (DR * wave + i) * PITCH), 16u, vo, 0u, 0, 0);
+            };
+            auto issue_rot = [&](uint8_t* lat, uint32_t lane) {  // the rotary parts of the wave's rows
+                const uint32_t i = lane >> 3, ch = (lane & 7u) ^ swz8((DR * wave + i) & 15u);
+                const uint32_t vo = 8u * ch < RP ? i * stride + 2u * L + 16u * ch : kOOB;
+                if (DR == 8 || lane < 8 * DR)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, WL_LDS(lat + ROT + DR * wave * 128u), 16u, vo, 0u, 0, 0);
             };
             auto issue_tile = [&](uint8_t* lat, uint32_t t, int32_t page) {
                 find_rows(t, page);
 #pragma unroll
-                for (uint32_t i = 0; i < DR; i++) issue_row(lat, i);
+                for (uint32_t i = 0; i < DR; i++) issue_row(lat, i, lane);
+                issue_rot(lat, lane);
             };
+            int32_t page = page_of(kt0), page1 = page_of(kt0 + 1);  // later: of tiles t + 2 and t + 3
             // the queries of rows sr + n, in the operand's layout: lane (row n, k group g)
             bf16x8 qf[NS];
             {
@@ -300,67 +319,64 @@ __global__ __launch_bounds__(64 * NW) void tree_bf16_kernel(Tree p, uint32_t min
                 }
             }
             auto has_nodes = [&](uint32_t t) { return (t + 1) * kKT > q.len; };  // tree nodes, or the end, in tile t
+            // A row that some nodes may not see must not reach them through 0 x inf: in
+            // a tile with nodes, those whose latent part is not finite are noted (their
+            // scores will be NaN for those that see them) and the part is cleared. The
+            // rotary part only enters scores. Each wave looks at the rows it called for.
+            auto note_flaws = [&](uint8_t* lat, uint32_t t) {
+                constexpr uint32_t LR = 64 / DR;  // lanes per row
+                const uint32_t i = DR * wave + lane / LR;
+                uint32_t nf = 0;
+                if (t * kKT + i >= q.len) {
+#pragma unroll 1
+                    for (uint32_t k = lane % LR; k < 16 * LC; k += LR) {
+                        u32x4* x = (u32x4*)(lat + i * PITCH + 16u * k);
+                        if (has_nonfinite(*x)) {
+                            nf = 1;
+                            *x = u32x4{0u, 0u, 0u, 0u};
+                        }
+                    }
+                }
+                for (uint32_t d = 1; d < LR; d <<= 1) nf |= __shfl_xor(nf, d, 64);
+                if (lane % LR == 0) ((uint8_t*)flaws)[i] = (uint8_t)nf;
+            };
+            // the key operand of step s: chunk 4 s + g of a row lies at (64 s) ^ (16 (g ^ swz))
+            auto kread = [&](const uint8_t* lat, uint32_t s, uint32_t lane) {
+                const uint32_t n = lane & 15u, g = lane >> 4;
+                return s < NL ? *(const u32x4*)(lat + (sk + n) * PITCH + ((16u * (g ^ swz(n))) ^ (64u * (s & 3u))) + 256u * (s >> 2))
+                              : *(const u32x4*)(lat + ROT + (sk + n) * 128u + ((16u * (g ^ swz8(n))) ^ (64u * (s - NL))));
+            };
             // the scores of row sr + n with keys sk + 4 g + j of tile t, in powers of two
             auto scores = [&](const uint8_t* lat, uint32_t t, uint32_t lane) {
+                constexpr uint32_t KP = NS < 6 ? NS : 6;  // steps that the key operands are read ahead
                 const uint32_t n = lane & 15u, g = lane >> 4;
-                // chunk 4 s + g of a row lies at (64 s) ^ (16 (g ^ swz))
-                const uint32_t ko = (sk + n) * PITCH, kx = 16u * (g ^ swz(n));
-                const uint32_t ro = (sk + n) * 128u + 16u * (g ^ swz8(n));
-                auto kread = [&](uint32_t s) {
-                    return s < NL ? *(const u32x4*)(lat + ko + (kx ^ (64u * (s & 3u))) + 256u * (s >> 2))
-                                  : *(const u32x4*)(lat + ROT + (ro ^ (64u * (s - NL))));
-                };
+                u32x4 kf[KP];
+#pragma unroll
+                for (uint32_t k = 0; k < KP; k++) kf[k] = kread(lat, k, lane);
                 f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
-                constexpr uint32_t KG = 2;  // reads a group of steps ahead of their products
-                u32x4 kf[2][KG];
 #pragma unroll
-                for (uint32_t k = 0; k < KG; k++) kf[0][k] = kread(k);
-#pragma unroll
-                for (uint32_t s = 0; s < NS; s += KG) {
-                    const uint32_t b = (s / KG) & 1u;
-                    if (s + KG < NS) {
-#pragma unroll
-                        for (uint32_t k = 0; k < KG; k++) kf[b ^ 1u][k] = kread(s + KG + k);
-                    }
-                    s0 = mma(as_bf16x8(kf[b][0]), qf[s], s0);
-                    s1 = mma(as_bf16x8(kf[b][1]), qf[s + 1], s1);
+                for (uint32_t s = 0; s < NS; s += 2) {
+                    s0 = mma(as_bf16x8(kf[s % KP]), qf[s], s0);
+                    s1 = mma(as_bf16x8(kf[(s + 1) % KP]), qf[s + 1], s1);
+                    if (s + KP < NS) kf[s % KP] = kread(lat, s + KP, lane);
+                    if (s + 1 + KP < NS) kf[(s + 1) % KP] = kread(lat, s + 1 + KP, lane);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 f32x4 sc;
 #pragma unroll
-                for (int j = 0; j < 4; j++) sc[j] = (s0[j] + s1[j]) * p.scale2;
+                for (int k = 0; k < 4; k++) sc[k] = (s0[k] + s1[k]) * p.scale2;
                 if (has_nodes(t)) {
-                    // a row that some nodes may not see must not reach them through
-                    // 0 x inf: where its latent part is not finite, its scores are NaN
-                    // for those that see it, and the part is cleared before the sums
-                    // (clear_flawed). The rotary part only enters scores.
-                    uint32_t nf = 0;
-                    if (t * kKT + sk + n >= q.len) {
-#pragma unroll 1
-                        for (uint32_t s = 0; s < NL; s++) nf |= has_nonfinite(*(const u32x4*)(lat + ko + 16u * g + 64u * s)) ? 1u : 0u;
-                    }
-                    uint64_t fl = __ballot(nf != 0);  // lane 16 g + n: key n
-                    fl |= fl >> 32;
-                    const uint32_t flawed = (uint32_t)(fl | (fl >> 16));
+                    const uint32_t fl = flaws[sk / 4u + g];
                     const uint64_t bits = seen[sr + n];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t kj = 4u * g + j, key = t * kKT + sk + kj;
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t key = t * kKT + sk + 4u * g + k;
                         const uint32_t bit = (uint32_t)(bits >> ((key - q.len) & 63u)) & (key < q.keys ? 1u : 0u);
-                        const float nan = (flawed >> kj) & 1u ? __builtin_nanf("") : 0.f;
-                        sc[j] = (bit | (key < q.len ? 1u : 0u)) ? sc[j] + nan : -INFINITY;
+                        const float nan = (fl >> (8 * k)) & 1u ? __builtin_nanf("") : 0.f;
+                        sc[k] = (bit | (key < q.len ? 1u : 0u)) ? sc[k] + nan : -INFINITY;
                     }
                 }
                 return sc;
-            };
-            auto clear_flawed = [&](uint8_t* lat, uint32_t t) {
-                if (wave < 2 && t * kKT + sk + n >= q.len) {
-#pragma unroll 1
-                    for (uint32_t s = 0; s < NL; s++) {
-                        u32x4* x = (u32x4*)(lat + (sk + n) * PITCH + 16u * g + 64u * s);
-                        if (has_nonfinite(*x)) *x = u32x4{0u, 0u, 0u, 0u};
-                    }
-                }
             };
             // m = the largest of x over the row's lanes and its two waves
             auto share_maxima = [&](float x) {
@@ -370,86 +386,108 @@ __global__ __launch_bounds__(64 * NW) void tree_bf16_kernel(Tree p, uint32_t min
                 ring_barrier();
                 m = fmaxf(kNone, fmaxf(rowred[0][sr + n], rowred[1][sr + n]));
             };
-            int32_t page = 0, page2 = 0;  // of tiles t + 3 and t + 4
             bool pass = false;
             uint32_t first = kt0;  // the tile that sets the reference
-            auto step = [&](uint8_t* lat, uint8_t* pb, uint8_t* nlat, uint32_t t) {
-                uint32_t lane = tid & 63u;
-                asm volatile("" : "+v"(lane));  // addresses are worked out per tile, not held in registers
-                const uint32_t n = lane & 15u, g = lane >> 4;
+            auto vread = [&](const uint8_t* lat, uint32_t k, uint32_t lane) {  // columns 16 k of the wave's, keys 8 g + [0, 8)
+                const uint32_t g = lane >> 4, vq = (lane & 15u) >> 2, vb = (lane & 3u) >> 1;
+                const uint32_t vo = (8u * g + vq) * PITCH + 16u * ((4u * LC * wv + vb) ^ swz((8u * g + vq) & 15u)) + 8u * (lane & 1u);
+                const uint8_t* pa = lat + (vo ^ (32u * k));
+                typedef __attribute__((address_space(3))) s16x4 l_s16x4;
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa));
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa + 4 * PITCH));
+                const u32x2 xx = __builtin_bit_cast(u32x2, x), yy = __builtin_bit_cast(u32x2, y);
+                return u32x4{xx[0], xx[1], yy[0], yy[1]};
+            };
+            auto opaque_lane = [&]() {  // addresses are worked out per tile, not held in registers
+                uint32_t x = tid & 63u;
+                asm volatile("" : "+v"(x));
+                return x;
+            };
+            // the weights of tile t
+            auto weigh = [&](const uint8_t* lat, uint8_t* pb, uint32_t t) {
+                const uint32_t lane = opaque_lane(), n = lane & 15u, g = lane >> 4;
                 const f32x4 sc = scores(lat, t, lane);
                 const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
                 if (t == first) share_maxima(top);
                 float e[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) e[k] = exp2_(sc[k] - m);
-                l += (e[0] + e[1]) + (e[2] + e[3]);
-                pass |= top > m + kSlack;
                 *(u32x2*)(pb + (sr + n) * 64u + 16u * ((sk / 8u + (g >> 1)) ^ ((n & 8u) >> 2)) + 8u * (g & 1u)) =
                     u32x2{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
-                vm_wait<2 * DR + 1>();  // tile t + 1 is there; t + 2 and a page may be on the way
-                ring_barrier();
-                if (has_nodes(t)) {
-                    clear_flawed(lat, t);
-                    ring_barrier();
-                }
-                find_rows(t + 3, page);
-                page = page2;
-                page2 = page_of(t + 5);
-                const uint32_t vq = (lane & 15u) >> 2, vb = (lane & 3u) >> 1;
-                const uint32_t vo = (8u * g + vq) * PITCH + 16u * ((4u * LC * wv + vb) ^ swz((8u * g + vq) & 15u)) + 8u * (lane & 1u);
-                auto vfrag = [&](uint32_t k) {  // columns 16 k of the wave's, keys 8 g + [0, 8)
-                    const uint8_t* pa = lat + (vo ^ (32u * k));
-                    typedef __attribute__((address_space(3))) s16x4 l_s16x4;
-                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa));
-                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa + 4 * PITCH));
-                    const u32x2 xx = __builtin_bit_cast(u32x2, x), yy = __builtin_bit_cast(u32x2, y);
-                    return u32x4{xx[0], xx[1], yy[0], yy[1]};
-                };
-                constexpr uint32_t VG = 2;
-                u32x4 vf[2][VG];
+                l += (e[0] + e[1]) + (e[2] + e[3]);
+                pass |= top > m + kSlack;
+            };
+            // finds tile t's rows (its page came two tiles ago)
+            auto next_rows = [&](uint32_t t) {
+                find_rows(t, page);
+                page = page1;
+                page1 = page_of(t + 2);
+            };
+            // the sums of a tile, its rows in `lat` and its weights in `pb`; the rows
+            // found are called for, into `nlat`
+            auto add = [&](const uint8_t* lat, const uint8_t* pb, uint8_t* nlat) {
+                constexpr uint32_t VP = CT < 4 ? CT : 4;  // column tiles that the values are read ahead
+                const uint32_t lane = opaque_lane(), n = lane & 15u, g = lane >> 4;
+                u32x4 vf[VP];
                 bf16x8 pf[2];
 #pragma unroll
                 for (int i = 0; i < 2; i++)
                     pf[i] = as_bf16x8(*(const u32x4*)(pb + (pr + 16u * i + n) * 64u + 16u * (g ^ ((n & 8u) >> 2))));
 #pragma unroll
-                for (uint32_t k = 0; k < VG; k++) vf[0][k] = vfrag(k);
+                for (uint32_t k = 0; k < VP; k++) vf[k] = vread(lat, k, lane);
 #pragma unroll
-                for (uint32_t v = 0; v < CT; v += VG) {
-                    const uint32_t b = (v / VG) & 1u;
-                    if (v + VG < CT) {
+                for (uint32_t v = 0; v < CT; v++) {
 #pragma unroll
-                        for (uint32_t k = 0; k < VG; k++) vf[b ^ 1u][k] = vfrag(v + VG + k);
-                    }
+                    for (int i = 0; i < 2; i++) acc[i][v] = mma(as_bf16x8(vf[v % VP]), pf[i], acc[i][v]);
+                    if (v + VP < CT) vf[v % VP] = vread(lat, v + VP, lane);
+                    constexpr uint32_t PER = (DR + CT - 1) / CT;
 #pragma unroll
-                    for (uint32_t k = 0; k < VG; k++)
-#pragma unroll
-                        for (int i = 0; i < 2; i++) acc[i][v + k] = mma(as_bf16x8(vf[b][k]), pf[i], acc[i][v + k]);
-                    constexpr uint32_t PER = (DR * VG + CT - 1) / CT;
-#pragma unroll
-                    for (uint32_t i = v / VG * PER; i < v / VG * PER + PER && i < DR; i++) issue_row(nlat, i);
+                    for (uint32_t k = 0; k < DR; k++)
+                        if (k >= v * PER && k < v * PER + PER) issue_row(nlat, k, lane);
+                    if (v + 1 == CT) issue_rot(nlat, lane);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
+            // between two barriers: tile t - 1 is in b0 with weights w0, tile t in b1 with
+            // weights w1 to be made, tile t + 2's place is b3; at t = kt1 the last sums
+            auto turn = [&](uint8_t* b0, uint8_t* b1, uint8_t* b3, uint8_t* w0, uint8_t* w1, uint32_t t) {
+                if (t < kt1 && has_nodes(t)) {
+                    note_flaws(b1, t);
+                    ring_barrier();
+                }
+                next_rows(t + 2);
+                if (GR > 1 && wave >= 4 && t < kt1) weigh(b1, w1, t);
+                add(b0, w0, b3);
+                if (t >= kt1) return false;
+                if (GR == 1 || wave < 4) weigh(b1, w1, t);
+                vm_wait<DR + 2>();  // tile t + 1 is there; t + 2 and a page may be on the way
+                ring_barrier();
+                return true;
+            };
             for (;;) {
                 clear();
-                const int32_t pg0 = page_of(kt0), pg1 = page_of(kt0 + 1), pg2 = page_of(kt0 + 2);
-                issue_tile(ring0, kt0, pg0);
-                issue_tile(ring1, kt0 + 1, pg1);
-                page = page_of(kt0 + 3);
-                page2 = page_of(kt0 + 4);
-                issue_tile(ring2, kt0 + 2, pg2);
-                vm_wait<4 * DR + 2>();
+                issue_tile(ring0, kt0, first == kt0 ? page : page_of(kt0));
+                issue_tile(ring1, kt0 + 1, first == kt0 ? page1 : page_of(kt0 + 1));
+                page = page_of(kt0 + 2);
+                page1 = page_of(kt0 + 3);
+                vm_wait<DR + 3>();
                 ring_barrier();
-                for (uint32_t t = kt0;;) {
-                    step(ring0, pb0, ring3, t);
-                    if (++t >= kt1) break;
-                    step(ring1, pb1, ring0, t);
-                    if (++t >= kt1) break;
-                    step(ring2, pb0, ring1, t);
-                    if (++t >= kt1) break;
-                    step(ring3, pb1, ring2, t);
-                    if (++t >= kt1) break;
+                if (has_nodes(kt0)) {
+                    note_flaws(ring0, kt0);
+                    ring_barrier();
+                }
+                next_rows(kt0 + 2);
+#pragma unroll
+                for (uint32_t i = 0; i < DR; i++) issue_row(ring2, i, lane);
+                issue_rot(ring2, lane);
+                weigh(ring0, pb0, kt0);
+                vm_wait<DR + 2>();
+                ring_barrier();
+                for (uint32_t t = kt0 + 1;; t += 4) {
+                    if (!turn(ring0, ring1, ring3, pb0, pb1, t)) break;
+                    if (!turn(ring1, ring2, ring0, pb1, pb0, t + 1)) break;
+                    if (!turn(ring2, ring3, ring1, pb0, pb1, t + 2)) break;
+                    if (!turn(ring3, ring0, ring2, pb1, pb0, t + 3)) break;
                 }
                 vm_wait<0>();
                 if (first != kt0) break;
@@ -463,6 +501,8 @@ __global__ __launch_bounds__(64 * NW) void tree_bf16_kernel(Tree p, uint32_t min
                 for (uint32_t t = kt0; t < kt1; t++) {
                     issue_tile(ring0, t, page_of(t));
                     vm_wait<0>();
+                    ring_barrier();
+                    note_flaws(ring0, t);
                     ring_barrier();
                     const f32x4 sc = scores(ring0, t, lane);
                     x = fmaxf(x, fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
@@ -484,7 +524,7 @@ __global__ __launch_bounds__(64 * NW) void tree_bf16_kernel(Tree p, uint32_t min
         if (g == 0) rowred[wave & 1u][sr + n] = l;
         const bool whole = kt1 - kt0 == q.nkt;
         if (!whole && sk == 0 && g == 0) p.part_ml[2u * (slot * ROWS + sr + n)] = m;
-        __syncthreads();
+        ring_barrier();
         const bool nan = bad_page != 0 || q.flaw;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -518,9 +558,9 @@ __global__ __launch_bounds__(64 * NW) void tree_bf16_kernel(Tree p, uint32_t min
             *(uint64_t*)(desc + 2) = base;
             *(uint64_t*)(desc + 4) = f.per;
         }
-        __syncthreads();
+        ring_barrier();
         if (tid == 0) bad_page = 0u;
-        __syncthreads();
+        ring_barrier();
     }
 }
 
@@ -551,8 +591,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
         if (tid < nc) {
             const uint32_t ka = chunk_at(q, nc, tid), kb = chunk_at(q, nc, tid + 1);
             start = base + (uint64_t)q.nrt * ka + (uint64_t)rt * (kb - ka);
-            w0 = (uint32_t)(start / per);
-            nw = (uint32_t)((start + (kb - ka) - 1) / per) - w0 + 1u;
+            w0 = (uint32_t)div64(start, per);
+            nw = (uint32_t)div64(start + (kb - ka) - 1, per) - w0 + 1u;
         }
         uint32_t inc = nw;
         for (uint32_t o = 1; o < 64; o <<= 1) {
@@ -722,12 +762,12 @@ size_t tree_scratch(const wl_tree_attn& a) {
     return rows * (128 * lat_class(a) + 2) * 4 + 2 * kGrid * 32;
 }
 
-template <int NW, int LC>
+template <int GR, int LC>
 int run_bf16(const Tree& p, hipStream_t st) {
-    hipLaunchKernelGGL((tree_bf16_kernel<NW, LC>), dim3(kGrid), dim3(64 * NW), 0, st, p, 1u);
+    hipLaunchKernelGGL((tree_bf16_kernel<GR, LC>), dim3(kGrid), dim3(256 * GR), 0, st, p, 1u);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL((tree_join_kernel<8 * NW, LC, true>), dim3(2 * kGrid, kJoinZ), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((tree_join_kernel<32 * GR, LC, true>), dim3(2 * kGrid, kJoinZ), dim3(256), 0, st, p);
     return (int)hipGetLastError();
 }
 
@@ -742,8 +782,8 @@ int launch_tree(const wl_tree_attn& a, void* stream) {
     p.part_ml = p.part + (size_t)2 * kGrid * 64 * 128 * lc;
     p.desc = (uint32_t*)(p.part_ml + (size_t)2 * kGrid * 64 * 2);
     if (a.dtype == WL_TYPE_BF16) {
-        if (rows == 64) return lc == 4 ? run_bf16<8, 4>(p, st) : lc == 2 ? run_bf16<8, 2>(p, st) : run_bf16<8, 1>(p, st);
-        return lc == 4 ? run_bf16<4, 4>(p, st) : lc == 2 ? run_bf16<4, 2>(p, st) : run_bf16<4, 1>(p, st);
+        if (rows == 64) return lc == 4 ? run_bf16<2, 4>(p, st) : lc == 2 ? run_bf16<2, 2>(p, st) : run_bf16<2, 1>(p, st);
+        return lc == 4 ? run_bf16<1, 4>(p, st) : lc == 2 ? run_bf16<1, 2>(p, st) : run_bf16<1, 1>(p, st);
     }
     const dim3 g(a.n_req, (a.n_heads + 3) / 4, 8);
     if (a.cache.dtype == WL_TYPE_BF16) hipLaunchKernelGGL((tree_attn_kernel<false, true>), g, dim3(256), 0, st, a);
