@@ -149,16 +149,17 @@ WL_DEV bool has_nonfinite(u32x4 v) {
         f |= (v[i] & 0x7F80u) == 0x7F80u || (v[i] & 0x7F800000u) == 0x7F800000u;
     return f;
 }
-// Where a row's 16-byte chunks lie in LDS: chunk c at c ^ swz(row) (rows of 256
-// bytes or more) or c ^ swz8(row) (rows of 128). LDS serves a 16-byte read 16
-// lanes at a time, lanes 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31 of either
-// half wave: for an MFMA operand (lane = row + 16 x chunk) those are 8 rows at
-// an even chunk and the other 8 at the odd one beside it, which these put into
-// 16 different places of the 256 bytes that the banks cover. A transposing
-// read's 32 lanes (8 rows x 2 chunks) fall into 16 different ones too.
-// Measured: 237 bytes a clock and CU, 127 with a swizzle over 16 rows in order.
-WL_DEV constexpr uint32_t swz(uint32_t row) { return ((row & 3u) << 1) | (row & 8u); }
+// LDS serves a 16-byte read 16 lanes at a time, lanes 0-3, 12-15, 20-27 and 4-11,
+// 16-19, 28-31 of either half wave: for an MFMA operand (lane = row + 16 x chunk)
+// those are 8 rows at an even chunk and the other 8 at the odd one beside it. Key
+// rows lie 32 bytes more than a multiple of 256 apart, which puts these 16 into 16
+// different places of the 256 bytes that the banks cover, as it does the 8 rows x 2
+// chunks that half a wave reads transposed. Rows of 128 and 64 bytes (rotary parts,
+// weights) have their chunk c at c ^ swz8(row) and c ^ swz4(row) instead.
+// Measured: 236 bytes a clock and CU (32 without).
+constexpr uint32_t kPad = 32;
 WL_DEV constexpr uint32_t swz8(uint32_t row) { return (row & 2u) | ((row & 8u) >> 1); }
+WL_DEV constexpr uint32_t swz4(uint32_t row) { return (row & 8u) >> 2; }
 
 // ---- 16-bit queries and cache --------------------------------------------------
 // ROWS = 32 GR rows (node, head) against 32 keys at a time, GR groups of four
@@ -169,18 +170,17 @@ WL_DEV constexpr uint32_t swz8(uint32_t row) { return (row & 2u) | ((row & 8u) >
 //   P = 2^(S - m) in bf16, through LDS, to the group's waves;
 //   O^T[cols][rows] += V^T P^T: wave w has columns [32 LC w, + 32 LC); the key
 //           rows are read again, transposed (ds_read_b64_tr_b16).
-// One barrier a tile: between two of them a wave makes the weights of tile t and
-// sums tile t - 1, group 0 the sums first, group 1 the weights first. A SIMD has
-// one wave of either group, so one's products fill the other's waits.
+// One barrier a tile: between two of them a wave makes the scores of tile t, then
+// sums tile t - 1 with the exponentials of tile t between the products.
 // m is a reference, not the maximum: that of the walk's first tile. Weights may
 // exceed 1 and lose nothing by it (bf16 and f32 keep their relative precision);
-// only where a score passes it by kSlack powers of two the walk is done again,
+// only where a weight passes kMost the walk is done again,
 // after one over the scores alone for the true maxima. So nothing is rescaled.
 // Key rows come into a ring of four tiles in LDS by DMA (16 bytes a lane): rows
 // behind the last key and columns behind the row's are read as zeros by the
 // resource's bounds. While tiles t - 1 and t are worked on, tile t + 2 is called
 // for between products; before the barrier each wave waits for its rows of t + 1.
-constexpr float kSlack = 64.f;  // a weight at most 2^64, 2^31 of them 2^95
+constexpr float kMost = 0x1p64f;  // 2^31 such weights sum to 2^95
 
 // s_waitcnt vmcnt(N): all but the last N memory operations of this wave are done.
 template <uint32_t N>
@@ -201,7 +201,7 @@ WL_DEV void ring_barrier() {
 
 template <int GR, int LC>
 __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t min_per) {
-    constexpr uint32_t NW = 4 * GR, ROWS = 32 * GR, PITCH = 256 * LC, NL = 4 * LC, NS = NL + 2, CT = 2 * LC, DR = 32 / NW;
+    constexpr uint32_t NW = 4 * GR, ROWS = 32 * GR, PITCH = 256 * LC + kPad, NL = 4 * LC, NS = NL + 2, CT = 2 * LC, DR = 32 / NW;
     // the ring: separate objects, so that the compiler's own waits for DMA-written LDS stay per tile
     __shared__ __align__(1024) uint8_t ring0[kKT * (PITCH + 128)], ring1[kKT * (PITCH + 128)], ring2[kKT * (PITCH + 128)],
         ring3[kKT * (PITCH + 128)];
@@ -277,23 +277,24 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                 rs = make_rsrc((const uint8_t*)p.a.cache.d_rows + (uint64_t)row * stride,
                                ok && left ? (left - 1u) * stride + 2u * (L + RP) : 0u);
             };
-            auto issue_row = [&](uint8_t* lat, uint32_t i, uint32_t lane) {  // the latent part of the wave's i-th row
-                const uint32_t ch = lane ^ swz((DR * wave + i) & 15u);
-                const uint32_t vo = 8u * ch < L ? i * stride + 16u * ch : kOOB;
+            // lane's chunk of a latent part, and of the wave's rows' rotary parts
+            const uint32_t lat_at = 8u * lane < L ? 16u * lane : kOOB;
+            const uint32_t rot_i = lane >> 3, rot_ch = (lane & 7u) ^ swz8((DR * wave + rot_i) & 15u);
+            const uint32_t rot_at = 8u * rot_ch < RP ? rot_i * stride + 2u * L + 16u * rot_ch : kOOB;
+            auto issue_row = [&](uint8_t* lat, uint32_t i) {
                 if (LC == 4 || lane < 16 * LC)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, WL_LDS(lat + (DR * wave + i) * PITCH), 16u, vo, 0u, 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, WL_LDS(lat + (DR * wave + i) * PITCH), 16u, lat_at + i * stride,
+                                                             0u, 0, 0);
             };
-            auto issue_rot = [&](uint8_t* lat, uint32_t lane) {  // the rotary parts of the wave's rows
-                const uint32_t i = lane >> 3, ch = (lane & 7u) ^ swz8((DR * wave + i) & 15u);
-                const uint32_t vo = 8u * ch < RP ? i * stride + 2u * L + 16u * ch : kOOB;
+            auto issue_rot = [&](uint8_t* lat) {
                 if (DR == 8 || lane < 8 * DR)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, WL_LDS(lat + ROT + DR * wave * 128u), 16u, vo, 0u, 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, WL_LDS(lat + ROT + DR * wave * 128u), 16u, rot_at, 0u, 0, 0);
             };
             auto issue_tile = [&](uint8_t* lat, uint32_t t, int32_t page) {
                 find_rows(t, page);
 #pragma unroll
-                for (uint32_t i = 0; i < DR; i++) issue_row(lat, i, lane);
-                issue_rot(lat, lane);
+                for (uint32_t i = 0; i < DR; i++) issue_row(lat, i);
+                issue_rot(lat);
             };
             int32_t page = page_of(kt0), page1 = page_of(kt0 + 1);  // later: of tiles t + 2 and t + 3
             // the queries of rows sr + n, in the operand's layout: lane (row n, k group g)
@@ -340,44 +341,46 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                 for (uint32_t d = 1; d < LR; d <<= 1) nf |= __shfl_xor(nf, d, 64);
                 if (lane % LR == 0) ((uint8_t*)flaws)[i] = (uint8_t)nf;
             };
-            // the key operand of step s: chunk 4 s + g of a row lies at (64 s) ^ (16 (g ^ swz))
-            auto kread = [&](const uint8_t* lat, uint32_t s, uint32_t lane) {
-                const uint32_t n = lane & 15u, g = lane >> 4;
-                return s < NL ? *(const u32x4*)(lat + (sk + n) * PITCH + ((16u * (g ^ swz(n))) ^ (64u * (s & 3u))) + 256u * (s >> 2))
-                              : *(const u32x4*)(lat + ROT + (sk + n) * 128u + ((16u * (g ^ swz8(n))) ^ (64u * (s - NL))));
+            // the key operand of step s: chunk 4 s + g of key row sk + n
+            const uint32_t key_at = (sk + n) * PITCH + 16u * g, key_rot = (sk + n) * 128u + 16u * (g ^ swz8(n));
+            auto kread = [&](const uint8_t* lat, uint32_t s) {
+                return s < NL ? *(const u32x4*)(lat + key_at + 64u * s)
+                              : *(const u32x4*)(lat + ROT + (key_rot ^ (64u * (s - NL))));
             };
-            // the scores of row sr + n with keys sk + 4 g + j of tile t, in powers of two
-            auto scores = [&](const uint8_t* lat, uint32_t t, uint32_t lane) {
-                constexpr uint32_t KP = NS < 6 ? NS : 6;  // steps that the key operands are read ahead
-                const uint32_t n = lane & 15u, g = lane >> 4;
+            // the products of rows sr + n with keys sk + 4 g + j, in two sums
+            auto products = [&](const uint8_t* lat, f32x4& s0, f32x4& s1) {
+                constexpr uint32_t KP = 4;  // steps that the key operands are read ahead
                 u32x4 kf[KP];
 #pragma unroll
-                for (uint32_t k = 0; k < KP; k++) kf[k] = kread(lat, k, lane);
-                f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+                for (uint32_t k = 0; k < KP; k++) kf[k] = kread(lat, k);
+                s0 = s1 = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (uint32_t s = 0; s < NS; s += 2) {
                     s0 = mma(as_bf16x8(kf[s % KP]), qf[s], s0);
                     s1 = mma(as_bf16x8(kf[(s + 1) % KP]), qf[s + 1], s1);
-                    if (s + KP < NS) kf[s % KP] = kread(lat, s + KP, lane);
-                    if (s + 1 + KP < NS) kf[(s + 1) % KP] = kread(lat, s + 1 + KP, lane);
+                    if (s + KP < NS) kf[s % KP] = kread(lat, s + KP);
+                    if (s + 1 + KP < NS) kf[(s + 1) % KP] = kread(lat, s + 1 + KP);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                f32x4 sc;
-#pragma unroll
-                for (int k = 0; k < 4; k++) sc[k] = (s0[k] + s1[k]) * p.scale2;
-                if (has_nodes(t)) {
-                    const uint32_t fl = flaws[sk / 4u + g];
-                    const uint64_t bits = seen[sr + n];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t key = t * kKT + sk + 4u * g + k;
-                        const uint32_t bit = (uint32_t)(bits >> ((key - q.len) & 63u)) & (key < q.keys ? 1u : 0u);
-                        const float nan = (fl >> (8 * k)) & 1u ? __builtin_nanf("") : 0.f;
-                        sc[k] = (bit | (key < q.len ? 1u : 0u)) ? sc[k] + nan : -INFINITY;
-                    }
-                }
-                return sc;
             };
+            // the scores in powers of two are s0 + s1 times the factor returned; those of
+            // keys that the row does not see become -inf
+            auto scores = [&](f32x4& s0, f32x4 s1, uint32_t t) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) s0[k] += s1[k];
+                if (!has_nodes(t)) return p.scale2;
+                const uint32_t fl = flaws[sk / 4u + g];
+                const uint64_t bits = seen[sr + n];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t key = t * kKT + sk + 4u * g + k;
+                    const uint32_t bit = (uint32_t)(bits >> ((key - q.len) & 63u)) & (key < q.keys ? 1u : 0u);
+                    const float nan = (fl >> (8 * k)) & 1u ? __builtin_nanf("") : 0.f;
+                    s0[k] = (bit | (key < q.len ? 1u : 0u)) ? s0[k] * p.scale2 + nan : -INFINITY;
+                }
+                return 1.0f;
+            };
+            auto largest = [&](f32x4 x, float f) { return fmaxf(fmaxf(x[0] * f, x[1] * f), fmaxf(x[2] * f, x[3] * f)); };
             // m = the largest of x over the row's lanes and its two waves
             auto share_maxima = [&](float x) {
                 x = fmaxf(x, __shfl_xor(x, 16, 64));
@@ -388,34 +391,16 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
             };
             bool pass = false;
             uint32_t first = kt0;  // the tile that sets the reference
-            auto vread = [&](const uint8_t* lat, uint32_t k, uint32_t lane) {  // columns 16 k of the wave's, keys 8 g + [0, 8)
-                const uint32_t g = lane >> 4, vq = (lane & 15u) >> 2, vb = (lane & 3u) >> 1;
-                const uint32_t vo = (8u * g + vq) * PITCH + 16u * ((4u * LC * wv + vb) ^ swz((8u * g + vq) & 15u)) + 8u * (lane & 1u);
-                const uint8_t* pa = lat + (vo ^ (32u * k));
+            // the value operand of columns 16 k of the wave's: lane group g has keys 4 g +
+            // [0, 4) and 16 + 4 g + [0, 4)
+            const uint32_t value_at = (4u * g + ((lane & 15u) >> 2)) * PITCH + 64u * LC * wv + 8u * (lane & 3u);
+            auto vread = [&](const uint8_t* lat, uint32_t k) {
+                const uint8_t* pa = lat + value_at + 32u * k;
                 typedef __attribute__((address_space(3))) s16x4 l_s16x4;
                 const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa));
-                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa + 4 * PITCH));
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa + 16 * PITCH));
                 const u32x2 xx = __builtin_bit_cast(u32x2, x), yy = __builtin_bit_cast(u32x2, y);
                 return u32x4{xx[0], xx[1], yy[0], yy[1]};
-            };
-            auto opaque_lane = [&]() {  // addresses are worked out per tile, not held in registers
-                uint32_t x = tid & 63u;
-                asm volatile("" : "+v"(x));
-                return x;
-            };
-            // the weights of tile t
-            auto weigh = [&](const uint8_t* lat, uint8_t* pb, uint32_t t) {
-                const uint32_t lane = opaque_lane(), n = lane & 15u, g = lane >> 4;
-                const f32x4 sc = scores(lat, t, lane);
-                const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-                if (t == first) share_maxima(top);
-                float e[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) e[k] = exp2_(sc[k] - m);
-                *(u32x2*)(pb + (sr + n) * 64u + 16u * ((sk / 8u + (g >> 1)) ^ ((n & 8u) >> 2)) + 8u * (g & 1u)) =
-                    u32x2{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
-                l += (e[0] + e[1]) + (e[2] + e[3]);
-                pass |= top > m + kSlack;
             };
             // finds tile t's rows (its page came two tiles ago)
             auto next_rows = [&](uint32_t t) {
@@ -423,43 +408,56 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                 page = page1;
                 page1 = page_of(t + 2);
             };
-            // the sums of a tile, its rows in `lat` and its weights in `pb`; the rows
-            // found are called for, into `nlat`
-            auto add = [&](const uint8_t* lat, const uint8_t* pb, uint8_t* nlat) {
-                constexpr uint32_t VP = CT < 4 ? CT : 4;  // column tiles that the values are read ahead
-                const uint32_t lane = opaque_lane(), n = lane & 15u, g = lane >> 4;
-                u32x4 vf[VP];
-                bf16x8 pf[2];
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-                    pf[i] = as_bf16x8(*(const u32x4*)(pb + (pr + 16u * i + n) * 64u + 16u * (g ^ ((n & 8u) >> 2))));
-#pragma unroll
-                for (uint32_t k = 0; k < VP; k++) vf[k] = vread(lat, k, lane);
-#pragma unroll
-                for (uint32_t v = 0; v < CT; v++) {
-#pragma unroll
-                    for (int i = 0; i < 2; i++) acc[i][v] = mma(as_bf16x8(vf[v % VP]), pf[i], acc[i][v]);
-                    if (v + VP < CT) vf[v % VP] = vread(lat, v + VP, lane);
-                    constexpr uint32_t PER = (DR + CT - 1) / CT;
-#pragma unroll
-                    for (uint32_t k = 0; k < DR; k++)
-                        if (k >= v * PER && k < v * PER + PER) issue_row(nlat, k, lane);
-                    if (v + 1 == CT) issue_rot(nlat, lane);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+            // the weights, in the order of the values' keys: chunk g of a row
+            const uint32_t put_at = (sr + n) * 64u + 16u * (g ^ swz4(n)) + sk / 2u;
+            const uint32_t get_at = (pr + n) * 64u + 16u * (g ^ swz4(n));
+            auto put_weights = [&](const float* e, uint8_t* pb) {
+                *(u32x2*)(pb + put_at) = u32x2{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
             };
             // between two barriers: tile t - 1 is in b0 with weights w0, tile t in b1 with
             // weights w1 to be made, tile t + 2's place is b3; at t = kt1 the last sums
             auto turn = [&](uint8_t* b0, uint8_t* b1, uint8_t* b3, uint8_t* w0, uint8_t* w1, uint32_t t) {
-                if (t < kt1 && has_nodes(t)) {
-                    note_flaws(b1, t);
-                    ring_barrier();
-                }
+                constexpr uint32_t VP = 2;  // column tiles that the values are read ahead
+                u32x4 vf[VP];
+                bf16x8 pf[2];
+                const bool live = t < kt1;
                 next_rows(t + 2);
-                if (GR > 1 && wave >= 4 && t < kt1) weigh(b1, w1, t);
-                add(b0, w0, b3);
-                if (t >= kt1) return false;
-                if (GR == 1 || wave < 4) weigh(b1, w1, t);
+                f32x4 s0, s1;
+                float e[4], f;
+                if (live) {
+                    if (has_nodes(t)) {
+                        note_flaws(b1, t);
+                        ring_barrier();
+                    }
+                    products(b1, s0, s1);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) pf[i] = as_bf16x8(*(const u32x4*)(w0 + get_at + 1024u * i));
+#pragma unroll
+                for (uint32_t k = 0; k < VP; k++) vf[k] = vread(b0, k);
+#pragma unroll
+                for (uint32_t v = 0; v < CT; v++) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) acc[i][v] = mma(as_bf16x8(vf[v % VP]), pf[i], acc[i][v]);
+                    if (v + VP < CT) vf[v % VP] = vread(b0, v + VP);
+                    if (live) {
+                        if (v == 0) f = scores(s0, s1, t);
+                        if (v == 1) {
+#pragma unroll
+                            for (int k = 0; k < 4; k++) e[k] = exp2_(fmaf(s0[k], f, -m));
+                        }
+                        if (v == (CT == 2 ? 1 : 2)) put_weights(e, w1);
+                    }
+                    constexpr uint32_t PER = (DR + CT - 1) / CT;
+#pragma unroll
+                    for (uint32_t k = 0; k < DR; k++)
+                        if (k >= v * PER && k < v * PER + PER) issue_row(b3, k);
+                    if (v + 1 == CT) issue_rot(b3);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (!live) return false;
+                l += (e[0] + e[1]) + (e[2] + e[3]);
+                pass |= fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) > kMost;
                 vm_wait<DR + 2>();  // tile t + 1 is there; t + 2 and a page may be on the way
                 ring_barrier();
                 return true;
@@ -478,9 +476,19 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                 }
                 next_rows(kt0 + 2);
 #pragma unroll
-                for (uint32_t i = 0; i < DR; i++) issue_row(ring2, i, lane);
-                issue_rot(ring2, lane);
-                weigh(ring0, pb0, kt0);
+                for (uint32_t i = 0; i < DR; i++) issue_row(ring2, i);
+                issue_rot(ring2);
+                {
+                    f32x4 s0, s1;
+                    products(ring0, s0, s1);
+                    const float f = scores(s0, s1, kt0);
+                    if (first == kt0) share_maxima(largest(s0, f));
+                    float e[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) e[k] = exp2_(fmaf(s0[k], f, -m));
+                    put_weights(e, pb0);
+                    l += (e[0] + e[1]) + (e[2] + e[3]);
+                }
                 vm_wait<DR + 2>();
                 ring_barrier();
                 for (uint32_t t = kt0 + 1;; t += 4) {
@@ -504,8 +512,10 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                     ring_barrier();
                     note_flaws(ring0, t);
                     ring_barrier();
-                    const f32x4 sc = scores(ring0, t, lane);
-                    x = fmaxf(x, fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])));
+                    f32x4 s0, s1;
+                    products(ring0, s0, s1);
+                    const float f = scores(s0, s1, t);
+                    x = fmaxf(x, largest(s0, f));
                     ring_barrier();
                 }
                 share_maxima(x);
