@@ -12,6 +12,9 @@ namespace paged {
 namespace {
 
 constexpr uint32_t kKT = 32;    // keys of a tile
+// Key tiles of a walk at least: a shorter one's parts cost more to join than it saves.
+// One token over 4096 keys, both launches: 32.6 us at 1, 28.6 at 2, 29.3 at 4, 32.5 at 8.
+constexpr uint32_t kMinPer = 2;
 constexpr uint32_t kGrid = 256; // work-groups of a launch: one per CU (LDS and registers allow one)
 constexpr float kNone = -3.0e38f;  // the running maximum of a row that has seen no key
 
@@ -224,24 +227,51 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
     if (tid < 2) p.desc[8 * (2 * c + tid)] = 0;
     if (f.u0 >= u1) return;
 
-    uint64_t u = f.u0, base = f.base;
-    uint32_t r = f.r, status = 0;
-    Req q = f.q;
-    while (u < u1) {
-        while (u >= base + (uint64_t)q.nrt * q.nkt) {  // the next request that has units
-            base += (uint64_t)q.nrt * q.nkt;
-            q = request<ROWS>(p, ++r, status);
+    // the walks of this work-group: a row tile's keys, or a part of them
+    struct Walk {
+        Req q;
+        uint64_t base;
+        uint32_t r, rt, kt0, kt1, slot;
+    };
+    uint64_t u = f.u0;
+    uint32_t status = 0;
+    Walk next{f.q, f.base, f.r, 0, 0, 0, 0};
+    auto find_walk = [&]() {  // the walk that begins at unit u < u1, from the last one's request on
+        Walk& w = next;
+        while (u >= w.base + (uint64_t)w.q.nrt * w.q.nkt) {  // the next request that has units
+            w.base += (uint64_t)w.q.nrt * w.q.nkt;
+            w.q = request<ROWS>(p, ++w.r, status);
         }
-        const uint64_t o = u - base;
-        const uint32_t nc = uni(chunks(q, f.per)), j = uni((uint32_t)div64((div64(o, q.nrt) + 1) * nc - 1, q.nkt));
-        const uint32_t ka = uni(chunk_at(q, nc, j)), kb = uni(chunk_at(q, nc, j + 1));
-        const uint64_t oj = o - (uint64_t)q.nrt * ka;
-        const uint32_t rt = uni((uint32_t)div64(oj, kb - ka)), kt0 = uni(ka + (uint32_t)(oj - (uint64_t)rt * (kb - ka)));
-        const uint32_t kt1 = uni(u1 - u < kb - kt0 ? kt0 + (uint32_t)(u1 - u) : kb);
-        const uint32_t slot = 2u * c + (u == f.u0 ? 0u : 1u);
-        u += kt1 - kt0;
-        const uint32_t rows = uni(q.nodes * H - rt * ROWS < ROWS ? q.nodes * H - rt * ROWS : ROWS);
-        const int32_t* table = p.a.d_table + (size_t)r * p.a.max_pages;
+        const uint64_t o = u - w.base;
+        const uint32_t nc = uni(chunks(w.q, f.per)), j = uni((uint32_t)div64((div64(o, w.q.nrt) + 1) * nc - 1, w.q.nkt));
+        const uint32_t ka = uni(chunk_at(w.q, nc, j)), kb = uni(chunk_at(w.q, nc, j + 1));
+        const uint64_t oj = o - (uint64_t)w.q.nrt * ka;
+        w.rt = uni((uint32_t)div64(oj, kb - ka));
+        w.kt0 = uni(ka + (uint32_t)(oj - (uint64_t)w.rt * (kb - ka)));
+        w.kt1 = uni(u1 - u < kb - w.kt0 ? w.kt0 + (uint32_t)(u1 - u) : kb);
+        w.slot = 2u * c + (u == f.u0 ? 0u : 1u);
+        u += w.kt1 - w.kt0;
+    };
+    // A wave's DR rows of a tile lie in one page (pages have at least 8 rows): its
+    // page in tile t of a walk; behind the last key, the last key's
+    auto page_at = [&](const Walk& w, uint32_t t) {
+        const uint32_t key = t * kKT + DR * wave;
+        return p.a.d_table[(size_t)w.r * p.a.max_pages + ((key < w.q.keys ? key : w.q.keys - 1u) >> p.psh)];
+    };
+    // the pages of the next walk's first four tiles are read while the last one ends
+    int32_t ahead[4] = {0, 0, 0, 0};
+    auto read_ahead = [&]() {
+        if (next.q.flaw) return;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) ahead[i] = page_at(next, next.kt0 + i);
+    };
+    find_walk();
+    read_ahead();
+    for (;;) {
+        const Walk w = next;
+        const Req& q = w.q;
+        const uint32_t rt = w.rt, kt0 = w.kt0, kt1 = w.kt1, slot = w.slot;
+        const uint32_t rows = q.nodes * H - rt * ROWS < ROWS ? q.nodes * H - rt * ROWS : ROWS;
 
         f32x4 acc[2][CT];
         float m = kNone, l = 0.f;  // of row sr + n: the reference, this lane's part of the weights' sum
@@ -253,15 +283,11 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                 for (uint32_t k = 0; k < CT; k++) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
         };
         bool bad = false;
+        const bool more = u < u1;
         if (q.flaw) {
             clear();
         } else {
-            // A wave's DR rows of a tile lie in one page (pages have at least 8 rows).
-            // Its page in tile t; behind the last key, the last key's
-            auto page_of = [&](uint32_t t) {
-                const uint32_t key = t * kKT + DR * wave;
-                return table[(key < q.keys ? key : q.keys - 1u) >> p.psh];
-            };
+            auto page_of = [&](uint32_t t) { return page_at(w, t); };
             // The wave's rows of tile t: one resource, whose bounds make zeros of rows
             // behind the last key. Tiles behind the walk's last are called for too, as
             // zeros, so that a wave's memory operations can be counted.
@@ -296,10 +322,10 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                 for (uint32_t i = 0; i < DR; i++) issue_row(lat, i);
                 issue_rot(lat);
             };
-            int32_t page = page_of(kt0), page1 = page_of(kt0 + 1);  // later: of tiles t + 2 and t + 3
+            int32_t page = 0, page1 = 0;  // of tiles t + 2 and t + 3
             // the queries of rows sr + n, in the operand's layout: lane (row n, k group g)
             bf16x8 qf[NS];
-            {
+            auto read_queries = [&]() {
                 const rsrc_t ql = make_rsrc((const uint16_t*)p.a.d_q_lat + q.t0 * p.a.q_lat_stride,
                                             2u * ((q.nodes - 1u) * (uint32_t)p.a.q_lat_stride + H * L));
                 const rsrc_t qr = make_rsrc((const uint16_t*)p.a.d_q_rope + q.t0 * p.a.q_rope_stride,
@@ -318,7 +344,7 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                     const uint32_t nd = live ? node : 0u;
                     seen[lr] = p.a.d_mask ? p.a.d_mask[q.t0 + nd] : (2ull << nd) - 1ull;
                 }
-            }
+            };
             auto has_nodes = [&](uint32_t t) { return (t + 1) * kKT > q.len; };  // tree nodes, or the end, in tile t
             // A row that some nodes may not see must not reach them through 0 x inf: in
             // a tile with nodes, those whose latent part is not finite are noted (their
@@ -464,11 +490,12 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
             };
             for (;;) {
                 clear();
-                issue_tile(ring0, kt0, first == kt0 ? page : page_of(kt0));
-                issue_tile(ring1, kt0 + 1, first == kt0 ? page1 : page_of(kt0 + 1));
-                page = page_of(kt0 + 2);
-                page1 = page_of(kt0 + 3);
-                vm_wait<DR + 3>();
+                issue_tile(ring0, kt0, ahead[0]);
+                issue_tile(ring1, kt0 + 1, ahead[1]);
+                page = ahead[2];
+                page1 = ahead[3];
+                if (first == kt0) read_queries();
+                vm_wait<0>();
                 ring_barrier();
                 if (has_nodes(kt0)) {
                     note_flaws(ring0, kt0);
@@ -523,6 +550,10 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                 first = ~0u;
             }
         }
+        if (more) {
+            find_walk();
+            read_ahead();
+        }
         // the weights' sums over the row's lanes and waves; flaws
         if (__ballot(bad) && lane == 0) {
             bad_page = 1u;
@@ -563,11 +594,12 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
         }
         if (!whole && tid == (slot & 1u)) {  // the thread that cleared it
             uint32_t* desc = p.desc + 8 * slot;
-            desc[0] = r + 1u;
+            desc[0] = w.r + 1u;
             desc[1] = rt;
-            *(uint64_t*)(desc + 2) = base;
+            *(uint64_t*)(desc + 2) = w.base;
             *(uint64_t*)(desc + 4) = f.per;
         }
+        if (!more) return;
         ring_barrier();
         if (tid == 0) bad_page = 0u;
         ring_barrier();
@@ -579,13 +611,13 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
 // join its share of the tile's rows, so the parts are read by as many CUs as
 // wrote them. The tile's parts are listed first, a thread per chunk of its keys.
 // Of few parts a wave joins a row by itself; many are dealt out to the four
-// waves and their sums added in order. Lane: columns 4 lane + 256 k.
+// waves, a quarter each, and their sums added in order. Lane: columns 4 lane + 256 k.
 constexpr uint32_t kJoinZ = 4, kManyParts = 16;
 template <int ROWS, int LC, bool OBF>
 __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
     constexpr uint32_t COLS = 128 * LC, NV = (COLS + 255) / 256;
     __shared__ f32x4 sums[4][NV][64];
-    __shared__ float wsum[4];
+    __shared__ float weight[4][2 * kGrid];
     __shared__ uint32_t count[4], list[2 * kGrid];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = uni(tid >> 6), mine = blockIdx.x;
     const uint32_t* desc = p.desc + 8 * mine;
@@ -628,27 +660,42 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
     const uint32_t r0 = rows * idx / S, r1 = rows * (idx + 1u) / S;
     for (uint32_t lr = r0 + (many ? blockIdx.y : 4u * blockIdx.y + wv); lr < r1; lr += many ? kJoinZ : 4u * kJoinZ) {
         auto at = [&](uint32_t s) { return (size_t)list[s] * ROWS + lr; };
-        float M = kNone;
-        for (uint32_t s = lane; s < S; s += 64) M = fmaxf(M, p.part_ml[2 * at(s)]);
-        for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
         f32x4 y[NV];
 #pragma unroll
         for (uint32_t k = 0; k < NV; k++) y[k] = f32x4{0.f, 0.f, 0.f, 0.f};
         float sum = 0.f;
-#pragma unroll 4
-        for (uint32_t s = many ? wv : 0u; s < S; s += many ? 4u : 1u) {
-            const float* ml = p.part_ml + 2 * at(s);
-            const float w = exp2_(ml[0] - M);
-            sum += w * ml[1];
+        auto take = [&](uint32_t s, float w) {
             const float* o = p.part + at(s) * COLS + 4u * lane;
 #pragma unroll
             for (uint32_t k = 0; k < NV; k++) {
-                if (4u * lane + 256u * k < COLS) {
+                if (COLS % 256 == 0 || 4u * lane < COLS) {
                     const f32x4 v = gld((const f32x4*)(o + 256u * k));
 #pragma unroll
                     for (int j = 0; j < 4; j++) y[k][j] += w * v[j];
                 }
             }
+        };
+        float M = kNone;
+        for (uint32_t s = lane; s < S; s += 64) M = fmaxf(M, p.part_ml[2 * at(s)]);
+        for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+        if (!many) {
+#pragma unroll 4
+            for (uint32_t s = 0; s < S; s++) {
+                const float* ml = p.part_ml + 2 * at(s);
+                const float w = exp2_(ml[0] - M);
+                sum += w * ml[1];
+                take(s, w);
+            }
+        } else {
+            for (uint32_t s = lane; s < S; s += 64) {
+                const float w = exp2_(p.part_ml[2 * at(s)] - M);
+                weight[wv][s] = w;
+                sum += w * p.part_ml[2 * at(s) + 1];
+            }
+            for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+            const uint32_t s1 = S * (wv + 1u) / 4u;
+#pragma unroll 4
+            for (uint32_t s = S * wv / 4u; s < s1; s++) take(s, weight[wv][s]);
         }
         const uint32_t row = rt * ROWS + lr, node = row / H, h = row - node * H;
         const size_t out = (size_t)(q.t0 + node) * p.a.out_stride + (size_t)h * L;
@@ -670,14 +717,13 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
         }
 #pragma unroll
         for (uint32_t k = 0; k < NV; k++) sums[wv][k][lane] = y[k];
-        if (lane == 0) wsum[wv] = sum;
         __syncthreads();
         if (wv < NV) {
             f32x4 v;
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 v[j] = (sums[0][wv][lane][j] + sums[1][wv][lane][j]) + (sums[2][wv][lane][j] + sums[3][wv][lane][j]);
-            put(v, (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]), wv);
+            put(v, sum, wv);
         }
         __syncthreads();
     }
@@ -774,7 +820,7 @@ size_t tree_scratch(const wl_tree_attn& a) {
 
 template <int GR, int LC>
 int run_bf16(const Tree& p, hipStream_t st) {
-    hipLaunchKernelGGL((tree_bf16_kernel<GR, LC>), dim3(kGrid), dim3(256 * GR), 0, st, p, 1u);
+    hipLaunchKernelGGL((tree_bf16_kernel<GR, LC>), dim3(kGrid), dim3(256 * GR), 0, st, p, kMinPer);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
     hipLaunchKernelGGL((tree_join_kernel<32 * GR, LC, true>), dim3(2 * kGrid, kJoinZ), dim3(256), 0, st, p);
