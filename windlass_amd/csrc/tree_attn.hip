@@ -152,6 +152,100 @@ WL_DEV bool has_nonfinite(u32x4 v) {
         f |= (v[i] & 0x7F80u) == 0x7F80u || (v[i] & 0x7F800000u) == 0x7F800000u;
     return f;
 }
+// The walks of work-group c: a row tile's keys, or a part of them.
+struct Walk {
+    Req q;
+    uint64_t base;
+    uint32_t r, rt, kt0, kt1, slot;
+};
+template <uint32_t ROWS>
+struct Walks {
+    const Tree& p;
+    const Place f;
+    const uint64_t u1;
+    const uint32_t c;
+    uint64_t u;
+    uint32_t status;
+    Walk next;
+    __device__ __forceinline__ Walks(const Tree& t, const Place& pl, uint32_t wg)
+        : p(t), f(pl), u1(pl.u0 + pl.per < pl.total ? pl.u0 + pl.per : pl.total), c(wg), u(pl.u0), status(0),
+          next{pl.q, pl.base, pl.r, 0, 0, 0, 0} {}
+    __device__ __forceinline__ bool more() const { return u < u1; }
+    __device__ __forceinline__ void find() {  // the walk that begins at unit u < u1, from the last one's request on
+        Walk& w = next;
+        while (u >= w.base + (uint64_t)w.q.nrt * w.q.nkt) {  // the next request that has units
+            w.base += (uint64_t)w.q.nrt * w.q.nkt;
+            w.q = request<ROWS>(p, ++w.r, status);
+        }
+        const uint64_t o = u - w.base;
+        const uint32_t nc = uni(chunks(w.q, f.per)), j = uni((uint32_t)div64((div64(o, w.q.nrt) + 1) * nc - 1, w.q.nkt));
+        const uint32_t ka = uni(chunk_at(w.q, nc, j)), kb = uni(chunk_at(w.q, nc, j + 1));
+        const uint64_t oj = o - (uint64_t)w.q.nrt * ka;
+        w.rt = uni((uint32_t)div64(oj, kb - ka));
+        w.kt0 = uni(ka + (uint32_t)(oj - (uint64_t)w.rt * (kb - ka)));
+        w.kt1 = uni(u1 - u < kb - w.kt0 ? w.kt0 + (uint32_t)(u1 - u) : kb);
+        w.slot = 2u * c + (u == f.u0 ? 0u : 1u);
+        u += w.kt1 - w.kt0;
+    }
+    __device__ __forceinline__ uint32_t rows(const Walk& w) const {
+        const uint32_t n = w.q.nodes * p.a.n_heads - w.rt * ROWS;
+        return n < ROWS ? n : ROWS;
+    }
+    // The page of DR consecutive keys of tile t, from its key k0 on (pages have at
+    // least 8 rows, and DR is at most 8); behind the last key, the last key's
+    __device__ __forceinline__ int32_t page(const Walk& w, uint32_t t, uint32_t k0) const {
+        const uint32_t key = t * kKT + k0;
+        return p.a.d_table[(size_t)w.r * p.a.max_pages + ((key < w.q.keys ? key : w.q.keys - 1u) >> p.psh)];
+    }
+    // names the row tile of the walk's part for the second launch
+    __device__ __forceinline__ void name_part(const Walk& w) const {
+        uint32_t* desc = p.desc + 8 * w.slot;
+        desc[0] = w.r + 1u;
+        desc[1] = w.rt;
+        *(uint64_t*)(desc + 2) = w.base;
+        *(uint64_t*)(desc + 4) = f.per;
+    }
+};
+// One lane's share of a row of sums (4 columns of every 16 from column `col` on,
+// n16 of them): finished, or as a part.
+template <uint32_t ROWS, int LC, bool OBF, uint32_t N16>
+WL_DEV void put_row(const Tree& p, const Walk& w, bool whole, uint32_t lr, float sum, const f32x4* y, uint32_t col) {
+    if (whole) {
+        const uint32_t H = p.a.n_heads, L = p.a.cache.kv_lora_rank;
+        const uint32_t row = w.rt * ROWS + lr, node = row / H, h = row - node * H;
+        const size_t o = (size_t)(w.q.t0 + node) * p.a.out_stride + (size_t)h * L + col;
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+        for (uint32_t k = 0; k < N16; k++) {
+            if (col + 16u * k >= L) continue;
+            const f32x4 v = {y[k][0] * inv, y[k][1] * inv, y[k][2] * inv, y[k][3] * inv};
+            if (OBF) gst((u32x2*)((uint16_t*)p.a.d_out + o + 16u * k), u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])});
+            else gst((f32x4*)((float*)p.a.d_out + o + 16u * k), v);
+        }
+    } else {
+        float* o = p.part + ((size_t)w.slot * ROWS + lr) * (128u * LC) + col;
+#pragma unroll
+        for (uint32_t k = 0; k < N16; k++) gst((f32x4*)(o + 16u * k), y[k]);
+    }
+}
+
+// s_waitcnt vmcnt(N): all but the last N memory operations of this wave are done.
+template <uint32_t N>
+WL_DEV void vm_wait() {
+    static_assert(N < 64u, "vmcnt is 6 bits");
+    __builtin_amdgcn_s_waitcnt((N & 15u) | ((N >> 4) << 14) | 0x0F70u);
+}
+// A barrier that orders LDS accesses of the waves' instructions only: DMA into
+// LDS, loads and stores go on across it (a release fence would wait for them).
+WL_DEV void ring_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
 // LDS serves a 16-byte read 16 lanes at a time, lanes 0-3, 12-15, 20-27 and 4-11,
 // 16-19, 28-31 of either half wave: for an MFMA operand (lane = row + 16 x chunk)
 // those are 8 rows at an even chunk and the other 8 at the odd one beside it. Key
@@ -185,23 +279,6 @@ WL_DEV constexpr uint32_t swz4(uint32_t row) { return (row & 8u) >> 2; }
 // for between products; before the barrier each wave waits for its rows of t + 1.
 constexpr float kMost = 0x1p64f;  // 2^31 such weights sum to 2^95
 
-// s_waitcnt vmcnt(N): all but the last N memory operations of this wave are done.
-template <uint32_t N>
-WL_DEV void vm_wait() {
-    static_assert(N < 64u, "vmcnt is 6 bits");
-    __builtin_amdgcn_s_waitcnt((N & 15u) | ((N >> 4) << 14) | 0x0F70u);
-}
-// A barrier that orders LDS accesses of the waves' instructions only: DMA into
-// LDS, loads and stores go on across it (a release fence would wait for them).
-WL_DEV void ring_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");
-}
-
 template <int GR, int LC>
 __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t min_per) {
     constexpr uint32_t NW = 4 * GR, ROWS = 32 * GR, PITCH = 256 * LC + kPad, NL = 4 * LC, NS = NL + 2, CT = 2 * LC, DR = 32 / NW;
@@ -223,55 +300,22 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
     const uint32_t H = p.a.n_heads, L = p.a.cache.kv_lora_rank, RP = p.a.cache.qk_rope;
     if (tid == 0) bad_page = again = 0;
     const Place f = find_place<ROWS, 64 * NW>(p, c, min_per, tmp, &found);
-    const uint64_t u1 = f.u0 + f.per < f.total ? f.u0 + f.per : f.total;
     if (tid < 2) p.desc[8 * (2 * c + tid)] = 0;
-    if (f.u0 >= u1) return;
-
-    // the walks of this work-group: a row tile's keys, or a part of them
-    struct Walk {
-        Req q;
-        uint64_t base;
-        uint32_t r, rt, kt0, kt1, slot;
-    };
-    uint64_t u = f.u0;
-    uint32_t status = 0;
-    Walk next{f.q, f.base, f.r, 0, 0, 0, 0};
-    auto find_walk = [&]() {  // the walk that begins at unit u < u1, from the last one's request on
-        Walk& w = next;
-        while (u >= w.base + (uint64_t)w.q.nrt * w.q.nkt) {  // the next request that has units
-            w.base += (uint64_t)w.q.nrt * w.q.nkt;
-            w.q = request<ROWS>(p, ++w.r, status);
-        }
-        const uint64_t o = u - w.base;
-        const uint32_t nc = uni(chunks(w.q, f.per)), j = uni((uint32_t)div64((div64(o, w.q.nrt) + 1) * nc - 1, w.q.nkt));
-        const uint32_t ka = uni(chunk_at(w.q, nc, j)), kb = uni(chunk_at(w.q, nc, j + 1));
-        const uint64_t oj = o - (uint64_t)w.q.nrt * ka;
-        w.rt = uni((uint32_t)div64(oj, kb - ka));
-        w.kt0 = uni(ka + (uint32_t)(oj - (uint64_t)w.rt * (kb - ka)));
-        w.kt1 = uni(u1 - u < kb - w.kt0 ? w.kt0 + (uint32_t)(u1 - u) : kb);
-        w.slot = 2u * c + (u == f.u0 ? 0u : 1u);
-        u += w.kt1 - w.kt0;
-    };
-    // A wave's DR rows of a tile lie in one page (pages have at least 8 rows): its
-    // page in tile t of a walk; behind the last key, the last key's
-    auto page_at = [&](const Walk& w, uint32_t t) {
-        const uint32_t key = t * kKT + DR * wave;
-        return p.a.d_table[(size_t)w.r * p.a.max_pages + ((key < w.q.keys ? key : w.q.keys - 1u) >> p.psh)];
-    };
-    // the pages of the next walk's first four tiles are read while the last one ends
+    Walks<ROWS> walks(p, f, c);
+    if (!walks.more()) return;
+    // the pages of a walk's first four tiles are read while the one before it ends
     int32_t ahead[4] = {0, 0, 0, 0};
     auto read_ahead = [&]() {
-        if (next.q.flaw) return;
+        if (walks.next.q.flaw) return;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) ahead[i] = page_at(next, next.kt0 + i);
+        for (uint32_t i = 0; i < 4; i++) ahead[i] = walks.page(walks.next, walks.next.kt0 + i, DR * wave);
     };
-    find_walk();
+    walks.find();
     read_ahead();
     for (;;) {
-        const Walk w = next;
+        const Walk w = walks.next;
         const Req& q = w.q;
-        const uint32_t rt = w.rt, kt0 = w.kt0, kt1 = w.kt1, slot = w.slot;
-        const uint32_t rows = q.nodes * H - rt * ROWS < ROWS ? q.nodes * H - rt * ROWS : ROWS;
+        const uint32_t rt = w.rt, kt0 = w.kt0, kt1 = w.kt1, rows = walks.rows(w);
 
         f32x4 acc[2][CT];
         float m = kNone, l = 0.f;  // of row sr + n: the reference, this lane's part of the weights' sum
@@ -283,11 +327,11 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                 for (uint32_t k = 0; k < CT; k++) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
         };
         bool bad = false;
-        const bool more = u < u1;
+        const bool more = walks.more();
         if (q.flaw) {
             clear();
         } else {
-            auto page_of = [&](uint32_t t) { return page_at(w, t); };
+            auto page_of = [&](uint32_t t) { return walks.page(w, t, DR * wave); };
             // The wave's rows of tile t: one resource, whose bounds make zeros of rows
             // behind the last key. Tiles behind the walk's last are called for too, as
             // zeros, so that a wave's memory operations can be counted.
@@ -551,7 +595,7 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
             }
         }
         if (more) {
-            find_walk();
+            walks.find();
             read_ahead();
         }
         // the weights' sums over the row's lanes and waves; flaws
@@ -564,7 +608,7 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
         l += __shfl_xor(l, 32, 64);
         if (g == 0) rowred[wave & 1u][sr + n] = l;
         const bool whole = kt1 - kt0 == q.nkt;
-        if (!whole && sk == 0 && g == 0) p.part_ml[2u * (slot * ROWS + sr + n)] = m;
+        if (!whole && sk == 0 && g == 0) p.part_ml[2u * (w.slot * ROWS + sr + n)] = m;
         ring_barrier();
         const bool nan = bad_page != 0 || q.flaw;
 #pragma unroll
@@ -573,32 +617,11 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
             float sum = rowred[0][lr] + rowred[1][lr];
             if (nan) sum = __builtin_nanf("");
             if (lr < rows) {
-                if (whole) {
-                    const uint32_t row = rt * ROWS + lr, node = row / H, h = row - node * H;
-                    uint16_t* o = (uint16_t*)p.a.d_out + (size_t)(q.t0 + node) * p.a.out_stride + (size_t)h * L;
-                    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-#pragma unroll
-                    for (uint32_t k = 0; k < CT; k++) {
-                        const uint32_t col = 32u * LC * wv + 16u * k + 4u * g;
-                        const f32x4 y = acc[i][k];
-                        if (col < L)
-                            gst((u32x2*)(o + col), u32x2{pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv)});
-                    }
-                } else {
-                    float* o = p.part + ((size_t)slot * ROWS + lr) * (128u * LC);
-#pragma unroll
-                    for (uint32_t k = 0; k < CT; k++) gst((f32x4*)(o + 32u * LC * wv + 16u * k + 4u * g), acc[i][k]);
-                    if (wv == 0 && g == 0) p.part_ml[2u * (slot * ROWS + lr) + 1u] = sum;
-                }
+                put_row<ROWS, LC, true, CT>(p, w, whole, lr, sum, acc[i], 32u * LC * wv + 4u * g);
+                if (!whole && wv == 0 && g == 0) p.part_ml[2u * (w.slot * ROWS + lr) + 1u] = sum;
             }
         }
-        if (!whole && tid == (slot & 1u)) {  // the thread that cleared it
-            uint32_t* desc = p.desc + 8 * slot;
-            desc[0] = w.r + 1u;
-            desc[1] = rt;
-            *(uint64_t*)(desc + 2) = w.base;
-            *(uint64_t*)(desc + 4) = f.per;
-        }
+        if (!whole && tid == (w.slot & 1u)) walks.name_part(w);  // the thread that cleared it
         if (!more) return;
         ring_barrier();
         if (tid == 0) bad_page = 0u;
@@ -728,80 +751,343 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
         __syncthreads();
     }
 }
-template <bool BF>
-WL_DEV float ld1(const void* p, size_t i) {
-    return BF ? bf2f(((const uint16_t*)p)[i]) : ((const float*)p)[i];
+// ---- 32-bit queries -------------------------------------------------------------
+// A 32-bit value is the sum of three bf16 ones (its leading 8 bits, the next 8, the
+// last 8: cut off, not rounded, so each remainder is exact), and a product of two
+// such sums is, but for terms below 2^-24 of it, the six products of parts whose
+// places add up to two at most (three of them where the other side is bf16 itself):
+// exact products in the matrix cores, summed in f32. 32 rows against 32 keys at a
+// time, four waves, split as in the 16-bit kernel; queries, weights and (WIDE)
+// cache rows in three parts each. One wave a SIMD: its 512 registers hold 16 rows'
+// queries (216), the sums (64) and the next tile (36, WIDE 72), which is read while
+// this one is worked on and then cut up into LDS. The products of the leading parts
+// and those of the others are summed apart in the scores.
+// Bound by the matrix cores: 102 (WIDE 204) MFMAs a wave and tile, 16 clocks each.
+WL_DEV void cut3(float x, float& h, float& m, float& l) {  // h + m + l = x, each with its low 16 bits clear
+    h = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+    const float r = x - h;
+    m = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u);
+    l = r - m;
 }
+// the leading halves of two floats, the first one's low
+WL_DEV uint32_t high2(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
+WL_DEV bool nonfinite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
-// One wave per (request, node, head): lane l holds columns l, l + 64, ... of
-// the query and of the output; one key after another, with the running
-// maximum and sum of the softmax.
-template <bool QBF, bool CBF>
-__global__ __launch_bounds__(256) void tree_attn_kernel(wl_tree_attn a) {
-    const uint32_t lane = threadIdx.x & 63u, wv = threadIdx.x >> 6;
-    const uint32_t r = blockIdx.x, h = blockIdx.y * 4u + wv, node0 = blockIdx.z;
-    if (h >= a.n_heads) return;
-    const uint32_t L = a.cache.kv_lora_rank, W = L + a.cache.qk_rope, ps = a.cache.page_size;
-    const int32_t t0 = a.d_cu[r], t1 = a.d_cu[r + 1], n = a.d_len[r];
-    uint32_t bad = 0;
-    if (t0 < 0 || t1 < t0 || (uint32_t)t1 > a.n_tokens) {
-        if (a.d_status && lane == 0) atomicOr(a.d_status, WL_PAGED_E_LEN);
-        return;
-    }
-    const uint32_t m = (uint32_t)(t1 - t0);
-    if (m == 0) return;
-    if (n < 0 || (uint64_t)n + m > (uint64_t)a.max_pages * ps) bad |= WL_PAGED_E_LEN;
-    if (m > WL_TREE_MAX_NODES) bad |= WL_PAGED_E_TREE;
-    const int32_t* table = a.d_table + (size_t)r * a.max_pages;
-    const uint32_t K = bad ? 0u : (uint32_t)n + m;
-    for (uint32_t k = lane; k * ps < K; k += 64)
-        if (table[k] < 0 || (uint32_t)table[k] >= a.cache.n_pages) bad |= WL_PAGED_E_PAGE;
-    for (int o = 32; o > 0; o >>= 1) bad |= __shfl_xor(bad, o, 64);
-    if (bad && a.d_status && lane == 0) atomicOr(a.d_status, bad);
-    for (uint32_t i = node0; i < m; i += gridDim.z) {
-        const uint32_t t = (uint32_t)t0 + i;
-        const uint64_t bits = a.d_mask ? a.d_mask[t] : (2ull << (i & 63u)) - 1ull;
-        float q[9], acc[8], mx = -INFINITY, sum = 0.f;
+template <int LC, bool WIDE>
+__global__ __launch_bounds__(256) void tree_f32_kernel(Tree p, uint32_t min_per) {
+    constexpr uint32_t ROWS = 32, PITCH = 256 * LC + kPad, NL = 4 * LC, NS = NL + 2, CT = 2 * LC, DR = 8, NP = WIDE ? 3 : 1;
+    constexpr uint32_t ROT = kKT * PITCH, PIECE = ROT + kKT * 128, ES = WIDE ? 4 : 2;
+    __shared__ __align__(1024) uint8_t tile[NP * PIECE];
+    __shared__ __align__(1024) uint8_t pb[3 * ROWS * 64];  // weights [part][row][32 keys]
+    __shared__ float rowred[2][ROWS];
+    __shared__ uint64_t seen[ROWS];
+    __shared__ uint32_t flaws[kKT / 4];
+    __shared__ uint32_t bad_page, again;
+    __shared__ uint64_t tmp[6];
+    __shared__ Req found;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uni(tid >> 6), n = lane & 15u, g = lane >> 4;
+    const uint32_t sr = 8u * (wave & ~1u), sk = 16u * (wave & 1u);  // first row and key of this wave's scores
+    const uint32_t c = (blockIdx.x % 8u) * (kGrid / 8u) + blockIdx.x / 8u;
+    const uint32_t H = p.a.n_heads, L = p.a.cache.kv_lora_rank, RP = p.a.cache.qk_rope;
+    if (tid == 0) bad_page = again = 0;
+    const Place f = find_place<ROWS, 256>(p, c, min_per, tmp, &found);
+    if (tid < 2) p.desc[8 * (2 * c + tid)] = 0;
+    Walks<ROWS> walks(p, f, c);
+    if (!walks.more()) return;
+    for (;;) {
+        walks.find();
+        const Walk w = walks.next;
+        const Req& q = w.q;
+        const uint32_t kt0 = w.kt0, kt1 = w.kt1, rows = walks.rows(w);
+        f32x4 acc[2][CT];
+        float m = kNone, l = 0.f;
+        auto clear = [&]() __attribute__((always_inline)) {
+            l = 0.f;
 #pragma unroll
-        for (uint32_t j = 0; j < 9; j++) {
-            const uint32_t c = lane + 64 * j;
-            q[j] = c < L ? ld1<QBF>(a.d_q_lat, t * a.q_lat_stride + (size_t)h * L + c)
-                   : c < W ? ld1<QBF>(a.d_q_rope, t * a.q_rope_stride + (size_t)h * (W - L) + (c - L)) : 0.f;
-        }
+            for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (uint32_t j = 0; j < 8; j++) acc[j] = 0.f;
-        for (uint32_t k = 0; k < K && !bad; k++) {
-            if (k >= (uint32_t)n && !((bits >> (k - (uint32_t)n)) & 1)) continue;
-            const size_t row = ((size_t)(uint32_t)table[k / ps] * ps + k % ps) * a.cache.row_stride;
-            float v[9], s = 0.f;
+                for (uint32_t k = 0; k < CT; k++) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        };
+        bool bad = false;
+        if (q.flaw) {
+            clear();
+        } else {
+            // the wave's 8 rows of a tile, in registers: chunk i 64 + lane of their latent
+            // parts (EL to a row), then of their rotary ones (ER)
+            constexpr uint32_t EL = 8 * ES * LC, NLAT = DR * EL / 64, ER = 4 * ES, NROT = DR * ER / 64;
+            const uint32_t stride = ES * p.a.cache.row_stride;
+            u32x4 raw[NLAT + NROT];
+            auto read_tile = [&](uint32_t t) __attribute__((always_inline)) {
+                const int32_t page = (int32_t)uni((uint32_t)walks.page(w, t, DR * wave));
+                const uint32_t key = t * kKT + DR * wave;
+                const uint32_t left = key < q.keys ? (q.keys - key < DR ? q.keys - key : DR) : 0u;
+                const bool ok = page >= 0 && (uint32_t)page < p.a.cache.n_pages;
+                bad |= left && !ok;
+                const uint32_t row = ok ? ((uint32_t)page << p.psh) + (key & (p.a.cache.page_size - 1u)) : 0u;
+                const rsrc_t rs = make_rsrc((const uint8_t*)p.a.cache.d_rows + (uint64_t)row * stride,
+                                            ok && left ? (left - 1u) * stride + ES * (L + RP) : 0u);
 #pragma unroll
-            for (uint32_t j = 0; j < 9; j++) {
-                const uint32_t c = lane + 64 * j;
-                v[j] = c < W ? ld1<CBF>(a.cache.d_rows, row + c) : 0.f;
-                s += q[j] * v[j];
+                for (uint32_t i = 0; i < NLAT; i++) {
+                    const uint32_t e = 64u * i + lane, k = e % EL;
+                    raw[i] = bld16(rs, 16u * k < ES * L ? (e / EL) * stride + 16u * k : kOOB, 0);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < NROT; i++) {
+                    const uint32_t e = 64u * i + lane, k = e % ER;
+                    raw[NLAT + i] = bld16(rs, 16u * k < ES * RP ? (e / ER) * stride + ES * L + 16u * k : kOOB, 0);
+                }
+            };
+            auto has_nodes = [&](uint32_t t) { return (t + 1) * kKT > q.len; };  // tree nodes, or the end, in tile t
+            // into LDS, in parts; of rows of nodes what is not finite is noted and cleared
+            // (their scores will be NaN for those that see them)
+            auto stage = [&](uint32_t t) __attribute__((always_inline)) {
+                auto put = [&](u32x4 x, uint32_t at) {
+                    if (WIDE) {
+                        float h[4], md[4], lo[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) cut3(__uint_as_float(x[k]), h[k], md[k], lo[k]);
+                        *(u32x2*)(tile + at) = u32x2{high2(h[0], h[1]), high2(h[2], h[3])};
+                        *(u32x2*)(tile + (NP > 1 ? PIECE : 0) + at) = u32x2{high2(md[0], md[1]), high2(md[2], md[3])};
+                        *(u32x2*)(tile + (NP > 1 ? 2 * PIECE : 0) + at) = u32x2{high2(lo[0], lo[1]), high2(lo[2], lo[3])};
+                    } else {
+                        *(u32x4*)(tile + at) = x;
+                    }
+                };
+                if (has_nodes(t)) {
+#pragma unroll
+                    for (uint32_t i = 0; i < NLAT + NROT; i++) {
+                        const uint32_t e = 64u * (i < NLAT ? i : i - NLAT) + lane, row = DR * wave + e / (i < NLAT ? EL : ER);
+                        bool nf = false;
+                        if (WIDE) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++) nf |= nonfinite(__uint_as_float(raw[i][j]));
+                        } else {
+                            nf = has_nonfinite(raw[i]);
+                        }
+                        if (nf && t * kKT + row >= q.len) {
+                            ((uint8_t*)flaws)[row] = 1;
+                            raw[i] = u32x4{0u, 0u, 0u, 0u};
+                        }
+                    }
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < NLAT + NROT; i++) {
+                    const bool lat = i < NLAT;
+                    const uint32_t e = 64u * (lat ? i : i - NLAT) + lane, row = DR * wave + e / (lat ? EL : ER), k = e % (lat ? EL : ER);
+                    const uint32_t b = WIDE ? 8u * k : 16u * k;  // of a bf16 row
+                    put(raw[i], lat ? row * PITCH + b : ROT + row * 128u + (b ^ (16u * swz8(row & 15u))));
+                }
+            };
+            // the queries of rows sr + n, in parts, in the operand's layout: lane (row n, k group g)
+            bf16x8 qf[3][NS];
+            auto read_queries = [&]() __attribute__((always_inline)) {
+                const rsrc_t ql = make_rsrc((const float*)p.a.d_q_lat + q.t0 * p.a.q_lat_stride,
+                                            4u * ((q.nodes - 1u) * (uint32_t)p.a.q_lat_stride + H * L));
+                const rsrc_t qr = make_rsrc((const float*)p.a.d_q_rope + q.t0 * p.a.q_rope_stride,
+                                            4u * ((q.nodes - 1u) * (uint32_t)p.a.q_rope_stride + H * RP));
+                const uint32_t lr = sr + n, row = w.rt * ROWS + lr, node = row / H, h = row - node * H;
+                const bool live = lr < rows;
+                const uint32_t vl = live ? 4u * (node * (uint32_t)p.a.q_lat_stride + h * L + 8u * g) : kOOB;
+                const uint32_t vr = live ? 4u * (node * (uint32_t)p.a.q_rope_stride + h * RP + 8u * g) : kOOB;
+#pragma unroll
+                for (uint32_t s = 0; s < NS; s++) {
+                    u32x4 x[2];
+#pragma unroll
+                    for (uint32_t k = 0; k < 2; k++) {
+                        x[k] = s < NL ? bld16(ql, vl + 128u * s + 16u * k, 0) : bld16(qr, vr + 128u * (s - NL) + 16u * k, 0);
+                        if (32u * (s < NL ? s : s - NL) + 8u * g >= (s < NL ? L : RP)) x[k] = u32x4{0u, 0u, 0u, 0u};
+                    }
+                    u32x4 part[3];
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; k++) {
+                        float a[3], b[3];
+                        cut3(__uint_as_float(x[k >> 1][2 * (k & 1)]), a[0], a[1], a[2]);
+                        cut3(__uint_as_float(x[k >> 1][2 * (k & 1) + 1]), b[0], b[1], b[2]);
+#pragma unroll
+                        for (int j = 0; j < 3; j++) part[j][k] = high2(a[j], b[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 3; j++) qf[j][s] = as_bf16x8(part[j]);
+                }
+                if (sk == 0 && g == 0) {
+                    const uint32_t nd = live ? node : 0u;
+                    seen[lr] = p.a.d_mask ? p.a.d_mask[q.t0 + nd] : (2ull << nd) - 1ull;
+                }
+            };
+            const uint32_t key_at = (sk + n) * PITCH + 16u * g, key_rot = (sk + n) * 128u + 16u * (g ^ swz8(n));
+            auto kread = [&](uint32_t s, uint32_t piece) {
+                const uint8_t* b = tile + PIECE * piece;
+                return as_bf16x8(s < NL ? *(const u32x4*)(b + key_at + 64u * s) : *(const u32x4*)(b + ROT + (key_rot ^ (64u * (s - NL)))));
+            };
+            // the scores in powers of two of row sr + n with keys sk + 4 g + j, -inf where unseen
+            auto scores = [&](uint32_t t) __attribute__((always_inline)) {
+                f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+                bf16x8 kf[2][NP];
+#pragma unroll
+                for (uint32_t j = 0; j < NP; j++) kf[0][j] = kread(0, j);
+#pragma unroll
+                for (uint32_t s = 0; s < NS; s++) {
+                    const uint32_t b = s & 1u;
+                    if (s + 1 < NS) {
+#pragma unroll
+                        for (uint32_t j = 0; j < NP; j++) kf[b ^ 1u][j] = kread(s + 1, j);
+                    }
+                    s0 = mma(kf[b][0], qf[0][s], s0);
+                    s1 = mma(kf[b][0], qf[2][s], s1);
+                    if (WIDE) {
+                        s1 = mma(kf[b][NP - 1], qf[0][s], s1);
+                        s1 = mma(kf[b][NP > 1 ? 1 : 0], qf[1][s], s1);
+                        s1 = mma(kf[b][NP > 1 ? 1 : 0], qf[0][s], s1);
+                    }
+                    s1 = mma(kf[b][0], qf[1][s], s1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                f32x4 sc;
+#pragma unroll
+                for (int k = 0; k < 4; k++) sc[k] = (s0[k] + s1[k]) * p.scale2;
+                if (has_nodes(t)) {
+                    const uint32_t fl = flaws[sk / 4u + g];
+                    const uint64_t bits = seen[sr + n];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t key = t * kKT + sk + 4u * g + k;
+                        const uint32_t bit = (uint32_t)(bits >> ((key - q.len) & 63u)) & (key < q.keys ? 1u : 0u);
+                        const float nan = (fl >> (8 * k)) & 1u ? __builtin_nanf("") : 0.f;
+                        sc[k] = (bit | (key < q.len ? 1u : 0u)) ? sc[k] + nan : -INFINITY;
+                    }
+                }
+                return sc;
+            };
+            auto largest = [&](f32x4 x) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); };
+            auto share_maxima = [&](float x) {
+                x = fmaxf(x, __shfl_xor(x, 16, 64));
+                x = fmaxf(x, __shfl_xor(x, 32, 64));
+                if (g == 0) rowred[wave & 1u][sr + n] = x;
+                ring_barrier();
+                m = fmaxf(kNone, fmaxf(rowred[0][sr + n], rowred[1][sr + n]));
+            };
+            const uint32_t value_at = (4u * g + ((lane & 15u) >> 2)) * PITCH + 64u * LC * wave + 8u * (lane & 3u);
+            auto vread = [&](uint32_t k, uint32_t piece) {
+                const uint8_t* pa = tile + PIECE * piece + value_at + 32u * k;
+                typedef __attribute__((address_space(3))) s16x4 l_s16x4;
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa));
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa + 16 * PITCH));
+                const u32x2 xx = __builtin_bit_cast(u32x2, x), yy = __builtin_bit_cast(u32x2, y);
+                return as_bf16x8(u32x4{xx[0], xx[1], yy[0], yy[1]});
+            };
+            const uint32_t put_at = (sr + n) * 64u + 16u * (g ^ swz4(n)) + sk / 2u, get_at = n * 64u + 16u * (g ^ swz4(n));
+            bool pass = false;
+            // a walk; SUMS false: over the scores alone, for their maxima
+            auto go = [&](bool known, auto sums) __attribute__((always_inline)) {
+                constexpr bool SUMS = decltype(sums)::value;
+                float x = kNone;
+                read_tile(kt0);
+                if (SUMS && !known) read_queries();
+                for (uint32_t t = kt0; t < kt1; t++) {
+                    if (has_nodes(t)) {
+                        if (tid < kKT / 4) flaws[tid] = 0;
+                        ring_barrier();
+                    }
+                    stage(t);
+                    ring_barrier();
+                    if (t + 1 < kt1) read_tile(t + 1);
+                    const f32x4 sc = scores(t);
+                    if (SUMS) {
+                        if (t == kt0 && !known) share_maxima(largest(sc));
+                        float e[3][4], top = 0.f;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const float v = exp2_(sc[k] - m);
+                            l += v;
+                            top = fmaxf(top, v);
+                            cut3(v, e[0][k], e[1][k], e[2][k]);
+                        }
+                        pass |= top > kMost;
+#pragma unroll
+                        for (uint32_t j = 0; j < 3; j++)
+                            *(u32x2*)(pb + j * ROWS * 64u + put_at) = u32x2{high2(e[j][0], e[j][1]), high2(e[j][2], e[j][3])};
+                        ring_barrier();
+                        bf16x8 pf[3][2];
+#pragma unroll
+                        for (uint32_t j = 0; j < 3; j++)
+#pragma unroll
+                            for (int i = 0; i < 2; i++)
+                                pf[j][i] = as_bf16x8(*(const u32x4*)(pb + j * ROWS * 64u + get_at + 1024u * i));
+                        bf16x8 vf[2][NP];
+#pragma unroll
+                        for (uint32_t j = 0; j < NP; j++) vf[0][j] = vread(0, j);
+#pragma unroll
+                        for (uint32_t v = 0; v < CT; v++) {
+                            const uint32_t b = v & 1u;
+                            if (v + 1 < CT) {
+#pragma unroll
+                                for (uint32_t j = 0; j < NP; j++) vf[b ^ 1u][j] = vread(v + 1, j);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                f32x4 y = acc[i][v];
+                                if (WIDE) {
+                                    y = mma(vf[b][NP - 1], pf[0][i], y);
+                                    y = mma(vf[b][NP > 1 ? 1 : 0], pf[1][i], y);
+                                    y = mma(vf[b][NP > 1 ? 1 : 0], pf[0][i], y);
+                                }
+                                y = mma(vf[b][0], pf[2][i], y);
+                                y = mma(vf[b][0], pf[1][i], y);
+                                acc[i][v] = mma(vf[b][0], pf[0][i], y);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    } else {
+                        x = fmaxf(x, largest(sc));
+                    }
+                    ring_barrier();
+                }
+                return x;
+            };
+            using Sums = std::integral_constant<bool, true>;
+            using Maxima = std::integral_constant<bool, false>;
+            clear();
+            go(false, Sums{});
+            if (__ballot(pass) && lane == 0) again = 1u;
+            ring_barrier();
+            const bool redo = again != 0;
+            ring_barrier();
+            if (redo) {
+                if (tid == 0) again = 0u;
+                share_maxima(go(true, Maxima{}));
+                clear();
+                go(true, Sums{});
             }
-            for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-            s *= a.scale;
-            const float mn = s != s ? s : fmaxf(mx, s);
-            const float al = mx == -INFINITY ? 0.f : expf(mx - mn), p = expf(s - mn);
-            sum = sum * al + p;
-#pragma unroll
-            for (uint32_t j = 0; j < 8; j++) acc[j] = acc[j] * al + p * v[j];
-            mx = mn;
         }
-        const float inv = bad ? __builtin_nanf("") : sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-        for (uint32_t j = 0; j < 8; j++) {
-            const uint32_t c = lane + 64 * j;
-            if (c >= L) break;
-            const size_t o = t * a.out_stride + (size_t)h * L + c;
-            const float y = acc[j] * inv;
-            if (QBF) ((uint16_t*)a.d_out)[o] = y != y ? 0x7FC0u : (uint16_t)f2bf(y);
-            else ((float*)a.d_out)[o] = y;
+        if (__ballot(bad) && lane == 0) {
+            bad_page = 1u;
+            if (p.a.d_status)
+                __hip_atomic_fetch_or(p.a.d_status, WL_PAGED_E_PAGE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (g == 0) rowred[wave & 1u][sr + n] = l;
+        const bool whole = kt1 - kt0 == q.nkt;
+        if (!whole && sk == 0 && g == 0) p.part_ml[2u * (w.slot * ROWS + sr + n)] = m;
+        ring_barrier();
+        const bool nan = bad_page != 0 || q.flaw;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t lr = 16u * i + n;
+            float sum = rowred[0][lr] + rowred[1][lr];
+            if (nan) sum = __builtin_nanf("");
+            if (lr < rows) {
+                put_row<ROWS, LC, false, CT>(p, w, whole, lr, sum, acc[i], 32u * LC * wave + 4u * g);
+                if (!whole && wave == 0 && g == 0) p.part_ml[2u * (w.slot * ROWS + lr) + 1u] = sum;
+            }
+        }
+        if (!whole && tid == (w.slot & 1u)) walks.name_part(w);  // the thread that cleared it
+        if (!walks.more()) return;
+        ring_barrier();
+        if (tid == 0) bad_page = 0u;
+        ring_barrier();
     }
 }
-
 }  // namespace
 
 uint32_t lat_class(const wl_tree_attn& a) {  // 128-column blocks of a row's latent part, as the kernels have them
@@ -827,6 +1113,15 @@ int run_bf16(const Tree& p, hipStream_t st) {
     return (int)hipGetLastError();
 }
 
+template <int LC, bool WIDE>
+int run_f32(const Tree& p, hipStream_t st) {
+    hipLaunchKernelGGL((tree_f32_kernel<LC, WIDE>), dim3(kGrid), dim3(256), 0, st, p, kMinPer);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    hipLaunchKernelGGL((tree_join_kernel<32, LC, false>), dim3(2 * kGrid, kJoinZ), dim3(256), 0, st, p);
+    return (int)hipGetLastError();
+}
+
 int launch_tree(const wl_tree_attn& a, void* stream) {
     hipStream_t st = (hipStream_t)stream;
     Tree p{};
@@ -841,10 +1136,8 @@ int launch_tree(const wl_tree_attn& a, void* stream) {
         if (rows == 64) return lc == 4 ? run_bf16<2, 4>(p, st) : lc == 2 ? run_bf16<2, 2>(p, st) : run_bf16<2, 1>(p, st);
         return lc == 4 ? run_bf16<1, 4>(p, st) : lc == 2 ? run_bf16<1, 2>(p, st) : run_bf16<1, 1>(p, st);
     }
-    const dim3 g(a.n_req, (a.n_heads + 3) / 4, 8);
-    if (a.cache.dtype == WL_TYPE_BF16) hipLaunchKernelGGL((tree_attn_kernel<false, true>), g, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((tree_attn_kernel<false, false>), g, dim3(256), 0, st, a);
-    return (int)hipGetLastError();
+    if (a.cache.dtype == WL_TYPE_BF16) return lc == 4 ? run_f32<4, false>(p, st) : lc == 2 ? run_f32<2, false>(p, st) : run_f32<1, false>(p, st);
+    return lc == 4 ? run_f32<4, true>(p, st) : lc == 2 ? run_f32<2, true>(p, st) : run_f32<1, true>(p, st);
 }
 
 }  // namespace paged
