@@ -15,7 +15,8 @@ constexpr uint32_t kKT = 32;    // keys of a tile
 // Key tiles of a walk at least: a shorter one's parts cost more to join than it saves.
 // One token over 4096 keys, both launches: 32.6 us at 1, 28.6 at 2, 29.3 at 4, 32.5 at 8.
 constexpr uint32_t kMinPer = 2;
-constexpr uint32_t kGrid = 256; // work-groups of a launch: one per CU (LDS and registers allow one)
+constexpr uint32_t kGrid = 256;      // work-groups of a launch of the 16-bit kernel: one per CU (LDS and registers allow one)
+constexpr uint32_t kGridF32 = 512;   // of the 32-bit one: two per CU
 constexpr float kNone = -3.0e38f;  // the running maximum of a row that has seen no key
 
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
@@ -27,9 +28,9 @@ struct Tree {
     wl_tree_attn a;
     uint32_t psh;      // log2 page_size
     float scale2;      // scale * log2(e): scores in powers of two
-    float* part;       // [2 kGrid][rows][cols] unnormalised sums of split tiles
-    float* part_ml;    // [2 kGrid][rows][2] their maxima and weight sums
-    uint32_t* desc;    // [2 kGrid][8] the parts' row tiles: {request + 1, row tile, base, per}, the last two 64-bit
+    float* part;       // [2 grid][rows][cols] unnormalised sums of split tiles
+    float* part_ml;    // [2 grid][rows][2] their maxima and weight sums
+    uint32_t* desc;    // [2 grid][8] the parts' row tiles: {request + 1, row tile, base, per}, the last two 64-bit
 };
 
 // ---- the work and its split --------------------------------------------------
@@ -80,7 +81,7 @@ struct Place {
     uint32_t r;
     Req q;
 };
-template <uint32_t ROWS, uint32_t THREADS>
+template <uint32_t ROWS, uint32_t THREADS, uint32_t GRID>
 WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* tmp, Req* found) {
     constexpr uint32_t NW = THREADS / 64;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = tid >> 6, R = p.a.n_req;
@@ -108,7 +109,7 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
     f.total = 0;
 #pragma unroll
     for (uint32_t w = 0; w < NW; w++) f.total += tmp[w];
-    f.per = (f.total + kGrid - 1) / kGrid;
+    f.per = (f.total + GRID - 1) / GRID;
     if (f.per < min_per) f.per = min_per;
     f.u0 = (uint64_t)c * f.per;
     uint64_t at = inc - mine;
@@ -299,7 +300,7 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
     const uint32_t c = (blockIdx.x % 8u) * (kGrid / 8u) + blockIdx.x / 8u;
     const uint32_t H = p.a.n_heads, L = p.a.cache.kv_lora_rank, RP = p.a.cache.qk_rope;
     if (tid == 0) bad_page = again = 0;
-    const Place f = find_place<ROWS, 64 * NW>(p, c, min_per, tmp, &found);
+    const Place f = find_place<ROWS, 64 * NW, kGrid>(p, c, min_per, tmp, &found);
     if (tid < 2) p.desc[8 * (2 * c + tid)] = 0;
     Walks<ROWS> walks(p, f, c);
     if (!walks.more()) return;
@@ -630,18 +631,18 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
 }
 
 // Joins the parts of split row tiles: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s
-// - M) l_s. Each part's writer (slot blockIdx.x) has four work-groups here that
+// - M) l_s. Each part's writer (slot blockIdx.x) has Z work-groups here that
 // join its share of the tile's rows, so the parts are read by as many CUs as
 // wrote them. The tile's parts are listed first, a thread per chunk of its keys.
 // Of few parts a wave joins a row by itself; many are dealt out to the four
 // waves, a quarter each, and their sums added in order. Lane: columns 4 lane + 256 k.
-constexpr uint32_t kJoinZ = 4, kManyParts = 16;
-template <int ROWS, int LC, bool OBF>
+constexpr uint32_t kManyParts = 16;
+template <uint32_t GRID, int ROWS, int LC, bool OBF>
 __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
-    constexpr uint32_t COLS = 128 * LC, NV = (COLS + 255) / 256;
+    constexpr uint32_t COLS = 128 * LC, NV = (COLS + 255) / 256, Z = 1024 / GRID;
     __shared__ f32x4 sums[4][NV][64];
-    __shared__ float weight[4][2 * kGrid];
-    __shared__ uint32_t count[4], list[2 * kGrid];
+    __shared__ float weight[4][2 * GRID];
+    __shared__ uint32_t count[4], list[2 * GRID];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = uni(tid >> 6), mine = blockIdx.x;
     const uint32_t* desc = p.desc + 8 * mine;
     if (desc[0] == 0) return;
@@ -650,26 +651,36 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
     const uint32_t rt = desc[1], H = p.a.n_heads, L = p.a.cache.kv_lora_rank;
     const uint64_t base = *(const uint64_t*)(desc + 2), per = *(const uint64_t*)(desc + 4);
     {
+        constexpr uint32_t C = GRID / 256;  // chunks of a thread
         const uint32_t nc = chunks(q, per);
-        uint64_t start = 0;
-        uint32_t w0 = 0, nw = 0;
-        if (tid < nc) {
-            const uint32_t ka = chunk_at(q, nc, tid), kb = chunk_at(q, nc, tid + 1);
-            start = base + (uint64_t)q.nrt * ka + (uint64_t)rt * (kb - ka);
-            w0 = (uint32_t)div64(start, per);
-            nw = (uint32_t)div64(start + (kb - ka) - 1, per) - w0 + 1u;
+        uint64_t start[C];
+        uint32_t w0[C], nw[C], all = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < C; i++) {
+            const uint32_t ch = C * tid + i;
+            start[i] = 0;
+            w0[i] = nw[i] = 0;
+            if (ch < nc) {
+                const uint32_t ka = chunk_at(q, nc, ch), kb = chunk_at(q, nc, ch + 1);
+                start[i] = base + (uint64_t)q.nrt * ka + (uint64_t)rt * (kb - ka);
+                w0[i] = (uint32_t)div64(start[i], per);
+                nw[i] = (uint32_t)div64(start[i] + (kb - ka) - 1, per) - w0[i] + 1u;
+            }
+            all += nw[i];
         }
-        uint32_t inc = nw;
+        uint32_t inc = all;
         for (uint32_t o = 1; o < 64; o <<= 1) {
             const uint32_t v = __shfl_up(inc, o, 64);
             if (lane >= o) inc += v;
         }
         if (lane == 63) count[wv] = inc;
         __syncthreads();
-        uint32_t at = inc - nw;
+        uint32_t at = inc - all;
         for (uint32_t w = 0; w < wv; w++) at += count[w];
-        for (uint32_t i = 0; i < nw; i++)  // a work-group's first walk has its even slot
-            list[at + i] = 2u * (w0 + i) + (start <= (w0 + i) * per ? 0u : 1u);
+#pragma unroll
+        for (uint32_t i = 0; i < C; i++)
+            for (uint32_t k = 0; k < nw[i]; k++)  // a work-group's first walk has its even slot
+                list[at++] = 2u * (w0[i] + k) + (start[i] <= (w0[i] + k) * per ? 0u : 1u);
         __syncthreads();
     }
     const uint32_t S = count[0] + count[1] + count[2] + count[3];
@@ -681,7 +692,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
     const uint32_t all = q.nodes * H - rt * ROWS, rows = all < ROWS ? all : ROWS;
     const bool many = S >= kManyParts;
     const uint32_t r0 = rows * idx / S, r1 = rows * (idx + 1u) / S;
-    for (uint32_t lr = r0 + (many ? blockIdx.y : 4u * blockIdx.y + wv); lr < r1; lr += many ? kJoinZ : 4u * kJoinZ) {
+    for (uint32_t lr = r0 + (many ? blockIdx.y : 4u * blockIdx.y + wv); lr < r1; lr += many ? Z : 4u * Z) {
         auto at = [&](uint32_t s) { return (size_t)list[s] * ROWS + lr; };
         f32x4 y[NV];
 #pragma unroll
@@ -754,15 +765,29 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
 // ---- 32-bit queries -------------------------------------------------------------
 // A 32-bit value is the sum of three bf16 ones (its leading 8 bits, the next 8, the
 // last 8: cut off, not rounded, so each remainder is exact), and a product of two
-// such sums is, but for terms below 2^-24 of it, the six products of parts whose
-// places add up to two at most (three of them where the other side is bf16 itself):
-// exact products in the matrix cores, summed in f32. 32 rows against 32 keys at a
-// time, four waves, split as in the 16-bit kernel; queries, weights and (WIDE)
-// cache rows in three parts each. One wave a SIMD: its 512 registers hold 16 rows'
-// queries (216), the sums (64) and the next tile (36, WIDE 72), which is read while
-// this one is worked on and then cut up into LDS. The products of the leading parts
-// and those of the others are summed apart in the scores.
-// Bound by the matrix cores: 102 (WIDE 204) MFMAs a wave and tile, 16 clocks each.
+// such sums is, but for terms below 2^-24 of it, the six products of parts h, m, l
+// whose places add up to two at most (three of them where the other side is bf16
+// itself): exact products in the matrix cores, summed in f32, the scores' leading
+// ones apart from the others.
+//
+// 32 rows against 32 keys (WIDE, a cache of 32-bit rows: 16) at a time, four waves.
+// The next tile's rows are read into registers while this one is worked on, then cut
+// up into LDS. Scores: a wave has 16 rows' queries, half of their columns, and adds
+// its sums to those of the wave with the other half, so a row's three parts take 108
+// registers; with the sums (64) and the next rows (36) that is what two work-groups a
+// CU leave a wave. They are what overlaps: one's products run while the other cuts,
+// takes exponentials or waits. (All columns in one wave and one work-group a CU,
+// first: one request of 64 nodes x 64 heads over 8192 keys 278 us, 5 requests of 7
+// nodes over up to 2000 32-bit rows 75 us; so, 242 and 58 us.) Values: 16 columns of
+// all rows at once. Of 16 keys, the 32 places of a product hold two parts of each:
+// (h, m) against the weights' (h, h) and (m, m), (h, l) against (l, h).
+// Lane addresses are computed where they are used (afresh): held, they spill.
+//
+// Bound by the matrix cores: 102 (WIDE 102 of 16 keys) products a wave and tile, 16
+// clocks each. The 64 nodes' 73 GFLOP, three products each, take 181 us at the rate
+// of a large library product (1211 TFLOP/s), 242 us and 18 us of joining here, 11 us
+// of them for the queries' reads at the start. Reading the next rows a piece at a
+// time between the scores' products made no difference (243 us).
 WL_DEV void cut3(float x, float& h, float& m, float& l) {  // h + m + l = x, each with its low 16 bits clear
     h = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
     const float r = x - h;
@@ -773,24 +798,34 @@ WL_DEV void cut3(float x, float& h, float& m, float& l) {  // h + m + l = x, eac
 WL_DEV uint32_t high2(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
 WL_DEV bool nonfinite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
+// x, of which nothing is computed ahead of this place: what is derived from it holds
+// no register before, over all the rest of the kernel.
+WL_DEV uint32_t afresh(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 template <int LC, bool WIDE>
-__global__ __launch_bounds__(256) void tree_f32_kernel(Tree p, uint32_t min_per) {
-    constexpr uint32_t ROWS = 32, PITCH = 256 * LC + kPad, NL = 4 * LC, NS = NL + 2, CT = 2 * LC, DR = 8, NP = WIDE ? 3 : 1;
-    constexpr uint32_t ROT = kKT * PITCH, PIECE = ROT + kKT * 128, ES = WIDE ? 4 : 2;
+__global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_per) {
+    constexpr uint32_t ROWS = 32, KT = WIDE ? 16 : 32, PITCH = 256 * LC + kPad, NL = 4 * LC, NH = NL / 2 + 1, CT = 2 * LC;
+    constexpr uint32_t DR = KT / 4, NK = KT / 8, NP = WIDE ? 3 : 1, ROT = KT * PITCH, PIECE = ROT + KT * 128, ES = WIDE ? 4 : 2;
     __shared__ __align__(1024) uint8_t tile[NP * PIECE];
-    __shared__ __align__(1024) uint8_t pb[3 * ROWS * 64];  // weights [part][row][32 keys]
+    __shared__ __align__(1024) uint8_t pb[3 * ROWS * 64];  // weights [operand][row][32 places]
+    __shared__ __align__(16) float other[4][64][NK];     // scores over half of the columns, for the wave of the others
     __shared__ float rowred[2][ROWS];
     __shared__ uint64_t seen[ROWS];
-    __shared__ uint32_t flaws[kKT / 4];
+    __shared__ uint32_t flaws[KT / 4];
     __shared__ uint32_t bad_page, again;
     __shared__ uint64_t tmp[6];
     __shared__ Req found;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uni(tid >> 6), n = lane & 15u, g = lane >> 4;
-    const uint32_t sr = 8u * (wave & ~1u), sk = 16u * (wave & 1u);  // first row and key of this wave's scores
-    const uint32_t c = (blockIdx.x % 8u) * (kGrid / 8u) + blockIdx.x / 8u;
+    const uint32_t tid = threadIdx.x, wave = uni(tid >> 6);
+    // the wave's scores: rows sr + n, over the 32-column slices NH hf .. of all of the
+    // tile's keys; it ends up with half of those keys
+    const uint32_t sr = 8u * (wave & ~1u), hf = wave & 1u;
+    const uint32_t c = (blockIdx.x % 8u) * (kGridF32 / 8u) + blockIdx.x / 8u;
     const uint32_t H = p.a.n_heads, L = p.a.cache.kv_lora_rank, RP = p.a.cache.qk_rope;
     if (tid == 0) bad_page = again = 0;
-    const Place f = find_place<ROWS, 256>(p, c, min_per, tmp, &found);
+    const Place f = find_place<ROWS, 256, kGridF32>(p, c, min_per, tmp, &found);
     if (tid < 2) p.desc[8 * (2 * c + tid)] = 0;
     Walks<ROWS> walks(p, f, c);
     if (!walks.more()) return;
@@ -812,24 +847,35 @@ __global__ __launch_bounds__(256) void tree_f32_kernel(Tree p, uint32_t min_per)
         if (q.flaw) {
             clear();
         } else {
-            // the wave's 8 rows of a tile, in registers: chunk i 64 + lane of their latent
+            // the wave's DR rows of a tile, in registers: chunk i 64 + lane of their latent
             // parts (EL to a row), then of their rotary ones (ER)
             constexpr uint32_t EL = 8 * ES * LC, NLAT = DR * EL / 64, ER = 4 * ES, NROT = DR * ER / 64;
             const uint32_t stride = ES * p.a.cache.row_stride;
             u32x4 raw[NLAT + NROT];
+            auto page_of = [&](uint32_t t) __attribute__((always_inline)) {  // of its rows in tile t (pages have at least 8)
+                const uint32_t key = t * KT + DR * wave;
+                return p.a.d_table[(size_t)w.r * p.a.max_pages + ((key < q.keys ? key : q.keys - 1u) >> p.psh)];
+            };
+            int32_t next_page;  // of the next tile to read
             auto read_tile = [&](uint32_t t) __attribute__((always_inline)) {
-                const int32_t page = (int32_t)uni((uint32_t)walks.page(w, t, DR * wave));
-                const uint32_t key = t * kKT + DR * wave;
+                const uint32_t lane = afresh(tid) & 63u;
+                const int32_t page = (int32_t)uni((uint32_t)next_page);
+                const uint32_t key = t * KT + DR * wave;
                 const uint32_t left = key < q.keys ? (q.keys - key < DR ? q.keys - key : DR) : 0u;
                 const bool ok = page >= 0 && (uint32_t)page < p.a.cache.n_pages;
                 bad |= left && !ok;
                 const uint32_t row = ok ? ((uint32_t)page << p.psh) + (key & (p.a.cache.page_size - 1u)) : 0u;
                 const rsrc_t rs = make_rsrc((const uint8_t*)p.a.cache.d_rows + (uint64_t)row * stride,
                                             ok && left ? (left - 1u) * stride + ES * (L + RP) : 0u);
+                next_page = page_of(t + 1);
 #pragma unroll
                 for (uint32_t i = 0; i < NLAT; i++) {
                     const uint32_t e = 64u * i + lane, k = e % EL;
-                    raw[i] = bld16(rs, 16u * k < ES * L ? (e / EL) * stride + 16u * k : kOOB, 0);
+                    // row j of whole chunks in the scalar offset (the first one's again for those
+                    // behind the last key, which no row of scores sees), not in address registers
+                    const uint32_t j = i / (EL < 64 ? 1 : EL / 64);
+                    if (EL < 64) raw[i] = bld16(rs, 16u * k < ES * L ? (e / EL) * stride + 16u * k : kOOB, 0);
+                    else raw[i] = bld16(rs, 16u * k < ES * L ? 16u * k : kOOB, j < left ? j * stride : 0u);
                 }
 #pragma unroll
                 for (uint32_t i = 0; i < NROT; i++) {
@@ -837,10 +883,11 @@ __global__ __launch_bounds__(256) void tree_f32_kernel(Tree p, uint32_t min_per)
                     raw[NLAT + i] = bld16(rs, 16u * k < ES * RP ? (e / ER) * stride + ES * L + 16u * k : kOOB, 0);
                 }
             };
-            auto has_nodes = [&](uint32_t t) { return (t + 1) * kKT > q.len; };  // tree nodes, or the end, in tile t
+            auto has_nodes = [&](uint32_t t) { return (t + 1) * KT > q.len; };  // tree nodes, or the end, in tile t
             // into LDS, in parts; of rows of nodes what is not finite is noted and cleared
             // (their scores will be NaN for those that see them)
             auto stage = [&](uint32_t t) __attribute__((always_inline)) {
+                const uint32_t lane = afresh(tid) & 63u;
                 auto put = [&](u32x4 x, uint32_t at) {
                     if (WIDE) {
                         float h[4], md[4], lo[4];
@@ -864,7 +911,7 @@ __global__ __launch_bounds__(256) void tree_f32_kernel(Tree p, uint32_t min_per)
                         } else {
                             nf = has_nonfinite(raw[i]);
                         }
-                        if (nf && t * kKT + row >= q.len) {
+                        if (nf && t * KT + row >= q.len) {
                             ((uint8_t*)flaws)[row] = 1;
                             raw[i] = u32x4{0u, 0u, 0u, 0u};
                         }
@@ -878,134 +925,191 @@ __global__ __launch_bounds__(256) void tree_f32_kernel(Tree p, uint32_t min_per)
                     put(raw[i], lat ? row * PITCH + b : ROT + row * 128u + (b ^ (16u * swz8(row & 15u))));
                 }
             };
-            // the queries of rows sr + n, in parts, in the operand's layout: lane (row n, k group g)
-            bf16x8 qf[3][NS];
+            // the queries of rows sr + n, in parts, in the operand's layout: lane (row n, k group g);
+            // slice s of the row's 2 NH: of the latent part's 32 columns each, and the rotary one's last two
+            bf16x8 qf[3][NH];
             auto read_queries = [&]() __attribute__((always_inline)) {
                 const rsrc_t ql = make_rsrc((const float*)p.a.d_q_lat + q.t0 * p.a.q_lat_stride,
                                             4u * ((q.nodes - 1u) * (uint32_t)p.a.q_lat_stride + H * L));
                 const rsrc_t qr = make_rsrc((const float*)p.a.d_q_rope + q.t0 * p.a.q_rope_stride,
                                             4u * ((q.nodes - 1u) * (uint32_t)p.a.q_rope_stride + H * RP));
-                const uint32_t lr = sr + n, row = w.rt * ROWS + lr, node = row / H, h = row - node * H;
+                const uint32_t ln = afresh(tid) & 63u, g = ln >> 4;
+                const uint32_t lr = sr + (ln & 15u), row = w.rt * ROWS + lr, node = row / H, h = row - node * H;
                 const bool live = lr < rows;
-                const uint32_t vl = live ? 4u * (node * (uint32_t)p.a.q_lat_stride + h * L + 8u * g) : kOOB;
-                const uint32_t vr = live ? 4u * (node * (uint32_t)p.a.q_rope_stride + h * RP + 8u * g) : kOOB;
+                const uint32_t vl = 4u * (node * (uint32_t)p.a.q_lat_stride + h * L);
+                const uint32_t vr = 4u * (node * (uint32_t)p.a.q_rope_stride + h * RP);
+                u32x4 x[NH][2];
 #pragma unroll
-                for (uint32_t s = 0; s < NS; s++) {
-                    u32x4 x[2];
+                for (uint32_t i = 0; i < NH; i++) {
+                    const bool rot = i + 1 == NH;  // the last of each half is a rotary one
+                    const uint32_t col = 32u * (rot ? hf : (NH - 1u) * hf + i) + 8u * g;
+                    const uint32_t at = live && col < (rot ? RP : L) ? (rot ? vr : vl) + 4u * col : kOOB;
 #pragma unroll
-                    for (uint32_t k = 0; k < 2; k++) {
-                        x[k] = s < NL ? bld16(ql, vl + 128u * s + 16u * k, 0) : bld16(qr, vr + 128u * (s - NL) + 16u * k, 0);
-                        if (32u * (s < NL ? s : s - NL) + 8u * g >= (s < NL ? L : RP)) x[k] = u32x4{0u, 0u, 0u, 0u};
-                    }
+                    for (uint32_t k = 0; k < 2; k++) x[i][k] = bld16(rot ? qr : ql, at, 16u * k);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < NH; i++) {
                     u32x4 part[3];
 #pragma unroll
                     for (uint32_t k = 0; k < 4; k++) {
                         float a[3], b[3];
-                        cut3(__uint_as_float(x[k >> 1][2 * (k & 1)]), a[0], a[1], a[2]);
-                        cut3(__uint_as_float(x[k >> 1][2 * (k & 1) + 1]), b[0], b[1], b[2]);
+                        cut3(__uint_as_float(x[i][k >> 1][2 * (k & 1)]), a[0], a[1], a[2]);
+                        cut3(__uint_as_float(x[i][k >> 1][2 * (k & 1) + 1]), b[0], b[1], b[2]);
 #pragma unroll
                         for (int j = 0; j < 3; j++) part[j][k] = high2(a[j], b[j]);
                     }
 #pragma unroll
-                    for (int j = 0; j < 3; j++) qf[j][s] = as_bf16x8(part[j]);
+                    for (int j = 0; j < 3; j++) qf[j][i] = as_bf16x8(part[j]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                if (sk == 0 && g == 0) {
+                if (hf == 0 && g == 0) {
                     const uint32_t nd = live ? node : 0u;
                     seen[lr] = p.a.d_mask ? p.a.d_mask[q.t0 + nd] : (2ull << nd) - 1ull;
                 }
             };
-            const uint32_t key_at = (sk + n) * PITCH + 16u * g, key_rot = (sk + n) * 128u + 16u * (g ^ swz8(n));
-            auto kread = [&](uint32_t s, uint32_t piece) {
-                const uint8_t* b = tile + PIECE * piece;
-                return as_bf16x8(s < NL ? *(const u32x4*)(b + key_at + 64u * s) : *(const u32x4*)(b + ROT + (key_rot ^ (64u * (s - NL)))));
+            // the scores in powers of two of row sr + n with keys own_keys(g) + k, -inf where unseen
+            constexpr uint32_t NB = KT / 16;
+            auto own_keys = [&](uint32_t g) { return WIDE ? 4u * g + 2u * hf : 16u * hf + 4u * g; };
+            struct Sc {
+                float v[NK];
             };
-            // the scores in powers of two of row sr + n with keys sk + 4 g + j, -inf where unseen
             auto scores = [&](uint32_t t) __attribute__((always_inline)) {
-                f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
-                bf16x8 kf[2][NP];
+                const uint32_t lane = afresh(tid) & 63u, n = lane & 15u, g = lane >> 4;
+                const uint32_t key_at = n * PITCH + 64u * (NH - 1u) * hf + 16u * g, key_rot = ROT + n * 128u + ((16u * (g ^ swz8(n))) ^ (64u * hf));
+                auto kread = [&](uint32_t i, uint32_t piece, uint32_t block) __attribute__((always_inline)) {
+                    return as_bf16x8(i + 1 < NH ? *(const u32x4*)(tile + PIECE * piece + 16u * block * PITCH + key_at + 64u * i)
+                                                : *(const u32x4*)(tile + PIECE * piece + 2048u * block + key_rot));
+                };
+                const uint32_t own = own_keys(g);
+                f32x4 s0[NB], s1[NB];
 #pragma unroll
-                for (uint32_t j = 0; j < NP; j++) kf[0][j] = kread(0, j);
+                for (uint32_t b = 0; b < NB; b++) s0[b] = s1[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+                bf16x8 kf[2][NB][NP];
+                auto kread_all = [&](uint32_t i) __attribute__((always_inline)) {
 #pragma unroll
-                for (uint32_t s = 0; s < NS; s++) {
-                    const uint32_t b = s & 1u;
-                    if (s + 1 < NS) {
+                    for (uint32_t b = 0; b < NB; b++)
 #pragma unroll
-                        for (uint32_t j = 0; j < NP; j++) kf[b ^ 1u][j] = kread(s + 1, j);
+                        for (uint32_t j = 0; j < NP; j++) kf[i & 1u][b][j] = kread(i, j, b);
+                };
+                kread_all(0);
+#pragma unroll
+                for (uint32_t i = 0; i < NH; i++) {
+                    if (i + 1 < NH) kread_all(i + 1);
+#pragma unroll
+                    for (uint32_t k = 0; k < (WIDE ? 6 : 3); k++) {
+#pragma unroll
+                        for (uint32_t b = 0; b < NB; b++) {
+                            const bf16x8* kp = kf[i & 1u][b];
+                            // h h apart; then h l, (l h, m m, m h,) h m
+                            if (k == 0) s0[b] = mma(kp[0], qf[0][i], s0[b]);
+                            else if (k == 1) s1[b] = mma(kp[0], qf[2][i], s1[b]);
+                            else if (k == (WIDE ? 5 : 2)) s1[b] = mma(kp[0], qf[1][i], s1[b]);
+                            else if (k == 2) s1[b] = mma(kp[NP - 1], qf[0][i], s1[b]);
+                            else s1[b] = mma(kp[NP > 1 ? 1 : 0], qf[k == 3 ? 1 : 0][i], s1[b]);
+                        }
                     }
-                    s0 = mma(kf[b][0], qf[0][s], s0);
-                    s1 = mma(kf[b][0], qf[2][s], s1);
-                    if (WIDE) {
-                        s1 = mma(kf[b][NP - 1], qf[0][s], s1);
-                        s1 = mma(kf[b][NP > 1 ? 1 : 0], qf[1][s], s1);
-                        s1 = mma(kf[b][NP > 1 ? 1 : 0], qf[0][s], s1);
-                    }
-                    s1 = mma(kf[b][0], qf[1][s], s1);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                f32x4 sc;
+                Sc sc;
+                if (WIDE) {
+                    const f32x4 y = s0[0] + s1[0];
 #pragma unroll
-                for (int k = 0; k < 4; k++) sc[k] = (s0[k] + s1[k]) * p.scale2;
+                    for (uint32_t k = 0; k < NK; k++) {
+                        sc.v[k] = hf ? y[2 + k] : y[k];
+                        other[wave][lane][k] = hf ? y[k] : y[2 + k];
+                    }
+                } else {
+                    const f32x4 a = s0[0] + s1[0], b = s0[NB - 1] + s1[NB - 1];
+#pragma unroll
+                    for (uint32_t k = 0; k < NK; k++) {
+                        sc.v[k] = hf ? b[k] : a[k];
+                        other[wave][lane][k] = hf ? a[k] : b[k];
+                    }
+                }
+                ring_barrier();
+#pragma unroll
+                for (uint32_t k = 0; k < NK; k++) sc.v[k] = (sc.v[k] + other[wave ^ 1u][lane][k]) * p.scale2;
                 if (has_nodes(t)) {
-                    const uint32_t fl = flaws[sk / 4u + g];
                     const uint64_t bits = seen[sr + n];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t key = t * kKT + sk + 4u * g + k;
+                    for (uint32_t k = 0; k < NK; k++) {
+                        const uint32_t key = t * KT + own + k;
                         const uint32_t bit = (uint32_t)(bits >> ((key - q.len) & 63u)) & (key < q.keys ? 1u : 0u);
-                        const float nan = (fl >> (8 * k)) & 1u ? __builtin_nanf("") : 0.f;
-                        sc[k] = (bit | (key < q.len ? 1u : 0u)) ? sc[k] + nan : -INFINITY;
+                        const float nan = ((const uint8_t*)flaws)[own + k] ? __builtin_nanf("") : 0.f;
+                        sc.v[k] = (bit | (key < q.len ? 1u : 0u)) ? sc.v[k] + nan : -INFINITY;
                     }
                 }
                 return sc;
             };
-            auto largest = [&](f32x4 x) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); };
+            auto largest = [&](const Sc& x) {
+                return WIDE ? fmaxf(x.v[0], x.v[1]) : fmaxf(fmaxf(x.v[0], x.v[1]), fmaxf(x.v[NK - 2], x.v[NK - 1]));
+            };
             auto share_maxima = [&](float x) {
+                const uint32_t lane = afresh(tid) & 63u, n = lane & 15u, g = lane >> 4;
                 x = fmaxf(x, __shfl_xor(x, 16, 64));
                 x = fmaxf(x, __shfl_xor(x, 32, 64));
                 if (g == 0) rowred[wave & 1u][sr + n] = x;
                 ring_barrier();
                 m = fmaxf(kNone, fmaxf(rowred[0][sr + n], rowred[1][sr + n]));
             };
-            const uint32_t value_at = (4u * g + ((lane & 15u) >> 2)) * PITCH + 64u * LC * wave + 8u * (lane & 3u);
-            auto vread = [&](uint32_t k, uint32_t piece) {
-                const uint8_t* pa = tile + PIECE * piece + value_at + 32u * k;
+            // 16 columns' values against 32 places of the weights: of KT = 32 keys, or of 16
+            // keys in their first part and in part j
+            auto vread = [&](uint32_t value_at, uint32_t k, uint32_t j) __attribute__((always_inline)) {
+                const uint8_t* pa = tile + value_at + 32u * k;
                 typedef __attribute__((address_space(3))) s16x4 l_s16x4;
                 const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa));
-                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa + 16 * PITCH));
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa + (WIDE ? j * PIECE : 16 * PITCH)));
                 const u32x2 xx = __builtin_bit_cast(u32x2, x), yy = __builtin_bit_cast(u32x2, y);
                 return as_bf16x8(u32x4{xx[0], xx[1], yy[0], yy[1]});
             };
-            const uint32_t put_at = (sr + n) * 64u + 16u * (g ^ swz4(n)) + sk / 2u, get_at = n * 64u + 16u * (g ^ swz4(n));
+            // the weights e of row sr + n in places: parts h, m, l against 32 keys; or
+            // against a key's value parts (h, m): h h and m m; against its (h, l): l h
+            auto put_weights = [&](uint32_t put_at, const float (&e)[3][NK]) __attribute__((always_inline)) {
+#pragma unroll
+                for (uint32_t j = 0; j < 3; j++) {
+                    uint8_t* o = pb + j * ROWS * 64u + put_at;
+                    if (WIDE) {
+                        *(uint32_t*)(o + 4u * hf) = high2(e[j][0], e[j][1]);
+                        *(uint32_t*)(o + 4u * hf + 8u) = j < 2 ? high2(e[j][0], e[j][1]) : high2(e[0][0], e[0][1]);
+                    } else {
+                        *(u32x2*)(o + 8u * hf) = u32x2{high2(e[j][0], e[j][1]), high2(e[j][NK - 2], e[j][NK - 1])};
+                    }
+                }
+            };
             bool pass = false;
             // a walk; SUMS false: over the scores alone, for their maxima
             auto go = [&](bool known, auto sums) __attribute__((always_inline)) {
                 constexpr bool SUMS = decltype(sums)::value;
                 float x = kNone;
-                read_tile(kt0);
+                const uint32_t t0 = kt0 * (kKT / KT), t1 = kt1 * (kKT / KT);
+                next_page = page_of(t0);
+                read_tile(t0);
                 if (SUMS && !known) read_queries();
-                for (uint32_t t = kt0; t < kt1; t++) {
+                if (SUMS) clear();
+                for (uint32_t t = t0; t < t1; t++) {
                     if (has_nodes(t)) {
-                        if (tid < kKT / 4) flaws[tid] = 0;
+                        if (const uint32_t i = afresh(tid); i < KT / 4) flaws[i] = 0;
                         ring_barrier();
                     }
                     stage(t);
                     ring_barrier();
-                    if (t + 1 < kt1) read_tile(t + 1);
-                    const f32x4 sc = scores(t);
+                    const Sc sc = scores(t);
+                    if (t + 1 < t1) read_tile(t + 1);
                     if (SUMS) {
-                        if (t == kt0 && !known) share_maxima(largest(sc));
-                        float e[3][4], top = 0.f;
+                        if (t == t0 && !known) share_maxima(largest(sc));
+                        float e[3][NK], top = 0.f;
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const float v = exp2_(sc[k] - m);
+                        for (uint32_t k = 0; k < NK; k++) {
+                            const float v = exp2_(sc.v[k] - m);
                             l += v;
                             top = fmaxf(top, v);
                             cut3(v, e[0][k], e[1][k], e[2][k]);
                         }
                         pass |= top > kMost;
-#pragma unroll
-                        for (uint32_t j = 0; j < 3; j++)
-                            *(u32x2*)(pb + j * ROWS * 64u + put_at) = u32x2{high2(e[j][0], e[j][1]), high2(e[j][2], e[j][3])};
+                        const uint32_t lane = afresh(tid) & 63u, n = lane & 15u, g = lane >> 4;
+                        const uint32_t put_at = (sr + n) * 64u + 16u * (g ^ swz4(n)), get_at = n * 64u + 16u * (g ^ swz4(n));
+                        const uint32_t value_at = (4u * g + (n >> 2)) * PITCH + 64u * LC * wave + 8u * (n & 3u);
+                        put_weights(put_at, e);
                         ring_barrier();
                         bf16x8 pf[3][2];
 #pragma unroll
@@ -1013,28 +1117,22 @@ __global__ __launch_bounds__(256) void tree_f32_kernel(Tree p, uint32_t min_per)
 #pragma unroll
                             for (int i = 0; i < 2; i++)
                                 pf[j][i] = as_bf16x8(*(const u32x4*)(pb + j * ROWS * 64u + get_at + 1024u * i));
-                        bf16x8 vf[2][NP];
-#pragma unroll
-                        for (uint32_t j = 0; j < NP; j++) vf[0][j] = vread(0, j);
+                        bf16x8 va[2], vb[2];
+                        auto vread_all = [&](uint32_t v) __attribute__((always_inline)) {
+                            va[v & 1u] = vread(value_at, v, 1);
+                            vb[v & 1u] = WIDE ? vread(value_at, v, 2) : va[v & 1u];
+                        };
+                        vread_all(0);
 #pragma unroll
                         for (uint32_t v = 0; v < CT; v++) {
-                            const uint32_t b = v & 1u;
-                            if (v + 1 < CT) {
+                            if (v + 1 < CT) vread_all(v + 1);
+                            f32x4 y[2];
 #pragma unroll
-                                for (uint32_t j = 0; j < NP; j++) vf[b ^ 1u][j] = vread(v + 1, j);
-                            }
+                            for (int i = 0; i < 2; i++) y[i] = mma(vb[v & 1u], pf[2][i], acc[i][v]);
 #pragma unroll
-                            for (int i = 0; i < 2; i++) {
-                                f32x4 y = acc[i][v];
-                                if (WIDE) {
-                                    y = mma(vf[b][NP - 1], pf[0][i], y);
-                                    y = mma(vf[b][NP > 1 ? 1 : 0], pf[1][i], y);
-                                    y = mma(vf[b][NP > 1 ? 1 : 0], pf[0][i], y);
-                                }
-                                y = mma(vf[b][0], pf[2][i], y);
-                                y = mma(vf[b][0], pf[1][i], y);
-                                acc[i][v] = mma(vf[b][0], pf[0][i], y);
-                            }
+                            for (int i = 0; i < 2; i++) y[i] = mma(va[v & 1u], pf[1][i], y[i]);
+#pragma unroll
+                            for (int i = 0; i < 2; i++) acc[i][v] = mma(va[v & 1u], pf[0][i], y[i]);
                             __builtin_amdgcn_sched_barrier(0);
                         }
                     } else {
@@ -1046,29 +1144,28 @@ __global__ __launch_bounds__(256) void tree_f32_kernel(Tree p, uint32_t min_per)
             };
             using Sums = std::integral_constant<bool, true>;
             using Maxima = std::integral_constant<bool, false>;
-            clear();
             go(false, Sums{});
-            if (__ballot(pass) && lane == 0) again = 1u;
+            if (__ballot(pass) && (tid & 63u) == 0) again = 1u;
             ring_barrier();
             const bool redo = again != 0;
             ring_barrier();
             if (redo) {
                 if (tid == 0) again = 0u;
                 share_maxima(go(true, Maxima{}));
-                clear();
                 go(true, Sums{});
             }
         }
-        if (__ballot(bad) && lane == 0) {
+        if (__ballot(bad) && (tid & 63u) == 0) {
             bad_page = 1u;
             if (p.a.d_status)
                 __hip_atomic_fetch_or(p.a.d_status, WL_PAGED_E_PAGE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
+        const uint32_t lane = afresh(tid) & 63u, n = lane & 15u, g = lane >> 4;
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         if (g == 0) rowred[wave & 1u][sr + n] = l;
         const bool whole = kt1 - kt0 == q.nkt;
-        if (!whole && sk == 0 && g == 0) p.part_ml[2u * (w.slot * ROWS + sr + n)] = m;
+        if (!whole && hf == 0 && g == 0) p.part_ml[2u * (w.slot * ROWS + sr + n)] = m;
         ring_barrier();
         const bool nan = bad_page != 0 || q.flaw;
 #pragma unroll
@@ -1100,8 +1197,8 @@ uint32_t row_class(const wl_tree_attn& a) {  // rows of a work-group's block
 }
 
 size_t tree_scratch(const wl_tree_attn& a) {
-    const size_t rows = 2 * kGrid * 64;
-    return rows * (128 * lat_class(a) + 2) * 4 + 2 * kGrid * 32;
+    const size_t rows = a.dtype == WL_TYPE_BF16 ? 2 * kGrid * row_class(a) : 2 * kGridF32 * 32;  // of parts
+    return rows * (128 * lat_class(a) + 2) * 4 + 2 * kGridF32 * 32;
 }
 
 template <int GR, int LC>
@@ -1109,16 +1206,16 @@ int run_bf16(const Tree& p, hipStream_t st) {
     hipLaunchKernelGGL((tree_bf16_kernel<GR, LC>), dim3(kGrid), dim3(256 * GR), 0, st, p, kMinPer);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL((tree_join_kernel<32 * GR, LC, true>), dim3(2 * kGrid, kJoinZ), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((tree_join_kernel<kGrid, 32 * GR, LC, true>), dim3(2 * kGrid, 4), dim3(256), 0, st, p);
     return (int)hipGetLastError();
 }
 
 template <int LC, bool WIDE>
 int run_f32(const Tree& p, hipStream_t st) {
-    hipLaunchKernelGGL((tree_f32_kernel<LC, WIDE>), dim3(kGrid), dim3(256), 0, st, p, kMinPer);
+    hipLaunchKernelGGL((tree_f32_kernel<LC, WIDE>), dim3(kGridF32), dim3(256), 0, st, p, kMinPer);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL((tree_join_kernel<32, LC, false>), dim3(2 * kGrid, kJoinZ), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((tree_join_kernel<kGridF32, 32, LC, false>), dim3(2 * kGridF32, 2), dim3(256), 0, st, p);
     return (int)hipGetLastError();
 }
 
@@ -1130,8 +1227,9 @@ int launch_tree(const wl_tree_attn& a, void* stream) {
     p.scale2 = a.scale * 1.44269504088896340736f;
     const uint32_t lc = lat_class(a), rows = row_class(a);
     p.part = (float*)a.d_scratch;
-    p.part_ml = p.part + (size_t)2 * kGrid * 64 * 128 * lc;
-    p.desc = (uint32_t*)(p.part_ml + (size_t)2 * kGrid * 64 * 2);
+    const size_t parts = a.dtype == WL_TYPE_BF16 ? 2 * kGrid * rows : 2 * kGridF32 * 32;
+    p.part_ml = p.part + parts * 128 * lc;
+    p.desc = (uint32_t*)(p.part_ml + parts * 2);
     if (a.dtype == WL_TYPE_BF16) {
         if (rows == 64) return lc == 4 ? run_bf16<2, 4>(p, st) : lc == 2 ? run_bf16<2, 2>(p, st) : run_bf16<2, 1>(p, st);
         return lc == 4 ? run_bf16<1, 4>(p, st) : lc == 2 ? run_bf16<1, 2>(p, st) : run_bf16<1, 1>(p, st);
