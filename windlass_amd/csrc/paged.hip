@@ -40,6 +40,12 @@ WL_DEV Sums shfl_up(const Sums& s, uint32_t o) {
     return r;
 }
 
+typedef __attribute__((ext_vector_type(4))) int32_t i32x4;
+// A thread takes four consecutive tokens, and looks once for their request, where
+// the step may hold that many runs of them; one token otherwise, so that a decode's
+// lookups do not queue up in a thread.
+__host__ __device__ inline bool runs_of_4(const wl_page_map& m) { return m.max_tokens >= 64u * m.n_req; }
+
 template <uint32_t THREADS, uint32_t RPT>
 __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
     constexpr uint32_t CAP = THREADS * RPT, NW = THREADS / 64;
@@ -141,8 +147,8 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
     };
     for (uint32_t j = gt; j < all.back; j += gn) m.d_free[(uint32_t)nf + j] = pushed(j);
     uint32_t flaw = 0;
-    // token i of request r: its slot; the first token of a new page writes the table's entry
-    auto place = [&](uint32_t r, uint32_t i, uint32_t t) {
+    // the slot of token i of request r; the first token of a new page writes the table's entry
+    auto place = [&](uint32_t r, uint32_t i) {
         const uint32_t row = len[r] + i, k = row >> psh;
         int32_t page;
         if (k < have[r]) {
@@ -154,7 +160,7 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
         }
         const bool ok = page >= 0 && (uint32_t)page < m.n_pages;
         if (!ok) flaw |= WL_PAGED_E_PAGE;
-        m.d_slot[t] = ok ? (int32_t)(((uint32_t)page << psh) + (row & pmask)) : -1;
+        return ok ? (int32_t)(((uint32_t)page << psh) + (row & pmask)) : -1;
     };
     if (trees) {
         for (uint32_t r = blockIdx.x * NW + wv; r < R; r += gridDim.x * NW) {
@@ -184,15 +190,45 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
                 }
             }
             if (i < a) {
-                place(r, i, t);
+                m.d_slot[t] = place(r, i);
                 if (m.d_mask) m.d_mask[t] = bits;
                 if (m.d_pos) m.d_pos[t] = (int32_t)(len[r] + depth);
+            }
+        }
+    } else if (runs_of_4(m)) {
+        const bool wide = (((uintptr_t)m.d_slot | (uintptr_t)m.d_pos) & 15u) == 0;
+        for (uint32_t t = 4u * gt; t < total; t += 4u * gn) {
+            uint32_t r = owner(cu, t);
+            int32_t slot[4], pos[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) {
+                if (t + k >= total) break;
+                uint32_t i = t + k - cu[r];
+                bool same = k > 0;
+                while (t + k >= cu[r + 1]) {  // on to its request: cu[R] is behind all of them
+                    i = t + k - cu[++r];
+                    same = false;
+                }
+                if (same && ((len[r] + i) & pmask)) slot[k] = slot[k ? k - 1 : 0] + (slot[k ? k - 1 : 0] >= 0 ? 1 : 0);
+                else slot[k] = place(r, i);
+                pos[k] = (int32_t)(len[r] + i);
+            }
+            if (wide && t + 4u <= total) {
+                *(i32x4*)(m.d_slot + t) = i32x4{slot[0], slot[1], slot[2], slot[3]};
+                if (m.d_pos) *(i32x4*)(m.d_pos + t) = i32x4{pos[0], pos[1], pos[2], pos[3]};
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < 4; k++) {
+                    if (t + k >= total) break;
+                    m.d_slot[t + k] = slot[k];
+                    if (m.d_pos) m.d_pos[t + k] = pos[k];
+                }
             }
         }
     } else {
         for (uint32_t t = gt; t < total; t += gn) {
             const uint32_t r = owner(cu, t), i = t - cu[r];
-            place(r, i, t);
+            m.d_slot[t] = place(r, i);
             if (m.d_pos) m.d_pos[t] = (int32_t)(len[r] + i);
         }
     }
@@ -349,7 +385,7 @@ int launch_map(const wl_page_map& m, void* stream) {
     // least, and no more work-groups than the chip has places for
     const uint32_t R = m.n_req;
     auto grid = [&](uint32_t threads) {
-        const uint64_t work = trees ? (uint64_t)R * 64u : m.max_tokens;
+        const uint64_t work = trees ? (uint64_t)R * 64u : runs_of_4(m) ? (m.max_tokens + 3u) / 4u : m.max_tokens;
         const uint64_t g = (work + threads - 1) / threads;
         return dim3((uint32_t)(g < 1 ? 1 : g > 512 ? 512 : g));
     };
