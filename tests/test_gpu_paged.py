@@ -78,6 +78,66 @@ def test_map_long_prompts_and_chain_masks(gpu):
     check_step(m, s)
 
 
+@pytest.mark.parametrize("shift", [0, 4])
+def test_map_long_runs(gpu, shift):
+    """More than 2^18 tokens, where a thread takes four: ends of requests inside the four,
+    requests of one and of no token, pages outside the cache, outputs that are not 16-byte aligned."""
+    adds = [70001, 0, 1, 0, 3, 130002, 64, 1, 2, 90000]
+    lens = [13, 40, 0, 16, 15, 31, 4096, 0, 7, 50]
+    have = [-(-n // 16) for n in lens]
+    need = [-(-(n + a) // 16) for n, a in zip(lens, adds)]
+    n_free = sum(need) - sum(have)
+    n_pages = sum(need) + 4
+    rng = np.random.default_rng(5)
+    pages = rng.permutation(n_pages).astype(np.int32)
+    table = np.full((10, max(need)), -9, np.int32)
+    at = n_free
+    for r, h in enumerate(have):
+        table[r, :h] = pages[at:at + h]
+        at += h
+    free = np.full(n_pages, -5, np.int32)
+    free[:n_free] = pages[:n_free]
+    free[n_free - 3] = n_pages  # the third page taken
+    s = dict(ps=16, n_pages=n_pages, max_pages=max(need), lens=lens, adds=adds, have=have, free=free, n_free=n_free,
+             table=table, parent=None)
+    m = P.Map(**s, max_tokens=sum(adds) + 7)
+    m.args.max_tokens -= shift // 4
+    m.args.d_slot += shift
+    m.args.d_pos += shift
+    paged.page_map(m.args)
+    hip.synchronize()
+    want = P.page_map(16, s["max_pages"], n_pages, lens, adds, have, free, n_free, table)
+    slot, n, o = want[5], sum(adds), shift // 4
+    slot[slot >= n_pages * 16] = -1
+    assert m.get("status")[0] == paged.E_PAGE
+    assert np.array_equal(m.get("table"), want[0]) and np.array_equal(m.get("cu"), want[4])
+    assert np.count_nonzero(slot == -1) == 16
+    assert np.array_equal(m.get("slot")[o:o + n], slot) and np.array_equal(m.get("pos")[o:o + n], want[6])
+    for x in (m.get("slot"), m.get("pos")):
+        assert np.all(x[:o] == -7) and np.all(x[o + n:] == -7)
+
+
+def test_map_many_pages_given_back(gpu):
+    """Ended requests' pages, far more of them than tokens."""
+    R, held = 40, 900
+    lens, adds = [0 if r % 3 else 100 + r for r in range(R)], [0 if r % 3 else 1 for r in range(R)]
+    have = [held - 7 * r for r in range(R)]
+    n_pages = sum(have) + 3
+    pages = np.random.default_rng(6).permutation(n_pages).astype(np.int32)
+    table, at = np.full((R, held), -9, np.int32), 3
+    for r, h in enumerate(have):
+        table[r, :h] = pages[at:at + h]
+        at += h
+    free = np.full(n_pages, -5, np.int32)
+    free[:3] = pages[:3]
+    s = dict(ps=8, n_pages=n_pages, max_pages=held, lens=lens, adds=adds, have=have, free=free, n_free=3, table=table,
+             parent=None)
+    m = P.Map(**s)
+    paged.page_map(m.args)
+    hip.synchronize()
+    check_step(m, s)
+
+
 def test_map_no_requests(gpu):
     m = P.Map(16, 4, 1, [], [], [], [0, 1, 2, 3], 4, np.zeros((0, 1), np.int32), max_tokens=2)
     paged.page_map(m.args)
@@ -224,6 +284,17 @@ class Write:
                                              (333, 256, 32, 20, 32, 8), (1030, 504, 56, 3, 8, 0)])
 def test_write(gpu, T, L, RP, H, ps, pad, x, cache):
     w = Write(T + L, T, x, cache, L, RP, H, ps, pad)
+    paged.write_rows(w.args)
+    hip.synchronize()
+    w.check()
+    assert w.status() == 0
+
+
+@pytest.mark.parametrize("x,cache", [("f32", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("T,RP,H", [(5, 64, 1), (5, 64, 9), (5, 64, 20), (1100, 64, 64), (3, 40, 1024)])
+def test_write_waves_of_a_token(gpu, T, RP, H, x, cache):
+    """One to four waves share a token's heads."""
+    w = Write(H, T, x, cache, 128, RP, H, 16, 8)
     paged.write_rows(w.args)
     hip.synchronize()
     w.check()

@@ -26,7 +26,11 @@ WL_DEV void set_status(uint32_t* status, uint32_t bits) {
 // outputs are written in the same launch: the k-th page, when it is one that
 // this step pushes, is looked up in the table it comes from, not on the stack.
 // In a call with trees a wave takes a request, lane i its node i; otherwise a
-// thread takes a token and finds its request by bisection.
+// thread takes a token, or four, and finds its request by bisection.
+// Bound by the launch and by latencies one after the other (lengths, the sums over
+// the requests, page, slot), not by bytes: 8 requests of 8 nodes 3.8 us, as an empty
+// kernel; 256 of 64 nodes 5.7 us; 1000 prompts, 690k tokens, 5.5 MB out, 10.5 us
+// (14.7 with one token a thread).
 struct Sums {
     uint64_t tok;
     uint32_t back, take;
@@ -41,10 +45,15 @@ WL_DEV Sums shfl_up(const Sums& s, uint32_t o) {
 }
 
 typedef __attribute__((ext_vector_type(4))) int32_t i32x4;
-// A thread takes four consecutive tokens, and looks once for their request, where
-// the step may hold that many runs of them; one token otherwise, so that a decode's
-// lookups do not queue up in a thread.
-__host__ __device__ inline bool runs_of_4(const wl_page_map& m) { return m.max_tokens >= 64u * m.n_req; }
+constexpr uint32_t kMapGrid = 512;  // work-groups at the most
+// A thread takes four consecutive tokens, and searches once for their request, where
+// a step holds many more of them than requests and one each would be more threads
+// than half of the chip's places; otherwise one, so that lookups do not queue up in a
+// thread. Token each / four each: 200 requests with 126k tokens 5.7 / 7.6 us, 1000
+// with 165k 8.2 / 11.3, 327k 11.9 / 11.1, 690k 14.6 / 10.9; 256 with one each 9.8 / 13.3.
+__host__ __device__ inline bool runs_of_4(const wl_page_map& m) {
+    return m.max_tokens >= 64u * m.n_req && m.max_tokens > (1u << 18);
+}
 
 template <uint32_t THREADS, uint32_t RPT>
 __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
@@ -242,6 +251,9 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
 // the angle of pair i: pos * theta^(-2 i / RP) in 64 bits, less its whole
 // turns, then sine and cosine of the rest in f32 with the rest's own rounding
 // added to first order; the other lanes take the pairs' values by permutes.
+// Bound by the bytes: 16384 bf16 tokens with 64 heads' queries, 306 MB read and
+// written in 61.4 us, 4.98 TB/s (a large copy: 5.05). 333 tokens 5.6 us, one token
+// 3.9 us, as an empty kernel.
 struct RowWrite {
     wl_row_write w;
     double inv[kMaxRope / 2];  // theta^(-2 i / qk_rope)
@@ -381,14 +393,18 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowWrite a) {
 
 int launch_map(const wl_page_map& m, void* stream) {
     const bool trees = m.d_parent || m.d_mask;
-    // a wave per request or a thread per token, four rounds of them at the
-    // least, and no more work-groups than the chip has places for
+    // a wave per request or a thread per token, and one for every page that may be
+    // given back (256 requests of which some end with 16176 pages: 4.7 us, 48 in one
+    // work-group), but no more work-groups than the chip has places for
     const uint32_t R = m.n_req;
     auto grid = [&](uint32_t threads) {
-        const uint64_t work = trees ? (uint64_t)R * 64u : runs_of_4(m) ? (m.max_tokens + 3u) / 4u : m.max_tokens;
+        uint64_t work = trees ? (uint64_t)R * 64u : runs_of_4(m) ? (m.max_tokens + 3u) / 4u : m.max_tokens;
+        if (work < m.n_pages) work = m.n_pages;
         const uint64_t g = (work + threads - 1) / threads;
         return dim3((uint32_t)(g < 1 ? 1 : g > 512 ? 512 : g));
     };
+    // a request a thread; up to 256 in small work-groups (8 requests 3.8 us, 5.1 in
+    // large ones; 200 of up to 64 tokens 5.4 and 6.5)
     hipStream_t st = (hipStream_t)stream;
     if (R <= 256) hipLaunchKernelGGL((page_map_kernel<256, 1>), grid(256), dim3(256), 0, st, m);
     else if (R <= 1024) hipLaunchKernelGGL((page_map_kernel<1024, 1>), grid(1024), dim3(1024), 0, st, m);
@@ -401,7 +417,11 @@ int launch_write(const wl_row_write& w, void* stream) {
     a.w = w;
     for (uint32_t i = 0; i < w.cache.qk_rope / 2; i++)
         a.inv[i] = 1.0 / std::pow((double)w.rope_theta, (double)(2 * i) / (double)w.cache.qk_rope);
-    a.wpt = w.n_tokens >= 1024 ? 1 : 4;
+    // a wave for every round of the heads, four at the most: more loads in flight. With
+    // one / four, 64 heads: 333 32-bit tokens 7.2 / 5.6 us, 1500 13.1 / 10.9, 8192
+    // 65 / 59; bf16 800 8.0 / 6.0, 8192 33.4 / 33.6, 16384 61.4 / 61.5
+    const uint32_t vpw = 64u / (w.cache.qk_rope / 8u), rounds = (w.n_heads + vpw - 1u) / vpw;
+    a.wpt = rounds < 1 ? 1 : rounds > 4 ? 4 : rounds;
     const uint32_t wgs = (uint32_t)(((uint64_t)w.n_tokens * a.wpt + 3) / 4);
     hipStream_t st = (hipStream_t)stream;
     if (w.dtype == WL_TYPE_BF16) hipLaunchKernelGGL(row_write_kernel<true>, dim3(wgs), dim3(256), 0, st, a);

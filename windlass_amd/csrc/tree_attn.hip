@@ -13,7 +13,8 @@ namespace {
 
 constexpr uint32_t kKT = 32;    // keys of a tile
 // Key tiles of a walk at least: a shorter one's parts cost more to join than it saves.
-// One token over 4096 keys, both launches: 32.6 us at 1, 28.6 at 2, 29.3 at 4, 32.5 at 8.
+// One token over 4096 keys, both launches: 32.3 us at 1, 28.7 at 2, 29.3 at 4, 32.0 at 8;
+// 12 requests of 5 nodes, 32-bit queries: 29.8 at 1, 29.8 at 2, 33.3 at 4, 37.1 at 6.
 constexpr uint32_t kMinPer = 2;
 constexpr uint32_t kGrid = 256;      // work-groups of a launch of the 16-bit kernel: one per CU (LDS and registers allow one)
 constexpr uint32_t kGridF32 = 512;   // of the 32-bit one: two per CU
@@ -278,6 +279,20 @@ WL_DEV constexpr uint32_t swz4(uint32_t row) { return (row & 8u) >> 2; }
 // behind the last key and columns behind the row's are read as zeros by the
 // resource's bounds. While tiles t - 1 and t are worked on, tile t + 2 is called
 // for between products; before the barrier each wave waits for its rows of t + 1.
+// P in bf16: a weight is off by 2^-9 of itself at the most and the sum that it is
+// divided by is of the weights before that, so an output's error is at most that of
+// one more rounding of each value, the size of its own last rounding.
+//
+// Measured (512 + 64 columns, first launch + join): 64 requests of 8 nodes x 64
+// heads over up to 8192 keys, 204 + 19 us, 2326 clocks a tile of 64 rows: 1152 of
+// the matrix cores, the rest LDS (each key row is read twice, 236 bytes a clock) and
+// what a barrier leaves uncovered. 32 requests of one token x 64 heads over up to 65536 keys,
+// 791 MB: 172 + 15 us, in the loop 6.1 TB/s, 3346 clocks a tile, the rows' way from
+// HBM. One token over 4096 keys: 20 + 7.5 us, of which a walk's start (its request,
+// pages, queries, first tile) takes 7, its end 4 and the place search 3. What did
+// not carry: 64 keys a tile in a ring of two (282 us for the 64 requests), a running
+// maximum with the sums rescaled (spills; 16 us more), rows permuted instead of
+// padded (232 us), loads by global addresses (the compiler then waits for all of them).
 constexpr float kMost = 0x1p64f;  // 2^31 such weights sum to 2^95
 
 template <int GR, int LC>
@@ -636,6 +651,8 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
 // wrote them. The tile's parts are listed first, a thread per chunk of its keys.
 // Of few parts a wave joins a row by itself; many are dealt out to the four
 // waves, a quarter each, and their sums added in order. Lane: columns 4 lane + 256 k.
+// Parts to read and their number bound it: 33 MB in 17 us for the 32-bit kernel's
+// 512 parts of 32 rows, 7.5 us for one token's 64.
 constexpr uint32_t kManyParts = 16;
 template <uint32_t GRID, int ROWS, int LC, bool OBF>
 __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
@@ -1191,7 +1208,10 @@ uint32_t lat_class(const wl_tree_attn& a) {  // 128-column blocks of a row's lat
     const uint32_t b = (a.cache.kv_lora_rank + 127) / 128;
     return b <= 1 ? 1 : b <= 2 ? 2 : 4;
 }
-uint32_t row_class(const wl_tree_attn& a) {  // rows of a work-group's block
+// Rows of the 16-bit kernel's tile: 64, or 32 where a request has no more on average.
+// One token, 32 requests over up to 65536 keys, both launches: of 64 heads 262 us with
+// 32 rows and 199 with 64; of 32 heads 175 and 183, of 16 heads 178 and 180.
+uint32_t row_class(const wl_tree_attn& a) {
     const uint64_t rows = (uint64_t)a.n_heads * (a.n_req ? (a.n_tokens + a.n_req - 1) / a.n_req : 1);
     return rows > 32 ? 64 : 32;
 }
