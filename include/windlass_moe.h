@@ -789,9 +789,10 @@ wl_status wl_paged_write(const wl_row_write* w, void* stream);
  * their rows hold; a NaN or an infinity in a row reaches the tokens that see
  * it. d_len, d_cu, d_mask and d_table are wl_paged_map's.
  * dtype: the type of queries and output; WL_TYPE_BF16 needs a BF16 cache.
- * Products are exact in f32 sums for 32-bit queries (and caches: three bf16
- * parts a value); in a BF16 output's call the softmax weights are rounded to
- * bf16 once. Strides in elements from token to token, multiples of 8 up to
+ * With 32-bit queries every product is right to 2^-23 of itself (exact with a
+ * BF16 cache) and summed in f32; a value beyond the largest bf16 number, 3.39e38,
+ * counts as an infinity. In a BF16 output's call the softmax weights are rounded
+ * to bf16 once. Strides in elements from token to token, multiples of 8 up to
  * 2^22; heads lie next to each other, at most 1024; 16-byte aligned. A request has at most
  * WL_TREE_MAX_NODES tokens (E_TREE). Tokens that no request holds stay as they
  * were. A request with an impossible length or more keys than its table row

@@ -780,12 +780,13 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
     }
 }
 // ---- 32-bit queries -------------------------------------------------------------
-// A 32-bit value is the sum of three bf16 ones (its leading 8 bits, the next 8, the
-// last 8: cut off, not rounded, so each remainder is exact), and a product of two
-// such sums is, but for terms below 2^-24 of it, the six products of parts h, m, l
-// whose places add up to two at most (three of them where the other side is bf16
-// itself): exact products in the matrix cores, summed in f32, the scores' leading
-// ones apart from the others.
+// A 32-bit value is the sum of three bf16 ones, h + m + l, each the rounding of what
+// the ones before it leave (which is exact: 24 bits, then 16, then 8), m at most 2^-8
+// of the value and l 2^-16. A product of two such sums is, but for its m l, l m and
+// l l, together 2^-23 of it at the most and of either sign, the six products
+// h h, h m, m h, m m, h l, l h; of a bf16 value and such a sum, all of three: exact
+// products in the matrix cores, summed in f32, the scores' leading ones apart from
+// the others.
 //
 // 32 rows against 32 keys (WIDE, a cache of 32-bit rows: 16) at a time, four waves.
 // The next tile's rows are read into registers while this one is worked on, then cut
@@ -802,17 +803,17 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
 //
 // Bound by the matrix cores: 102 (WIDE 102 of 16 keys) products a wave and tile, 16
 // clocks each. The 64 nodes' 73 GFLOP, three products each, take 181 us at the rate
-// of a large library product (1211 TFLOP/s), 242 us and 18 us of joining here, 11 us
-// of them for the queries' reads at the start. Reading the next rows a piece at a
+// of a large library product (1211 TFLOP/s), 222 us with the joining here, 11 us
+// of them for the queries' reads at the start and some 15 for the parts. Reading the next rows a piece at a
 // time between the scores' products made no difference (243 us).
-WL_DEV void cut3(float x, float& h, float& m, float& l) {  // h + m + l = x, each with its low 16 bits clear
-    h = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
-    const float r = x - h;
-    m = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u);
-    l = r - m;
+WL_DEV void cut3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {  // two values' parts, x in the low halves
+    auto low = [](uint32_t v) { return __uint_as_float(v << 16); };
+    auto high = [](uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); };
+    h = pack_bf16(x, y);
+    x -= low(h), y -= high(h);
+    m = pack_bf16(x, y);
+    l = pack_bf16(x - low(m), y - high(m));
 }
-// the leading halves of two floats, the first one's low
-WL_DEV uint32_t high2(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
 WL_DEV bool nonfinite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
 // x, of which nothing is computed ahead of this place: what is derived from it holds
@@ -907,12 +908,12 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
                 const uint32_t lane = afresh(tid) & 63u;
                 auto put = [&](u32x4 x, uint32_t at) {
                     if (WIDE) {
-                        float h[4], md[4], lo[4];
+                        uint32_t v[3][2];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) cut3(__uint_as_float(x[k]), h[k], md[k], lo[k]);
-                        *(u32x2*)(tile + at) = u32x2{high2(h[0], h[1]), high2(h[2], h[3])};
-                        *(u32x2*)(tile + (NP > 1 ? PIECE : 0) + at) = u32x2{high2(md[0], md[1]), high2(md[2], md[3])};
-                        *(u32x2*)(tile + (NP > 1 ? 2 * PIECE : 0) + at) = u32x2{high2(lo[0], lo[1]), high2(lo[2], lo[3])};
+                        for (int k = 0; k < 2; k++)
+                            cut3(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1]), v[0][k], v[1][k], v[2][k]);
+#pragma unroll
+                        for (uint32_t j = 0; j < NP; j++) *(u32x2*)(tile + j * PIECE + at) = u32x2{v[j][0], v[j][1]};
                     } else {
                         *(u32x4*)(tile + at) = x;
                     }
@@ -969,11 +970,11 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
                     u32x4 part[3];
 #pragma unroll
                     for (uint32_t k = 0; k < 4; k++) {
-                        float a[3], b[3];
-                        cut3(__uint_as_float(x[i][k >> 1][2 * (k & 1)]), a[0], a[1], a[2]);
-                        cut3(__uint_as_float(x[i][k >> 1][2 * (k & 1) + 1]), b[0], b[1], b[2]);
+                        uint32_t v[3];
+                        cut3(__uint_as_float(x[i][k >> 1][2 * (k & 1)]), __uint_as_float(x[i][k >> 1][2 * (k & 1) + 1]), v[0], v[1],
+                             v[2]);
 #pragma unroll
-                        for (int j = 0; j < 3; j++) part[j][k] = high2(a[j], b[j]);
+                        for (int j = 0; j < 3; j++) part[j][k] = v[j];
                     }
 #pragma unroll
                     for (int j = 0; j < 3; j++) qf[j][i] = as_bf16x8(part[j]);
@@ -1081,15 +1082,15 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
             };
             // the weights e of row sr + n in places: parts h, m, l against 32 keys; or
             // against a key's value parts (h, m): h h and m m; against its (h, l): l h
-            auto put_weights = [&](uint32_t put_at, const float (&e)[3][NK]) __attribute__((always_inline)) {
+            auto put_weights = [&](uint32_t put_at, const uint32_t (&e)[3][NK / 2]) __attribute__((always_inline)) {
 #pragma unroll
                 for (uint32_t j = 0; j < 3; j++) {
                     uint8_t* o = pb + j * ROWS * 64u + put_at;
                     if (WIDE) {
-                        *(uint32_t*)(o + 4u * hf) = high2(e[j][0], e[j][1]);
-                        *(uint32_t*)(o + 4u * hf + 8u) = j < 2 ? high2(e[j][0], e[j][1]) : high2(e[0][0], e[0][1]);
+                        *(uint32_t*)(o + 4u * hf) = e[j][0];
+                        *(uint32_t*)(o + 4u * hf + 8u) = j < 2 ? e[j][0] : e[0][0];
                     } else {
-                        *(u32x2*)(o + 8u * hf) = u32x2{high2(e[j][0], e[j][1]), high2(e[j][NK - 2], e[j][NK - 1])};
+                        *(u32x2*)(o + 8u * hf) = u32x2{e[j][0], e[j][NK / 2 - 1]};
                     }
                 }
             };
@@ -1114,13 +1115,14 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
                     if (t + 1 < t1) read_tile(t + 1);
                     if (SUMS) {
                         if (t == t0 && !known) share_maxima(largest(sc));
-                        float e[3][NK], top = 0.f;
+                        float top = 0.f;
+                        uint32_t e[3][NK / 2];
 #pragma unroll
-                        for (uint32_t k = 0; k < NK; k++) {
-                            const float v = exp2_(sc.v[k] - m);
-                            l += v;
-                            top = fmaxf(top, v);
-                            cut3(v, e[0][k], e[1][k], e[2][k]);
+                        for (uint32_t k = 0; k < NK / 2; k++) {
+                            const float v = exp2_(sc.v[2 * k] - m), v1 = exp2_(sc.v[2 * k + 1] - m);
+                            l += v + v1;
+                            top = fmaxf(top, fmaxf(v, v1));
+                            cut3(v, v1, e[0][k], e[1][k], e[2][k]);
                         }
                         pass |= top > kMost;
                         const uint32_t lane = afresh(tid) & 63u, n = lane & 15u, g = lane >> 4;
