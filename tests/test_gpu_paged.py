@@ -478,6 +478,34 @@ def test_attention_long_and_uneven(gpu, q, cache):
 
 
 @pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("H,lens,adds", [(20, [900, 0, 333, 4000], [5, 1, 64, 9]), (64, [2500], [7]), (33, [31, 0, 64], [2, 0, 3]),
+                                         (64, list(range(0, 1200, 20)), [2] * 60), (128, [70, 2100], [64, 1])],
+                         ids=["uneven", "one", "short", "sixty", "tall"])
+def test_attention_pieces(gpu, q, cache, H, lens, adds):
+    """Fewer row tiles than work-groups: each has a piece of one."""
+    rng = np.random.default_rng(21)
+    Tree(22, q, cache, 128, 32, H, 16, lens, adds, random_trees(rng, adds)).upload().run().check()
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
+def test_attention_refused_among_pieces(gpu, q, cache):
+    lens, adds = [2000, 300, 9, 1400], [2, 3, 1, 2]
+    def tree():
+        return Tree(23, q, cache, 128, 16, 70, 16, lens, adds, tail=3)
+    t = tree()
+    table = t.table.copy()
+    table[0, 77] = -3
+    t.upload(table=table).run().check(nan=(0,))
+    assert t.status() == paged.E_PAGE
+    t = tree()
+    t.upload(lens=[2000, -5, 9, 2 ** 31 - 1]).run().check(nan=(1, 3))
+    assert t.status() == paged.E_LEN
+    t = tree()
+    t.upload(cu=[0, 2, 5, 6, 12]).run().check(skip=(3,))
+    assert t.status() == paged.E_LEN
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
 def test_attention_many_requests(gpu, q, cache):
     rng = np.random.default_rng(10)
     R = 300
