@@ -88,7 +88,7 @@ def tree_attention(q, rows, L, scale, seen, q_type):
         return np.zeros((H, L)), np.zeros((H, L))
     q, k = q.astype(np.float64), rows[seen].astype(np.float64)
     s = scale * q @ k.T
-    es = ((k.shape[1] + 16) * U32 * scale * (np.abs(q) @ np.abs(k).T) + 4 * U32 * np.abs(s)).max(1, keepdims=True)
+    es = ((k.shape[1] + 16) * U32 * abs(scale) * (np.abs(q) @ np.abs(k).T) + 4 * U32 * np.abs(s)).max(1, keepdims=True)
     p = np.exp(s - s.max(1, keepdims=True))
     p /= p.sum(1, keepdims=True)
     out, size = p @ k[:, :L], p @ np.abs(k[:, :L])

@@ -514,6 +514,40 @@ def test_attention_many_requests(gpu, q, cache):
 
 
 @pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("R", [600, 1500, 4096])
+def test_attention_requests_beyond_a_thread_each(gpu, q, cache, R):
+    rng = np.random.default_rng(R)
+    lens, adds = [int(x) for x in rng.integers(0, 40, R)], [int(x) for x in rng.integers(0, 3, R)]
+    Tree(24, q, cache, 64, 8, 2, 8, lens, adds, random_trees(rng, adds)).upload().run().check()
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("scale", [-0.07, 0.0])
+def test_attention_scales_that_are_not_positive(gpu, q, cache, scale):
+    rng = np.random.default_rng(25)
+    lens, adds = [70, 0, 611], [5, 2, 33]
+    t = Tree(26, q, cache, 96, 16, 5, 16, lens, adds, random_trees(rng, adds))
+    t.scale = scale
+    t.upload().run().check()
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
+def test_attention_magnitudes(gpu, q, cache):
+    """Large queries against small rows, scaled by powers of two: exact in every type."""
+    t = Tree(27, q, cache, 128, 32, 6, 16, [300, 40], [3, 9])
+    t.ql, t.qr = t.ql * np.float32(2.0 ** 60), t.qr * np.float32(2.0 ** 60)
+    t.rows = [x * np.float32(2.0 ** -60) for x in t.rows]
+    t.pages = t.pages * np.float32(2.0 ** -60)
+    t.upload().run().check()
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
+def test_attention_most_heads(gpu, q, cache):
+    rng = np.random.default_rng(28)
+    Tree(29, q, cache, 16, 8, 1024, 8, [40, 3], [2, 1], random_trees(rng, [2, 1])).upload().run().check()
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
 def test_attention_rows_that_see_nothing(gpu, q, cache):
     """Masks of nothing: zeros without a context, the context alone with one. Any 64-bit mask, not only a tree's."""
     rng = np.random.default_rng(12)

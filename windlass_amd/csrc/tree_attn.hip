@@ -106,7 +106,7 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
         if (r < R) {
             q = request<ROWS>(p, r, status);
             mine += (uint64_t)q.nrt * q.nkt;
-            tiles += q.nrt;
+            tiles += q.nrt < GRID ? q.nrt : GRID;  // (of a refused request it may be any number)
         }
     }
     rq[tid] = u32x2{q.nrt, q.nkt};
