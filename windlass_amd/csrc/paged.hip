@@ -28,8 +28,8 @@ WL_DEV void set_status(uint32_t* status, uint32_t bits) {
 // In a call with trees a wave takes a request, lane i its node i; otherwise a
 // thread takes a token, or four, and finds its request by bisection.
 // Bound by the launch and by latencies one after the other (lengths, the sums over
-// the requests, page, slot), not by bytes: 8 requests of 8 nodes 3.8 us, as an empty
-// kernel; 256 of 64 nodes 5.7 us; 1000 prompts, 690k tokens, 5.5 MB out, 10.5 us
+// the requests, page, slot), not by bytes: 8 requests of 8 nodes 3.7 us (an empty
+// kernel takes 1.4); 256 of 64 nodes 5.7 us; 1000 prompts, 690k tokens, 5.5 MB out, 10.5 us
 // (14.7 with one token a thread).
 struct Sums {
     uint64_t tok;
@@ -64,6 +64,7 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = tid >> 6, R = m.n_req;
     const uint32_t psh = 31u - (uint32_t)__clz((int)m.page_size), pmask = m.page_size - 1u;
     const bool trees = m.d_parent || m.d_mask;
+    const int32_t nf = *m.d_n_free;
     if (tid == 0) err = 0;
     __syncthreads();
     // thread tid's requests are [RPT tid, RPT tid + RPT)
@@ -119,7 +120,6 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
         back[CAP] = at.back;
         take[CAP] = at.take;
     }
-    const int32_t nf = *m.d_n_free;
     uint32_t refuse = err;  // set before the barrier above
     if (all.tok > m.max_tokens) refuse |= WL_PAGED_E_LEN;
     if (nf < 0 || (uint32_t)nf > m.n_pages || (uint64_t)(uint32_t)nf + all.back > m.n_pages) refuse |= WL_PAGED_E_PAGE;
@@ -252,8 +252,9 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
 // turns, then sine and cosine of the rest in f32 with the rest's own rounding
 // added to first order; the other lanes take the pairs' values by permutes.
 // Bound by the bytes: 16384 bf16 tokens with 64 heads' queries, 306 MB read and
-// written in 61.4 us, 4.98 TB/s (a large copy: 5.05). 333 tokens 5.6 us, one token
-// 3.9 us, as an empty kernel.
+// written in 61.4 us, 4.98 TB/s (a large copy: 5.05). 333 tokens 5.3 us, one token
+// 3.7 us: a kernel's 1.4 and two trips to memory (3.9 with the row called for only
+// when its slot had come).
 struct RowWrite {
     wl_row_write w;
     double inv[kMaxRope / 2];  // theta^(-2 i / qk_rope)
@@ -317,8 +318,25 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowWrite a) {
     const uint32_t t = wave / a.wpt, part = wave % a.wpt;
     if (t >= w.n_tokens) return;
     const uint32_t L = w.cache.kv_lora_rank, RP = w.cache.qk_rope, HP = RP / 2;
-    const int32_t pos = w.d_pos[t];
     const bool cbf = w.cache.dtype == WL_TYPE_BF16;
+    // everything the wave needs first is called for before anything is waited for
+    const int32_t pos = w.d_pos[t], slot = part == 0 ? w.d_slot[t] : -1, src = part == 0 && w.d_src ? w.d_src[t] : (int32_t)t;
+    const uint32_t cph = RP / 8, vpw = 64 / cph, c = lane % cph, vl = lane / cph;
+    const uint32_t i = 8 * lane;
+    const bool src_ok = !w.d_src || (src >= 0 && (uint32_t)src < w.n_kv);
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, r[8], g[8], qv[8];
+    if (part == 0 && src_ok) {
+        const size_t in = (size_t)src * w.kv_stride;
+        if (i < L) {
+            load8<BF>(w.d_kv, in + i, v);
+            load8<true>(w.d_norm_w, i, g);
+        }
+        if (lane < cph) load8<BF>(w.d_kv, in + L + i, r);
+    }
+    auto load_q = [&](uint32_t h0) {
+        if (vl < vpw && h0 + vl < w.n_heads) load8<BF>(w.d_q_rope, (size_t)t * w.q_stride + (size_t)(h0 + vl) * RP + 8 * c, qv);
+    };
+    load_q(part * vpw);
     if (pos < 0) {
         if (lane == 0 && part == 0) set_status(w.d_status, WL_PAGED_E_LEN);
         return;
@@ -326,7 +344,6 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowWrite a) {
     float sn = 0.f, cs = 0.f;
     if (lane < HP) sincos_of((double)pos * a.inv[lane], sn, cs);
     // this lane's 4 pairs: chunk c of the RP / 8 chunks of a rotary vector, of vector vl of the wave's vpw
-    const uint32_t cph = RP / 8, vpw = 64 / cph, c = lane % cph, vl = lane / cph;
     float s4[4], c4[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
@@ -341,19 +358,11 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowWrite a) {
         }
     };
     if (part == 0) {
-        const int32_t slot = w.d_slot[t], src = w.d_src ? w.d_src[t] : (int32_t)t;
         const uint32_t rows = w.cache.n_pages * w.cache.page_size;
-        const bool bad = slot < -1 || (slot >= 0 && (uint32_t)slot >= rows) || (w.d_src && (src < 0 || (uint32_t)src >= w.n_kv));
+        const bool bad = slot < -1 || (slot >= 0 && (uint32_t)slot >= rows) || !src_ok;
         if (bad && lane == 0) set_status(w.d_status, WL_PAGED_E_SLOT);
         if (!bad && slot >= 0) {
-            const size_t in = (size_t)src * w.kv_stride, out = (size_t)slot * w.cache.row_stride;
-            const uint32_t i = 8 * lane;
-            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, r[8], g[8];
-            if (i < L) {
-                load8<BF>(w.d_kv, in + i, v);
-                load8<true>(w.d_norm_w, i, g);
-            }
-            if (lane < cph) load8<BF>(w.d_kv, in + L + i, r);
+            const size_t out = (size_t)slot * w.cache.row_stride;
             float ss = 0.f;
 #pragma unroll
             for (int k = 0; k < 8; k++) ss += v[k] * v[k];
@@ -377,11 +386,11 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowWrite a) {
     for (uint32_t h0 = part * vpw; h0 < w.n_heads; h0 += a.wpt * vpw) {
         const uint32_t h = h0 + vl;
         const bool ok = vl < vpw && h < w.n_heads;
-        float v[8], lo[4], hi[4];
-        if (ok) load8<BF>(w.d_q_rope, (size_t)t * w.q_stride + (size_t)h * RP + 8 * c, v);
+        float lo[4], hi[4];
+        if (h0 != part * vpw) load_q(h0);
         __builtin_amdgcn_wave_barrier();
         if (ok) {
-            turn(v, lo, hi);
+            turn(qv, lo, hi);
             const size_t out = (size_t)t * w.q_out_stride + (size_t)h * RP + 4 * c;
             store_n<4>(w.d_q_rope_out, out, lo, BF);
             store_n<4>(w.d_q_rope_out, out + HP, hi, BF);
