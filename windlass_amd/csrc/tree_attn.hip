@@ -83,6 +83,27 @@ WL_DEV uint64_t div64(uint64_t a, uint64_t b) {
     return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
+// The sum of x over this lane and those below it: within rows of 16 lanes, then the
+// rows' last lanes handed on. (Shuffles go through LDS, some 130 clocks a step.)
+template <int CTRL, int ROWMASK>
+WL_DEV uint32_t dpp0(uint32_t x) {  // lanes without a source get 0
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWMASK, 0xf, false);
+}
+template <int CTRL, int ROWMASK>
+WL_DEV uint64_t dpp0(uint64_t x) {
+    return (uint64_t)dpp0<CTRL, ROWMASK>((uint32_t)(x >> 32)) << 32 | dpp0<CTRL, ROWMASK>((uint32_t)x);
+}
+template <class T>
+WL_DEV T sum_up(T x) {
+    x += dpp0<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+    x += dpp0<0x112, 0xf>(x);
+    x += dpp0<0x114, 0xf>(x);
+    x += dpp0<0x118, 0xf>(x);
+    x += dpp0<0x142, 0xa>(x);  // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+    x += dpp0<0x143, 0xc>(x);
+    return x;
+}
+
 // The launch's units (or pieces), and the request (with its first one) that unit
 // u0 = c per (piece c) falls into. Each thread sums the requests of its share; tmp: two
 // words per wave, and ten; rq: a pair per thread.
@@ -112,12 +133,8 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
     rq[tid] = u32x2{q.nrt, q.nkt};
     if (c == 0 && status && p.a.d_status)
         __hip_atomic_fetch_or(p.a.d_status, status, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    uint64_t inc = mine;
-    for (uint32_t o = 1; o < 64; o <<= 1) {
-        const uint64_t v = (uint64_t)__shfl_up((unsigned long long)inc, o, 64);
-        if (lane >= o) inc += v;
-        tiles += __shfl_xor(tiles, o, 64);
-    }
+    const uint64_t inc = sum_up(mine);
+    tiles = sum_up(tiles);
     if (lane == 63) {
         tmp[wv] = inc;
         tmp[NW + 2 + wv] = tiles;
@@ -144,8 +161,8 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
             const uint32_t len = per + k * step;
             uint32_t n = 0;
             for (uint32_t r = lane; r < R; r += 64) n += rq[r][0] * ((rq[r][1] + len - 1u) / len);
-            for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-            if (lane == 0) ((uint32_t*)(tmp + 2 * NW + 2))[k] = n;
+            n = sum_up(n);
+            if (lane == 63) ((uint32_t*)(tmp + 2 * NW + 2))[k] = n;
         }
         __syncthreads();
         for (uint32_t k = kTries; k-- > 0;)
@@ -156,11 +173,7 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
         f.per = f.pieces;
         f.u0 = c;
         mine = q.nrt * ((q.nkt + f.pieces - 1u) / f.pieces);
-        uint32_t sum = (uint32_t)mine;
-        for (uint32_t o = 1; o < 64; o <<= 1) {
-            const uint32_t v = __shfl_up(sum, o, 64);
-            if (lane >= o) sum += v;
-        }
+        const uint32_t sum = sum_up((uint32_t)mine);
         if (lane == 63) tmp[wv] = sum;
         __syncthreads();
         f.total = 0;
@@ -190,7 +203,8 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
     f.per = uni64(f.per);
     f.base = uni64(tmp[NW]);
     f.r = uni((uint32_t)tmp[NW + 1]);
-    f.q = Req{uni(found->t0), uni(found->nodes), uni(found->len), uni(found->keys), uni(found->nrt), uni(found->nkt), uni(found->flaw)};
+    f.q = Req{uni(found->t0),  uni(found->nodes), uni(found->len), uni(found->keys),
+              uni(found->nrt), uni(found->nkt),   uni(found->flaw)};
     return f;
 }
 
@@ -229,16 +243,20 @@ struct Walks {
     uint32_t status;
     Walk next;
     __device__ __forceinline__ Walks(const Tree& t, const Place& pl, uint32_t wg)
-        : p(t), f(pl), u1(pl.pieces ? (pl.u0 < pl.total ? pl.u0 + 1 : pl.u0) : pl.u0 + pl.per < pl.total ? pl.u0 + pl.per : pl.total), c(wg), u(pl.u0), status(0),
-          next{pl.q, pl.base, pl.r, 0, 0, 0, 0} {}
+        : p(t), f(pl), u1(end(pl)), c(wg), u(pl.u0), status(0), next{pl.q, pl.base, pl.r, 0, 0, 0, 0} {}
+    static __device__ __forceinline__ uint64_t end(const Place& pl) {
+        const uint64_t u = pl.u0 + (pl.pieces ? 1u : pl.per);
+        return u < pl.total ? u : pl.total;  // (a work-group without work begins behind it)
+    }
     __device__ __forceinline__ bool more() const { return u < u1; }
     __device__ __forceinline__ void find() {  // the walk that begins at unit u < u1, from the last one's request on
         Walk& w = next;
         if (f.pieces) {
             const uint32_t i = (uint32_t)(u++ - w.base), nc = uni(pieces_of(w.q, f.pieces)), j = uni(i / w.q.nrt);
+            const uint32_t len = uni(w.q.nkt / nc), longer = w.q.nkt - len * nc;  // the first ones one tile more
             w.rt = uni(i - j * w.q.nrt);
-            w.kt0 = uni(chunk_at(w.q, nc, j));
-            w.kt1 = uni(chunk_at(w.q, nc, j + 1));
+            w.kt0 = uni(j * len + (j < longer ? j : longer));
+            w.kt1 = uni(w.kt0 + len + (j < longer ? 1u : 0u));
             w.slot = 2u * c;
             return;
         }
@@ -357,7 +375,7 @@ WL_DEV constexpr uint32_t swz4(uint32_t row) { return (row & 8u) >> 2; }
 // what a barrier leaves uncovered. 32 requests of one token x 64 heads over up to 65536 keys,
 // 791 MB: 172 + 15 us, in the loop 6.1 TB/s, 3346 clocks a tile, the rows' way from
 // HBM. One token over 4096 keys: 20 + 7.5 us, of which a walk's start (its request,
-// pages, queries, first tile) takes 7, its end 4 and the place search 3. What did
+// pages, queries, first tile) takes 7, its end 4 and the place search 2.5. What did
 // not carry: 64 keys a tile in a ring of two (282 us for the 64 requests), a running
 // maximum with the sums rescaled (spills; 16 us more), rows permuted instead of
 // padded (232 us), loads by global addresses (the compiler then waits for all of them).
@@ -883,9 +901,10 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
 //
 // Bound by the matrix cores: 102 (WIDE 102 of 16 keys) products a wave and tile, 16
 // clocks each. The 64 nodes' 73 GFLOP, three products each, take 181 us at the rate
-// of a large library product (1211 TFLOP/s), 222 us with the joining here, 11 us
-// of them for the queries' reads at the start and some 15 for the parts. Reading the next rows a piece at a
-// time between the scores' products made no difference (243 us).
+// of a large library product (1211 TFLOP/s), 207 to 217 us with the joining here
+// (cards differ), 11 of them for the queries' reads at the start and 12 for the join.
+// Reading the next rows a piece at a time between the scores' products made no
+// difference.
 WL_DEV void cut3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {  // two values' parts, x in the low halves
     auto low = [](uint32_t v) { return __uint_as_float(v << 16); };
     auto high = [](uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); };
@@ -1018,7 +1037,8 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
 #pragma unroll
                 for (uint32_t i = 0; i < NLAT + NROT; i++) {
                     const bool lat = i < NLAT;
-                    const uint32_t e = 64u * (lat ? i : i - NLAT) + lane, row = DR * wave + e / (lat ? EL : ER), k = e % (lat ? EL : ER);
+                    const uint32_t e = 64u * (lat ? i : i - NLAT) + lane, k = e % (lat ? EL : ER);
+                    const uint32_t row = DR * wave + e / (lat ? EL : ER);
                     const uint32_t b = WIDE ? 8u * k : 16u * k;  // of a bf16 row
                     put(raw[i], lat ? row * PITCH + b : ROT + row * 128u + (b ^ (16u * swz8(row & 15u))));
                 }
@@ -1026,7 +1046,10 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
             // the queries of rows sr + n, in parts, in the operand's layout: lane (row n, k group g);
             // slice s of the row's 2 NH: of the latent part's 32 columns each, and the rotary one's last two
             bf16x8 qf[3][NH];
-            auto read_queries = [&]() __attribute__((always_inline)) {
+            struct Queries {
+                u32x4 x[NH][2];
+            };
+            auto read_queries = [&](Queries& f) __attribute__((always_inline)) {
                 const rsrc_t ql = make_rsrc((const float*)p.a.d_q_lat + q.t0 * p.a.q_lat_stride,
                                             4u * ((q.nodes - 1u) * (uint32_t)p.a.q_lat_stride + H * L));
                 const rsrc_t qr = make_rsrc((const float*)p.a.d_q_rope + q.t0 * p.a.q_rope_stride,
@@ -1036,23 +1059,24 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
                 const bool live = lr < rows;
                 const uint32_t vl = 4u * (node * (uint32_t)p.a.q_lat_stride + h * L);
                 const uint32_t vr = 4u * (node * (uint32_t)p.a.q_rope_stride + h * RP);
-                u32x4 x[NH][2];
 #pragma unroll
                 for (uint32_t i = 0; i < NH; i++) {
                     const bool rot = i + 1 == NH;  // the last of each half is a rotary one
                     const uint32_t col = 32u * (rot ? hf : (NH - 1u) * hf + i) + 8u * g;
                     const uint32_t at = live && col < (rot ? RP : L) ? (rot ? vr : vl) + 4u * col : kOOB;
 #pragma unroll
-                    for (uint32_t k = 0; k < 2; k++) x[i][k] = bld16(rot ? qr : ql, at, 16u * k);
+                    for (uint32_t k = 0; k < 2; k++) f.x[i][k] = bld16(rot ? qr : ql, at, 16u * k);
                 }
+            };
+            auto cut_queries = [&](const Queries& f) __attribute__((always_inline)) {
 #pragma unroll
                 for (uint32_t i = 0; i < NH; i++) {
                     u32x4 part[3];
 #pragma unroll
                     for (uint32_t k = 0; k < 4; k++) {
                         uint32_t v[3];
-                        cut3(__uint_as_float(x[i][k >> 1][2 * (k & 1)]), __uint_as_float(x[i][k >> 1][2 * (k & 1) + 1]), v[0], v[1],
-                             v[2]);
+                        const u32x4 x = f.x[i][k >> 1];
+                        cut3(__uint_as_float(x[2 * (k & 1)]), __uint_as_float(x[2 * (k & 1) + 1]), v[0], v[1], v[2]);
 #pragma unroll
                         for (int j = 0; j < 3; j++) part[j][k] = v[j];
                     }
@@ -1060,8 +1084,9 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
                     for (int j = 0; j < 3; j++) qf[j][i] = as_bf16x8(part[j]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                if (hf == 0 && g == 0) {
-                    const uint32_t nd = live ? node : 0u;
+                const uint32_t ln = afresh(tid) & 63u, lr = sr + (ln & 15u);
+                if (hf == 0 && (ln >> 4) == 0) {
+                    const uint32_t nd = lr < rows ? (w.rt * ROWS + lr) / H : 0u;
                     seen[lr] = p.a.d_mask ? p.a.d_mask[q.t0 + nd] : (2ull << nd) - 1ull;
                 }
             };
@@ -1073,7 +1098,8 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
             };
             auto scores = [&](uint32_t t) __attribute__((always_inline)) {
                 const uint32_t lane = afresh(tid) & 63u, n = lane & 15u, g = lane >> 4;
-                const uint32_t key_at = n * PITCH + 64u * (NH - 1u) * hf + 16u * g, key_rot = ROT + n * 128u + ((16u * (g ^ swz8(n))) ^ (64u * hf));
+                const uint32_t key_at = n * PITCH + 64u * (NH - 1u) * hf + 16u * g;
+                const uint32_t key_rot = ROT + n * 128u + ((16u * (g ^ swz8(n))) ^ (64u * hf));
                 auto kread = [&](uint32_t i, uint32_t piece, uint32_t block) __attribute__((always_inline)) {
                     return as_bf16x8(i + 1 < NH ? *(const u32x4*)(tile + PIECE * piece + 16u * block * PITCH + key_at + 64u * i)
                                                 : *(const u32x4*)(tile + PIECE * piece + 2048u * block + key_rot));
@@ -1181,8 +1207,11 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
                 float x = kNone;
                 const uint32_t t0 = kt0 * (kKT / KT), t1 = kt1 * (kKT / KT);
                 next_page = page_of(t0);
+                Queries first;
+                if (SUMS && !known) read_queries(first);
+                __builtin_amdgcn_sched_barrier(0);
                 read_tile(t0);
-                if (SUMS && !known) read_queries();
+                if (SUMS && !known) cut_queries(first);
                 if (SUMS) clear();
                 for (uint32_t t = t0; t < t1; t++) {
                     if (has_nodes(t)) {
@@ -1336,7 +1365,8 @@ int launch_tree(const wl_tree_attn& a, void* stream) {
         if (rows == 64) return lc == 4 ? run_bf16<2, 4>(p, st) : lc == 2 ? run_bf16<2, 2>(p, st) : run_bf16<2, 1>(p, st);
         return lc == 4 ? run_bf16<1, 4>(p, st) : lc == 2 ? run_bf16<1, 2>(p, st) : run_bf16<1, 1>(p, st);
     }
-    if (a.cache.dtype == WL_TYPE_BF16) return lc == 4 ? run_f32<4, false>(p, st) : lc == 2 ? run_f32<2, false>(p, st) : run_f32<1, false>(p, st);
+    if (a.cache.dtype == WL_TYPE_BF16)
+        return lc == 4 ? run_f32<4, false>(p, st) : lc == 2 ? run_f32<2, false>(p, st) : run_f32<1, false>(p, st);
     return lc == 4 ? run_f32<4, true>(p, st) : lc == 2 ? run_f32<2, true>(p, st) : run_f32<1, true>(p, st);
 }
 
