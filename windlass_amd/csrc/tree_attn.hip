@@ -370,10 +370,10 @@ WL_DEV constexpr uint32_t swz4(uint32_t row) { return (row & 8u) >> 2; }
 // one more rounding of each value, the size of its own last rounding.
 //
 // Measured (512 + 64 columns, first launch + join): 64 requests of 8 nodes x 64
-// heads over up to 8192 keys, 204 + 19 us, 2326 clocks a tile of 64 rows: 1152 of
-// the matrix cores, the rest LDS (each key row is read twice, 236 bytes a clock) and
-// what a barrier leaves uncovered. 32 requests of one token x 64 heads over up to 65536 keys,
-// 791 MB: 172 + 15 us, in the loop 6.1 TB/s, 3346 clocks a tile, the rows' way from
+// heads over up to 8192 keys, 205 + 17 us, 2326 clocks a tile of 64 rows: 1090 of
+// the matrix cores and 1120 of LDS (265 KB at 236 bytes a clock), mostly in turn.
+// 32 requests of one token x 64 heads over up to 65536 keys,
+// 791 MB: 162 + 13 us, in the loop 6.1 TB/s, 3346 clocks a tile, the rows' way from
 // HBM. One token over 4096 keys: 20 + 7.5 us, of which a walk's start (its request,
 // pages, queries, first tile) takes 7, its end 4 and the place search 2.5. What did
 // not carry: 64 keys a tile in a ring of two (282 us for the 64 requests), a running
