@@ -705,7 +705,9 @@ typedef struct wl_paged_cache {
  *   d_have_out[r]    pages held (not d_have itself)
  *   *d_n_free_out    pages left on the stack (not d_n_free itself)
  *   d_cu[r]          sum of d_add before r; d_cu[n_req] the step's tokens
- *   per token t = d_cu[r] + i (arrays of max_tokens, the rest as it was):
+ *   per token t = d_cu[r] + i (arrays of max_tokens; behind the step's tokens
+ *   d_slot is -1, d_pos 0 and d_mask as it was, so that a step captured with
+ *   room for more tokens writes no row for them):
  *   d_slot[t]        where its row goes
  *   d_pos[t]         its position: d_len[r] + i, or in a tree d_len[r] + the
  *                    number of its ancestors (may be NULL)

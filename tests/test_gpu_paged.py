@@ -49,7 +49,7 @@ def check_step(m, s, extra=0):
     if "d_mask" in m.b:
         assert np.array_equal(m.get("mask")[:n], np.array(mask, np.uint64))
         assert np.all(m.get("mask")[n:] == 77)
-    assert np.all(m.get("slot")[n:] == -7) and np.all(m.get("pos")[n:] == -7)  # behind the last request: as it was
+    assert np.all(m.get("slot")[n:] == -1) and np.all(m.get("pos")[n:] == 0)  # behind the last request: no tokens
 
 
 @pytest.mark.parametrize("trees", [False, True])
@@ -113,8 +113,46 @@ def test_map_long_runs(gpu, shift):
     assert np.array_equal(m.get("table"), want[0]) and np.array_equal(m.get("cu"), want[4])
     assert np.count_nonzero(slot == -1) == 16
     assert np.array_equal(m.get("slot")[o:o + n], slot) and np.array_equal(m.get("pos")[o:o + n], want[6])
-    for x in (m.get("slot"), m.get("pos")):
-        assert np.all(x[:o] == -7) and np.all(x[o + n:] == -7)
+    for x, none in (m.get("slot"), -1), (m.get("pos"), 0):
+        assert np.all(x[:o] == -7) and np.all(x[o + n:] == none)
+
+
+@pytest.mark.parametrize("trees", [False, True])
+def test_map_and_write_with_room_for_more(gpu, trees):
+    """Buffers for 40 tokens: a step of 30, then one of 3. Its write leaves the rows of the first alone."""
+    L, RP, ps, n_pages = 32, 8, 8, 12
+    W = L + RP
+    rng = np.random.default_rng(31)
+    parent = np.full(40, -1, np.int32) if trees else None
+    m = P.Map(ps, n_pages, 6, [0, 0], [10, 20], [0, 0], np.arange(n_pages), n_pages, np.full((2, 6), -1), parent, max_tokens=40)
+    norm = P.as_type(np.ones(L), "bf16")
+    b = dict(d_kv=P.upload(rng.standard_normal((40, W)), "f32"), d_norm_w=P.upload(norm, "bf16"),
+             cache=P.upload(np.zeros((n_pages * ps, W)), "f32"))
+    c = paged.Cache(d_rows=b["cache"].ptr, dtype=paged.TYPE["f32"], n_pages=n_pages, page_size=ps, kv_lora_rank=L, qk_rope=RP,
+                    row_stride=W)
+    w = paged.RowWrite(cache=c, dtype=paged.TYPE["f32"], n_tokens=40, eps=1e-6, rope_theta=1e4, kv_stride=W, d_kv=b["d_kv"].ptr,
+                       d_norm_w=b["d_norm_w"].ptr, d_pos=m.b["d_pos"].ptr, d_slot=m.b["d_slot"].ptr,
+                       d_status=m.b["d_status"].ptr)
+    kept = None
+    for lens, adds in ([0, 0], [10, 20]), ([10, 20], [1, 2]):
+        m.b["d_len"].upload(np.asarray(lens, np.int32))
+        m.b["d_add"].upload(np.asarray(adds, np.int32))
+        if kept is not None:
+            m.b["d_have"].upload(m.get("have_out").astype(np.int32))
+            m.b["d_n_free"].upload(m.get("n_free_out").astype(np.int32))
+            b["d_kv"].upload(rng.standard_normal((40, W)).astype(np.float32))
+        paged.page_map(m.args)
+        paged.write_rows(w)
+        hip.synchronize()
+        assert m.get("status")[0] == 0
+        slots, rows = m.get("slot"), P.download(b["cache"], "f32", (n_pages * ps, W))
+        n = sum(adds)
+        assert np.all(slots[:n] >= 0) and np.all(slots[n:] == -1)
+        if kept is not None:
+            still = np.setdiff1d(np.arange(n_pages * ps), slots[:n])
+            assert np.array_equal(rows[still], kept[still])
+            assert not np.any(np.all(rows[slots[:n]] == kept[slots[:n]], axis=1))
+        kept = rows
 
 
 def test_map_many_pages_given_back(gpu):

@@ -140,6 +140,10 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
     for (uint32_t r = gt; r < R; r += gn) m.d_have_out[r] = (int32_t)need[r];
     for (uint32_t r = gt; r <= R; r += gn) m.d_cu[r] = (int32_t)cu[r];
     if (gt == 0) *m.d_n_free_out = (int32_t)(F - all.take);
+    for (uint32_t t = total + gt; t < m.max_tokens; t += gn) {  // behind the step's tokens: none
+        m.d_slot[t] = -1;
+        if (m.d_pos) m.d_pos[t] = 0;
+    }
     // the last r with base[r] <= x: the owner of element x (empty ranges before it share its base)
     auto owner = [&](const uint32_t* base, uint32_t x) {
         uint32_t lo = 0, hi = R;
