@@ -24,6 +24,7 @@ typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 #define WL_LDS(p) ((__attribute__((address_space(3))) void*)(p))
 
+constexpr uint32_t kDesc = 16;
 // What a launch needs beside the call's arguments.
 struct Tree {
     wl_tree_attn a;
@@ -31,7 +32,7 @@ struct Tree {
     float scale2;      // scale * log2(e): scores in powers of two
     float* part;       // [2 grid][rows][cols] unnormalised sums of split tiles
     float* part_ml;    // [2 grid][rows][2] their maxima and weight sums
-    uint32_t* desc;    // [2 grid][8] the parts' row tiles: {request + 1, row tile, base, per, pieces}, base and per 64-bit
+    uint32_t* desc;    // [2 grid][kDesc] the parts' row tiles, as name_part writes them, or 0
 };
 
 // ---- the work and its split --------------------------------------------------
@@ -286,12 +287,16 @@ struct Walks {
     }
     // names the row tile of the walk's part for the second launch
     __device__ __forceinline__ void name_part(const Walk& w) const {
-        uint32_t* desc = p.desc + 8 * w.slot;
-        desc[0] = w.r + 1u;
+        uint32_t* desc = p.desc + kDesc * w.slot;
+        desc[0] = 1u;
         desc[1] = w.rt;
         *(uint64_t*)(desc + 2) = w.base;
         *(uint64_t*)(desc + 4) = f.per;
         desc[6] = f.pieces;
+        desc[7] = w.q.t0;
+        desc[8] = w.q.nodes;
+        desc[9] = w.q.nrt;
+        desc[10] = w.q.nkt;
     }
 };
 // One lane's share of a row of sums (4 columns of every 16 from column `col` on,
@@ -402,7 +407,7 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
     const uint32_t H = p.a.n_heads, L = p.a.cache.kv_lora_rank, RP = p.a.cache.qk_rope;
     if (tid == 0) bad_page = again = 0;
     const Place f = find_place<ROWS, 64 * NW, kGrid>(p, c, min_per, tmp, (u32x2*)pb0, &found);
-    if (tid < 2) p.desc[8 * (2 * c + tid)] = 0;
+    if (tid < 2) p.desc[kDesc * (2 * c + tid)] = 0;
     Walks<ROWS> walks(p, f, c);
     if (!walks.more()) return;
     // the pages of a walk's first four tiles are read while the one before it ends
@@ -747,10 +752,10 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
     __shared__ float weight[4][2 * GRID];
     __shared__ uint32_t count[4], list[2 * GRID];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = uni(tid >> 6), mine = blockIdx.x;
-    const uint32_t* desc = p.desc + 8 * mine;
+    const uint32_t* desc = p.desc + kDesc * mine;
     if (desc[0] == 0) return;
-    uint32_t status = 0;
-    const Req q = request<ROWS>(p, desc[0] - 1u, status);
+    Req q{};  // as the first launch found it, in one read
+    q.t0 = desc[7], q.nodes = desc[8], q.nrt = desc[9], q.nkt = desc[10];
     const uint32_t rt = desc[1], H = p.a.n_heads, L = p.a.cache.kv_lora_rank;
     const uint64_t base = *(const uint64_t*)(desc + 2), per = *(const uint64_t*)(desc + 4);
     const uint32_t pieces = desc[6];
@@ -943,7 +948,7 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
     const uint32_t H = p.a.n_heads, L = p.a.cache.kv_lora_rank, RP = p.a.cache.qk_rope;
     if (tid == 0) bad_page = again = 0;
     const Place f = find_place<ROWS, 256, kGridF32>(p, c, min_per, tmp, (u32x2*)pb, &found);
-    if (tid < 2) p.desc[8 * (2 * c + tid)] = 0;
+    if (tid < 2) p.desc[kDesc * (2 * c + tid)] = 0;
     Walks<ROWS> walks(p, f, c);
     if (!walks.more()) return;
     for (;;) {
@@ -1329,7 +1334,7 @@ uint32_t row_class(const wl_tree_attn& a) {
 
 size_t tree_scratch(const wl_tree_attn& a) {
     const size_t rows = a.dtype == WL_TYPE_BF16 ? 2 * kGrid * row_class(a) : 2 * kGridF32 * 32;  // of parts
-    return rows * (128 * lat_class(a) + 2) * 4 + 2 * kGridF32 * 32;
+    return rows * (128 * lat_class(a) + 2) * 4 + 2 * kGridF32 * kDesc * 4;
 }
 
 template <int GR, int LC>
