@@ -52,7 +52,7 @@ struct Tree {
 // pieces of row tiles (all of a request's equally long, as many as need be) at most
 // that much longer than `per` (and a sixteenth) are no more than the work-groups,
 // work-group c takes piece c. One request of 64 nodes over 8192 keys, 32 bits: 222 us
-// without, 207 with; 5 of 7 nodes 67 and 59; 12 of 5 nodes 28 and 23. (A request of
+// without, 207 with; 5 of 7 nodes 67 and 59; 12 of 5 nodes 28 and 23; 32 contexts 191 and 179. (A request of
 // one row tile needs neither chunks nor pieces: its keys stand in a row.)
 constexpr uint32_t kSlack = 6;
 struct Req {
@@ -375,11 +375,11 @@ WL_DEV constexpr uint32_t swz4(uint32_t row) { return (row & 8u) >> 2; }
 // one more rounding of each value, the size of its own last rounding.
 //
 // Measured (512 + 64 columns, first launch + join): 64 requests of 8 nodes x 64
-// heads over up to 8192 keys, 205 + 17 us, 2326 clocks a tile of 64 rows: 1090 of
+// heads over up to 8192 keys, 205 + 16 us, 2326 clocks a tile of 64 rows: 1090 of
 // the matrix cores and 1120 of LDS (265 KB at 236 bytes a clock), mostly in turn.
 // 32 requests of one token x 64 heads over up to 65536 keys,
-// 791 MB: 162 + 13 us, in the loop 6.1 TB/s, 3346 clocks a tile, the rows' way from
-// HBM. One token over 4096 keys: 20 + 7.5 us, of which a walk's start (its request,
+// 791 MB: 162 + 12 us, in the loop 6.1 TB/s, 3346 clocks a tile, the rows' way from
+// HBM. One token over 4096 keys: 20 + 6.7 us, of which a walk's start (its request,
 // pages, queries, first tile) takes 7, its end 4 and the place search 2.5. What did
 // not carry: 64 keys a tile in a ring of two (282 us for the 64 requests), a running
 // maximum with the sums rescaled (spills; 16 us more), rows permuted instead of
@@ -742,8 +742,8 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
 // wrote them. The tile's parts are listed first, a thread per chunk of its keys.
 // Of few parts a wave joins a row by itself; many are dealt out to the four
 // waves, a quarter each, and their sums added in order. Lane: columns 4 lane + 256 k.
-// Parts to read and their number bound it: 33 MB in 17 us for the 32-bit kernel's
-// 512 parts of 32 rows, 7.5 us for one token's 64.
+// Parts to read and their number bound it: 33 MB in 12 us for 512 parts of 32 rows,
+// 6.7 us for one token's 65.
 constexpr uint32_t kManyParts = 16;
 template <uint32_t GRID, int ROWS, int LC, bool OBF>
 __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
