@@ -794,7 +794,8 @@ wl_status wl_paged_write(const wl_row_write* w, void* stream);
  * With 32-bit queries every product is right to 2^-23 of itself (exact with a
  * BF16 cache) and summed in f32; a value beyond the largest bf16 number, 3.39e38,
  * counts as an infinity. In a BF16 output's call the softmax weights are rounded
- * to bf16 once. Strides in elements from token to token, multiples of 8 up to
+ * to bf16 once and divided by the sum of what they are then. Of finite rows, scores
+ * in f32's range given, results are finite: they lie between the values. Strides in elements from token to token, multiples of 8 up to
  * 2^22; heads lie next to each other, at most 1024; 16-byte aligned. A request has at most
  * WL_TREE_MAX_NODES tokens (E_TREE). Tokens that no request holds stay as they
  * were. A request with an impossible length or more keys than its table row

@@ -98,6 +98,21 @@ def tree_attention(q, rows, L, scale, seen, q_type):
     return out, far + 1e-37
 
 
+def tree_attention_mean(q, rows, L, scale, seen, q_type):
+    """tree_attention for results that are means by rounded weights. For a bf16 output: with weights p (1 + d), |d| <=
+    2^-8, over their own sum the result is off by sum p d (c - out) / sum p (1 + d), at most 2^-8 / (1 - 2^-8) sum p |c -
+    out|, and 2^-8 of itself for its own rounding; f32 sums and exponentials as there."""
+    out, far = tree_attention(q, rows, L, scale, seen, "f32")
+    if q_type == "bf16" and seen.any():
+        k = rows[seen].astype(np.float64)
+        s = scale * q.astype(np.float64) @ k.T
+        p = np.exp(s - s.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        dev = np.stack([w @ np.abs(k[:, :L] - o) for w, o in zip(p, out)])
+        far = (far + U16 / (1 - U16) * dev) * (1 + U16) + U16 * np.abs(out)
+    return out, far
+
+
 class Map:
     """The buffers of a wl_page_map."""
 

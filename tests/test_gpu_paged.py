@@ -467,6 +467,17 @@ class Tree:
                     assert np.all(np.abs(got - y) <= far), (r, i, np.max(np.abs(got - y) / far))
 
 
+class Mean(Tree):
+    """A Tree whose bound is that of a mean by rounded weights."""
+    def want(self, r, i):
+        t, n, a = self.cu[r] + i, self.lens[r], self.adds[r]
+        bits = (2 << i) - 1 if self.masks is None else int(self.masks[t])
+        seen = np.array([True] * n + [bool(bits >> j & 1) for j in range(a)], bool)
+        q = np.concatenate([self.ql[t, :self.H * self.L].reshape(self.H, self.L),
+                            self.qr[t, :self.H * (self.W - self.L)].reshape(self.H, -1)], 1)
+        return P.tree_attention_mean(q, self.rows[r], self.L, self.scale, seen, self.qt)
+
+
 def random_trees(rng, adds):
     masks = []
     for a in adds:
@@ -577,6 +588,47 @@ def test_attention_magnitudes(gpu, q, cache):
     t.rows = [x * np.float32(2.0 ** -60) for x in t.rows]
     t.pages = t.pages * np.float32(2.0 ** -60)
     t.upload().run().check()
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("H,n", [(4, 500), (64, 1500)])
+def test_attention_large_rows_with_rising_scores(gpu, q, cache, H, n):
+    """Rows of some 2^66 against queries of 2^-66 (exact scalings): scores that rise by some 50 powers of two from a
+    tile of keys to the next, so that weights relative to an early tile, times the values, are beyond f32 where the
+    result is not."""
+    for sign in (1.0, -1.0):
+        t = Mean(32, q, cache, 128, 16, H, 16, [n], [2])
+        ramp = P.as_type(sign * 30.0 * (np.arange(n + 2) % 500 - 250) / 250, "bf16")
+        for k in range(n + 2):
+            t.rows[0][k, 128] = ramp[k]
+            t.pages[t.table[0, k // 16], k % 16, 128] = ramp[k]
+        t.qr[:, 0::16] = 128.0
+        t.ql, t.qr = t.ql * np.float32(2.0 ** -66), t.qr * np.float32(2.0 ** -66)
+        t.rows = [x * np.float32(2.0 ** 66) for x in t.rows]
+        t.pages = t.pages * np.float32(2.0 ** 66)
+        t.upload().run().check()
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("L,H,lens,adds", [(128, 4, [40, 900], [1, 3]), (512, 64, [5000], [1]), (256, 20, [700] * 40, [2] * 40),
+                                           (96, 16, [90] * 300, [1] * 300)], ids=["short", "parts", "pieces", "whole"])
+def test_attention_values_at_the_end_of_the_range(gpu, q, cache, L, H, lens, adds):
+    """Latent values next to the largest bf16 number, scores of the rotary parts alone: any result lies between the
+    values, whatever their unnormalised sums come to. (A call that is off by more than half a bf16 step of the largest
+    would give an infinity, which no bound lets pass.)"""
+    top = float(np.float32(2.0 ** 127 * (2 - 2.0 ** -7)))
+    for signs in (1.0, -1.0), (1.0, 1.0):
+        t = Mean(33, q, cache, L, 16, H, 16, lens, adds)
+        rng = np.random.default_rng(34)
+        t.ql[:] = 0.0
+        for r, rows in enumerate(t.rows):
+            n = len(rows)
+            big = np.where(rng.random((n, 1)) < 0.5, signs[0], signs[1]) * top * (1 - 0.1 * rng.random((n, L)))
+            rows[:, :L] = np.clip(P.as_type(big, cache), -top, top)
+            rows[:n // 2, :L] = np.where(rng.random((n // 2, 1)) < 0.5, signs[0], signs[1]) * top
+            for k in range(n):
+                t.pages[t.table[r, k // 16], k % 16, :L] = rows[k, :L]
+        t.upload().run().check()
 
 
 @pytest.mark.parametrize("q,cache", TYPES)

@@ -363,16 +363,20 @@ WL_DEV constexpr uint32_t swz4(uint32_t row) { return (row & 8u) >> 2; }
 // One barrier a tile: between two of them a wave makes the scores of tile t, then
 // sums tile t - 1 with the exponentials of tile t between the products.
 // m is a reference, not the maximum: that of the walk's first tile. Weights may
-// exceed 1 and lose nothing by it (bf16 and f32 keep their relative precision);
-// only where a weight passes kMost the walk is done again,
-// after one over the scores alone for the true maxima. So nothing is rescaled.
+// exceed 1 and lose nothing by it (bf16 and f32 keep their relative precision); only
+// where a weight passes kMost, or a sum of weighted values is not finite, the walk is
+// done again, after one over the scores alone for the true maxima, with a reference
+// above them (lift_of). So nothing is rescaled, and finite rows have finite results.
 // Key rows come into a ring of four tiles in LDS by DMA (16 bytes a lane): rows
 // behind the last key and columns behind the row's are read as zeros by the
 // resource's bounds. While tiles t - 1 and t are worked on, tile t + 2 is called
 // for between products; before the barrier each wave waits for its rows of t + 1.
-// P in bf16: a weight is off by 2^-9 of itself at the most and the sum that it is
-// divided by is of the weights before that, so an output's error is at most that of
-// one more rounding of each value, the size of its own last rounding.
+// P in bf16: a weight p is off by 2^-8 of itself at the most, and the sum that it is
+// divided by is of the rounded weights. So a result stays a mean of the values c: it is
+// off by 2^-8 sum p |c - out| / sum p at the most, never outside of them, and exact where
+// they are equal; its own rounding adds 2^-8 |out|. (Against 64 bits, 2-norms of all
+// outputs: 64 requests of 8 nodes 2.1e-3, with the sum of weights in 32 bits 2.2e-3,
+// their weights in 32 bits 1.7e-3, which is the outputs' own rounding.)
 //
 // Measured (512 + 64 columns, first launch + join): 64 requests of 8 nodes x 64
 // heads over up to 8192 keys, 205 + 16 us, 2326 clocks a tile of 64 rows: 1090 of
@@ -385,6 +389,22 @@ WL_DEV constexpr uint32_t swz4(uint32_t row) { return (row & 8u) >> 2; }
 // maximum with the sums rescaled (spills; 16 us more), rows permuted instead of
 // padded (232 us), loads by global addresses (the compiler then waits for all of them).
 constexpr float kMost = 0x1p64f;  // 2^31 such weights sum to 2^95
+// How far above its true maximum the reference of a walk that is done again lies, in
+// powers of two: the weights of all its keys then sum to 1/2 at the most, and no sum of
+// them and values is more than the largest of these. (The exponentials' arguments are
+// rounded at that size, 2^-20 for up to 2^15 keys. Scores of such a walk, 64 powers of
+// two apart, have no finer step; where only values are large, it is what they cost.)
+WL_DEV float lift_of(uint32_t keys) { return (float)(33u - (uint32_t)__clz((int)(keys - 1u))); }  // 1 + ceil(log2 keys), keys >= 2
+// Whether a value is not finite (a NaN is the largest of any).
+template <uint32_t N>
+WL_DEV bool nonfinite(const f32x4 (&y)[N]) {
+    float z = 0.f;
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) z = __builtin_elementwise_maximum(z, fabsf(y[k][j]));
+    return !(z <= 3.402823466e38f);
+}
 
 template <int GR, int LC>
 __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t min_per) {
@@ -589,7 +609,12 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
             const uint32_t put_at = (sr + n) * 64u + 16u * (g ^ swz4(n)) + sk / 2u;
             const uint32_t get_at = (pr + n) * 64u + 16u * (g ^ swz4(n));
             auto put_weights = [&](const float* e, uint8_t* pb) {
-                *(u32x2*)(pb + put_at) = u32x2{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
+                const u32x2 x = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
+                *(u32x2*)(pb + put_at) = x;
+                const float r[4] = {__uint_as_float(x[0] << 16), __uint_as_float(x[0] & 0xFFFF0000u),
+                                    __uint_as_float(x[1] << 16), __uint_as_float(x[1] & 0xFFFF0000u)};
+                l += (r[0] + r[1]) + (r[2] + r[3]);
+                pass |= fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])) > kMost;
             };
             // between two barriers: tile t - 1 is in b0 with weights w0, tile t in b1 with
             // weights w1 to be made, tile t + 2's place is b3; at t = kt1 the last sums
@@ -633,8 +658,6 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 if (!live) return false;
-                l += (e[0] + e[1]) + (e[2] + e[3]);
-                pass |= fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) > kMost;
                 vm_wait<DR + 2>();  // tile t + 1 is there; t + 2 and a page may be on the way
                 ring_barrier();
                 return true;
@@ -665,7 +688,6 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
 #pragma unroll
                     for (int k = 0; k < 4; k++) e[k] = exp2_(fmaf(s0[k], f, -m));
                     put_weights(e, pb0);
-                    l += (e[0] + e[1]) + (e[2] + e[3]);
                 }
                 vm_wait<DR + 2>();
                 ring_barrier();
@@ -677,9 +699,11 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                 }
                 vm_wait<0>();
                 if (first != kt0) break;
+#pragma unroll
+                for (uint32_t i = 0; i < 2; i++) pass |= pr + 16u * i + n < rows && nonfinite(acc[i]);
                 if (__ballot(pass) && lane == 0) again = 1u;
                 ring_barrier();
-                const bool redo = again != 0;
+                const bool redo = uni(again) != 0;
                 ring_barrier();
                 if (!redo) break;
                 if (tid == 0) again = 0u;
@@ -697,6 +721,7 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                     ring_barrier();
                 }
                 share_maxima(x);
+                m += lift_of((kt1 - kt0) * kKT);
                 ring_barrier();
                 first = ~0u;
             }
@@ -745,6 +770,8 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
 // Parts to read and their number bound it: 33 MB in 12 us for 512 parts of 32 rows,
 // 6.7 us for one token's 65.
 constexpr uint32_t kManyParts = 16;
+// The parts' weights are 1 at the most: as many finite sums, each times this, are finite.
+constexpr float kPart = 0.5f / (2 * kGridF32);
 template <uint32_t GRID, int ROWS, int LC, bool OBF>
 __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
     constexpr uint32_t COLS = 128 * LC, NV = (COLS + 255) / 256, Z = 1024 / GRID;
@@ -836,13 +863,13 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
 #pragma unroll 4
             for (uint32_t s = 0; s < S; s++) {
                 const float* ml = p.part_ml + 2 * at(s);
-                const float w = exp2_(ml[0] - M);
+                const float w = exp2_(ml[0] - M) * kPart;
                 sum += w * ml[1];
                 take(s, w);
             }
         } else {
             for (uint32_t s = lane; s < S; s += 64) {
-                const float w = exp2_(p.part_ml[2 * at(s)] - M);
+                const float w = exp2_(p.part_ml[2 * at(s)] - M) * kPart;
                 weight[wv][s] = w;
                 sum += w * p.part_ml[2 * at(s) + 1];
             }
@@ -1278,13 +1305,16 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
             using Sums = std::integral_constant<bool, true>;
             using Maxima = std::integral_constant<bool, false>;
             go(false, Sums{});
+#pragma unroll
+            for (uint32_t i = 0; i < 2; i++) pass |= 16u * i + (afresh(tid) & 15u) < rows && nonfinite(acc[i]);
             if (__ballot(pass) && (tid & 63u) == 0) again = 1u;
             ring_barrier();
-            const bool redo = again != 0;
+            const bool redo = uni(again) != 0;
             ring_barrier();
             if (redo) {
                 if (tid == 0) again = 0u;
                 share_maxima(go(true, Maxima{}));
+                m += lift_of((kt1 - kt0) * kKT);
                 go(true, Sums{});
             }
         }
