@@ -720,8 +720,9 @@ typedef struct wl_paged_cache {
  * E_LEN, E_SPACE, E_PAGE (*d_n_free, or what would be pushed, does not fit the
  * stack of n_pages entries) or too many nodes (E_TREE): the step is refused as
  * a whole: d_have_out and *d_n_free_out are what came in, d_cu is all 0, every
- * d_slot is -1, nothing else is written. A page outside the cache, in a table
- * or on the stack: E_PAGE, its tokens' slots are -1. n_req * max_pages < 2^31. */
+ * d_slot is -1, nothing else is written. A page outside the cache that this
+ * step uses or gives back: E_PAGE; its tokens' slots are -1, and one given back
+ * goes onto the stack as it is. n_req * max_pages < 2^31. */
 typedef struct wl_page_map {
     uint32_t n_req, page_size, n_pages;
     uint32_t max_pages;      /* entries per row of d_table */

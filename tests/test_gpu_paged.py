@@ -248,6 +248,21 @@ def test_map_pages_outside_the_cache(gpu):
     assert m.get("slot").tolist() == [-1, 15, -1, -1]  # a held page, a held one, and a taken one
 
 
+@pytest.mark.parametrize("flaw", [-1, 6, 2 ** 31 - 1])
+@pytest.mark.parametrize("trees", [False, True])
+def test_map_gives_back_pages_outside_the_cache(gpu, flaw, trees):
+    """Entries of an ended request that are no pages, with nobody who takes them in this step: they are found where
+    they are given back, not when another request is served with them."""
+    s = dict(ps=8, n_pages=6, max_pages=3, lens=[0, 7], adds=[0, 1], have=[3, 1], n_free=1, parent=np.array([-1]) if trees else None,
+             free=np.array([5, 0, 0, 0, 0, 0], np.int32), table=np.array([[2, flaw, 3], [1, -1, -1]], np.int32))
+    m = P.Map(**s)
+    paged.page_map(m.args)
+    hip.synchronize()
+    assert m.get("status")[0] == paged.E_PAGE
+    assert m.get("slot").tolist() == [15] and m.get("have_out").tolist() == [0, 1]
+    assert m.get("n_free_out")[0] == 4 and m.get("free")[:4].tolist() == [5, 2, flaw, 3]  # counts and order as always
+
+
 # ---- the write ----------------------------------------------------------------
 class Write:
     def __init__(self, seed, T, x, cache, L, RP, H, ps, pad=0, pos=None, slot=None, n_pages=None, src=None, n_kv=None,

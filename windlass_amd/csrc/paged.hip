@@ -158,8 +158,13 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
         const uint32_t r = owner(back, j);
         return m.d_table[(size_t)r * m.max_pages + need[r] + (j - back[r])];
     };
-    for (uint32_t j = gt; j < all.back; j += gn) m.d_free[(uint32_t)nf + j] = pushed(j);
     uint32_t flaw = 0;
+    auto in_cache = [&](int32_t page) { return page >= 0 && (uint32_t)page < m.n_pages; };
+    for (uint32_t j = gt; j < all.back; j += gn) {  // what is no page is told of here, and given back all the same
+        const int32_t page = pushed(j);
+        if (!in_cache(page)) flaw |= WL_PAGED_E_PAGE;
+        m.d_free[(uint32_t)nf + j] = page;
+    }
     // the slot of token i of request r; the first token of a new page writes the table's entry
     auto place = [&](uint32_t r, uint32_t i) {
         const uint32_t row = len[r] + i, k = row >> psh;
@@ -171,7 +176,7 @@ __global__ __launch_bounds__(THREADS) void page_map_kernel(wl_page_map m) {
             page = s >= (uint32_t)nf ? pushed(s - (uint32_t)nf) : m.d_free[s];
             if ((row & pmask) == 0) m.d_table[(size_t)r * m.max_pages + k] = page;
         }
-        const bool ok = page >= 0 && (uint32_t)page < m.n_pages;
+        const bool ok = in_cache(page);
         if (!ok) flaw |= WL_PAGED_E_PAGE;
         return ok ? (int32_t)(((uint32_t)page << psh) + (row & pmask)) : -1;
     };
