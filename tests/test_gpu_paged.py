@@ -552,6 +552,21 @@ def test_attention_pieces(gpu, q, cache, H, lens, adds):
 
 
 @pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("H,lens,adds,R", [(64, [2500], [7], 64), (20, [900, 333, 4000], [5, 64, 9], 64), (128, [70, 2100], [64, 1], 250)])
+def test_attention_requests_without_tokens_change_nothing(gpu, q, cache, H, lens, adds, R):
+    """A step with room for R requests of which a few are live: the others' results, bit for bit, of a call of the live
+    ones alone."""
+    a = Mean(35, q, cache, 128, 32, H, 16, lens, adds)
+    alone = a.upload().run().out()
+    at = [(k + 1) * R // (len(lens) + 1) for k in range(len(lens))]  # the live ones' places
+    b = Mean(35, q, cache, 128, 32, H, 16, [lens[at.index(r)] if r in at else 0 for r in range(R)],
+             [adds[at.index(r)] if r in at else 0 for r in range(R)])
+    assert np.array_equal(a.ql, b.ql) and np.array_equal(a.pages, b.pages, equal_nan=True)
+    assert np.array_equal(b.upload().run().out(), alone)
+    b.check()
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
 def test_attention_refused_among_pieces(gpu, q, cache):
     lens, adds = [2000, 300, 9, 1400], [2, 3, 1, 2]
     def tree():

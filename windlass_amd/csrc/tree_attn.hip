@@ -51,9 +51,11 @@ struct Tree {
 // a walk's start, its end and its part cost as much as some kSlack tiles. So where
 // pieces of row tiles (all of a request's equally long, as many as need be) at most
 // that much longer than `per` (and a sixteenth) are no more than the work-groups,
-// work-group c takes piece c. One request of 64 nodes over 8192 keys, 32 bits: 222 us
-// without, 207 with; 5 of 7 nodes 67 and 59; 12 of 5 nodes 28 and 23; 32 contexts 191 and 179. (A request of
-// one row tile needs neither chunks nor pieces: its keys stand in a row.)
+// work-group c takes piece c. (Requests without tokens change nothing of this, as
+// long as a launch has a thread for each: up to 256, 512 in work-groups of eight waves.)
+// One request of 64 nodes over 8192 keys, 32 bits: 222 us
+// without, 207 with; 5 of 7 nodes 67 and 59; 12 of 5 nodes 28 and 23; 32 contexts 191 and 179. (Requests of
+// one row tile need neither chunks nor pieces: their keys stand in a row.)
 constexpr uint32_t kSlack = 6;
 struct Req {
     uint32_t t0, nodes, len, keys, nrt, nkt, flaw;  // flaw: WL_PAGED_E_* (its rows get NaN)
@@ -136,18 +138,19 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
         __hip_atomic_fetch_or(p.a.d_status, status, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const uint64_t inc = sum_up(mine);
     tiles = sum_up(tiles);
+    const uint64_t several = __ballot(q.nrt > 1) ? 1ull << 32 : 0;  // a request (of a thread with one) has more than one
     if (lane == 63) {
         tmp[wv] = inc;
-        tmp[NW + 2 + wv] = tiles;
+        tmp[NW + 2 + wv] = several | tiles;
     }
     __syncthreads();
     Place f;
     f.total = 0;
-    tiles = 0;
+    uint64_t all = 0;
 #pragma unroll
     for (uint32_t w = 0; w < NW; w++) {
         f.total += tmp[w];
-        tiles += (uint32_t)tmp[NW + 2 + w];
+        all += tmp[NW + 2 + w];
     }
     f.per = (f.total + GRID - 1) / GRID;
     if (f.per < min_per) f.per = min_per;
@@ -155,7 +158,7 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
     f.pieces = 0;
     uint64_t at = inc - mine;
     for (uint32_t w = 0; w < wv; w++) at += tmp[w];
-    if (share == 1 && tiles > R && tiles < GRID && (f.total >> 32) == 0) {
+    if (share == 1 && (all >> 32) != 0 && (uint32_t)all < GRID && (f.total >> 32) == 0) {
         // the least of some lengths with which the pieces are no more than the work-groups
         const uint32_t per = (uint32_t)f.per, step = (kSlack + per / 16u + kTries - 2u) / (kTries - 1u);
         for (uint32_t k = wv; k < kTries; k += NW) {
