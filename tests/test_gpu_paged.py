@@ -725,6 +725,32 @@ def test_attention_rising_scores(gpu, q, cache):
         t.upload().run().check()
 
 
+@pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("lens,adds", [([9000], [2]), ([9000] + [1000] * 300, [2] + [1] * 300)], ids=["parts", "whole"])
+def test_attention_scores_that_rise_by_more_than_a_walk_can_hold(gpu, q, cache, lens, adds):
+    """Scores that rise by 70 powers of two from a tile of 32 keys to the next, in ramps of 11 tiles: every longer walk
+    is done again, the ones of five tiles and more around the ring of four, and every ramp's top counts."""
+    t = Mean(36, q, cache, 128, 16, 64 if len(lens) > 1 else 256, 16, lens, adds, spread=0.5)
+    n = max(lens) + max(adds)
+    powers = 70.0 * (np.arange(n) % (11 * 32)) / 32
+    t.qr[:, 0::16] = 128.0
+    ramp = P.as_type((powers - 385) * np.log(2) / (128 * t.scale), "bf16")
+    assert np.ptp(ramp[:32].astype(np.float64)) * 128 * t.scale / np.log(2) > 66
+    for r, rows in enumerate(t.rows):
+        rows[:, 128] = ramp[:len(rows)]
+        for k in range(len(rows)):
+            t.pages[t.table[r, k // 16], k % 16, 128] = ramp[k]
+    t.upload().run().check()
+
+
+@pytest.mark.parametrize("L,RP,H,lens,adds", [(256, 64, 4, [30, 0, 500], [3, 1, 2]), (200, 40, 4, [9000], [3]), (136, 8, 1, [700] * 280, [1] * 280),
+                                              (256, 64, 8, [40000, 5, 6], [1, 2, 1])], ids=["short", "parts", "whole", "long"])
+def test_attention_few_rows_and_a_middling_latent_part(gpu, L, RP, H, lens, adds):
+    """16-bit calls of at most 32 rows a request with latent parts of 129 to 256 columns, whole row tiles and parts."""
+    rng = np.random.default_rng(37)
+    Mean(38, "bf16", "bf16", L, RP, H, 16, lens, adds, random_trees(rng, adds)).upload().run().check()
+
+
 def test_attention_refused_requests(gpu):
     """Flaws that only the device sees spoil their own request and set their bit; everyone else is exact."""
     lens, adds = [20, 30, 9, 40], [2, 3, 1, 2]
