@@ -756,7 +756,7 @@ wl_status wl_paged_map(const wl_page_map* m, void* stream);
  * token's row; its rotary queries are written). d_src (may be NULL): token t's
  * kv row is d_kv[d_src[t]], of n_kv rows: after a verification the accepted
  * nodes' rows are written again, at their final slots, from the same
- * projections. A slot or source row outside its buffer: E_SLOT, passed over; a
+ * projections. A slot, or a source row for one, outside its buffer: E_SLOT, passed over; a
  * negative position: E_LEN, passed over and its queries not written. Slots are
  * distinct: where two tokens have the same one, its row is made of parts of
  * either. */

@@ -378,6 +378,17 @@ def test_write_accepted_rows_again(gpu):
     assert w.status() == 0
 
 
+@pytest.mark.parametrize("x,cache", [("f32", "f32"), ("bf16", "bf16")])
+def test_write_sources_behind_the_tokens(gpu, x, cache):
+    """A step captured with room for more writes rows again: what stands in d_src where the slots are -1 is not looked
+    at, and no flaw."""
+    w = Write(39, 7, x, cache, 64, 16, 2, 16, src=[2, 0, 3, -1, 4, 2 ** 31 - 1, -7], n_kv=4, slot=[5, 9, 0, -1, -1, -1, -1])
+    paged.write_rows(w.args)
+    hip.synchronize()
+    w.check()
+    assert w.status() == 0
+
+
 def test_write_flaws(gpu):
     w = Write(4, 6, "f32", "f32", 64, 16, 3, 16, n_pages=2, src=[0, 1, -1, 7, 3, 4], n_kv=7,
               slot=[32, -2, 4, 5, 6, 7], pos=[4, 5, 6, 7, -1, 8])

@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowWrite a) {
     };
     if (part == 0) {
         const uint32_t rows = w.cache.n_pages * w.cache.page_size;
-        const bool bad = slot < -1 || (slot >= 0 && (uint32_t)slot >= rows) || !src_ok;
+        const bool bad = slot < -1 || (slot >= 0 && ((uint32_t)slot >= rows || !src_ok));
         if (bad && lane == 0) set_status(w.d_status, WL_PAGED_E_SLOT);
         if (!bad && slot >= 0) {
             const size_t out = (size_t)slot * w.cache.row_stride;
