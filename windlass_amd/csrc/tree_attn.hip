@@ -13,11 +13,13 @@ namespace {
 
 constexpr uint32_t kKT = 32;    // keys of a tile
 // Key tiles of a walk at least: a shorter one's parts cost more to join than it saves.
-// One token over 4096 keys, both launches: 32.3 us at 1, 28.7 at 2, 29.3 at 4, 32.0 at 8;
-// 12 requests of 5 nodes, 32-bit queries: 29.8 at 1, 29.8 at 2, 33.3 at 4, 37.1 at 6.
+// Both launches in us at 1, 2, 3 and 4: one token x 64 heads over 4096 keys 31.0, 27.5, 27.8,
+// 28.0, with 32-bit queries 30.4, 28.6, 29.9, 31.6, 32 bits throughout (two of 16 keys)
+// 35.5, 38.4, 42.9, 49.8; 12 requests of up to 5 nodes, 32-bit queries, 22.1, 22.1, 22.9, 24.9.
 constexpr uint32_t kMinPer = 2;
 constexpr uint32_t kGrid = 256;      // work-groups of a launch of the 16-bit kernel: one per CU (LDS and registers allow one)
 constexpr uint32_t kGridF32 = 512;   // of the 32-bit one: two per CU
+constexpr uint32_t kRows16 = 64, kRows32 = 32;  // rows of their tiles
 constexpr float kNone = -3.0e38f;  // the running maximum of a row that has seen no key
 
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
@@ -355,8 +357,10 @@ WL_DEV constexpr uint32_t swz8(uint32_t row) { return (row & 2u) | ((row & 8u) >
 WL_DEV constexpr uint32_t swz4(uint32_t row) { return (row & 8u) >> 2; }
 
 // ---- 16-bit queries and cache --------------------------------------------------
-// ROWS = 32 GR rows (node, head) against 32 keys at a time, GR groups of four
-// waves with 32 rows each. In a group
+// 64 rows (node, head) against 32 keys at a time, two groups of four waves with 32
+// rows each. (One group for requests of at most 32 rows: one token of 32 heads over up to
+// 65536 keys, 32 requests, 512 columns, 163 us against 165; 256 columns 137 against 130,
+// 128 columns and 16 heads 121 against 113.) In a group
 //   S^T[keys][rows] = K Q^T: wave w takes row tile w / 2 and 16-key tile w % 2;
 //           its 16 rows' queries stay in its registers through the whole walk
 //           (4 LC + 2 steps of 32 columns);
@@ -409,9 +413,9 @@ WL_DEV bool nonfinite(const f32x4 (&y)[N]) {
     return !(z <= 3.402823466e38f);
 }
 
-template <int GR, int LC>
-__global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t min_per) {
-    constexpr uint32_t NW = 4 * GR, ROWS = 32 * GR, PITCH = 256 * LC + kPad, NL = 4 * LC, NS = NL + 2, CT = 2 * LC, DR = 32 / NW;
+template <int LC>
+__global__ __launch_bounds__(512) void tree_bf16_kernel(Tree p, uint32_t min_per) {
+    constexpr uint32_t NW = 8, ROWS = kRows16, PITCH = 256 * LC + kPad, NL = 4 * LC, NS = NL + 2, CT = 2 * LC, DR = 32 / NW;
     // the ring: separate objects, so that the compiler's own waits for DMA-written LDS stay per tile
     __shared__ __align__(1024) uint8_t ring0[kKT * (PITCH + 128)], ring1[kKT * (PITCH + 128)], ring2[kKT * (PITCH + 128)],
         ring3[kKT * (PITCH + 128)];
@@ -487,7 +491,7 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
                                                              0u, 0, 0);
             };
             auto issue_rot = [&](uint8_t* lat) {
-                if (DR == 8 || lane < 8 * DR)
+                if (lane < 8 * DR)
                     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, WL_LDS(lat + ROT + DR * wave * 128u), 16u, rot_at, 0u, 0, 0);
             };
             auto issue_tile = [&](uint8_t* lat, uint32_t t, int32_t page) {
@@ -775,7 +779,7 @@ __global__ __launch_bounds__(256 * GR) void tree_bf16_kernel(Tree p, uint32_t mi
 constexpr uint32_t kManyParts = 16;
 // The parts' weights are 1 at the most: as many finite sums, each times this, are finite.
 constexpr float kPart = 0.5f / (2 * kGridF32);
-template <uint32_t GRID, int ROWS, int LC, bool OBF>
+template <uint32_t GRID, uint32_t ROWS, int LC, bool OBF>
 __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
     constexpr uint32_t COLS = 128 * LC, NV = (COLS + 255) / 256, Z = 1024 / GRID;
     __shared__ f32x4 sums[4][NV][64];
@@ -959,7 +963,7 @@ WL_DEV uint32_t afresh(uint32_t x) {
 
 template <int LC, bool WIDE>
 __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_per) {
-    constexpr uint32_t ROWS = 32, KT = WIDE ? 16 : 32, PITCH = 256 * LC + kPad, NL = 4 * LC, NH = NL / 2 + 1, CT = 2 * LC;
+    constexpr uint32_t ROWS = kRows32, KT = WIDE ? 16 : 32, PITCH = 256 * LC + kPad, NL = 4 * LC, NH = NL / 2 + 1, CT = 2 * LC;
     constexpr uint32_t DR = KT / 4, NK = KT / 8, NP = WIDE ? 3 : 1, ROT = KT * PITCH, PIECE = ROT + KT * 128, ES = WIDE ? 4 : 2;
     __shared__ __align__(1024) uint8_t tile[NP * PIECE];
     __shared__ __align__(1024) uint8_t pb[3 * ROWS * 64];  // weights [operand][row][32 places]
@@ -1357,25 +1361,18 @@ uint32_t lat_class(const wl_tree_attn& a) {  // 128-column blocks of a row's lat
     const uint32_t b = (a.cache.kv_lora_rank + 127) / 128;
     return b <= 1 ? 1 : b <= 2 ? 2 : 4;
 }
-// Rows of the 16-bit kernel's tile: 64, or 32 where a request has no more on average.
-// One token, 32 requests over up to 65536 keys, both launches: of 64 heads 262 us with
-// 32 rows and 199 with 64; of 32 heads 175 and 183, of 16 heads 178 and 180.
-uint32_t row_class(const wl_tree_attn& a) {
-    const uint64_t rows = (uint64_t)a.n_heads * (a.n_req ? (a.n_tokens + a.n_req - 1) / a.n_req : 1);
-    return rows > 32 ? 64 : 32;
-}
+size_t part_rows(const wl_tree_attn& a) { return a.dtype == WL_TYPE_BF16 ? 2 * kGrid * kRows16 : 2 * kGridF32 * kRows32; }
 
 size_t tree_scratch(const wl_tree_attn& a) {
-    const size_t rows = a.dtype == WL_TYPE_BF16 ? 2 * kGrid * row_class(a) : 2 * kGridF32 * 32;  // of parts
-    return rows * (128 * lat_class(a) + 2) * 4 + 2 * kGridF32 * kDesc * 4;
+    return part_rows(a) * (128 * lat_class(a) + 2) * 4 + 2 * kGridF32 * kDesc * 4;
 }
 
-template <int GR, int LC>
+template <int LC>
 int run_bf16(const Tree& p, hipStream_t st) {
-    hipLaunchKernelGGL((tree_bf16_kernel<GR, LC>), dim3(kGrid), dim3(256 * GR), 0, st, p, kMinPer);
+    hipLaunchKernelGGL((tree_bf16_kernel<LC>), dim3(kGrid), dim3(512), 0, st, p, kMinPer);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL((tree_join_kernel<kGrid, 32 * GR, LC, true>), dim3(2 * kGrid, 4), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((tree_join_kernel<kGrid, kRows16, LC, true>), dim3(2 * kGrid, 4), dim3(256), 0, st, p);
     return (int)hipGetLastError();
 }
 
@@ -1384,7 +1381,7 @@ int run_f32(const Tree& p, hipStream_t st) {
     hipLaunchKernelGGL((tree_f32_kernel<LC, WIDE>), dim3(kGridF32), dim3(256), 0, st, p, kMinPer);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL((tree_join_kernel<kGridF32, 32, LC, false>), dim3(2 * kGridF32, 2), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((tree_join_kernel<kGridF32, kRows32, LC, false>), dim3(2 * kGridF32, 2), dim3(256), 0, st, p);
     return (int)hipGetLastError();
 }
 
@@ -1394,15 +1391,11 @@ int launch_tree(const wl_tree_attn& a, void* stream) {
     p.a = a;
     p.psh = 31u - (uint32_t)__builtin_clz(a.cache.page_size);
     p.scale2 = a.scale * 1.44269504088896340736f;
-    const uint32_t lc = lat_class(a), rows = row_class(a);
+    const uint32_t lc = lat_class(a);
     p.part = (float*)a.d_scratch;
-    const size_t parts = a.dtype == WL_TYPE_BF16 ? 2 * kGrid * rows : 2 * kGridF32 * 32;
-    p.part_ml = p.part + parts * 128 * lc;
-    p.desc = (uint32_t*)(p.part_ml + parts * 2);
-    if (a.dtype == WL_TYPE_BF16) {
-        if (rows == 64) return lc == 4 ? run_bf16<2, 4>(p, st) : lc == 2 ? run_bf16<2, 2>(p, st) : run_bf16<2, 1>(p, st);
-        return lc == 4 ? run_bf16<1, 4>(p, st) : lc == 2 ? run_bf16<1, 2>(p, st) : run_bf16<1, 1>(p, st);
-    }
+    p.part_ml = p.part + part_rows(a) * 128 * lc;
+    p.desc = (uint32_t*)(p.part_ml + part_rows(a) * 2);
+    if (a.dtype == WL_TYPE_BF16) return lc == 4 ? run_bf16<4>(p, st) : lc == 2 ? run_bf16<2>(p, st) : run_bf16<1>(p, st);
     if (a.cache.dtype == WL_TYPE_BF16)
         return lc == 4 ? run_f32<4, false>(p, st) : lc == 2 ? run_f32<2, false>(p, st) : run_f32<1, false>(p, st);
     return lc == 4 ? run_f32<4, true>(p, st) : lc == 2 ? run_f32<2, true>(p, st) : run_f32<1, true>(p, st);
