@@ -787,7 +787,8 @@ wl_status wl_paged_write(const wl_row_write* w, void* stream);
  * over the keys k that t sees, c_k | r_k the cache row of token k of its
  * request: every k < d_len[r], and of the request's tokens of this call (rows
  * d_len[r] + j, node j = token d_cu[r] + j, written before) those whose bit j
- * is set in d_mask[t]; d_mask NULL: j <= t - d_cu[r]. A token that sees no key
+ * is set in d_mask[t]; d_mask NULL: j <= t - d_cu[r]. There is no selection among
+ * the keys (wl_run_attention attends to index_topk of a longer context). A token that sees no key
  * gets zeros. Keys that a token does not see count for nothing, whatever
  * their rows hold; a NaN or an infinity in a row reaches the tokens that see
  * it. d_len, d_cu, d_mask and d_table are wl_paged_map's.
@@ -796,7 +797,8 @@ wl_status wl_paged_write(const wl_row_write* w, void* stream);
  * BF16 cache) and summed in f32; a value beyond the largest bf16 number, 3.39e38,
  * counts as an infinity. In a BF16 output's call the softmax weights are rounded
  * to bf16 once and divided by the sum of what they are then. Of finite rows, scores
- * in f32's range given, results are finite: they lie between the values. Strides in elements from token to token, multiples of 8 up to
+ * in f32's range given, results are finite and, to rounding, between the values.
+ * Strides in elements from token to token, multiples of 8 up to
  * 2^22; heads lie next to each other, at most 1024; 16-byte aligned. A request has at most
  * WL_TREE_MAX_NODES tokens (E_TREE). Tokens that no request holds stay as they
  * were. A request with an impossible length or more keys than its table row

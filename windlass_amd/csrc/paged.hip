@@ -28,9 +28,10 @@ WL_DEV void set_status(uint32_t* status, uint32_t bits) {
 // In a call with trees a wave takes a request, lane i its node i; otherwise a
 // thread takes a token, or four, and finds its request by bisection.
 // Bound by the launch and by latencies one after the other (lengths, the sums over
-// the requests, page, slot), not by bytes: 8 requests of 8 nodes 3.7 us (an empty
-// kernel takes 1.4); 256 of 64 nodes 5.7 us; 1000 prompts, 690k tokens, 5.5 MB out, 10.5 us
-// (14.7 with one token a thread).
+// the requests, page, slot), not by bytes: 8 requests of up to 8 nodes 3.8 us (an empty
+// kernel takes 1.4); 256 of up to 64 nodes, 5083 in all, 5.8 us; 1000 prompts, 661k
+// tokens, 5.3 MB out, 11 us (14.8 with one token a thread), of which the search over all
+// requests for every four tokens is most.
 struct Sums {
     uint64_t tok;
     uint32_t back, take;
@@ -49,8 +50,8 @@ constexpr uint32_t kMapGrid = 512;  // work-groups at the most
 // A thread takes four consecutive tokens, and searches once for their request, where
 // a step holds many more of them than requests and one each would be more threads
 // than half of the chip's places; otherwise one, so that lookups do not queue up in a
-// thread. Token each / four each: 200 requests with 126k tokens 5.7 / 7.6 us, 1000
-// with 165k 8.2 / 11.3, 327k 11.9 / 11.1, 690k 14.6 / 10.9; 256 with one each 9.8 / 13.3.
+// thread. Token each / four each: 200 requests with 126k tokens 5.6 / 7.5 us, 1000
+// with 165k 8.3 / 11.5, 327k 12.2 / 11.2, 661k 14.8 / 11.0; 256 with 1345 5.4 / 8.3.
 __host__ __device__ inline bool runs_of_4(const wl_page_map& m) {
     return m.max_tokens >= 64u * m.n_req && m.max_tokens > (1u << 18);
 }

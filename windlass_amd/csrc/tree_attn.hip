@@ -385,8 +385,8 @@ WL_DEV constexpr uint32_t swz4(uint32_t row) { return (row & 8u) >> 2; }
 // outputs: 64 requests of 8 nodes 2.1e-3, with the sum of weights in 32 bits 2.2e-3,
 // their weights in 32 bits 1.7e-3, which is the outputs' own rounding.)
 //
-// Measured (512 + 64 columns, first launch + join): 64 requests of 8 nodes x 64
-// heads over up to 8192 keys, 205 + 16 us, 2326 clocks a tile of 64 rows: 1090 of
+// Measured (512 + 64 columns, first launch + join): 64 requests of up to 8 nodes, 284
+// in all, x 64 heads over up to 8192 keys, 205 + 16 us, 2326 clocks a tile of 64 rows: 1090 of
 // the matrix cores and 1120 of LDS (265 KB at 236 bytes a clock), mostly in turn.
 // 32 requests of one token x 64 heads over up to 65536 keys,
 // 791 MB: 162 + 12 us, in the loop 6.1 TB/s, 3346 clocks a tile, the rows' way from
@@ -936,7 +936,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Tree p) {
 // nodes over up to 2000 32-bit rows 75 us; so, 242 and 58 us.) Values: 16 columns of
 // all rows at once. Of 16 keys, the 32 places of a product hold two parts of each:
 // (h, m) against the weights' (h, h) and (m, m), (h, l) against (l, h).
-// Lane addresses are computed where they are used (afresh): held, they spill.
+// Lane addresses are computed where they are used (afresh): held, they spill. (With 512
+// columns 2 registers a lane still do, 8 in WIDE.)
 //
 // Bound by the matrix cores: 102 (WIDE 102 of 16 keys) products a wave and tile, 16
 // clocks each. The 64 nodes' 73 GFLOP, three products each, take 181 us at the rate
