@@ -4,16 +4,12 @@
 
 #include <cmath>
 
-#include "dev_common.h"
 #include "paged.h"
+#include "paged_dev.h"
 
 namespace wl {
 namespace paged {
 namespace {
-
-WL_DEV void set_status(uint32_t* status, uint32_t bits) {
-    if (status && bits) __hip_atomic_fetch_or(status, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 
 // ---- the page map ---------------------------------------------------------
 // One launch. With n = len, a = add, h = have of a request and w = ceil((n +
@@ -300,19 +296,13 @@ WL_DEV void load8(const void* p, size_t i, float* v) {
         }
     }
 }
-WL_DEV uint32_t pack2(float a, float b) {
-    bf16x2 r;
-    r[0] = (__bf16)a;  // round to nearest even
-    r[1] = (__bf16)b;
-    return __builtin_bit_cast(uint32_t, r);
-}
 template <int N>
 WL_DEV void store_n(void* p, size_t i, const float* v, bool bf) {
     if (bf) {
 #pragma unroll
         for (int k = 0; k < N; k += 4) {
             typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
-            const u32x2 x = {pack2(v[k], v[k + 1]), pack2(v[k + 2], v[k + 3])};
+            const u32x2 x = {pack_bf16(v[k], v[k + 1]), pack_bf16(v[k + 2], v[k + 3])};
             gst((u32x2*)((uint16_t*)p + i + k), x);
         }
     } else {

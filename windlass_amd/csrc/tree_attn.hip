@@ -4,8 +4,8 @@
 
 #include <type_traits>
 
-#include "dev_common.h"
 #include "paged.h"
+#include "paged_dev.h"
 
 namespace wl {
 namespace paged {
@@ -136,8 +136,7 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
         }
     }
     rq[tid] = u32x2{q.nrt, q.nkt};
-    if (c == 0 && status && p.a.d_status)
-        __hip_atomic_fetch_or(p.a.d_status, status, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (c == 0 && status) set_status(p.a.d_status, status);
     const uint64_t inc = sum_up(mine);
     tiles = sum_up(tiles);
     const uint64_t several = __ballot(q.nrt > 1) ? 1ull << 32 : 0;  // a request (of a thread with one) has more than one
@@ -219,12 +218,6 @@ WL_DEV uint32_t chunks(const Req& q, uint64_t per) { return q.nrt == 1 || per > 
 WL_DEV uint32_t pieces_of(const Req& q, uint32_t len) { return (q.nkt + len - 1u) / len; }
 WL_DEV uint32_t chunk_at(const Req& q, uint32_t nc, uint32_t j) { return (uint32_t)div64((uint64_t)j * q.nkt, nc); }
 
-WL_DEV uint32_t pack_bf16(float a, float b) {
-    bf16x2 r;
-    r[0] = (__bf16)a;  // round to nearest even
-    r[1] = (__bf16)b;
-    return __builtin_bit_cast(uint32_t, r);
-}
 WL_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 WL_DEV bool has_nonfinite(u32x4 v) {
     bool f = false;
@@ -740,8 +733,7 @@ __global__ __launch_bounds__(512) void tree_bf16_kernel(Tree p, uint32_t min_per
         // the weights' sums over the row's lanes and waves; flaws
         if (__ballot(bad) && lane == 0) {
             bad_page = 1u;
-            if (p.a.d_status)
-                __hip_atomic_fetch_or(p.a.d_status, WL_PAGED_E_PAGE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            set_status(p.a.d_status, WL_PAGED_E_PAGE);
         }
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
@@ -1328,8 +1320,7 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
         }
         if (__ballot(bad) && (tid & 63u) == 0) {
             bad_page = 1u;
-            if (p.a.d_status)
-                __hip_atomic_fetch_or(p.a.d_status, WL_PAGED_E_PAGE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            set_status(p.a.d_status, WL_PAGED_E_PAGE);
         }
         const uint32_t lane = afresh(tid) & 63u, n = lane & 15u, g = lane >> 4;
         l += __shfl_xor(l, 16, 64);
