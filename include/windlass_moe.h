@@ -649,7 +649,11 @@ wl_status   wl_attn_taps(wl_attn* a, wl_attn_taps_out* out);
  *   per layer:
  *   wl_paged_write           the new tokens' cache rows (wl_run_attention's
  *                            prep stage) and their heads' rotary queries
- *   wl_paged_tree_attention  the new tokens' attention over the cache
+ *   wl_paged_tree_attention  the new tokens' attention over the cache, or
+ *   wl_paged_window_attention  through a sliding window with sinks
+ *   wl_token_logprobs        the drafted tokens' log probabilities, from the logits
+ *
+ * and wl_paged_read gives rows of the cache back as values.
  *
  * These calls have no context: every buffer is the caller's, named by an
  * argument block that may be kept and used again (a program keeps one per
@@ -669,6 +673,7 @@ wl_status   wl_attn_taps(wl_attn* a, wl_attn_taps_out* out);
  * written. */
 #define WL_TYPE_F32  0
 #define WL_TYPE_BF16 1
+#define WL_TYPE_MXFP4 4          /* of a cache's rows only */
 #define WL_PAGED_MAX_REQ   4096  /* requests in one call */
 #define WL_TREE_MAX_NODES  64    /* drafted tokens of one request in one call */
 #define WL_PAGED_E_LEN   1u      /* a length, a page count or a token range that cannot be */
@@ -683,8 +688,17 @@ const char* wl_paged_last_error(void);
  * kv_lora_rank + qk_rope, a multiple of 8), 16-byte aligned. A row holds the
  * normalised compressed key/value (kv_lora_rank values: a multiple of 8, at
  * most 512) and behind it the rotated key (qk_rope: a multiple of 8, 8 to 64).
- * dtype: WL_TYPE_F32, the precision of wl_run_attention's caches, or
- * WL_TYPE_BF16, half the bytes. A slot is page * page_size + row. */
+ * dtype: WL_TYPE_F32, the precision of wl_run_attention's caches, WL_TYPE_BF16,
+ * half the bytes, or WL_TYPE_MXFP4, the experts' format. Of a WL_TYPE_MXFP4 cache
+ * kv_lora_rank is a multiple of 32 and row_stride counts bytes, a multiple of 16; a
+ * row is kv_lora_rank / 2 bytes of E2M1 values (the low nibble is the even
+ * column), 16 bytes with one E8M0 scale per 32 columns (block b's at 4 (b % 4) + b /
+ * 4, 0 where there is no block) and the rotated key in bf16: 400 bytes at 512 + 64
+ * columns, 1152 in bf16. A block's scale is the least 2^e, -125 <= e <= 125,
+ * with which its largest magnitude is at most 6 (beyond that values are held to 6),
+ * a value the nearest of 0, 1/2, 1, 3/2, 2, 3, 4 and 6 times it, of two as near the
+ * one with the even code; a block with a NaN or an infinity has scale 255 and counts
+ * as NaN. A slot is page * page_size + row. */
 typedef struct wl_paged_cache {
     void*    d_rows;
     uint32_t dtype;
@@ -752,7 +766,8 @@ wl_status wl_paged_map(const wl_page_map* m, void* stream);
  * for every head's rotary query (d_q_rope_out may be d_q_rope itself). dtype:
  * the type of d_kv, d_q_rope and d_q_rope_out; strides in elements from token
  * to token, multiples of 8 up to 2^22; 16-byte aligned. Angles are computed in 64 bits,
- * everything else in 32, rounded once. A slot of -1 is passed over (as is its
+ * everything else in 32, rounded once; the compressed part for a 4-bit cache in 64
+ * bits (a rounding to 4 bits is a step of a third). A slot of -1 is passed over (as is its
  * token's row; its rotary queries are written). d_src (may be NULL): token t's
  * kv row is d_kv[d_src[t]], of n_kv rows: after a verification the accepted
  * nodes' rows are written again, at their final slots, from the same
@@ -779,6 +794,29 @@ typedef struct wl_row_write {
 } wl_row_write;
 wl_status wl_paged_write(const wl_row_write* w, void* stream);
 
+/* Reads rows back as values: of request r the tokens [d_first[r], d_first[r] + n),
+ * n = d_cu[r + 1] - d_cu[r], into rows d_cu[r], .. of d_out (kv_lora_rank + qk_rope
+ * values each, out_stride elements apart, a multiple of 8 up to 2^22; dtype:
+ * WL_TYPE_F32 or WL_TYPE_BF16, 16-byte aligned), whatever the cache's type: the matrix
+ * that kv_b_proj is multiplied with where a prefix is needed as keys and values. A
+ * value of the cache that d_out's type does not hold is rounded to nearest. d_first
+ * may be NULL: all 0. n_rows: rows of d_out; rows behind the last request's stay as
+ * they were. A negative d_first, tokens behind the table row's entries or rows
+ * outside [0, n_rows) (E_LEN): the request is left out. A page outside the cache
+ * (E_PAGE): NaN in its tokens' rows. */
+typedef struct wl_row_read {
+    wl_paged_cache cache;
+    uint32_t dtype, n_req, n_rows;
+    uint32_t max_pages;        /* entries per row of d_table */
+    const int32_t* d_table;    /* [n_req][max_pages] */
+    const int32_t* d_first;    /* [n_req] or NULL */
+    const int32_t* d_cu;       /* [n_req + 1] */
+    void* d_out;               /* [n_rows][kv_lora_rank + qk_rope] */
+    uint64_t out_stride;
+    uint32_t* d_status;
+} wl_row_read;
+wl_status wl_paged_read(const wl_row_read* r, void* stream);
+
 /* Attention of the tokens of n_req requests over the paged cache, in the
  * absorbed form: token t's head h has the query d_q_lat[t][h] (kv_lora_rank
  * values, the query taken through the key half of kv_b_proj) and
@@ -792,9 +830,11 @@ wl_status wl_paged_write(const wl_row_write* w, void* stream);
  * gets zeros. Keys that a token does not see count for nothing, whatever
  * their rows hold; a NaN or an infinity in a row reaches the tokens that see
  * it. d_len, d_cu, d_mask and d_table are wl_paged_map's.
- * dtype: the type of queries and output; WL_TYPE_BF16 needs a BF16 cache.
+ * dtype: the type of queries and output; WL_TYPE_BF16 needs a BF16 or MXFP4 cache.
+ * (Of 32 bf16 queries that meet one scale of an MXFP4 cache, those under a 120th of
+ * the largest are held to 2^-14 of it.)
  * With 32-bit queries every product is right to 2^-23 of itself (exact with a
- * BF16 cache) and summed in f32; a value beyond the largest bf16 number, 3.39e38,
+ * BF16 or MXFP4 cache) and summed in f32; a value beyond the largest bf16 number, 3.39e38,
  * counts as an infinity. In a BF16 output's call the softmax weights are rounded
  * to bf16 once and divided by the sum of what they are then. Of finite rows, scores
  * in f32's range given, results are finite and, to rounding, between the values.
@@ -829,6 +869,58 @@ typedef struct wl_tree_attn {
 } wl_tree_attn;
 size_t    wl_paged_tree_scratch(const wl_tree_attn* a);
 wl_status wl_paged_tree_attention(const wl_tree_attn* a, void* stream);
+
+/* The same through a sliding window that leaves the first tokens visible: of the keys
+ * that wl_paged_tree_attention gives token t, those at positions below n_sinks, and
+ * those fewer than `window` positions before t's own (window 1: itself), which is
+ * d_len[r] + the number of its ancestors. Key k of a request's d_len[r] tokens is
+ * at position k, a node that t sees at d_len[r] + the number of nodes that t sees
+ * before it. window 0: no window (n_sinks counts for nothing). Every type,
+ * d_scratch (wl_paged_tree_scratch(&w->tree) bytes) and refusal is
+ * wl_paged_tree_attention's. Pages without a key that the window or the sinks reach,
+ * 32 keys from key 0 on taken together, are not looked at: their entries of
+ * d_table may name pages that have been given to others. */
+typedef struct wl_window_attn {
+    wl_tree_attn tree;
+    uint32_t window, n_sinks;
+} wl_window_attn;
+wl_status wl_paged_window_attention(const wl_window_attn* w, void* stream);
+
+/* What a verification of drafted tokens reads from the model's logits. Row i of
+ * d_logits (n_vocab values, `stride` elements from row to row, dtype WL_TYPE_F32 or
+ * WL_TYPE_BF16) gives the distribution p = softmax(d_logits[i]):
+ *   d_logp[t]         log p of token d_token[t] in row d_row[t], of n_tokens tokens (a
+ *                     drafted node's row is its parent's); d_row NULL: row t
+ *   d_entropy[i]      -sum p log p, in nats (may be NULL)
+ *   d_top_id[i][j], d_top_logp[i][j]
+ *                     the n_top (0 to WL_LOGPROB_MAX_TOP, at most n_vocab) largest
+ *                     logits' ids, largest first, of equal ones the lowest id first,
+ *                     and their log p (both may be NULL if n_top is 0)
+ * Computed in f32 from the logits as they are. A logit of -infinity has p = 0 and
+ * log p = -infinity. In a row without a finite logit, or with a NaN or +infinity, log p
+ * and the entropy are NaN; ids are by order all the same, a NaN before any number. A
+ * token outside [0, n_vocab) or a row outside [0, n_rows): NaN, and E_SLOT.
+ * n_vocab up to 2^20, n_rows and n_tokens up to 2^20. Alignment: d_logits 16 bytes
+ * and stride a multiple of 8 are fastest, the elements' size is enough. d_scratch:
+ * wl_token_logprobs_scratch(a) bytes (0 if `a` is invalid), 16-byte aligned; it
+ * holds nothing between calls. Errors as the paged calls' (wl_paged_last_error). */
+#define WL_LOGPROB_MAX_TOP 32
+typedef struct wl_logprobs {
+    uint32_t dtype, n_rows, n_vocab, n_tokens, n_top;
+    const void* d_logits;      /* [n_rows][n_vocab] */
+    uint64_t stride;
+    const int32_t* d_token;    /* [n_tokens] */
+    const int32_t* d_row;      /* [n_tokens] or NULL */
+    float* d_logp;             /* [n_tokens] */
+    float* d_entropy;          /* [n_rows] or NULL */
+    float* d_top_logp;         /* [n_rows][n_top] */
+    int32_t* d_top_id;         /* [n_rows][n_top] */
+    void* d_scratch;
+    size_t scratch_bytes;
+    uint32_t* d_status;
+} wl_logprobs;
+size_t    wl_token_logprobs_scratch(const wl_logprobs* a);
+wl_status wl_token_logprobs(const wl_logprobs* a, void* stream);
 
 /* ---- single-expert building blocks ---------------------------------------
  * y[N] = W . x for MXFP4 W ([N,K/2] packed nibbles + [N,K/32] E8M0 scales) and

@@ -1,8 +1,9 @@
-// paged.hip — the page map of a step (wl_paged_map) and the write of its
-// latent cache rows (wl_paged_write).
+// paged.hip — the page map of a step (wl_paged_map), the write of its latent
+// cache rows (wl_paged_write) and their reading back (wl_paged_read).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "paged.h"
 #include "paged_dev.h"
@@ -311,7 +312,53 @@ WL_DEV void store_n(void* p, size_t i, const float* v, bool bf) {
     }
 }
 
-template <bool BF>
+// The compressed part of a row of a 4-bit cache, a lane's 8 values v with weights g:
+// everything in 64 bits, so that a value is on the side of a border between two 4-bit
+// ones that its exact value is on (in 32 bits about one in 2^20 is not, and a step is a
+// third of the value). Four lanes hold a block. It adds 512 x 7 64-bit comparisons a
+// token, some 3 us of the chip in 16384 tokens, beside their bytes.
+WL_DEV void store_mx(uint8_t* row, uint32_t lane, uint32_t L, const float* v, const float* g, float eps) {
+    double c[8], ss = 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; k++) ss += (double)v[k] * (double)v[k];
+    for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    const double rs = 1.0 / sqrt(ss / (double)L + (double)eps);
+    double most = 0.0;
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        c[k] = (double)v[k] * rs * (double)g[k];
+        bad |= !(fabs(c[k]) < INFINITY);
+        most = fmax(most, fabs(c[k]));
+    }
+    uint32_t nf = bad ? 1u : 0u;
+    for (int o = 1; o < 4; o <<= 1) {
+        most = fmax(most, __shfl_xor(most, o, 64));
+        nf |= __shfl_xor(nf, o, 64);
+    }
+    // the least e with most <= 6 2^e: 6 is 3/2 of 4
+    const uint64_t bits = (uint64_t)__double_as_longlong(most);
+    int32_t e = (int32_t)(bits >> 52) - 1023 - 2 + ((bits & 0xFFFFFFFFFFFFFull) > 0x8000000000000ull ? 1 : 0);
+    e = e < (int32_t)kMxLo - 127 ? (int32_t)kMxLo - 127 : e > (int32_t)kMxHi - 127 ? (int32_t)kMxHi - 127 : e;
+    const double inv = __longlong_as_double((int64_t)(1023 - e) << 52);
+    uint32_t word = 0;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const double a = fabs(c[k]) * inv;
+        const uint32_t code = (a > 0.25 ? 1u : 0u) + (a >= 0.75 ? 1u : 0u) + (a > 1.25 ? 1u : 0u) + (a >= 1.75 ? 1u : 0u) +
+                              (a > 2.5 ? 1u : 0u) + (a >= 3.5 ? 1u : 0u) + (a > 5.0 ? 1u : 0u);
+        word |= (code | (code && c[k] < 0.0 ? 8u : 0u)) << (4 * k);
+    }
+    if (8u * lane < L) gst((uint32_t*)row + lane, word);
+    // lane j < 4 has the scales of blocks j, 4 + j, 8 + j and 12 + j, each from its block's first lane
+    const uint32_t mine = 8u * lane < L ? (nf ? 255u : (uint32_t)(e + 127)) : 0u;
+    uint32_t scales = 0;
+#pragma unroll
+    for (uint32_t s = 0; s < 4; s++) scales |= __shfl(mine, (int)(16u * s + 4u * (lane & 3u)), 64) << (8u * s);
+    if (lane < 4) gst((uint32_t*)(row + L / 2) + lane, scales);
+}
+
+template <bool BF, bool MX>
 __global__ __launch_bounds__(256) void row_write_kernel(RowWrite a) {
     const wl_row_write& w = a.w;
     const uint32_t lane = threadIdx.x & 63u, wave = blockIdx.x * 4u + (threadIdx.x >> 6);
@@ -361,7 +408,21 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowWrite a) {
         const uint32_t rows = w.cache.n_pages * w.cache.page_size;
         const bool bad = slot < -1 || (slot >= 0 && ((uint32_t)slot >= rows || !src_ok));
         if (bad && lane == 0) set_status(w.d_status, WL_PAGED_E_SLOT);
-        if (!bad && slot >= 0) {
+        if (MX && !bad && slot >= 0) {
+            uint8_t* row = (uint8_t*)w.cache.d_rows + (size_t)slot * w.cache.row_stride;
+            if (i >= L) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) g[k] = 0.f;
+            }
+            store_mx(row, lane, L, v, g, w.eps);
+            if (lane < cph) {
+                float lo[4], hi[4];
+                turn(r, lo, hi);
+                store_n<4>(row + L / 2 + kMxScales, 4 * c, lo, true);
+                store_n<4>(row + L / 2 + kMxScales, HP + 4 * c, hi, true);
+            }
+        }
+        if (!MX && !bad && slot >= 0) {
             const size_t out = (size_t)slot * w.cache.row_stride;
             float ss = 0.f;
 #pragma unroll
@@ -398,7 +459,72 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowWrite a) {
     }
 }
 
+// ---- rows as values -----------------------------------------------------------
+// A thread has 8 values of a row, so a row's chunks, the rotary ones among them, lie in
+// a row over the threads; a request's rows are dealt out to the work-groups of its
+// column of the grid. Bound by the bytes.
+template <int CT, bool OBF>
+__global__ __launch_bounds__(256) void row_read_kernel(wl_row_read p, uint32_t psh) {
+    constexpr bool MX = CT == WL_TYPE_MXFP4;
+    const uint32_t r = blockIdx.y, L = p.cache.kv_lora_rank, RP = p.cache.qk_rope, cl = L / 8u, per = cl + RP / 8u;
+    const int32_t c0 = p.d_cu[r], c1 = p.d_cu[r + 1], first = p.d_first ? p.d_first[r] : 0;
+    const bool head = blockIdx.x == 0 && threadIdx.x == 0;
+    if (c0 == c1) return;
+    if (c0 < 0 || c1 < c0 || (uint32_t)c1 > p.n_rows || first < 0 ||
+        (uint64_t)(uint32_t)first + (uint32_t)(c1 - c0) > ((uint64_t)p.max_pages << psh)) {
+        if (head) set_status(p.d_status, WL_PAGED_E_LEN);
+        return;
+    }
+    const uint32_t n = (uint32_t)(c1 - c0) * per;  // n_rows <= 2^24, per <= 72
+    for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < n; i += gridDim.x * 256u) {
+        const uint32_t j = i / per, k = i - j * per, key = (uint32_t)first + j;
+        const int32_t page = p.d_table[(size_t)r * p.max_pages + (key >> psh)];
+        float v[8];
+        if (page < 0 || (uint32_t)page >= p.cache.n_pages) {
+            if (k == 0) set_status(p.d_status, WL_PAGED_E_PAGE);
+#pragma unroll
+            for (int m = 0; m < 8; m++) v[m] = __builtin_nanf("");
+        } else {
+            const size_t at = (((size_t)(uint32_t)page << psh) + (key & (p.cache.page_size - 1u))) * p.cache.row_stride;
+            if (MX) {
+                const uint8_t* row = (const uint8_t*)p.cache.d_rows + at;
+                if (k < cl) {
+                    const uint32_t s = gld1(row + L / 2 + mx_scale_at(k / 4u));
+                    const u32x4 x = __builtin_bit_cast(u32x4, fp4x8_bf16(gld((const uint32_t*)row + k), e8m0f(s)));
+#pragma unroll
+                    for (int m = 0; m < 4; m++) {
+                        v[2 * m] = s == 255u ? __builtin_nanf("") : __uint_as_float(x[m] << 16);
+                        v[2 * m + 1] = s == 255u ? __builtin_nanf("") : __uint_as_float(x[m] & 0xFFFF0000u);
+                    }
+                } else {
+                    load8<true>(row + L / 2 + kMxScales, 8u * (k - cl), v);
+                }
+            } else {
+                load8<CT == WL_TYPE_BF16>(p.cache.d_rows, at + 8u * k, v);
+            }
+        }
+        store_n<8>(p.d_out, (size_t)((uint32_t)c0 + j) * p.out_stride + 8u * k, v, OBF);
+    }
+}
+
 }  // namespace
+
+int launch_read(const wl_row_read& r, void* stream) {
+    const uint32_t psh = 31u - (uint32_t)__builtin_clz(r.cache.page_size), per = (r.cache.kv_lora_rank + r.cache.qk_rope) / 8u;
+    // enough work-groups for the longest request, whichever it is, 4096 in all at the most
+    const uint32_t most = r.n_req >= 4096u ? 1u : 4096u / r.n_req, need = (uint32_t)(((uint64_t)r.n_rows * per + 255u) / 256u);
+    const dim3 grid(need < most ? need : most, r.n_req);
+    hipStream_t st = (hipStream_t)stream;
+    auto go = [&](auto ct) {
+        constexpr int CT = decltype(ct)::value;
+        if (r.dtype == WL_TYPE_BF16) hipLaunchKernelGGL((row_read_kernel<CT, true>), grid, dim3(256), 0, st, r, psh);
+        else hipLaunchKernelGGL((row_read_kernel<CT, false>), grid, dim3(256), 0, st, r, psh);
+        return (int)hipGetLastError();
+    };
+    return r.cache.dtype == WL_TYPE_MXFP4  ? go(std::integral_constant<int, WL_TYPE_MXFP4>{})
+           : r.cache.dtype == WL_TYPE_BF16 ? go(std::integral_constant<int, WL_TYPE_BF16>{})
+                                           : go(std::integral_constant<int, WL_TYPE_F32>{});
+}
 
 int launch_map(const wl_page_map& m, void* stream) {
     const bool trees = m.d_parent || m.d_mask;
@@ -433,8 +559,10 @@ int launch_write(const wl_row_write& w, void* stream) {
     a.wpt = rounds < 1 ? 1 : rounds > 4 ? 4 : rounds;
     const uint32_t wgs = (uint32_t)(((uint64_t)w.n_tokens * a.wpt + 3) / 4);
     hipStream_t st = (hipStream_t)stream;
-    if (w.dtype == WL_TYPE_BF16) hipLaunchKernelGGL(row_write_kernel<true>, dim3(wgs), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(row_write_kernel<false>, dim3(wgs), dim3(256), 0, st, a);
+    const bool mx = w.cache.dtype == WL_TYPE_MXFP4;
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(wgs), dim3(256), 0, st, a); };
+    if (w.dtype == WL_TYPE_BF16) mx ? go(row_write_kernel<true, true>) : go(row_write_kernel<true, false>);
+    else mx ? go(row_write_kernel<false, true>) : go(row_write_kernel<false, false>);
     return (int)hipGetLastError();
 }
 

@@ -1,6 +1,8 @@
 // paged_dev.h — device helpers that the paged-cache kernels (paged.hip,
 // tree_attn.hip) share. Not public ABI.
 #pragma once
+#include <type_traits>
+
 #include "dev_common.h"
 
 namespace wl {
@@ -15,6 +17,31 @@ WL_DEV uint32_t pack_bf16(float a, float b) {  // a in the low half
     r[0] = (__bf16)a;  // round to nearest even
     r[1] = (__bf16)b;
     return __builtin_bit_cast(uint32_t, r);
+}
+
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+// A block of 32 E2M1 values and its scale byte as bf16 (exact) into LDS at dst, the
+// 16-byte pieces in the order turn, turn + 1, .. (mod 4). A block of scale 255 (NaN) is
+// `nan`, two values.
+WL_DEV void put_mx(u32x4 x, uint32_t scale, uint8_t* dst, uint32_t turn, uint32_t nan) {
+    const bool t1 = turn & 1u, t2 = turn & 2u;
+    const u32x4 y = t1 ? u32x4{x[1], x[2], x[3], x[0]} : x, z = t2 ? u32x4{y[2], y[3], y[0], y[1]} : y;
+    const float s = __uint_as_float(scale << 23);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) {
+        u32x4 v = __builtin_bit_cast(u32x4, fp4x8_bf16(z[j], s));
+        if (scale == 255u) v = u32x4{nan, nan, nan, nan};
+        *(u32x4*)(dst + 16u * ((turn + j) & 3u)) = v;
+    }
+}
+
+// f(0), .., f(N - 1) with constants
+template <int N, class F>
+WL_DEV void static_for(F f) {
+    if constexpr (N > 0) {
+        static_for<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
 }
 
 }  // namespace paged

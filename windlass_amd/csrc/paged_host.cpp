@@ -1,6 +1,7 @@
-// paged_host.cpp — the C ABI of the paged cache (wl_paged_*): checks of the
-// argument blocks, then the launches of paged.hip and tree_attn.hip. No state
-// but this thread's last message.
+// paged_host.cpp — the C ABI of the paged cache (wl_paged_*) and of the drafted
+// tokens' log probabilities: checks of the argument blocks, then the launches of
+// paged.hip, tree_attn.hip, tree_mx4.hip and logprobs.hip. No state but this
+// thread's last message.
 #include <hip/hip_runtime.h>
 
 #include <cstdarg>
@@ -30,9 +31,19 @@ bool overlap(const void* a, size_t na, const void* b, size_t nb) {
 }
 size_t esize(uint32_t t) { return t == WL_TYPE_F32 ? 4 : 2; }
 
+// Bytes of a cache's row, of all its rows.
+size_t row_bytes(const wl_paged_cache& c) {
+    if (c.dtype == WL_TYPE_MXFP4) return c.kv_lora_rank / 2 + wl::paged::kMxScales + 2 * c.qk_rope;
+    return (c.kv_lora_rank + c.qk_rope) * esize(c.dtype);
+}
+size_t cache_bytes(const wl_paged_cache& c) {
+    const size_t stride = c.row_stride * (c.dtype == WL_TYPE_MXFP4 ? 1 : esize(c.dtype));
+    return ((size_t)c.n_pages * c.page_size - 1) * stride + row_bytes(c);
+}
+
 wl_status check_cache(const wl_paged_cache& c) {
     if (!c.d_rows || !aligned(c.d_rows, 16)) return fail(WL_ERR_INVALID, "the cache must be 16-byte aligned and not null");
-    if (c.dtype > WL_TYPE_BF16) return fail(WL_ERR_INVALID, "cache type %u", c.dtype);
+    if (c.dtype > WL_TYPE_BF16 && c.dtype != WL_TYPE_MXFP4) return fail(WL_ERR_INVALID, "cache type %u", c.dtype);
     if (!pow2_page(c.page_size)) return fail(WL_ERR_INVALID, "page_size %u: a power of two, 8 to 1024", c.page_size);
     if (c.n_pages == 0 || (uint64_t)c.n_pages * c.page_size >= (1ull << 31))
         return fail(WL_ERR_INVALID, "n_pages x page_size must be in [1, 2^31)");
@@ -40,6 +51,12 @@ wl_status check_cache(const wl_paged_cache& c) {
         return fail(WL_ERR_INVALID, "kv_lora_rank %u: a multiple of 8, 8 to 512", c.kv_lora_rank);
     if (c.qk_rope == 0 || c.qk_rope % 8 || c.qk_rope > wl::paged::kMaxRope)
         return fail(WL_ERR_INVALID, "qk_rope %u: a multiple of 8, 8 to %u", c.qk_rope, wl::paged::kMaxRope);
+    if (c.dtype == WL_TYPE_MXFP4) {
+        if (c.kv_lora_rank % 32) return fail(WL_ERR_INVALID, "kv_lora_rank %u: a multiple of 32 in a 4-bit cache", c.kv_lora_rank);
+        if (c.row_stride % 16 || c.row_stride < row_bytes(c) || c.row_stride > (1u << 21))
+            return fail(WL_ERR_INVALID, "row_stride %u: bytes, a multiple of 16, %zu to 2^21", c.row_stride, row_bytes(c));
+        return WL_OK;
+    }
     if (c.row_stride % 8 || c.row_stride < c.kv_lora_rank + c.qk_rope || c.row_stride > (1u << 20))
         return fail(WL_ERR_INVALID, "row_stride %u: a multiple of 8, at least kv_lora_rank + qk_rope", c.row_stride);
     return WL_OK;
@@ -84,13 +101,58 @@ wl_status check_tree(const wl_tree_attn* a) {
     wl_status s = check_cache(a->cache);
     if (s != WL_OK) return s;
     if (a->dtype > WL_TYPE_BF16) return fail(WL_ERR_INVALID, "type %u", a->dtype);
-    if (a->dtype == WL_TYPE_BF16 && a->cache.dtype != WL_TYPE_BF16)
-        return fail(WL_ERR_INVALID, "bf16 queries need a bf16 cache");
+    if (a->dtype == WL_TYPE_BF16 && a->cache.dtype == WL_TYPE_F32)
+        return fail(WL_ERR_INVALID, "bf16 queries need a bf16 or 4-bit cache");
     if (a->n_req > WL_PAGED_MAX_REQ) return fail(WL_ERR_INVALID, "n_req %u exceeds %u", a->n_req, WL_PAGED_MAX_REQ);
     if (a->n_heads == 0 || a->n_heads > 1024) return fail(WL_ERR_INVALID, "n_heads %u: 1 to 1024", a->n_heads);
     if (a->n_tokens > (1u << 20)) return fail(WL_ERR_INVALID, "n_tokens %u exceeds 2^20", a->n_tokens);
     if (a->max_pages == 0 || (uint64_t)a->max_pages * a->cache.page_size >= (1ull << 31))
         return fail(WL_ERR_INVALID, "max_pages x page_size must be in [1, 2^31)");
+    return WL_OK;
+}
+
+// The call through a window (0: none).
+wl_status attend(const wl_tree_attn* a, uint32_t window, uint32_t sinks, const char* what, void* stream) {
+    wl_status s = check_tree(a);
+    if (s != WL_OK) return s;
+    if (a->n_req == 0 || a->n_tokens == 0) return WL_OK;
+    const wl_paged_cache& c = a->cache;
+    const uint64_t H = a->n_heads, L = c.kv_lora_rank, P = c.qk_rope;
+    if ((s = check_rows(a->d_q_lat, a->q_lat_stride, H * L, "d_q_lat")) != WL_OK) return s;
+    if ((s = check_rows(a->d_q_rope, a->q_rope_stride, H * P, "d_q_rope")) != WL_OK) return s;
+    if ((s = check_rows(a->d_out, a->out_stride, H * L, "d_out")) != WL_OK) return s;
+    if (!a->d_table || !a->d_len || !a->d_cu || !aligned(a->d_table, 4) || !aligned(a->d_len, 4) || !aligned(a->d_cu, 4) ||
+        !aligned(a->d_mask, 8) || !aligned(a->d_status, 4))
+        return fail(WL_ERR_INVALID, "d_table, d_len and d_cu must be set and 4-byte aligned, d_mask 8-byte");
+    const size_t need = wl::paged::tree_scratch(*a);
+    if (!a->d_scratch || !aligned(a->d_scratch, 16) || a->scratch_bytes < need)
+        return fail(WL_ERR_INVALID, "scratch of %zu bytes (%zu needed, 16-byte aligned)", a->scratch_bytes, need);
+    const size_t on = span(a->out_stride, H * L, a->n_tokens, a->dtype);
+    const struct {
+        const void* p;
+        size_t n;
+    } in[] = {{a->d_q_lat, span(a->q_lat_stride, H * L, a->n_tokens, a->dtype)},
+              {a->d_q_rope, span(a->q_rope_stride, H * P, a->n_tokens, a->dtype)},
+              {c.d_rows, cache_bytes(c)},
+              {a->d_table, 4 * (size_t)a->n_req * a->max_pages},
+              {a->d_len, 4 * (size_t)a->n_req},
+              {a->d_cu, 4 * ((size_t)a->n_req + 1)},
+              {a->d_mask, 8 * (size_t)a->n_tokens},
+              {a->d_status, 4}};
+    for (const auto& x : in)
+        if (overlap(a->d_out, on, x.p, x.n) || overlap(a->d_scratch, need, x.p, x.n))
+            return fail(WL_ERR_INVALID, "d_out or d_scratch overlaps an input");
+    if (overlap(a->d_out, on, a->d_scratch, need)) return fail(WL_ERR_INVALID, "d_scratch overlaps d_out");
+    return on_device_of(stream, what, [&] { return wl::paged::launch_tree(*a, window, sinks, stream); });
+}
+
+wl_status check_logprobs(const wl_logprobs* a) {
+    if (!a) return fail(WL_ERR_INVALID, "the argument block is null");
+    if (a->dtype > WL_TYPE_BF16) return fail(WL_ERR_INVALID, "type %u", a->dtype);
+    if (a->n_vocab == 0 || a->n_vocab > (1u << 20)) return fail(WL_ERR_INVALID, "n_vocab %u: 1 to 2^20", a->n_vocab);
+    if (a->n_rows > (1u << 20) || a->n_tokens > (1u << 20)) return fail(WL_ERR_INVALID, "n_rows and n_tokens: up to 2^20");
+    if (a->n_top > WL_LOGPROB_MAX_TOP || a->n_top > a->n_vocab)
+        return fail(WL_ERR_INVALID, "n_top %u: up to %u and n_vocab", a->n_top, WL_LOGPROB_MAX_TOP);
     return WL_OK;
 }
 
@@ -155,8 +217,7 @@ wl_status wl_paged_write(const wl_row_write* w, void* stream) {
     if (!w->d_pos || !w->d_slot || !aligned(w->d_pos, 4) || !aligned(w->d_slot, 4) || !aligned(w->d_src, 4) ||
         !aligned(w->d_status, 4))
         return fail(WL_ERR_INVALID, "d_pos and d_slot must be set, and index arrays 4-byte aligned");
-    const size_t rows = (size_t)c.n_pages * c.page_size;
-    const size_t cache_n = span(c.row_stride, W, rows, c.dtype);
+    const size_t cache_n = cache_bytes(c);
     const size_t kv_n = span(w->kv_stride, W, w->d_src ? w->n_kv : w->n_tokens, w->dtype);
     if (overlap(c.d_rows, cache_n, w->d_kv, kv_n)) return fail(WL_ERR_INVALID, "the cache overlaps d_kv");
     if (w->n_heads) {
@@ -179,37 +240,79 @@ size_t wl_paged_tree_scratch(const wl_tree_attn* a) {
 }
 
 wl_status wl_paged_tree_attention(const wl_tree_attn* a, void* stream) {
-    wl_status s = check_tree(a);
+    return attend(a, 0, 0, "wl_paged_tree_attention", stream);
+}
+
+wl_status wl_paged_window_attention(const wl_window_attn* w, void* stream) {
+    if (!w) return fail(WL_ERR_INVALID, "the argument block is null");
+    // positions are below 2^31: a longer window, or more sinks, leave out no more
+    const uint32_t most = 0x7FFFFFFFu;
+    return attend(&w->tree, w->window < most ? w->window : most, w->n_sinks < most ? w->n_sinks : most,
+                  "wl_paged_window_attention", stream);
+}
+
+wl_status wl_paged_read(const wl_row_read* r, void* stream) {
+    if (!r) return fail(WL_ERR_INVALID, "the argument block is null");
+    wl_status s = check_cache(r->cache);
     if (s != WL_OK) return s;
-    if (a->n_req == 0 || a->n_tokens == 0) return WL_OK;
-    const wl_paged_cache& c = a->cache;
-    const uint64_t H = a->n_heads, L = c.kv_lora_rank, P = c.qk_rope;
-    if ((s = check_rows(a->d_q_lat, a->q_lat_stride, H * L, "d_q_lat")) != WL_OK) return s;
-    if ((s = check_rows(a->d_q_rope, a->q_rope_stride, H * P, "d_q_rope")) != WL_OK) return s;
-    if ((s = check_rows(a->d_out, a->out_stride, H * L, "d_out")) != WL_OK) return s;
-    if (!a->d_table || !a->d_len || !a->d_cu || !aligned(a->d_table, 4) || !aligned(a->d_len, 4) || !aligned(a->d_cu, 4) ||
-        !aligned(a->d_mask, 8) || !aligned(a->d_status, 4))
-        return fail(WL_ERR_INVALID, "d_table, d_len and d_cu must be set and 4-byte aligned, d_mask 8-byte");
-    const size_t need = wl::paged::tree_scratch(*a);
-    if (!a->d_scratch || !aligned(a->d_scratch, 16) || a->scratch_bytes < need)
-        return fail(WL_ERR_INVALID, "scratch of %zu bytes (%zu needed, 16-byte aligned)", a->scratch_bytes, need);
-    const size_t on = span(a->out_stride, H * L, a->n_tokens, a->dtype);
+    if (r->dtype > WL_TYPE_BF16) return fail(WL_ERR_INVALID, "type %u", r->dtype);
+    if (r->n_req > WL_PAGED_MAX_REQ) return fail(WL_ERR_INVALID, "n_req %u exceeds %u", r->n_req, WL_PAGED_MAX_REQ);
+    if (r->n_rows > (1u << 24)) return fail(WL_ERR_INVALID, "n_rows %u exceeds 2^24", r->n_rows);
+    if (r->max_pages == 0 || (uint64_t)r->max_pages * r->cache.page_size >= (1ull << 31))
+        return fail(WL_ERR_INVALID, "max_pages x page_size must be in [1, 2^31)");
+    if (r->n_req == 0 || r->n_rows == 0) return WL_OK;
+    const uint64_t W = r->cache.kv_lora_rank + r->cache.qk_rope;
+    if ((s = check_rows(r->d_out, r->out_stride, W, "d_out")) != WL_OK) return s;
+    if (!r->d_table || !r->d_cu || !aligned(r->d_table, 4) || !aligned(r->d_first, 4) || !aligned(r->d_cu, 4) ||
+        !aligned(r->d_status, 4))
+        return fail(WL_ERR_INVALID, "d_table and d_cu must be set, and index arrays 4-byte aligned");
+    const size_t on = span(r->out_stride, W, r->n_rows, r->dtype);
     const struct {
         const void* p;
         size_t n;
-    } in[] = {{a->d_q_lat, span(a->q_lat_stride, H * L, a->n_tokens, a->dtype)},
-              {a->d_q_rope, span(a->q_rope_stride, H * P, a->n_tokens, a->dtype)},
-              {c.d_rows, span(c.row_stride, L + P, (size_t)c.n_pages * c.page_size, c.dtype)},
-              {a->d_table, 4 * (size_t)a->n_req * a->max_pages},
-              {a->d_len, 4 * (size_t)a->n_req},
-              {a->d_cu, 4 * ((size_t)a->n_req + 1)},
-              {a->d_mask, 8 * (size_t)a->n_tokens},
-              {a->d_status, 4}};
+    } in[] = {{r->cache.d_rows, cache_bytes(r->cache)},
+              {r->d_table, 4 * (size_t)r->n_req * r->max_pages},
+              {r->d_first, 4 * (size_t)r->n_req},
+              {r->d_cu, 4 * ((size_t)r->n_req + 1)},
+              {r->d_status, 4}};
     for (const auto& x : in)
-        if (overlap(a->d_out, on, x.p, x.n) || overlap(a->d_scratch, need, x.p, x.n))
-            return fail(WL_ERR_INVALID, "d_out or d_scratch overlaps an input");
-    if (overlap(a->d_out, on, a->d_scratch, need)) return fail(WL_ERR_INVALID, "d_scratch overlaps d_out");
-    return on_device_of(stream, "wl_paged_tree_attention", [&] { return wl::paged::launch_tree(*a, stream); });
+        if (overlap(r->d_out, on, x.p, x.n)) return fail(WL_ERR_INVALID, "d_out overlaps an input");
+    return on_device_of(stream, "wl_paged_read", [&] { return wl::paged::launch_read(*r, stream); });
+}
+
+size_t wl_token_logprobs_scratch(const wl_logprobs* a) {
+    return check_logprobs(a) == WL_OK ? wl::paged::logprobs_scratch(*a) : 0;
+}
+
+wl_status wl_token_logprobs(const wl_logprobs* a, void* stream) {
+    wl_status s = check_logprobs(a);
+    if (s != WL_OK) return s;
+    const size_t es = esize(a->dtype), R = a->n_rows, T = a->n_tokens, N = a->n_top;
+    if (R == 0) return T == 0 ? WL_OK : fail(WL_ERR_INVALID, "tokens without rows");
+    if (!a->d_logits || !aligned(a->d_logits, es)) return fail(WL_ERR_INVALID, "d_logits must be aligned to its type and not null");
+    if (a->stride < a->n_vocab || a->stride > (1u << 24))
+        return fail(WL_ERR_INVALID, "a stride of %llu elements (%u to 2^24)", (unsigned long long)a->stride, a->n_vocab);
+    if (T && (!a->d_token || !a->d_logp)) return fail(WL_ERR_INVALID, "d_token and d_logp must be set for tokens");
+    if (T > R && !a->d_row) return fail(WL_ERR_INVALID, "%u tokens of %u rows without d_row", a->n_tokens, a->n_rows);
+    if (N && (!a->d_top_id || !a->d_top_logp)) return fail(WL_ERR_INVALID, "d_top_id and d_top_logp must be set for n_top");
+    for (const void* p : {(const void*)a->d_token, (const void*)a->d_row, (const void*)a->d_logp, (const void*)a->d_entropy,
+                          (const void*)a->d_top_logp, (const void*)a->d_top_id, (const void*)a->d_status})
+        if (!aligned(p, 4)) return fail(WL_ERR_INVALID, "the arrays must be 4-byte aligned");
+    const size_t need = wl::paged::logprobs_scratch(*a);
+    if (!a->d_scratch || !aligned(a->d_scratch, 16) || a->scratch_bytes < need)
+        return fail(WL_ERR_INVALID, "scratch of %zu bytes (%zu needed, 16-byte aligned)", a->scratch_bytes, need);
+    const struct Range {
+        const void* p;
+        size_t n;
+    } in[] = {{a->d_logits, ((R - 1) * a->stride + a->n_vocab) * es}, {a->d_token, 4 * T}, {a->d_row, 4 * T}, {a->d_status, 4}},
+      out[] = {{a->d_logp, 4 * T}, {a->d_entropy, 4 * R}, {a->d_top_logp, 4 * R * N}, {a->d_top_id, 4 * R * N}, {a->d_scratch, need}};
+    for (const Range& o : out) {
+        for (const Range& x : in)
+            if (overlap(o.p, o.n, x.p, x.n)) return fail(WL_ERR_INVALID, "an output overlaps an input");
+        for (const Range& x : out)
+            if (&x != &o && overlap(o.p, o.n, x.p, x.n)) return fail(WL_ERR_INVALID, "two outputs overlap");
+    }
+    return on_device_of(stream, "wl_token_logprobs", [&] { return wl::paged::launch_logprobs(*a, stream); });
 }
 
 }  // extern "C"

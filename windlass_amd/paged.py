@@ -1,5 +1,6 @@
 """ctypes binding of the paged-cache calls of include/windlass_moe.h: the page
-map, the write of latent cache rows, and attention for trees of drafted tokens.
+map, the write of latent cache rows and their reading back, attention for trees of
+drafted tokens, through a sliding window too, and their log probabilities.
 
 An argument block is one of the structures below, its pointers device
 addresses; a program fills it once and passes it to every call whose buffers
@@ -8,9 +9,10 @@ import ctypes
 
 from . import moe
 
-TYPE = {"f32": 0, "bf16": 1}
+TYPE = {"f32": 0, "bf16": 1, "mxfp4": 4}  # (mxfp4: of a cache's rows)
 MAX_REQ = 4096
 TREE_MAX_NODES = 64
+LOGPROB_MAX_TOP = 32
 E_LEN, E_SPACE, E_PAGE, E_TREE, E_SLOT = 1, 2, 4, 8, 16
 
 _vp, _u32, _u64, _f32 = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_float
@@ -46,6 +48,26 @@ class TreeAttention(ctypes.Structure):
                 ("d_status", _vp)]
 
 
+class WindowAttention(ctypes.Structure):
+    """wl_window_attn"""
+    _fields_ = [("tree", TreeAttention), ("window", _u32), ("n_sinks", _u32)]
+
+
+class RowRead(ctypes.Structure):
+    """wl_row_read"""
+    _fields_ = [("cache", Cache), ("dtype", _u32), ("n_req", _u32), ("n_rows", _u32), ("max_pages", _u32),
+                ("d_table", _vp), ("d_first", _vp), ("d_cu", _vp), ("d_out", _vp), ("out_stride", _u64),
+                ("d_status", _vp)]
+
+
+class TokenLogprobs(ctypes.Structure):
+    """wl_logprobs"""
+    _fields_ = [(n, _u32) for n in ["dtype", "n_rows", "n_vocab", "n_tokens", "n_top"]] + \
+               [("d_logits", _vp), ("stride", _u64), ("d_token", _vp), ("d_row", _vp), ("d_logp", _vp),
+                ("d_entropy", _vp), ("d_top_logp", _vp), ("d_top_id", _vp), ("d_scratch", _vp),
+                ("scratch_bytes", ctypes.c_size_t), ("d_status", _vp)]
+
+
 _lib = None
 
 
@@ -54,12 +76,15 @@ def _load():
     if _lib is None:
         lib = moe.load()
         for name, block in [("wl_paged_map", PageMap), ("wl_paged_write", RowWrite),
-                            ("wl_paged_tree_attention", TreeAttention)]:
+                            ("wl_paged_tree_attention", TreeAttention), ("wl_paged_window_attention", WindowAttention),
+                            ("wl_paged_read", RowRead), ("wl_token_logprobs", TokenLogprobs)]:
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(block), _vp]
             fn.restype = ctypes.c_int
         lib.wl_paged_tree_scratch.argtypes = [ctypes.POINTER(TreeAttention)]
         lib.wl_paged_tree_scratch.restype = ctypes.c_size_t
+        lib.wl_token_logprobs_scratch.argtypes = [ctypes.POINTER(TokenLogprobs)]
+        lib.wl_token_logprobs_scratch.restype = ctypes.c_size_t
         lib.wl_paged_last_error.argtypes = []
         lib.wl_paged_last_error.restype = ctypes.c_char_p
         _lib = lib
@@ -81,6 +106,26 @@ def write_rows(args, stream=0):
 
 def tree_attention(args, stream=0):
     _ck(_load().wl_paged_tree_attention(args, stream), "wl_paged_tree_attention")
+
+
+def window_attention(args, stream=0):
+    _ck(_load().wl_paged_window_attention(args, stream), "wl_paged_window_attention")
+
+
+def read_rows(args, stream=0):
+    _ck(_load().wl_paged_read(args, stream), "wl_paged_read")
+
+
+def token_logprobs(args, stream=0):
+    _ck(_load().wl_token_logprobs(args, stream), "wl_token_logprobs")
+
+
+def token_logprobs_scratch(args):
+    """Bytes of scratch that token_logprobs needs for these shapes (raises if they are invalid)."""
+    n = _load().wl_token_logprobs_scratch(args)
+    if n == 0:
+        raise moe.WindlassError(1, f"wl_token_logprobs_scratch: {_lib.wl_paged_last_error().decode()}")
+    return n
 
 
 def tree_attention_scratch(args):
