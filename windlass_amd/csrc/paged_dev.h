@@ -20,19 +20,22 @@ WL_DEV uint32_t pack_bf16(float a, float b) {  // a in the low half
 }
 
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
-// A block of 32 E2M1 values and its scale byte as bf16 (exact) into LDS at dst, the
-// 16-byte pieces in the order turn, turn + 1, .. (mod 4). A block of scale 255 (NaN) is
-// `nan`, two values.
-WL_DEV void put_mx(u32x4 x, uint32_t scale, uint8_t* dst, uint32_t turn, uint32_t nan) {
-    const bool t1 = turn & 1u, t2 = turn & 2u;
+// A block of 32 E2M1 values and its scale, on their way to bf16 (exact): 16-byte pieces
+// j = 0 .. 3 go into LDS, piece (turn + j) % 4 of the block at dst. (The lanes of a wave
+// write with different turns, so that they meet different banks.) A block of scale 255,
+// a NaN, becomes zeros.
+struct MxBlock {
+    u32x4 x;
+    float scale;
+    uint32_t turn;
+};
+WL_DEV MxBlock mx_block(u32x4 x, uint32_t scale, uint32_t turn) {
+    const bool t1 = turn & 1u, t2 = turn & 2u, nan = scale == 255u;
     const u32x4 y = t1 ? u32x4{x[1], x[2], x[3], x[0]} : x, z = t2 ? u32x4{y[2], y[3], y[0], y[1]} : y;
-    const float s = __uint_as_float(scale << 23);
-#pragma unroll
-    for (uint32_t j = 0; j < 4; j++) {
-        u32x4 v = __builtin_bit_cast(u32x4, fp4x8_bf16(z[j], s));
-        if (scale == 255u) v = u32x4{nan, nan, nan, nan};
-        *(u32x4*)(dst + 16u * ((turn + j) & 3u)) = v;
-    }
+    return MxBlock{nan ? u32x4{0u, 0u, 0u, 0u} : z, __uint_as_float(nan ? 0u : scale << 23), turn};
+}
+WL_DEV void mx_put(const MxBlock& b, uint32_t j, uint8_t* dst) {
+    *(u32x4*)(dst + 16u * ((b.turn + j) & 3u)) = __builtin_bit_cast(u32x4, fp4x8_bf16(b.x[j], b.scale));
 }
 
 // f(0), .., f(N - 1) with constants

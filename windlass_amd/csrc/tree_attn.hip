@@ -459,13 +459,6 @@ WL_DEV void cut3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {  // 
 }
 WL_DEV bool nonfinite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
-// x, of which nothing is computed ahead of this place: what is derived from it holds
-// no register before, over all the rest of the kernel.
-WL_DEV uint32_t afresh(uint32_t x) {
-    asm volatile("" : "+v"(x));
-    return x;
-}
-
 // The cache that 32-bit queries meet: 32-bit rows (WIDE), 16-bit ones, or 4-bit ones.
 enum : int { kCacheF32 = 0, kCacheBf16 = 1, kCacheMx4 = 2 };
 template <int LC, int CK, bool WIN>
@@ -600,7 +593,12 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
                     const uint32_t e = 64u * (lat ? i : i - NLAT) + lane, k = e % (lat ? EL : ER);
                     const uint32_t row = DR * wave + e / (lat ? EL : ER);
                     if (MX && lat) {
-                        if (e / EL < DR) put_mx(raw[i], mx[i], tile + row * PITCH + 64u * k, k >> 2, 0x7FC07FC0u);
+                        if (e / EL < DR) {
+                            const MxBlock b = mx_block(raw[i], mx[i], k >> 2);
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; j++) mx_put(b, j, tile + row * PITCH + 64u * k);
+                            if (mx[i] == 255u) *(u32x4*)(tile + row * PITCH + 64u * k) = u32x4{~0u, ~0u, ~0u, ~0u};  // NaN, and so its scores
+                        }
                         continue;
                     }
                     const uint32_t b = WIDE ? 8u * k : 16u * k;  // of a bf16 row
