@@ -21,8 +21,9 @@ template <int LC, bool WIN>
 __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per) {
     constexpr uint32_t NW = 8, ROWS = kRows16, PITCH = 256 * LC + kPad, CT = LC, DR = 32 / NW, QP = kQueryPieces, NB = 4 * LC;
     // a tile as it comes: 256 bytes of values a row, chunk c at c ^ swap(row); then by
-    // wave its rows' rotary parts, chunk c at c ^ swz8(row), and scales (1 KB, so that all
-    // lanes take part: loads under a condition the compiler cannot count, and waits for)
+    // wave its rows' rotary parts, chunk c at c ^ swz8(row), and scales, behind 64 bytes a
+    // wave (1 KB, so that all lanes take part: loads under a condition the compiler cannot
+    // count, and waits for)
     constexpr uint32_t AUX = kKT * 256, AUXW = 1024, RAW = AUX + NW * AUXW;
     // the queries' pieces on their way to the registers, 24 bytes a block: half of the
     // blocks of all rows in one place each
@@ -31,8 +32,11 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
     // (the tiles in the first 64 KB, by their alignment: an LDS instruction's own offset
     // reaches that far)
     __shared__ __align__(16384) uint8_t raw0[RAW], raw1[RAW], raw2[RAW], raw3[RAW];
-    __shared__ __align__(1024) uint8_t vb0[kKT * PITCH], vb1[kKT * PITCH];  // its values in bf16
-    __shared__ __align__(1024) uint8_t pb0[ROWS * 64], pb1[ROWS * 64];      // weights [row][32 keys], of tiles in turn
+    __shared__ __align__(1024) uint8_t vb[2 * kKT * PITCH];  // values in bf16 and
+    __shared__ __align__(1024) uint8_t pb[2 * ROWS * 64];    // weights [row][32 keys], of tiles in turn
+    // Where these two lie: a lane's place is kept with it added, as an LDS instruction's
+    // own offset does not reach that far (elsewhere they would cost an addition each)
+    constexpr uint32_t VB = 4 * RAW, PB = VB + 2 * kKT * PITCH;
     __shared__ uint8_t qscale[ROWS][NB];  // exponents of the queries' first pieces (255: not finite)
     __shared__ float rowred[2][ROWS];
     __shared__ uint64_t seen[ROWS];
@@ -46,7 +50,7 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
     const uint32_t H = p.a.n_heads, L = p.a.cache.kv_lora_rank, RP = p.a.cache.qk_rope;
     const uint32_t stride = p.a.cache.row_stride;
     if (tid == 0) bad_page = again = 0;
-    const Place f = find_place<ROWS, 64 * NW, kGrid, WIN>(p, c, min_per, tmp, (u32x2*)pb0, &found);
+    const Place f = find_place<ROWS, 64 * NW, kGrid, WIN>(p, c, min_per, tmp, (u32x2*)pb, &found);
     if (tid < 2) p.desc[kDesc * (2 * c + tid)] = 0;
     Walks<ROWS, WIN> walks(p, f, c);
     auto swap = [](uint32_t row) { return 2u * (row & 7u); };
@@ -56,9 +60,10 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
         const Req& q = w.q;
         const uint32_t rt = w.rt, kt0 = w.kt0, kt1 = w.kt1, rows = walks.rows(w);
         f32x4 acc[4][CT];  // of all rows, columns 16 LC wave + [0, 16 LC)
-        float m = kNone, l = 0.f;  // of row sr + n: the reference, this lane's part of the weights' sum
+        float m = kNone;  // the reference of row sr + n
+        f32x4 l;          // the sum of row 16 (wave % 4) + n's weights, four times
         auto clear = [&]() __attribute__((always_inline)) {
-            l = 0.f;
+            l = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -94,8 +99,8 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
             const uint32_t val_i = lane >> 4, val_ch = (lane & 15u) ^ swap(DR * wave + val_i);
             const uint32_t val_at = 32u * val_ch < L ? val_i * stride + 16u * val_ch : kOOB;
             const uint32_t rot_i = (lane >> 3) & 3u, rot_ch = (lane & 7u) ^ swz8((DR * wave + rot_i) & 15u);
-            const uint32_t aux_at = lane >= 32u + DR   ? kOOB
-                                    : lane >= 32u      ? (lane & 3u) * stride + L / 2u
+            // (the scales in other banks for each wave's rows)
+            const uint32_t aux_at = lane >= 32u ? ((lane - 32u) / DR == wave ? (lane & 3u) * stride + L / 2u : kOOB)
                                     : 8u * rot_ch < RP ? rot_i * stride + L / 2u + kMxScales + 16u * rot_ch
                                                        : kOOB;
             auto issue = [&](uint8_t* raw, uint32_t t) __attribute__((always_inline)) {
@@ -146,7 +151,7 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                         // (the conversions take several passes: their operands stay live)
                         const u32x6 y = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, sc);
                         asm volatile("" ::"v"(y), "v"(even), "v"(odd), "v"(sc));
-                        uint8_t* o = j == 0 ? (half ? vb1 : vb0) : j == 1 ? (half ? vb1 : vb0) + ROWS * QROW : half ? raw3 : raw2;
+                        uint8_t* o = j < 2 ? vb + (half ? kKT * PITCH : 0u) + j * (ROWS * QROW) : half ? raw3 : raw2;
 #pragma unroll
                         for (uint32_t k = 0; k < 3; k++) *(u32x2*)(o + to + 8u * k) = u32x2{y[2 * k], y[2 * k + 1]};
                         if (j + 1 < QP) {
@@ -188,7 +193,7 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                     e |= (uint32_t)qscale[lr][b] << (8u * s);
 #pragma unroll
                     for (uint32_t j = 0; j < QP; j++) {
-                        const uint8_t* o = j == 0 ? (half ? vb1 : vb0) : j == 1 ? (half ? vb1 : vb0) + ROWS * QROW : half ? raw3 : raw2;
+                        const uint8_t* o = j < 2 ? vb + (half ? kKT * PITCH : 0u) + j * (ROWS * QROW) : half ? raw3 : raw2;
 #pragma unroll
                         for (uint32_t k = 0; k < 3; k++) {
                             const u32x2 y = *(const u32x2*)(o + from + 8u * k);
@@ -213,11 +218,15 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
             // the key operands of step s: values of columns 128 s + 32 g of key row sk + n, or its rotary part
             const uint32_t key = sk + n, key_at = key * 256u + (16u * g ^ 16u * swap(key));
             const uint32_t key_aux = AUX + (key >> 2) * AUXW, key_rot = key_aux + (key & 3u) * 128u + 16u * (g ^ swz8(n));
-            const uint32_t key_scale = key_aux + 128u * DR + (key & 3u) * 16u + 4u * g;
+            const uint32_t key_scale = key_aux + 128u * DR + 64u * (key >> 2) + (key & 3u) * 16u + 4u * g;
             // the tile's values in bf16: lane's chunk of row wave + 8 (lane / 16)
             const uint32_t cv_row = wave + 8u * (lane >> 4), cv_ch = lane & 15u;
-            const uint32_t cv_at = cv_row * 256u + 16u * (cv_ch ^ swap(cv_row)), cv_to = cv_row * PITCH + 64u * cv_ch;
-            const uint32_t cv_scale = AUX + (cv_row >> 2) * AUXW + 128u * DR + (cv_row & 3u) * 16u + mx_scale_at(cv_ch);
+            // (Its four pieces of 8 columns go in two pairs to the row's two halves, the pairs of
+            // columns 16 k at 32 ((k / 2) + half (k % 2)): 8 lanes write to 8 places of 128 bytes,
+            // with the pieces of a pair in opposite order for half of them.)
+            const bool cv_odd = ((cv_ch >> 2) ^ (cv_ch >> 3)) & 1u;
+            const uint32_t cv_at = cv_row * 256u + 16u * (cv_ch ^ swap(cv_row)), cv_to = cv_row * PITCH + 32u * cv_ch + (cv_odd ? 16u : 0u);
+            const uint32_t cv_scale = AUX + (cv_row >> 2) * (AUXW + 64u) + 128u * DR + (cv_row & 3u) * 16u + mx_scale_at(cv_ch);
             // a tile's operands, read ahead: two steps' values, and what a lane converts
             struct Keys {
                 u32x4 k[2], v;
@@ -231,14 +240,19 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                 x.v_scale = raw[cv_scale];
             };
             // the products of rows sr + n with keys sk + 4 g + j; between them the tile's values
-            // are brought to bf16 in vb (VALUES): the matrix cores run on meanwhile
-            auto products = [&](const uint8_t* raw, Keys& x, f32x4& s0, uint8_t* vb, auto values) __attribute__((always_inline)) {
+            // are brought to bf16 in place (VALUES): the matrix cores run on meanwhile
+            auto products = [&](const uint8_t* raw, Keys& x, f32x4& s0, uint32_t place, auto values) __attribute__((always_inline)) {
                 constexpr bool VALUES = decltype(values)::value;
-                const uint32_t to = afresh(cv_to);
+                const uint32_t to = afresh(cv_to + VB) - VB + place * (kKT * PITCH), to2 = afresh((cv_to ^ 16u) + VB) - VB + place * (kKT * PITCH);
                 f32x4 y[QP];
 #pragma unroll
                 for (uint32_t j = 0; j < QP; j++) y[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-                const MxBlock v = mx_block(x.v, x.v_scale, cv_ch >> 2);
+                if (VALUES && __ballot(x.v_scale == 255u)) {  // a block that is NaN: zeros (its key's scores are NaN)
+                    const bool nan = x.v_scale == 255u;
+                    x.v = nan ? u32x4{0u, 0u, 0u, 0u} : x.v;
+                    x.v_scale = nan ? 0u : x.v_scale;
+                }
+                const float v_scale = __uint_as_float(x.v_scale << 23);
                 static_for<LC>([&](auto si) __attribute__((always_inline)) {
                     constexpr int s = decltype(si)::value;
                     const u32x4 k = x.k[s % 2];
@@ -252,7 +266,11 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                     if (LC > 1 || s > 0) x.k[s % 2] = *(const u32x4*)(raw + (s + 2 < LC ? key_at ^ (64u * (s + 2)) : key_rot ^ (64u * (s + 2 - LC))));
                     if (VALUES && (LC == 4 || cv_ch < NB)) {
 #pragma unroll
-                        for (uint32_t j = 4 * s / LC; j < 4 * (s + 1) / LC; j++) mx_put(v, j, vb + to);
+                        for (uint32_t j = 4 * s / LC; j < 4 * (s + 1) / LC; j++) {  // piece j / 2 of pair j % 2
+                            const uint32_t lo = x.v[2 * (j & 1u)], hi = x.v[2 * (j & 1u) + 1u], piece = (j < 2) != cv_odd ? lo : hi;
+                            *(u32x4*)(vb + (j < 2 ? to : to2) + (j & 1u) * (128u * LC)) =
+                                __builtin_bit_cast(u32x4, fp4x8_bf16(piece, v_scale));
+                        }
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 });
@@ -294,57 +312,61 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
             };
             bool pass = false;
             uint32_t first = kt0;  // the tile that sets the reference
-            const uint32_t value_at = (4u * g + ((lane & 15u) >> 2)) * PITCH + 32u * LC * wave + 8u * (lane & 3u);
-            auto vread = [&](const uint8_t* vb, uint32_t at, uint32_t k) __attribute__((always_inline)) {
-                const uint8_t* pa = vb + at + 32u * k;
+            const uint32_t value_at = (4u * g + ((lane & 15u) >> 2)) * PITCH + (LC == 1 ? 32u * (wave / 2u) + 128u * (wave % 2u) : 16u * LC * wave) + 8u * (lane & 3u);
+            auto vread = [&](uint32_t at, uint32_t k) __attribute__((always_inline)) {
+                // columns 16 (LC wave + k): (with a single 128 columns the wave is k)
+                const uint8_t* pa = vb + at + (LC == 1 ? 0u : 32u * (k / 2u) + 128u * LC * (k % 2u));
                 typedef __attribute__((address_space(3))) s16x4 l_s16x4;
                 const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa));
                 const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)WL_LDS(pa + 16 * PITCH));
                 const u32x2 xx = __builtin_bit_cast(u32x2, x), yy = __builtin_bit_cast(u32x2, y);
                 return u32x4{xx[0], xx[1], yy[0], yy[1]};
             };
-            const uint32_t put_at = (sr + n) * 64u + 16u * (g ^ swz4(n)) + sk / 2u;
-            const uint32_t get_at = n * 64u + 16u * (g ^ swz4(n));
-            auto put_weights = [&](f32x4 s0, float f, uint8_t* pb) __attribute__((always_inline)) {
+            // chunk g of a row of weights (operand order) at g ^ turned(row): 8-byte writes meet two
+            // by two, reads not at all (swz4's four by four: 49 clocks a tile more)
+            const uint32_t turned = ((n & 4u) ? 3u : 0u) ^ ((n >> 1) & 1u);
+            const uint32_t put_at = (sr + n) * 64u + 16u * (g ^ turned) + sk / 2u;
+            const uint32_t get_at = n * 64u + 16u * (g ^ turned);
+            auto put_weights = [&](f32x4 s0, float f, uint32_t place) __attribute__((always_inline)) {
                 float e[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) e[k] = exp2_(fmaf(s0[k], f, -m));
-                const u32x2 x = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
-                *(u32x2*)(pb + afresh(put_at)) = x;
-                const float r[4] = {__uint_as_float(x[0] << 16), __uint_as_float(x[0] & 0xFFFF0000u),
-                                    __uint_as_float(x[1] << 16), __uint_as_float(x[1] & 0xFFFF0000u)};
-                l += (r[0] + r[1]) + (r[2] + r[3]);
-                pass |= fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])) > kMost;
+                *(u32x2*)(pb + (afresh(put_at + PB) - PB) + place * (ROWS * 64u)) = u32x2{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3])};
             };
-            // the values in v0 by the weights in w0
+            // the values by the weights of one place; the weights' own sums are products with ones
             constexpr uint32_t VP = CT < 2 ? CT : 2;  // column tiles that the values are read ahead
             struct Values {
-                bf16x8 p[4];
+                bf16x8 p[4], own;
                 u32x4 v[VP];
                 uint32_t at;
             };
-            auto read_values = [&](const uint8_t* v0, const uint8_t* w0, Values& x) __attribute__((always_inline)) {
-                const uint32_t get = afresh(get_at);
+            auto read_values = [&](uint32_t place, Values& x) __attribute__((always_inline)) {
+                const uint32_t get = afresh(get_at + PB) - PB + place * (ROWS * 64u);
 #pragma unroll
-                for (int i = 0; i < 4; i++) x.p[i] = as_bf16x8(*(const u32x4*)(w0 + get + 1024u * i));
-                x.at = afresh(value_at);
+                for (int i = 0; i < 4; i++) x.p[i] = as_bf16x8(*(const u32x4*)(pb + get + 1024u * i));
+                x.own = as_bf16x8(*(const u32x4*)(pb + afresh(get_at + 1024u * (wave & 3u) + PB) - PB + place * (ROWS * 64u)));
+                x.at = afresh(value_at + VB) - VB + place * (kKT * PITCH);
 #pragma unroll
-                for (uint32_t k = 0; k < VP; k++) x.v[k] = vread(v0, x.at, k);
+                for (uint32_t k = 0; k < VP; k++) x.v[k] = vread(x.at, k);
             };
-            auto sums = [&](const uint8_t* v0, Values& x, auto then) __attribute__((always_inline)) {
+            auto sums = [&](Values& x, auto then) __attribute__((always_inline)) {
+                const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
 #pragma unroll
                 for (uint32_t v = 0; v < CT; v++) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) acc[i][v] = mma(as_bf16x8(x.v[v % VP]), x.p[i], acc[i][v]);
-                    if (v + VP < CT) x.v[v % VP] = vread(v0, x.at, v + VP);
-                    if (v == 0) then();
+                    if (v + VP < CT) x.v[v % VP] = vread(x.at, v + VP);
+                    if (v == 0) {
+                        l = mma(as_bf16x8(ones), x.own, l);
+                        then();
+                    }
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
-            // between two barriers: tile t - 1 has its values in v0 and weights in w0; tile t
-            // is in b1, to be brought to v1 and w1; tile t + 3's place is b0; at t = kt1 the last sums
-            auto turn = [&](uint8_t* b0, const uint8_t* b1, const uint8_t* v0, uint8_t* v1, const uint8_t* w0, uint8_t* w1,
-                            uint32_t t) __attribute__((always_inline)) {
+            // between two barriers: tile t - 1 has its values and weights in place 1 - E; tile t
+            // is in b1, to be brought to place E; tile t + 3's place is b0; at t = kt1 the last sums
+            auto turn = [&](uint8_t* b0, const uint8_t* b1, auto place, uint32_t t) __attribute__((always_inline)) {
+                constexpr uint32_t E = decltype(place)::value;
                 const bool live = t < kt1;
                 f32x4 s0;
                 float f = 0.f;
@@ -353,15 +375,15 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                     read_keys(b1, x);
                     __builtin_amdgcn_sched_barrier(0);
                     issue(b0, t + 3);
-                    products(b1, x, s0, v1, std::true_type{});
+                    products(b1, x, s0, E, std::true_type{});
                     f = scores(s0, t);
                     if (WIN && masked(t)) late_maxima(largest(s0, f));
                 }
                 Values y;
-                read_values(v0, w0, y);
+                read_values(1u - E, y);
                 __builtin_amdgcn_sched_barrier(0);
-                sums(v0, y, [&]() __attribute__((always_inline)) {
-                    if (live) put_weights(s0, f, w1);
+                sums(y, [&]() __attribute__((always_inline)) {
+                    if (live) put_weights(s0, f, E);
                 });
                 if (!live) return false;
                 vm_wait<4>();  // tile t + 1 is there; t + 2 and t + 3 may be on the way
@@ -384,24 +406,25 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                     f32x4 s0;
                     Keys x;
                     read_keys(raw0, x);
-                    products(raw0, x, s0, vb0, std::true_type{});
+                    products(raw0, x, s0, 0, std::true_type{});
                     const float f = scores(s0, kt0);
                     if (first == kt0) share_maxima(largest(s0, f));
                     clear();
-                    put_weights(s0, f, pb0);
+                    put_weights(s0, f, 0);
                 }
                 ring_barrier();
                 for (uint32_t t = kt0 + 1;; t += 4) {
-                    if (!turn(raw0, raw1, vb0, vb1, pb0, pb1, t)) break;
-                    if (!turn(raw1, raw2, vb1, vb0, pb1, pb0, t + 1)) break;
-                    if (!turn(raw2, raw3, vb0, vb1, pb0, pb1, t + 2)) break;
-                    if (!turn(raw3, raw0, vb1, vb0, pb1, pb0, t + 3)) break;
+                    if (!turn(raw0, raw1, std::integral_constant<uint32_t, 1>{}, t)) break;
+                    if (!turn(raw1, raw2, std::integral_constant<uint32_t, 0>{}, t + 1)) break;
+                    if (!turn(raw2, raw3, std::integral_constant<uint32_t, 1>{}, t + 2)) break;
+                    if (!turn(raw3, raw0, std::integral_constant<uint32_t, 0>{}, t + 3)) break;
                 }
                 vm_wait<0>();
                 if (first != kt0) break;
                 const uint32_t nr = afresh(tid) & 15u;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++) pass |= 16u * i + nr < rows && nonfinite(acc[i]);
+                pass |= l[0] > kMost;
                 if (__ballot(pass) && (afresh(tid) & 63u) == 0) again = 1u;
                 ring_barrier();
                 const bool redo = uni(again) != 0;
@@ -417,7 +440,7 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                     f32x4 s0;
                     Keys y;
                     read_keys(raw0, y);
-                    products(raw0, y, s0, nullptr, std::false_type{});
+                    products(raw0, y, s0, 0, std::false_type{});
                     const float f = scores(s0, t);
                     x = fmaxf(x, largest(s0, f));
                     ring_barrier();
@@ -435,9 +458,7 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
             bad_page = 1u;
             set_status(p.a.d_status, WL_PAGED_E_PAGE);
         }
-        l += __shfl_xor(l, 16, 64);
-        l += __shfl_xor(l, 32, 64);
-        if (g == 0) rowred[wave & 1u][sr + n] = l;
+        if (wave < 4u && g == 0) rowred[0][16u * wave + n] = l[0];
         const bool whole = kt1 - kt0 == q.nkt;
         if (!whole && sk == 0 && g == 0) p.part_ml[2u * (w.slot * ROWS + sr + n)] = m;
         ring_barrier();
@@ -445,7 +466,7 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t lr = 16u * i + n;
-            float sum = rowred[0][lr] + rowred[1][lr];
+            float sum = rowred[0][lr];
             if (nan) sum = __builtin_nanf("");
             if (lr < rows) {
                 put_row<ROWS, LC, true, CT>(p, w, whole, lr, sum, acc[i], 16u * LC * wave + 4u * g);
