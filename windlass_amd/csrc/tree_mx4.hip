@@ -15,7 +15,7 @@ typedef __attribute__((ext_vector_type(32))) float f32x32;
 
 // Pieces of 32 queries that meet one scale of a key: q = sum of p_i 2^s_i, p_i of E2M3;
 // s_1 puts the largest into (3.75, 7.5], the others fall by 4 and 9 powers of two.
-constexpr uint32_t kQueryPieces = 3;
+constexpr uint32_t kQueryPieces = 3;  // (they are moved as three)
 
 template <int LC, bool WIN>
 __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per) {
@@ -25,10 +25,7 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
     // wave (1 KB, so that all lanes take part: loads under a condition the compiler cannot
     // count, and waits for)
     constexpr uint32_t AUX = kKT * 256, AUXW = 1024, RAW = AUX + NW * AUXW;
-    // the queries' pieces on their way to the registers, 24 bytes a block: half of the
-    // blocks of all rows in one place each
-    constexpr uint32_t QROW = NB / 2 * 24;
-    static_assert(2 * ROWS * QROW <= kKT * PITCH && ROWS * QROW <= RAW, "the queries' pieces fit");
+    static_assert(ROWS * NB * 64 <= 2 * kKT * PITCH && ROWS * NB * 8 <= RAW, "the queries fit where the values go");
     // (the tiles in the first 64 KB, by their alignment: an LDS instruction's own offset
     // reaches that far)
     __shared__ __align__(16384) uint8_t raw0[RAW], raw1[RAW], raw2[RAW], raw3[RAW];
@@ -113,26 +110,49 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, WL_LDS(raw + AUX + AUXW * wave), 16u, aux_at, 0u, 0, 0);
             };
             // The queries of rows sr + n: lane (row n, block g) has 32 columns of each 128 in
-            // pieces, and the rotary part in bf16. A thread cuts up a block of a row, for the
-            // two waves that need it (one round of code: a walk's start is the time that its
-            // instructions take to come); the pieces go through the places of values (the
-            // first two of a half of the blocks each) and of the last two tiles.
+            // pieces, and the rotary part in bf16. They come by DMA to where the values will be,
+            // 64 bytes a block; a thread cuts up a block for the two waves that need it, the
+            // pieces going to the block's place and, 8 bytes of them, to the last tile's. (One
+            // trip to memory, and one round of code: a walk's start takes the time that its
+            // instructions take to come.)
             u32x6 qf[LC][QP];
             uint32_t qs[QP];  // the pieces' scales, a byte for each 128 columns
             bf16x8 qr[2];
-            auto cut_queries = [&]() __attribute__((always_inline)) {
+            auto call_queries = [&]() __attribute__((always_inline)) {
                 const rsrc_t ql = make_rsrc((const uint16_t*)p.a.d_q_lat + q.t0 * p.a.q_lat_stride,
                                             2u * ((q.nodes - 1u) * (uint32_t)p.a.q_lat_stride + H * L));
-                const uint32_t id = afresh(tid);
+                const rsrc_t qro = make_rsrc((const uint16_t*)p.a.d_q_rope + q.t0 * p.a.q_rope_stride,
+                                             2u * ((q.nodes - 1u) * (uint32_t)p.a.q_rope_stride + H * RP));
+                // lane i has row i's place; a load brings 1 KB, of 4 / LC rows
+                const uint32_t ln = afresh(tid) & 63u, row = rt * ROWS + ln, node = row / H, h = row - node * H;
+                const uint32_t lat = 2u * (node * (uint32_t)p.a.q_lat_stride + h * L), chunk = ln % (16u * LC);
 #pragma unroll 1
-                for (uint32_t i = id; i < ROWS * NB; i += 64u * NW) {
-                    const uint32_t lr = i / NB, b = i % NB, row = rt * ROWS + lr, node = row / H, h = row - node * H;
-                    const uint32_t at = lr < rows && 32u * b < L ? 2u * (node * (uint32_t)p.a.q_lat_stride + h * L + 32u * b) : kOOB;
+                for (uint32_t i = 2u * LC * wave; i < 2u * LC * (wave + 1u); i++) {
+                    const uint32_t r = i * (4u / LC) + ln / (16u * LC), at = __shfl(lat, (int)r, 64);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(ql, WL_LDS(vb + 1024u * i), 16u,
+                                                             r < rows && 8u * chunk < L ? at + 16u * chunk : kOOB, 0u, 0, 0);
+                }
+                const uint32_t lr = sr + (ln & 15u), mine = 2u * (node * (uint32_t)p.a.q_rope_stride + h * RP), vr = __shfl(mine, (int)lr, 64);
+#pragma unroll
+                for (uint32_t s = 0; s < 2; s++) {
+                    const uint32_t col = 32u * s + 8u * (ln >> 4);
+                    qr[s] = as_bf16x8(bld16(qro, lr < rows && col < RP ? vr + 2u * col : kOOB, 0));
+                }
+                if (wave == 0) {
+                    uint32_t from;
+                    seen[ln] = sees<WIN>(p, q, ln < rows ? node : 0u, from);
+                    if (WIN) low[ln] = from;
+                }
+            };
+            auto cut_queries = [&]() __attribute__((always_inline)) {
+#pragma unroll 1
+                for (uint32_t i = afresh(tid); i < ROWS * NB; i += 64u * NW) {
                     f32x16 even, odd;
                     uint32_t most = 0;
                     u32x4 x[4];
+                    u32x4* const at = (u32x4*)(vb + 64u * i);
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; k++) x[k] = bld16(ql, at, 16u * k);
+                    for (uint32_t k = 0; k < 4; k++) x[k] = at[k];
 #pragma unroll
                     for (uint32_t k = 0; k < 16; k++) {
                         const uint32_t v = x[k / 4][k % 4];
@@ -143,20 +163,17 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                     constexpr uint32_t lo = 5u * (QP - 1u);
                     uint32_t e = (most >> 23) + ((most & 0x7FFFFFu) > 0x700000u ? 1u : 0u);
                     e = e < lo + 2u ? lo : e - 2u;
-                    qscale[lr][b] = (uint8_t)(most >= 0x7F800000u ? 255u : e);
-                    const uint32_t half = b / (NB / 2), to = lr * QROW + (b % (NB / 2)) * 24u;
+                    qscale[i / NB][i % NB] = (uint8_t)(most >= 0x7F800000u ? 255u : e);
+                    u32x6 y[QP];
 #pragma unroll
                     for (uint32_t j = 0; j < QP; j++) {
                         const float sc = __uint_as_float((e - (j ? 5u * j - 1u : 0u)) << 23);
                         // (the conversions take several passes: their operands stay live)
-                        const u32x6 y = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, sc);
-                        asm volatile("" ::"v"(y), "v"(even), "v"(odd), "v"(sc));
-                        uint8_t* o = j < 2 ? vb + (half ? kKT * PITCH : 0u) + j * (ROWS * QROW) : half ? raw3 : raw2;
-#pragma unroll
-                        for (uint32_t k = 0; k < 3; k++) *(u32x2*)(o + to + 8u * k) = u32x2{y[2 * k], y[2 * k + 1]};
+                        y[j] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, sc);
+                        asm volatile("" ::"v"(y[j]), "v"(even), "v"(odd), "v"(sc));
                         if (j + 1 < QP) {
-                            const f32x32 z = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(y, sc);
-                            asm volatile("" ::"v"(z), "v"(y), "v"(sc));
+                            const f32x32 z = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(y[j], sc);
+                            asm volatile("" ::"v"(z), "v"(y[j]), "v"(sc));
 #pragma unroll
                             for (int k = 0; k < 16; k++) {
                                 even[k] -= z[2 * k];
@@ -164,43 +181,25 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                             }
                         }
                     }
+                    at[0] = u32x4{y[0][0], y[0][1], y[0][2], y[0][3]};
+                    at[1] = u32x4{y[0][4], y[0][5], y[1][0], y[1][1]};
+                    at[2] = u32x4{y[1][2], y[1][3], y[1][4], y[1][5]};
+                    at[3] = u32x4{y[2][0], y[2][1], y[2][2], y[2][3]};
+                    *(u32x2*)(raw3 + 8u * i) = u32x2{y[2][4], y[2][5]};
                 }
             };
             auto read_queries = [&]() __attribute__((always_inline)) {
-                const rsrc_t qro = make_rsrc((const uint16_t*)p.a.d_q_rope + q.t0 * p.a.q_rope_stride,
-                                             2u * ((q.nodes - 1u) * (uint32_t)p.a.q_rope_stride + H * RP));
-                const uint32_t ln = afresh(tid) & 63u, lr = sr + (ln & 15u), gr = ln >> 4;
-                const uint32_t row = rt * ROWS + lr, node = row / H, h = row - node * H;
-                const bool live = lr < rows;
-                const uint32_t vr = 2u * (node * (uint32_t)p.a.q_rope_stride + h * RP);
-#pragma unroll
-                for (uint32_t s = 0; s < 2; s++) {
-                    const uint32_t col = 32u * s + 8u * gr;
-                    qr[s] = as_bf16x8(bld16(qro, live && col < RP ? vr + 2u * col : kOOB, 0));
-                }
-                if (sk == 0 && gr == 0) {
-                    uint32_t from;
-                    seen[lr] = sees<WIN>(p, q, live ? node : 0u, from);
-                    if (WIN) low[lr] = from;
-                }
-                ring_barrier();
+                const uint32_t ln = afresh(tid) & 63u, lr = sr + (ln & 15u), at = lr * NB + (ln >> 4);
                 uint32_t e = 0;
 #pragma unroll
                 for (uint32_t s = 0; s < LC; s++) {
-                    const uint32_t b = 4u * s + gr;  // (of one half for all lanes, but with a single 128 columns)
-                    const bool half = LC == 1 ? b >= NB / 2 : s >= LC / 2;
-                    const uint32_t from = lr * QROW + (b % (NB / 2)) * 24u;
-                    e |= (uint32_t)qscale[lr][b] << (8u * s);
-#pragma unroll
-                    for (uint32_t j = 0; j < QP; j++) {
-                        const uint8_t* o = j < 2 ? vb + (half ? kKT * PITCH : 0u) + j * (ROWS * QROW) : half ? raw3 : raw2;
-#pragma unroll
-                        for (uint32_t k = 0; k < 3; k++) {
-                            const u32x2 y = *(const u32x2*)(o + from + 8u * k);
-                            qf[s][j][2 * k] = y[0];
-                            qf[s][j][2 * k + 1] = y[1];
-                        }
-                    }
+                    const u32x4* b = (const u32x4*)(vb + 64u * (at + 4u * s));
+                    const u32x4 x0 = b[0], x1 = b[1], x2 = b[2], x3 = b[3];
+                    const u32x2 x4 = *(const u32x2*)(raw3 + 8u * (at + 4u * s));
+                    qf[s][0] = u32x6{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1]};
+                    qf[s][1] = u32x6{x1[2], x1[3], x2[0], x2[1], x2[2], x2[3]};
+                    qf[s][2] = u32x6{x3[0], x3[1], x3[2], x3[3], x4[0], x4[1]};
+                    e |= (uint32_t)qscale[lr][4u * s + (ln >> 4)] << (8u * s);
                 }
 #pragma unroll
                 for (uint32_t j = 0; j < QP; j++) {
@@ -212,7 +211,6 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                         qs[j] |= (x == 255u ? 255u : x - drop) << (8u * s);
                     }
                 }
-                ring_barrier();
             };
             auto masked = [&](uint32_t t) { return is_masked<WIN>(p, q, key_of<WIN>(q, t), kKT); };
             // the key operands of step s: values of columns 128 s + 32 g of key row sk + n, or its rotary part
@@ -311,7 +309,6 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                 if (before != kNone) m = before;
             };
             bool pass = false;
-            uint32_t first = kt0;  // the tile that sets the reference
             const uint32_t value_at = (4u * g + ((lane & 15u) >> 2)) * PITCH + (LC == 1 ? 32u * (wave / 2u) + 128u * (wave % 2u) : 16u * LC * wave) + 8u * (lane & 3u);
             auto vread = [&](uint32_t at, uint32_t k) __attribute__((always_inline)) {
                 // columns 16 (LC wave + k): (with a single 128 columns the wave is k)
@@ -363,64 +360,66 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
-            // between two barriers: tile t - 1 has its values and weights in place 1 - E; tile t
-            // is in b1, to be brought to place E; tile t + 3's place is b0; at t = kt1 the last sums
+            // A turn: tile t, in b1, becomes values and weights in place E; tile t + 3's place
+            // is b0. Of a SIMD's two waves the first sums tile t - 1 before the turn's barrier,
+            // the second tile t behind it, so that one's sums run beside the other's scores.
+            constexpr bool late = false;
+            uint32_t fresh = kt0;  // the tile whose maxima are the references
             auto turn = [&](uint8_t* b0, const uint8_t* b1, auto place, uint32_t t) __attribute__((always_inline)) {
                 constexpr uint32_t E = decltype(place)::value;
-                const bool live = t < kt1;
-                f32x4 s0;
-                float f = 0.f;
-                if (live) {
+                if (t < kt1) {
                     Keys x;
+                    f32x4 s0;
                     read_keys(b1, x);
                     __builtin_amdgcn_sched_barrier(0);
                     issue(b0, t + 3);
                     products(b1, x, s0, E, std::true_type{});
-                    f = scores(s0, t);
-                    if (WIN && masked(t)) late_maxima(largest(s0, f));
+                    const float f = scores(s0, t);
+                    if (t == fresh || (WIN && masked(t))) late_maxima(largest(s0, f));
+                    put_weights(s0, f, E);
+                    if (late) {
+                        vm_wait<4>();  // tile t + 1 is there; t + 2 and t + 3 may be on the way
+                        ring_barrier();
+                    }
+                } else if (late) {
+                    return false;
                 }
-                Values y;
-                read_values(1u - E, y);
-                __builtin_amdgcn_sched_barrier(0);
-                sums(y, [&]() __attribute__((always_inline)) {
-                    if (live) put_weights(s0, f, E);
-                });
-                if (!live) return false;
-                vm_wait<4>();  // tile t + 1 is there; t + 2 and t + 3 may be on the way
-                ring_barrier();
+                if (late || t > kt0) {
+                    Values y;
+                    read_values(late ? E : 1u - E, y);
+                    __builtin_amdgcn_sched_barrier(0);
+                    sums(y, [] {});
+                }
+                if (t >= kt1) return false;
+                if (!late) {
+                    vm_wait<4>();
+                    ring_barrier();
+                }
                 return true;
             };
+            call_queries();
             first_rows();
             for (;;) {
                 issue(raw0, kt0);
                 issue(raw1, kt0 + 1);
-                if (first == kt0) {
-                    cut_queries();
-                    read_queries();
-                }
                 issue(raw2, kt0 + 2);
                 vm_wait<0>();
                 ring_barrier();
-                {
-                    issue(raw3, kt0 + 3);
-                    f32x4 s0;
-                    Keys x;
-                    read_keys(raw0, x);
-                    products(raw0, x, s0, 0, std::true_type{});
-                    const float f = scores(s0, kt0);
-                    if (first == kt0) share_maxima(largest(s0, f));
-                    clear();
-                    put_weights(s0, f, 0);
+                if (fresh == kt0) {
+                    cut_queries();
+                    ring_barrier();
+                    read_queries();
+                    ring_barrier();
                 }
-                ring_barrier();
-                for (uint32_t t = kt0 + 1;; t += 4) {
-                    if (!turn(raw0, raw1, std::integral_constant<uint32_t, 1>{}, t)) break;
-                    if (!turn(raw1, raw2, std::integral_constant<uint32_t, 0>{}, t + 1)) break;
-                    if (!turn(raw2, raw3, std::integral_constant<uint32_t, 1>{}, t + 2)) break;
-                    if (!turn(raw3, raw0, std::integral_constant<uint32_t, 0>{}, t + 3)) break;
+                clear();
+                for (uint32_t t = kt0;; t += 4) {
+                    if (!turn(raw3, raw0, std::integral_constant<uint32_t, 0>{}, t)) break;
+                    if (!turn(raw0, raw1, std::integral_constant<uint32_t, 1>{}, t + 1)) break;
+                    if (!turn(raw1, raw2, std::integral_constant<uint32_t, 0>{}, t + 2)) break;
+                    if (!turn(raw2, raw3, std::integral_constant<uint32_t, 1>{}, t + 3)) break;
                 }
                 vm_wait<0>();
-                if (first != kt0) break;
+                if (fresh != kt0) break;
                 const uint32_t nr = afresh(tid) & 15u;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++) pass |= 16u * i + nr < rows && nonfinite(acc[i]);
@@ -448,7 +447,7 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                 share_maxima(x);
                 m += lift_of((kt1 - kt0) * kKT);
                 ring_barrier();
-                first = ~0u;
+                fresh = ~0u;
                 first_rows();
             }
         }
