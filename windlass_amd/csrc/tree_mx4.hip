@@ -34,7 +34,7 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
     // Where these two lie: a lane's place is kept with it added, as an LDS instruction's
     // own offset does not reach that far (elsewhere they would cost an addition each)
     constexpr uint32_t VB = 4 * RAW, PB = VB + 2 * kKT * PITCH;
-    __shared__ uint8_t qscale[ROWS][NB];  // exponents of the queries' first pieces (255: not finite)
+    __shared__ uint8_t qscale[NB][ROWS];  // exponents of the queries' first pieces (255: not finite)
     __shared__ float rowred[2][ROWS];
     __shared__ uint64_t seen[ROWS];
     __shared__ uint32_t low[WIN ? ROWS : 1];
@@ -114,7 +114,10 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
             // 64 bytes a block; a thread cuts up a block for the two waves that need it, the
             // pieces going to the block's place and, 8 bytes of them, to the last tile's. (One
             // trip to memory, and one round of code: a walk's start takes the time that its
-            // instructions take to come.)
+            // instructions take to come.) 16 bytes c of a row are at c ^ apart(row), which is
+            // another place for each of 16 rows, and for the 8 rows at c and 8 at c + 4 that
+            // are served together.
+            auto apart = [](uint32_t row) { return 4u * ((0x1320u >> (row & 12u)) & 3u) + (row & 3u); };
             u32x6 qf[LC][QP];
             uint32_t qs[QP];  // the pieces' scales, a byte for each 128 columns
             bf16x8 qr[2];
@@ -125,10 +128,11 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                                              2u * ((q.nodes - 1u) * (uint32_t)p.a.q_rope_stride + H * RP));
                 // lane i has row i's place; a load brings 1 KB, of 4 / LC rows
                 const uint32_t ln = afresh(tid) & 63u, row = rt * ROWS + ln, node = row / H, h = row - node * H;
-                const uint32_t lat = 2u * (node * (uint32_t)p.a.q_lat_stride + h * L), chunk = ln % (16u * LC);
+                const uint32_t lat = 2u * (node * (uint32_t)p.a.q_lat_stride + h * L);
 #pragma unroll 1
                 for (uint32_t i = 2u * LC * wave; i < 2u * LC * (wave + 1u); i++) {
                     const uint32_t r = i * (4u / LC) + ln / (16u * LC), at = __shfl(lat, (int)r, 64);
+                    const uint32_t chunk = (ln % (16u * LC)) ^ apart(r);
                     __builtin_amdgcn_raw_ptr_buffer_load_lds(ql, WL_LDS(vb + 1024u * i), 16u,
                                                              r < rows && 8u * chunk < L ? at + 16u * chunk : kOOB, 0u, 0, 0);
                 }
@@ -150,9 +154,10 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                     f32x16 even, odd;
                     uint32_t most = 0;
                     u32x4 x[4];
-                    u32x4* const at = (u32x4*)(vb + 64u * i);
+                    const uint32_t lr = i % ROWS, b = i / ROWS;
+                    auto at = [&](uint32_t k) { return (u32x4*)(vb + lr * (64u * NB) + 16u * ((4u * b + k) ^ apart(lr))); };
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; k++) x[k] = at[k];
+                    for (uint32_t k = 0; k < 4; k++) x[k] = *at(k);
 #pragma unroll
                     for (uint32_t k = 0; k < 16; k++) {
                         const uint32_t v = x[k / 4][k % 4];
@@ -163,7 +168,7 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                     constexpr uint32_t lo = 5u * (QP - 1u);
                     uint32_t e = (most >> 23) + ((most & 0x7FFFFFu) > 0x700000u ? 1u : 0u);
                     e = e < lo + 2u ? lo : e - 2u;
-                    qscale[i / NB][i % NB] = (uint8_t)(most >= 0x7F800000u ? 255u : e);
+                    qscale[b][lr] = (uint8_t)(most >= 0x7F800000u ? 255u : e);
                     u32x6 y[QP];
 #pragma unroll
                     for (uint32_t j = 0; j < QP; j++) {
@@ -181,25 +186,26 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                             }
                         }
                     }
-                    at[0] = u32x4{y[0][0], y[0][1], y[0][2], y[0][3]};
-                    at[1] = u32x4{y[0][4], y[0][5], y[1][0], y[1][1]};
-                    at[2] = u32x4{y[1][2], y[1][3], y[1][4], y[1][5]};
-                    at[3] = u32x4{y[2][0], y[2][1], y[2][2], y[2][3]};
+                    *at(0) = u32x4{y[0][0], y[0][1], y[0][2], y[0][3]};
+                    *at(1) = u32x4{y[0][4], y[0][5], y[1][0], y[1][1]};
+                    *at(2) = u32x4{y[1][2], y[1][3], y[1][4], y[1][5]};
+                    *at(3) = u32x4{y[2][0], y[2][1], y[2][2], y[2][3]};
                     *(u32x2*)(raw3 + 8u * i) = u32x2{y[2][4], y[2][5]};
                 }
             };
             auto read_queries = [&]() __attribute__((always_inline)) {
-                const uint32_t ln = afresh(tid) & 63u, lr = sr + (ln & 15u), at = lr * NB + (ln >> 4);
+                const uint32_t ln = afresh(tid) & 63u, lr = sr + (ln & 15u);
                 uint32_t e = 0;
 #pragma unroll
                 for (uint32_t s = 0; s < LC; s++) {
-                    const u32x4* b = (const u32x4*)(vb + 64u * (at + 4u * s));
-                    const u32x4 x0 = b[0], x1 = b[1], x2 = b[2], x3 = b[3];
-                    const u32x2 x4 = *(const u32x2*)(raw3 + 8u * (at + 4u * s));
+                    const uint32_t b = 4u * s + (ln >> 4);
+                    auto at = [&](uint32_t k) { return *(const u32x4*)(vb + lr * (64u * NB) + 16u * ((4u * b + k) ^ apart(lr))); };
+                    const u32x4 x0 = at(0), x1 = at(1), x2 = at(2), x3 = at(3);
+                    const u32x2 x4 = *(const u32x2*)(raw3 + 8u * (b * ROWS + lr));
                     qf[s][0] = u32x6{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1]};
                     qf[s][1] = u32x6{x1[2], x1[3], x2[0], x2[1], x2[2], x2[3]};
                     qf[s][2] = u32x6{x3[0], x3[1], x3[2], x3[3], x4[0], x4[1]};
-                    e |= (uint32_t)qscale[lr][4u * s + (ln >> 4)] << (8u * s);
+                    e |= (uint32_t)qscale[b][lr] << (8u * s);
                 }
 #pragma unroll
                 for (uint32_t j = 0; j < QP; j++) {
