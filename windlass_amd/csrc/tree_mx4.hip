@@ -100,14 +100,23 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
             const uint32_t aux_at = lane >= 32u ? ((lane - 32u) / DR == wave ? (lane & 3u) * stride + L / 2u : kOOB)
                                     : 8u * rot_ch < RP ? rot_i * stride + L / 2u + kMxScales + 16u * rot_ch
                                                        : kOOB;
-            auto issue = [&](uint8_t* raw, uint32_t t) __attribute__((always_inline)) {
+            auto rows_of = [&](uint32_t t) __attribute__((always_inline)) {
                 if (t - first_tile >= 64u) find_rows(first_tile + 64u, more_pages);
                 const int i = (int)(t - first_tile);
                 const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)t_hi, i) << 32 |
                                     (uint32_t)__builtin_amdgcn_readlane((int)t_lo, i);
-                const rsrc_t rs = make_rsrc((const void*)at, (uint32_t)__builtin_amdgcn_readlane((int)t_size, i));
+                return make_rsrc((const void*)at, (uint32_t)__builtin_amdgcn_readlane((int)t_size, i));
+            };
+            auto call_values = [&](rsrc_t rs, uint8_t* raw) __attribute__((always_inline)) {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, WL_LDS(raw + 1024u * wave), 16u, val_at, 0u, 0, 0);
+            };
+            auto call_others = [&](rsrc_t rs, uint8_t* raw) __attribute__((always_inline)) {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, WL_LDS(raw + AUX + AUXW * wave), 16u, aux_at, 0u, 0, 0);
+            };
+            auto call_tile = [&](uint8_t* raw, uint32_t t) __attribute__((always_inline)) {
+                const rsrc_t rs = rows_of(t);
+                call_values(rs, raw);
+                call_others(rs, raw);
             };
             // The queries of rows sr + n: lane (row n, block g) has 32 columns of each 128 in
             // pieces, and the rotary part in bf16. They come by DMA to where the values will be,
@@ -244,8 +253,8 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                 x.v_scale = raw[cv_scale];
             };
             // the products of rows sr + n with keys sk + 4 g + j; between them the tile's values
-            // are brought to bf16 in place (VALUES): the matrix cores run on meanwhile
-            auto products = [&](const uint8_t* raw, Keys& x, f32x4& s0, uint32_t place, auto values) __attribute__((always_inline)) {
+            // are brought to bf16 in place (VALUES), and mid(step) runs: the matrix cores run on meanwhile
+            auto products = [&](const uint8_t* raw, Keys& x, f32x4& s0, uint32_t place, auto values, auto mid) __attribute__((always_inline)) {
                 constexpr bool VALUES = decltype(values)::value;
                 const uint32_t to = afresh(cv_to + VB) - VB + place * (kKT * PITCH), to2 = afresh((cv_to ^ 16u) + VB) - VB + place * (kKT * PITCH);
                 f32x4 y[QP];
@@ -268,6 +277,7 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                         y[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, bb, y[j], 4, 2, s, (int)x.scale, s, (int)qs[j]);
                     }
                     if (LC > 1 || s > 0) x.k[s % 2] = *(const u32x4*)(raw + (s + 2 < LC ? key_at ^ (64u * (s + 2)) : key_rot ^ (64u * (s + 2 - LC))));
+                    mid(si);
                     if (VALUES && (LC == 4 || cv_ch < NB)) {
 #pragma unroll
                         for (uint32_t j = 4 * s / LC; j < 4 * (s + 1) / LC; j++) {  // piece j / 2 of pair j % 2
@@ -352,24 +362,21 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
 #pragma unroll
                 for (uint32_t k = 0; k < VP; k++) x.v[k] = vread(x.at, k);
             };
-            auto sums = [&](Values& x, auto then) __attribute__((always_inline)) {
+            auto sums = [&](Values& x) __attribute__((always_inline)) {
                 const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
 #pragma unroll
                 for (uint32_t v = 0; v < CT; v++) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) acc[i][v] = mma(as_bf16x8(x.v[v % VP]), x.p[i], acc[i][v]);
                     if (v + VP < CT) x.v[v % VP] = vread(x.at, v + VP);
-                    if (v == 0) {
-                        l = mma(as_bf16x8(ones), x.own, l);
-                        then();
-                    }
+                    if (v == 0) l = mma(as_bf16x8(ones), x.own, l);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             };
-            // A turn: tile t, in b1, becomes values and weights in place E; tile t + 3's place
-            // is b0. Of a SIMD's two waves the first sums tile t - 1 before the turn's barrier,
-            // the second tile t behind it, so that one's sums run beside the other's scores.
-            constexpr bool late = false;
+            // A turn, between two barriers: tile t, in b1, becomes values and weights in place E,
+            // tile t - 1 is summed from the other one; tile t + 3 is called for to b0, between the
+            // products (at their beginning a wave stands still for it: 170 us for 163, the 64 x
+            // 8). At t = kt1 the last sums.
             uint32_t fresh = kt0;  // the tile whose maxima are the references
             auto turn = [&](uint8_t* b0, const uint8_t* b1, auto place, uint32_t t) __attribute__((always_inline)) {
                 constexpr uint32_t E = decltype(place)::value;
@@ -378,37 +385,33 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                     f32x4 s0;
                     read_keys(b1, x);
                     __builtin_amdgcn_sched_barrier(0);
-                    issue(b0, t + 3);
-                    products(b1, x, s0, E, std::true_type{});
+                    const rsrc_t rs = rows_of(t + 3);
+                    products(b1, x, s0, E, std::true_type{}, [&](auto si) __attribute__((always_inline)) {
+                        constexpr int s = decltype(si)::value;
+                        if (s == (LC > 1 ? 1 : 0)) call_values(rs, b0);
+                        if (s == LC - 1) call_others(rs, b0);
+                    });
                     const float f = scores(s0, t);
                     if (t == fresh || (WIN && masked(t))) late_maxima(largest(s0, f));
                     put_weights(s0, f, E);
-                    if (late) {
-                        vm_wait<4>();  // tile t + 1 is there; t + 2 and t + 3 may be on the way
-                        ring_barrier();
-                    }
-                } else if (late) {
-                    return false;
                 }
-                if (late || t > kt0) {
+                if (t > kt0) {
                     Values y;
-                    read_values(late ? E : 1u - E, y);
+                    read_values(1u - E, y);
                     __builtin_amdgcn_sched_barrier(0);
-                    sums(y, [] {});
+                    sums(y);
                 }
                 if (t >= kt1) return false;
-                if (!late) {
-                    vm_wait<4>();
-                    ring_barrier();
-                }
+                vm_wait<4>();  // tile t + 1 is there; t + 2 and t + 3 may be on the way
+                ring_barrier();
                 return true;
             };
             call_queries();
             first_rows();
             for (;;) {
-                issue(raw0, kt0);
-                issue(raw1, kt0 + 1);
-                issue(raw2, kt0 + 2);
+                call_tile(raw0, kt0);
+                call_tile(raw1, kt0 + 1);
+                call_tile(raw2, kt0 + 2);
                 vm_wait<0>();
                 ring_barrier();
                 if (fresh == kt0) {
@@ -439,13 +442,13 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                 float x = kNone;
                 first_rows();
                 for (uint32_t t = kt0; t < kt1; t++) {
-                    issue(raw0, t);
+                    call_tile(raw0, t);
                     vm_wait<0>();
                     ring_barrier();
                     f32x4 s0;
                     Keys y;
                     read_keys(raw0, y);
-                    products(raw0, y, s0, 0, std::false_type{});
+                    products(raw0, y, s0, 0, std::false_type{}, [](auto) {});
                     const float f = scores(s0, t);
                     x = fmaxf(x, largest(s0, f));
                     ring_barrier();
