@@ -15,13 +15,21 @@ namespace {
 // (u + (m - M) s). (Sums of exp times z itself would lose what z has over z - M.)
 //
 // First launch: a wave has a part of a row, one pass over it. A lane has 32 values at a
-// time, their largest, and its own m, s and u, brought to a new m once for the 32. The
-// n_top largest so far stand in the wave's lanes, in order: value as an ordered integer,
-// id. What is at least the last of them (one comparison for each 8 values; few pass)
-// goes in one by one: its place is the number of lanes before it, those behind take
-// their neighbour's. The first 32 x 64 values' bound is the n_top-th of the lanes' largest:
-// that many are at least as large. Second launch: a work-group a row joins its parts, a
-// wave a token looks up its logit.
+// time, their largest, and its own m, s and u, brought to a new m once for the 32. Second
+// launch: a work-group a row joins its parts, a wave a token looks up its logit.
+//
+// The n_top most likely: the first launch leaves the largest value that each lane has met
+// (one comparison in 32 values). The n-th largest of these, over the lanes of all parts, is
+// a bound that at least n values reach and few others: the second launch finds it, reads
+// again what the lanes that reach it have met, and what reaches it too goes into lists in
+// LDS, ordered by counting. Where more than kLanes lanes reach the bound (rows of equal
+// values) the whole row is read again; a list that runs full is cut down to its n best.
+//
+// Bound by the read of the logits where rows are many, by two launches where they are few.
+// 284 rows of 154880: f32 30 us (5.8 TB/s) with no n_top, 42 with 20; bf16 22 us (4.0 TB/s,
+// two exponentials' time a value) and 31. One row of them 9 us and 15. 2048 rows of 32000
+// bf16: 32 us and 47. (Lists kept in the first launch, by insertion into each lane's
+// registers: 57 us at 284 rows bf16 and n_top 20, 31 at one row.)
 constexpr uint32_t kPer = 32;             // values a lane has at a time
 constexpr uint32_t kPart = 64 * kPer;     // of a wave
 constexpr float kLowest = -3.402823466e38f;
@@ -31,7 +39,7 @@ struct Logp {
     wl_logprobs a;
     uint32_t parts;   // per row
     float* sums;      // [n_rows][parts][4] m, s, u
-    uint32_t* top;    // [n_rows][parts][n_top][2] ordered value, id
+    float* most;      // [n_rows][parts][64] the largest value of each lane
 };
 
 // Integers in the order of the values, NaN (any) the largest and -0 as +0; no value's is 0.
@@ -61,30 +69,88 @@ WL_DEV Sums wave_join(Sums x) {
     return x;
 }
 
-// The largest of a wave's values so far: lane i the i-th.
-struct Best {
-    uint32_t key = 0, id = ~0u;
-    float least = -INFINITY;  // what is below it is not among the n
-    __device__ __forceinline__ bool before(uint32_t k, uint32_t i) const { return key > k || (key == k && id < i); }
-    __device__ __forceinline__ void put(uint32_t lane, uint32_t n, uint32_t k, uint32_t i, uint32_t floor) {  // k, i uniform
-        const uint32_t p = (uint32_t)__popcll(__ballot(before(k, i)));
-        if (p >= n) return;
-        const uint32_t pk = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)key, 0x138, 0xf, 0xf, false);  // the lane below's
-        const uint32_t pi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)id, 0x138, 0xf, 0xf, false);
-        key = lane < p ? key : lane == p ? k : pk;
-        id = lane < p ? id : lane == p ? i : pi;
-        const uint32_t last = (uint32_t)__builtin_amdgcn_readlane((int)key, (int)(n - 1u));
-        least = value_of(last > floor ? last : floor);
+// A wave's list of the values that may be among the n largest, of (ordered value, id).
+constexpr uint32_t kList = 640;
+constexpr uint32_t kLanes = 256;  // whose values are read again
+constexpr uint32_t kShare = 10, kAhead = 4;  // loads in flight
+
+struct List {
+    u32x2* const at;         // [kList] in LDS
+    const uint32_t lane, n;
+    uint32_t count = 0;
+    uint32_t floor = 0;      // ordered: n values are at least this
+    float least = -INFINITY; // the same
+    __device__ __forceinline__ List(u32x2* a, uint32_t l, uint32_t n_top) : at(a), lane(l), n(n_top) {}
+    static __device__ __forceinline__ bool before(uint32_t k, uint32_t i, uint32_t k2, uint32_t i2) { return k > k2 || (k == k2 && i < i2); }
+    __device__ __forceinline__ void raise(uint32_t f) {
+        if (f <= floor) return;
+        floor = f;
+        least = value_of(f);
     }
-    // every lane's value z of id `i` (where ok)
-    __device__ __forceinline__ void take(uint32_t lane, uint32_t n, float z, uint32_t i, bool ok, uint32_t floor) {
-        uint64_t left = __ballot(ok && !(z < least));
-        while (left) {
-            const int l = __ffsll((unsigned long long)left) - 1;
-            left &= left - 1;
-            put(lane, n, (uint32_t)__builtin_amdgcn_readlane((int)ordered(z), l), (uint32_t)__builtin_amdgcn_readlane((int)i, l),
-                floor);
+    // From four values a lane (0: none): the n-th largest of them, to 16 bits, from below. (A
+    // NaN's bound, to 16 bits, is one too.)
+    __device__ __forceinline__ void bound(u32x4 mine) {
+        uint32_t f = 0;
+#pragma unroll
+        for (uint32_t b = 31; b >= 16; b--) {
+            const uint32_t c = f | 1u << b;
+            uint32_t reach = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) reach += (uint32_t)__popcll(__ballot(mine[k] >= c));
+            if (reach >= n) f = c;
         }
+        raise(uni(f));
+    }
+    // Leaves the n best, in order.
+    __device__ __forceinline__ void cut() {
+        uint32_t k[kList / 64], id[kList / 64], bk = 0, bi = ~0u;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (uint32_t j = 0; j < kList / 64; j++) {
+            const u32x2 x = 64u * j + lane < count ? at[64u * j + lane] : u32x2{0u, ~0u};
+            k[j] = x[0];
+            id[j] = x[1];
+        }
+        const uint32_t m = count < n ? count : n;
+        for (uint32_t r = 0; r < m; r++) {
+            uint32_t x = 0, i = ~0u;
+#pragma unroll
+            for (uint32_t j = 0; j < kList / 64; j++)
+                if (before(k[j], id[j], x, i)) {
+                    x = k[j];
+                    i = id[j];
+                }
+            for (int o = 32; o > 0; o >>= 1) {
+                const uint32_t x2 = __shfl_xor(x, o, 64), i2 = __shfl_xor(i, o, 64);
+                if (before(x2, i2, x, i)) {
+                    x = x2;
+                    i = i2;
+                }
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kList / 64; j++)
+                if (id[j] == i) k[j] = 0, id[j] = ~0u;  // (an id stands in a list once)
+            if (lane == r) {
+                bk = x;
+                bi = i;
+            }
+        }
+        if (lane < m) at[lane] = u32x2{bk, bi};
+        __builtin_amdgcn_wave_barrier();
+        count = m;
+        if (m == n) raise((uint32_t)__builtin_amdgcn_readlane((int)bk, (int)(n - 1u)));
+    }
+    // every lane's value o (ordered) of id i, where ok
+    __device__ __forceinline__ void add(uint32_t o, uint32_t i, bool ok) {
+        ok = ok && o >= floor;
+        const uint64_t m = __ballot(ok);
+        if (!m) return;
+        if (ok) at[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u))] = u32x2{o, i};
+        count += (uint32_t)__popcll(m);
+    }
+    // before `more` values a lane come
+    __device__ __forceinline__ void make_room(uint32_t more) {
+        if (__builtin_expect(count > kList - 64u * more, 0)) cut();
     }
 };
 
@@ -92,11 +158,7 @@ template <bool BF, bool TOP, bool ENT>
 struct Stream {
     static constexpr uint32_t VE = BF ? 8 : 4, U = kPer / VE;
     Sums x{kLowest, 0.f, 0.f};
-    Best best;
-    uint32_t floor = 0;
-    bool fresh = true;
-    const uint32_t lane, n;
-    __device__ __forceinline__ Stream(uint32_t l, uint32_t n_top) : lane(l), n(n_top) {}
+    float largest = -INFINITY;  // of this lane
     static __device__ __forceinline__ void open(u32x4 r, float* v) {
 #pragma unroll
         for (uint32_t k = 0; k < 4; k++) {
@@ -118,97 +180,82 @@ struct Stream {
             if (ENT) x.u = fmaf(e, fmaxf(d, -1e30f), x.u);
         }
     }
-    // U vectors of a lane, the first of id `id0`, the others 64 VE ids apart; vectors
-    // from `end` ids on do not count (CUT)
+    // U vectors of a lane, 64 apart, of which those before `count` count (CUT)
     template <bool CUT>
-    __device__ __forceinline__ void block(const u32x4 (&raw)[U], uint32_t id0, uint32_t end) {
-        float v[kPer], top[U], most = -INFINITY;
+    __device__ __forceinline__ void block(const u32x4 (&raw)[U], uint32_t first, uint32_t count) {
+        float v[kPer], most = -INFINITY;
 #pragma unroll
         for (uint32_t i = 0; i < U; i++) {
             open(raw[i], v + VE * i);
-            const bool ok = !CUT || id0 + 64u * VE * i < end;
-            float t = -INFINITY;
 #pragma unroll
             for (uint32_t k = 0; k < VE; k++) {
-                if (CUT && !ok) v[VE * i + k] = -INFINITY;
-                t = larger(t, v[VE * i + k]);
+                if (CUT && first + 64u * i >= count) v[VE * i + k] = -INFINITY;
+                most = larger(most, v[VE * i + k]);
             }
-            top[i] = t;
-            most = larger(most, t);
         }
         add(v, kPer, most);
-        if (!TOP) return;
-        if (fresh) {  // the n-th largest of the lanes' largest: at least n values are no less
-            fresh = false;
-            const uint32_t mine = ordered(most);
-            uint32_t rank = 0;
-#pragma unroll 8
-            for (uint32_t l = 0; l < 64; l++) {
-                const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)l);
-                rank += o > mine || (o == mine && l < lane) ? 1u : 0u;
-            }
-            const uint64_t nth = __ballot(rank == n - 1u);
-            floor = (uint32_t)__builtin_amdgcn_readlane((int)mine, __ffsll((unsigned long long)nth) - 1);
-            best.least = value_of(floor);
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < U; i++) {
-            if (!__ballot(!(top[i] < best.least))) continue;
-            const uint32_t id = id0 + 64u * VE * i;
-#pragma unroll
-            for (uint32_t k = 0; k < VE; k++) best.take(lane, n, v[VE * i + k], id + k, !CUT || id < end, floor);
-        }
+        if (TOP) largest = larger(largest, most);
     }
+};
+
+// A row's 16-byte vectors: the first value of vector 0, and how many there are. What is
+// before and behind them is the first part's.
+template <bool BF>
+struct Row {
+    static constexpr uint32_t VE = BF ? 8 : 4, ES = BF ? 2 : 4;
+    const uint8_t* base;
+    uint32_t head, nv, tail;
+    __device__ __forceinline__ Row(const Logp& p, uint32_t row) {
+        base = (const uint8_t*)p.a.d_logits + (uint64_t)row * p.a.stride * ES;
+        const uint32_t off = (uint32_t)((0u - (uint32_t)(uintptr_t)base) & 15u) / ES;
+        head = off < p.a.n_vocab ? off : p.a.n_vocab;
+        nv = (p.a.n_vocab - head) / VE;
+        tail = head + nv * VE;
+    }
+    __device__ __forceinline__ uint32_t part_at(const Logp& p, uint32_t part) const { return (uint32_t)((uint64_t)nv * part / p.parts); }
+    __device__ __forceinline__ float value(uint32_t id) const {
+        return BF ? bf2f(gld((const uint16_t*)base + id)) : gld((const float*)base + id);
+    }
+    // the value before or behind the vectors that a lane has (of id < n_vocab)
+    __device__ __forceinline__ uint32_t edge(uint32_t lane) const { return lane < head ? lane : tail + lane - head; }
 };
 
 template <bool BF, bool TOP, bool ENT>
 __global__ __launch_bounds__(256) void logp_part_kernel(Logp p) {
     using St = Stream<BF, TOP, ENT>;
-    constexpr uint32_t VE = St::VE, U = St::U, ES = BF ? 2 : 4;
+    constexpr uint32_t U = St::U;
     const uint32_t lane = threadIdx.x & 63u, wave = uni(blockIdx.x * 4u + (threadIdx.x >> 6));
     const uint32_t row = wave / p.parts, part = wave - row * p.parts;
     if (row >= p.a.n_rows) return;
-    const uint32_t V = p.a.n_vocab;
-    const uint8_t* base = (const uint8_t*)p.a.d_logits + (uint64_t)row * p.a.stride * ES;
-    // whole 16 bytes from the first aligned value on; what is before and behind them is
-    // the first part's
-    const uint32_t off = (uint32_t)((0u - (uint32_t)(uintptr_t)base) & 15u) / ES, head = off < V ? off : V;
-    const uint32_t nv = (V - head) / VE, tail = head + nv * VE;
-    const uint32_t v0 = (uint32_t)((uint64_t)nv * part / p.parts), v1 = (uint32_t)((uint64_t)nv * (part + 1u) / p.parts);
-    St st(lane, p.a.n_top);
-    const rsrc_t rs = make_rsrc(base + (uint64_t)head * ES, nv * 16u);
+    const Row<BF> r(p, row);
+    const uint32_t v0 = r.part_at(p, part), v1 = r.part_at(p, part + 1u);
+    St st;
+    const rsrc_t rs = make_rsrc(r.base + (uint64_t)r.head * Row<BF>::ES, r.nv * 16u);
     auto load = [&](u32x4 (&raw)[U], uint32_t v) {
 #pragma unroll
         for (uint32_t i = 0; i < U; i++) raw[i] = bld16_nt(rs, (v + 64u * i + lane) * 16u, 0);
     };
     uint32_t v = v0;
-    const uint32_t end = head + v1 * VE;
     u32x4 a[U], b[U];
     if (v < v1) load(a, v);
     while (v < v1) {
         const uint32_t next = v + 64u * U;
         if (next < v1) load(b, next);
-        if (next <= v1) st.template block<false>(a, head + (v + lane) * VE, end);
-        else st.template block<true>(a, head + (v + lane) * VE, end);
+        if (next <= v1) st.template block<false>(a, v + lane, v1);
+        else st.template block<true>(a, v + lane, v1);
         v = next;
 #pragma unroll
         for (uint32_t i = 0; i < U; i++) a[i] = b[i];
     }
-    if (part == 0 && head + (V - tail) > 0) {
-        const uint32_t id = lane < head ? lane : tail + lane - head;
-        const bool ok = id < V;
-        float z = -INFINITY;
-        if (ok) z = BF ? bf2f(gld((const uint16_t*)base + id)) : gld((const float*)base + id);
+    if (part == 0 && r.head + (p.a.n_vocab - r.tail) > 0) {
+        const uint32_t id = r.edge(lane);
+        const float z = id < p.a.n_vocab ? r.value(id) : -INFINITY;
         st.add(&z, 1, z);
-        if (TOP) st.best.take(lane, p.a.n_top, z, id, ok, st.floor);
     }
     const Sums x = wave_join(st.x);
     const uint64_t slot = (uint64_t)row * p.parts + part;
     if (lane == 0) gst((f32x4*)(p.sums + 4u * slot), f32x4{x.m, x.s, x.u, 0.f});
-    if (TOP && lane < p.a.n_top) {
-        uint32_t* o = p.top + 2u * (slot * p.a.n_top + lane);
-        gst((u32x2*)o, u32x2{st.best.key, st.best.id});
-    }
+    if (TOP) gst(p.most + 64u * slot + lane, st.largest);
 }
 
 WL_DEV Sums row_sums(const Logp& p, uint32_t row, uint32_t lane) {
@@ -223,7 +270,11 @@ WL_DEV Sums row_sums(const Logp& p, uint32_t row, uint32_t lane) {
 // Work-groups [0, rows): a row's entropy and most likely tokens; behind them a wave a token.
 template <bool BF>
 __global__ __launch_bounds__(256) void logp_join_kernel(Logp p, uint32_t rows) {
-    __shared__ u32x2 lists[4][WL_LOGPROB_MAX_TOP];
+    constexpr uint32_t VE = Row<BF>::VE;
+    __shared__ u32x2 lists[4][kList];
+    __shared__ uint32_t lanes[kLanes];  // those whose largest reach the bound
+    __shared__ u32x4 highs[64];
+    __shared__ uint32_t n_lanes, counts[4];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = uni(tid >> 6), n = p.a.n_top;
     if (blockIdx.x >= rows) {
         const uint32_t t = (blockIdx.x - rows) * 4u + wv;
@@ -247,33 +298,103 @@ __global__ __launch_bounds__(256) void logp_join_kernel(Logp p, uint32_t rows) {
     const float log_s = logf(x.s);
     if (tid == 0 && p.a.d_entropy) gst(p.a.d_entropy + row, log_s - x.u / x.s);
     if (n == 0) return;
-    // the parts' lists, dealt out to the waves, then the waves' to the first
-    Best best;
-    const uint32_t all = p.parts * n;
-    const u32x2* top = (const u32x2*)(p.top + 2ull * row * all);
-    for (uint32_t i = 64u * wv; i < all; i += 256u) {
-        const bool ok = i + lane < all;
-        u32x2 c = {0u, ~0u};
-        if (ok) c = gld(top + i + lane);
-        best.take(lane, n, value_of(c[0]), c[1], ok && c[0] != 0u, 0u);
-    }
-    if (lane < n) lists[wv][lane] = u32x2{best.key, best.id};
+    // a bound from the largest values of the lanes, a share of them to a thread
+    List list(lists[wv], lane, n);
+    const uint32_t all = 64u * p.parts;  // lanes
+    const float* most = p.most + 64ull * row * p.parts;
+    auto shares = [&](auto&& f) {
+        for (uint32_t i0 = tid; i0 < all; i0 += 256u * kShare) {
+            float v[kShare];
+#pragma unroll
+            for (uint32_t k = 0; k < kShare; k++) v[k] = gld(most + (i0 + 256u * k < all ? i0 + 256u * k : i0));
+#pragma unroll
+            for (uint32_t k = 0; k < kShare; k++)
+                if (i0 + 256u * k < all) f(ordered(v[k]), i0 + 256u * k);
+        }
+    };
+    uint32_t high = 0;
+    shares([&](uint32_t o, uint32_t) { high = max(high, o); });
+    ((uint32_t*)highs)[tid] = high;
+    if (tid == 0) n_lanes = 0;
     __syncthreads();
-    if (wv != 0) return;
-    for (uint32_t w = 1; w < 4; w++) {
-        const u32x2 c = lane < n ? lists[w][lane] : u32x2{0u, ~0u};
-        best.take(lane, n, value_of(c[0]), c[1], c[0] != 0u, 0u);
+    list.bound(highs[lane]);
+    shares([&](uint32_t o, uint32_t i) {
+        if (o < list.floor) return;
+        const uint32_t k = atomicAdd(&n_lanes, 1u);  // (their order changes no result)
+        if (k < kLanes) lanes[k] = i;
+    });
+    __syncthreads();
+    const uint32_t found = uni(n_lanes);
+    const bool whole = found > kLanes;
+    // what these lanes have met, or the whole row: 64 vectors, one a lane, make a step
+    const Row<BF> r(p, row);
+    const rsrc_t rs = make_rsrc(r.base + (uint64_t)r.head * Row<BF>::ES, r.nv * 16u);
+    const uint32_t each = (r.nv / p.parts + 64u) / 64u;  // vectors of a lane, at most
+    const uint32_t sh = each > 1u ? 32u - (uint32_t)__builtin_clz(each - 1u) : 0u;
+    const uint32_t steps = ((whole ? r.nv : found << sh) + 63u) / 64u;
+    for (uint32_t i0 = wv; i0 < steps; i0 += 4u * kAhead) {
+        u32x4 raw[kAhead];
+        uint32_t at[kAhead];  // the lane's vector (from nv on: none)
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; k++) {
+            const uint32_t i = 64u * (i0 + 4u * k) + lane;
+            at[k] = ~0u;
+            if (whole) {
+                at[k] = i;
+            } else if (i >> sh < found) {
+                const uint32_t x = lanes[i >> sh], v = r.part_at(p, x / 64u) + x % 64u + 64u * (i & ((1u << sh) - 1u));
+                if (v < r.part_at(p, x / 64u + 1u)) at[k] = v;
+            }
+            raw[k] = bld16(rs, at[k] < r.nv ? at[k] * 16u : kOOB, 0);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; k++) {
+            float v[VE];
+            Stream<BF, true, true>::open(raw[k], v);
+            list.make_room(VE);
+#pragma unroll
+            for (uint32_t e = 0; e < VE; e++) list.add(ordered(v[e]), r.head + at[k] * VE + e, at[k] < r.nv);
+        }
     }
-    if (lane < n) {
-        gst(p.a.d_top_id + (uint64_t)row * n + lane, (int32_t)best.id);
-        gst(p.a.d_top_logp + (uint64_t)row * n + lane, (value_of(best.key) - x.m) - log_s);
+    if (wv == 0) {
+        const uint32_t id = r.edge(lane);
+        const bool ok = id < p.a.n_vocab && lane < 32u;
+        list.make_room(1);
+        list.add(ordered(ok ? r.value(id) : 0.f), id, ok);
+    }
+    // the waves' lists as one, ordered by counting
+    if (list.count > 64u) list.cut();
+    const u32x2 own = lane < list.count ? lists[wv][lane] : u32x2{0u, ~0u};
+    if (lane == 0) counts[wv] = list.count;
+    __syncthreads();
+    uint32_t before = 0, count = 0;
+    for (uint32_t w = 0; w < 4; w++) {
+        if (w < wv) before += counts[w];
+        count += counts[w];
+    }
+    u32x2* const one = lists[0];  // at most 256, and zeros up to a multiple of 8
+    if (lane < list.count) one[before + lane] = own;
+    if (tid < 8u) one[count + tid] = u32x2{0u, ~0u};
+    __syncthreads();
+    if (lane >= list.count) return;
+    uint32_t rank = 0;
+    for (uint32_t i = 0; i < count; i += 8u)
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) rank += List::before(one[i + k][0], one[i + k][1], own[0], own[1]) ? 1u : 0u;
+    if (rank < n) {
+        gst(p.a.d_top_id + (uint64_t)row * n + rank, (int32_t)own[1]);
+        gst(p.a.d_top_logp + (uint64_t)row * n + rank, (value_of(own[0]) - x.m) - log_s);
     }
 }
 
-// Parts of a row: waves for the whole chip where there are few rows, and no part
-// shorter than what a wave has at a time.
+// Parts of a row: waves for the whole chip where there are few rows, and no part shorter
+// than what a wave has at a time. With n_top more and shorter parts: there is less to read
+// again, which outweighs the longer join (in us at 2048, 4096 and 8192 waves, bf16 and n_top
+// 20: 284 x 154880 33.0, 31.2, 30.7, 2048 x 32000 62.9, 53.6, 46.7; without n_top 22.2, 22.8,
+// 22.9 and 32.7, 32.8, 32.4; 1024 waves 33.3 at the former).
 uint32_t parts_of(const wl_logprobs& a) {
-    const uint32_t most = (a.n_vocab + kPart - 1u) / kPart, want = a.n_rows >= 4096u ? 1u : 4096u / (a.n_rows ? a.n_rows : 1u);
+    const uint32_t waves = a.n_top ? 8192u : 2048u, most = (a.n_vocab + kPart - 1u) / kPart;
+    const uint32_t want = a.n_rows >= waves ? 1u : waves / (a.n_rows ? a.n_rows : 1u);
     return want < most ? want : most;
 }
 
@@ -281,7 +402,7 @@ uint32_t parts_of(const wl_logprobs& a) {
 
 size_t logprobs_scratch(const wl_logprobs& a) {
     const size_t slots = (size_t)(a.n_rows ? a.n_rows : 1) * parts_of(a);
-    return slots * (16 + 8 * (size_t)a.n_top);
+    return slots * (16 + (a.n_top ? 256 : 0));
 }
 
 int launch_logprobs(const wl_logprobs& a, void* stream) {
@@ -289,7 +410,7 @@ int launch_logprobs(const wl_logprobs& a, void* stream) {
     p.a = a;
     p.parts = parts_of(a);
     p.sums = (float*)a.d_scratch;
-    p.top = (uint32_t*)(p.sums + 4 * (size_t)a.n_rows * p.parts);
+    p.most = p.sums + 4 * (size_t)a.n_rows * p.parts;
     hipStream_t st = (hipStream_t)stream;
     const bool bf = a.dtype == WL_TYPE_BF16;
     const dim3 grid((uint32_t)(((uint64_t)a.n_rows * p.parts + 3u) / 4u));
