@@ -140,3 +140,14 @@ def test_offsets_past_32_bits(gpu):
     x.args.d_logits, x.args.stride = big.ptr, stride
     x.run().check()
     big.free()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [33, 700, 2100, 8000, 17000, 70000])
+def test_rows_of_few_values(gpu, V, t):
+    """Many values reach the bound of the most likely: the lists run full, or the row is read again."""
+    rng = np.random.default_rng(V)
+    z = np.stack([np.full(V, -2.0), rng.integers(0, 2, V).astype(float), np.where(rng.random(V) < 0.03, 4.0, rng.standard_normal(V)),
+                  np.where(np.arange(V) < V // 2, 1.0, 0.0)])
+    for n_top in (1, 32):
+        Logprobs(z, t, rng.integers(0, V, 4), n_top=n_top).run().check()
