@@ -59,8 +59,10 @@ struct Tree {
 // work-group c takes piece c. (Requests without tokens change nothing of this, as
 // long as a launch has a thread for each: up to 256, 512 in work-groups of eight waves.)
 // One request of 64 nodes over 8192 keys, 32 bits: 222 us
-// without, 207 with; 5 of 7 nodes 67 and 59; 12 of 5 nodes 28 and 23; 32 contexts 191 and 179. (Requests of
-// one row tile need neither chunks nor pieces: their keys stand in a row.)
+// without, 207 with; 5 of 7 nodes 67 and 59; 12 of 5 nodes 28 and 23; 32 contexts 191 and 179. Requests of
+// one row tile, 16-bit queries: 32 contexts of up to 65536 keys 180 and 170, of 4-bit rows 129 and 121, these
+// through a window of 4096 57 and 46; 8 of up to 3016 keys 25 and 19. (They need no chunks: their keys stand
+// in a row.)
 constexpr uint32_t kSlack = 6;
 //
 // Through a window (WIN) a request's keys are those that some node may see: tiles
@@ -189,10 +191,9 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
     if (c == 0 && status) set_status(p.a.d_status, status);
     const uint64_t inc = sum_up(mine);
     tiles = sum_up(tiles);
-    const uint64_t several = __ballot(q.nrt > 1) ? 1ull << 32 : 0;  // a request (of a thread with one) has more than one
     if (lane == 63) {
         tmp[wv] = inc;
-        tmp[NW + 2 + wv] = several | tiles;
+        tmp[NW + 2 + wv] = tiles;
     }
     __syncthreads();
     Place f;
@@ -209,7 +210,7 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
     f.pieces = 0;
     uint64_t at = inc - mine;
     for (uint32_t w = 0; w < wv; w++) at += tmp[w];
-    if (share == 1 && (all >> 32) != 0 && (uint32_t)all < GRID && (f.total >> 32) == 0) {
+    if (share == 1 && all < GRID && (f.total >> 32) == 0) {
         // the least of some lengths with which the pieces are no more than the work-groups
         const uint32_t per = (uint32_t)f.per, step = (kSlack + per / 16u + kTries - 2u) / (kTries - 1u);
         for (uint32_t k = wv; k < kTries; k += NW) {
