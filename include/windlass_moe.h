@@ -697,8 +697,8 @@ const char* wl_paged_last_error(void);
  * columns, 1152 in bf16. A block's scale is the least 2^e, -125 <= e <= 125,
  * with which its largest magnitude is at most 6 (beyond that values are held to 6),
  * a value the nearest of 0, 1/2, 1, 3/2, 2, 3, 4 and 6 times it, of two as near the
- * one with the even code; a block with a NaN or an infinity has scale 255 and counts
- * as NaN. A slot is page * page_size + row. */
+ * one with the even code; a block with a NaN or an infinity has scale 255; blocks
+ * of scale 253 and more count as NaN. A slot is page * page_size + row. */
 typedef struct wl_paged_cache {
     void*    d_rows;
     uint32_t dtype;

@@ -439,3 +439,43 @@ def test_attention_most_heads(gpu):
     rng = np.random.default_rng(28)
     for q in Q:
         S.Serving(29, q, "mxfp4", 32, 8, 1024, 8, [40, 3], [2, 1], random_trees(rng, [2, 1])).upload().run().check()
+
+
+@pytest.mark.parametrize("scale", [252, 253, 254])
+def test_read_scales_beyond_those_of_the_write(gpu, scale):
+    """253 and more count as NaN; 252 gives its values, up to 6 x 2^125."""
+    t = S.Serving(11, "f32", "mxfp4", 96, 16, 2, 16, [20], [0])
+    page = t.table[0, 0]
+    t.bytes[page, 3, 48 + S.scale_at(1)] = scale
+    t.upload()
+    want = np.array(t.rows[0])
+    code = t.bytes[page, 3, 16:32]
+    code = np.stack([code & 15, code >> 4], 1).reshape(1, 32).astype(np.int64)
+    want[3, 32:64] = S.values(code, np.array([[252]]))[0] if scale == 252 else np.nan
+    for dtype in ("f32", "bf16"):
+        assert np.array_equal(read(t, dtype, None, [20])[0][:20], P.as_type(want, dtype), equal_nan=True)
+
+
+@pytest.mark.parametrize("q", Q)
+@pytest.mark.parametrize("scale", [253, 254, 255])
+@pytest.mark.parametrize("window", [0, 40])
+def test_rows_of_any_bytes(gpu, q, scale, window):
+    """Rows that nobody sees hold anything; the same bytes in a row that some see make their results NaN."""
+    masks = [1, 3, 5, 9, 17, 33, 65, 129]  # node 1 is seen by itself alone
+    n = 150
+    t = S.Serving(36, q, "mxfp4", 512, 64, 4, 32, [n, n], [8, 8], masks + masks, window=window, sinks=0)
+    def spoil(k):
+        row = t.bytes[t.table[0, k // 32], k % 32]
+        row[:256], row[256:272], row[272:] = 0x77, scale, 0x7F
+    spoil(n + 1)
+    if window:
+        for k in range(n - window + 1):
+            spoil(k)
+    t.upload().run()
+    out = t.out()[:, :4 * 512].reshape(16, 4, 512)
+    for i in range(16):
+        if i == 1:
+            assert np.isnan(out[i]).all()
+        else:
+            y, far = t.want(i // 8, i % 8)
+            assert np.all(np.abs(out[i] - y) <= far)

@@ -411,6 +411,8 @@ int launch_logprobs(const wl_logprobs& a, void* stream) {
     p.parts = parts_of(a);
     p.sums = (float*)a.d_scratch;
     p.most = p.sums + 4 * (size_t)a.n_rows * p.parts;
+    const uint32_t rows = a.d_entropy || a.n_top ? a.n_rows : 0u, wgs = rows + (a.n_tokens + 3u) / 4u;
+    if (wgs == 0) return 0;
     hipStream_t st = (hipStream_t)stream;
     const bool bf = a.dtype == WL_TYPE_BF16;
     const dim3 grid((uint32_t)(((uint64_t)a.n_rows * p.parts + 3u) / 4u));
@@ -421,8 +423,6 @@ int launch_logprobs(const wl_logprobs& a, void* stream) {
     else bf ? part(logp_part_kernel<true, false, false>) : part(logp_part_kernel<false, false, false>);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    const uint32_t rows = a.d_entropy || a.n_top ? a.n_rows : 0u, wgs = rows + (a.n_tokens + 3u) / 4u;
-    if (wgs == 0) return 0;
     if (bf) hipLaunchKernelGGL(logp_join_kernel<true>, dim3(wgs), dim3(256), 0, st, p, rows);
     else hipLaunchKernelGGL(logp_join_kernel<false>, dim3(wgs), dim3(256), 0, st, p, rows);
     return (int)hipGetLastError();

@@ -26,7 +26,7 @@ constexpr uint32_t kMxScales = 16;
 // Where among them block b's stands: a lane of the scaled products has blocks g, 4 + g,
 // 8 + g and 12 + g, whose scales are then one word.
 constexpr uint32_t mx_scale_at(uint32_t b) { return 4u * (b % 4u) + b / 4u; }
-constexpr uint32_t kMxLo = 2, kMxHi = 252;  // the scales that the write gives a block
+constexpr uint32_t kMxLo = 2, kMxHi = 252;  // the scales that the write gives a block (above: a block that is NaN)
 
 }  // namespace paged
 }  // namespace wl

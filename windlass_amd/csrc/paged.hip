@@ -493,8 +493,8 @@ __global__ __launch_bounds__(256) void row_read_kernel(wl_row_read p, uint32_t p
                     const u32x4 x = __builtin_bit_cast(u32x4, fp4x8_bf16(gld((const uint32_t*)row + k), e8m0f(s)));
 #pragma unroll
                     for (int m = 0; m < 4; m++) {
-                        v[2 * m] = s == 255u ? __builtin_nanf("") : __uint_as_float(x[m] << 16);
-                        v[2 * m + 1] = s == 255u ? __builtin_nanf("") : __uint_as_float(x[m] & 0xFFFF0000u);
+                        v[2 * m] = s > kMxHi ? __builtin_nanf("") : __uint_as_float(x[m] << 16);
+                        v[2 * m + 1] = s > kMxHi ? __builtin_nanf("") : __uint_as_float(x[m] & 0xFFFF0000u);
                     }
                 } else {
                     load8<true>(row + L / 2 + kMxScales, 8u * (k - cl), v);

@@ -1,9 +1,10 @@
 // paged_dev.h — device helpers that the paged-cache kernels (paged.hip,
-// tree_attn.hip) share. Not public ABI.
+// tree_dev.h, tree_attn.hip, tree_mx4.hip, logprobs.hip) share. Not public ABI.
 #pragma once
 #include <type_traits>
 
 #include "dev_common.h"
+#include "paged.h"
 
 namespace wl {
 namespace paged {
@@ -22,15 +23,15 @@ WL_DEV uint32_t pack_bf16(float a, float b) {  // a in the low half
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 // A block of 32 E2M1 values and its scale, on their way to bf16 (exact): 16-byte pieces
 // j = 0 .. 3 go into LDS, piece (turn + j) % 4 of the block at dst. (The lanes of a wave
-// write with different turns, so that they meet different banks.) A block of scale 255,
-// a NaN, becomes zeros.
+// write with different turns, so that they meet different banks.) A block that is NaN
+// becomes zeros.
 struct MxBlock {
     u32x4 x;
     float scale;
     uint32_t turn;
 };
 WL_DEV MxBlock mx_block(u32x4 x, uint32_t scale, uint32_t turn) {
-    const bool t1 = turn & 1u, t2 = turn & 2u, nan = scale == 255u;
+    const bool t1 = turn & 1u, t2 = turn & 2u, nan = scale > kMxHi;
     const u32x4 y = t1 ? u32x4{x[1], x[2], x[3], x[0]} : x, z = t2 ? u32x4{y[2], y[3], y[0], y[1]} : y;
     return MxBlock{nan ? u32x4{0u, 0u, 0u, 0u} : z, __uint_as_float(nan ? 0u : scale << 23), turn};
 }

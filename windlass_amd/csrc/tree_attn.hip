@@ -573,7 +573,7 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
                         const uint32_t e = 64u * (i < NLAT ? i : i - NLAT) + lane, row = DR * wave + e / (i < NLAT ? EL : ER);
                         bool nf = false;
                         if (MX && i < NLAT) {
-                            nf = mx[i] == 255u;
+                            nf = mx[i] > kMxHi;
                         } else if (WIDE) {
 #pragma unroll
                             for (int j = 0; j < 4; j++) nf |= nonfinite(__uint_as_float(raw[i][j]));
@@ -597,7 +597,7 @@ __global__ __launch_bounds__(256, 2) void tree_f32_kernel(Tree p, uint32_t min_p
                             const MxBlock b = mx_block(raw[i], mx[i], k >> 2);
 #pragma unroll
                             for (uint32_t j = 0; j < 4; j++) mx_put(b, j, tile + row * PITCH + 64u * k);
-                            if (mx[i] == 255u) *(u32x4*)(tile + row * PITCH + 64u * k) = u32x4{~0u, ~0u, ~0u, ~0u};  // NaN, and so its scores
+                            if (mx[i] > kMxHi) *(u32x4*)(tile + row * PITCH + 64u * k) = u32x4{~0u, ~0u, ~0u, ~0u};  // NaN, and so its scores
                         }
                         continue;
                     }

@@ -260,8 +260,8 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                 f32x4 y[QP];
 #pragma unroll
                 for (uint32_t j = 0; j < QP; j++) y[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (VALUES && __ballot(x.v_scale == 255u)) {  // a block that is NaN: zeros (its key's scores are NaN)
-                    const bool nan = x.v_scale == 255u;
+                if (VALUES && __ballot(x.v_scale > kMxHi)) {  // a block that is NaN: zeros (its key's scores are NaN)
+                    const bool nan = x.v_scale > kMxHi;
                     x.v = nan ? u32x4{0u, 0u, 0u, 0u} : x.v;
                     x.v_scale = nan ? 0u : x.v_scale;
                 }
@@ -294,6 +294,14 @@ __global__ __launch_bounds__(512) void tree_mx4_kernel(Tree p, uint32_t min_per)
                     y[s] = mma(as_bf16x8(x.k[(LC + s) % 2]), qr[s], y[s]);
                 }
                 s0 = y[0] + (QP > 2 ? y[1] + y[QP - 1] : y[1]);
+                // (255 is a NaN in the products too, 253 and 254 are not)
+                const uint64_t beyond = __ballot((((x.scale & 0x7F7F7F7Fu) + 0x01010101u * (0x7Fu - kMxHi % 128u)) & x.scale & 0x80808080u) != 0u);
+                if (__builtin_expect(beyond != 0u, 0)) {
+                    const uint64_t keys = beyond | beyond >> 32;  // bit n: of key sk + n
+                    const uint32_t nan = (uint32_t)(keys | keys >> 16) >> (4u * ((afresh(tid) & 63u) >> 4));
+#pragma unroll
+                    for (int k = 0; k < 4; k++) s0[k] = (nan >> k) & 1u ? __builtin_nanf("") : s0[k];
+                }
             };
             // the scores in powers of two are s0 times the factor returned; those of keys
             // that the row does not see become -inf
