@@ -27,7 +27,7 @@ namespace {
 //
 // Bound by the read of the logits where rows are many, by two launches where they are few.
 // 284 rows of 154880: f32 30 us (5.8 TB/s) with no n_top, 42 with 20; bf16 22 us (4.0 TB/s,
-// two exponentials' time a value) and 31. One row of them 9 us and 15. 2048 rows of 32000
+// two exponentials' time a value) and 31. One row of them 9 us and 13. 2048 rows of 32000
 // bf16: 32 us and 47. (Lists kept in the first launch, by insertion into each lane's
 // registers: 57 us at 284 rows bf16 and n_top 20, 31 at one row.)
 constexpr uint32_t kPer = 32;             // values a lane has at a time
@@ -72,7 +72,7 @@ WL_DEV Sums wave_join(Sums x) {
 // A wave's list of the values that may be among the n largest, of (ordered value, id).
 constexpr uint32_t kList = 640;
 constexpr uint32_t kLanes = 256;  // whose values are read again
-constexpr uint32_t kShare = 10, kAhead = 4;  // loads in flight
+constexpr uint32_t kShare = 20, kAhead = 4;  // loads in flight
 
 struct List {
     u32x2* const at;         // [kList] in LDS
@@ -258,10 +258,16 @@ __global__ __launch_bounds__(256) void logp_part_kernel(Logp p) {
     if (TOP) gst(p.most + 64u * slot + lane, st.largest);
 }
 
-WL_DEV Sums row_sums(const Logp& p, uint32_t row, uint32_t lane) {
+// Part i's m, s and u (behind the last part: the last one's, taken away by row_sums).
+WL_DEV f32x4 part_sums(const Logp& p, uint32_t row, uint32_t i) {
+    return gld((const f32x4*)(p.sums + 4u * ((uint64_t)row * p.parts + (i < p.parts ? i : p.parts - 1u))));
+}
+// All parts', of which the lane has part `lane` already.
+WL_DEV Sums row_sums(const Logp& p, uint32_t row, uint32_t lane, f32x4 v) {
     Sums x{kLowest, 0.f, 0.f};
-    for (uint32_t i = lane; i < p.parts; i += 64u) {
-        const f32x4 v = gld((const f32x4*)(p.sums + 4u * ((uint64_t)row * p.parts + i)));
+    if (lane < p.parts) x = Sums{v[0], v[1], v[2]};
+    for (uint32_t i = lane + 64u; i < p.parts; i += 64u) {
+        v = part_sums(p, row, i);
         x = join(x, Sums{v[0], v[1], v[2]});
     }
     return wave_join(x);
@@ -285,7 +291,7 @@ __global__ __launch_bounds__(256) void logp_join_kernel(Logp p, uint32_t rows) {
         if (ok) {
             const uint64_t at = (uint64_t)(uint32_t)row * p.a.stride + (uint32_t)token;
             z = BF ? bf2f(gld((const uint16_t*)p.a.d_logits + at)) : gld((const float*)p.a.d_logits + at);
-            const Sums x = row_sums(p, (uint32_t)row, lane);
+            const Sums x = row_sums(p, (uint32_t)row, lane, part_sums(p, (uint32_t)row, lane));
             z = (z - x.m) - logf(x.s);
         } else if (lane == 0) {
             set_status(p.a.d_status, WL_PAGED_E_SLOT);
@@ -294,23 +300,26 @@ __global__ __launch_bounds__(256) void logp_join_kernel(Logp p, uint32_t rows) {
         return;
     }
     const uint32_t row = blockIdx.x;
-    const Sums x = row_sums(p, row, lane);
+    const f32x4 first = part_sums(p, row, lane);
+    const uint32_t all = 64u * p.parts;  // lanes
+    const float* most = p.most + 64ull * row * p.parts;
+    float share[kShare];  // of their largest values
+    if (n) {
+#pragma unroll
+        for (uint32_t k = 0; k < kShare; k++)
+            if (256u * k < all) share[k] = gld(most + (tid + 256u * k < all ? tid + 256u * k : lane));
+    }
+    const Sums x = row_sums(p, row, lane, first);
     const float log_s = logf(x.s);
     if (tid == 0 && p.a.d_entropy) gst(p.a.d_entropy + row, log_s - x.u / x.s);
     if (n == 0) return;
     // a bound from the largest values of the lanes, a share of them to a thread
     List list(lists[wv], lane, n);
-    const uint32_t all = 64u * p.parts;  // lanes
-    const float* most = p.most + 64ull * row * p.parts;
     auto shares = [&](auto&& f) {
-        for (uint32_t i0 = tid; i0 < all; i0 += 256u * kShare) {
-            float v[kShare];
 #pragma unroll
-            for (uint32_t k = 0; k < kShare; k++) v[k] = gld(most + (i0 + 256u * k < all ? i0 + 256u * k : i0));
-#pragma unroll
-            for (uint32_t k = 0; k < kShare; k++)
-                if (i0 + 256u * k < all) f(ordered(v[k]), i0 + 256u * k);
-        }
+        for (uint32_t k = 0; k < kShare; k++)
+            if (tid + 256u * k < all) f(ordered(share[k]), tid + 256u * k);
+        for (uint32_t i = tid + 256u * kShare; i < all; i += 256u) f(ordered(gld(most + i)), i);
     };
     uint32_t high = 0;
     shares([&](uint32_t o, uint32_t) { high = max(high, o); });
