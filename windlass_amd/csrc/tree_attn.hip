@@ -1,5 +1,6 @@
 // tree_attn.hip — attention of trees of drafted tokens over a paged cache of
-// latent rows (wl_paged_tree_attention).
+// latent rows (wl_paged_tree_attention, wl_paged_window_attention); 16-bit queries
+// over 4-bit rows are tree_mx4.hip's.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -43,7 +44,7 @@ namespace {
 // in all, x 64 heads over up to 8192 keys, 205 + 16 us, 2326 clocks a tile of 64 rows: 1090 of
 // the matrix cores and 1120 of LDS (265 KB at 236 bytes a clock), mostly in turn.
 // 32 requests of one token x 64 heads over up to 65536 keys,
-// 791 MB: 162 + 12 us, in the loop 6.1 TB/s, 3346 clocks a tile, the rows' way from
+// 791 MB: 157 + 12 us, in the loop 6.1 TB/s, 3346 clocks a tile, the rows' way from
 // HBM. One token over 4096 keys: 20 + 6.7 us, of which a walk's start (its request,
 // pages, queries, first tile) takes 7, its end 4 and the place search 2.5. What did
 // not carry: 64 keys a tile in a ring of two (282 us for the 64 requests), a running
@@ -448,7 +449,9 @@ __global__ __launch_bounds__(512) void tree_bf16_kernel(Tree p, uint32_t min_per
 // of a large library product (1211 TFLOP/s), 207 to 217 us with the joining here
 // (cards differ), 11 of them for the queries' reads at the start and 12 for the join.
 // Reading the next rows a piece at a time between the scores' products made no
-// difference.
+// difference. Rows of 4 bits are read as they lie in the cache and brought to bf16, which
+// holds them, on their way into LDS: 5 requests of up to 7 nodes (16 in all) over up to 2000
+// keys 34 us, of which the join takes 9 and a walk's start and end most.
 WL_DEV void cut3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {  // two values' parts, x in the low halves
     auto low = [](uint32_t v) { return __uint_as_float(v << 16); };
     auto high = [](uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); };

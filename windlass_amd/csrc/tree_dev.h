@@ -62,13 +62,17 @@ struct Tree {
 // without, 207 with; 5 of 7 nodes 67 and 59; 12 of 5 nodes 28 and 23; 32 contexts 191 and 179. Requests of
 // one row tile, 16-bit queries: 32 contexts of up to 65536 keys 180 and 170, of 4-bit rows 129 and 121, these
 // through a window of 4096 57 and 46; 8 of up to 3016 keys 25 and 19. (They need no chunks: their keys stand
-// in a row.)
+// in a row; of one such request alone that makes equal pieces by itself.)
 constexpr uint32_t kSlack = 6;
 //
 // Through a window (WIN) a request's keys are those that some node may see: tiles
 // [0, st) with the sinks and those from the first key on that its first node sees;
 // `skip` tiles between them are no units. A walk counts the others (nkt); the first
-// key of its tile t is key_of(t).
+// key of its tile t is key_of(t). Nodes of a request see windows a few keys apart, so
+// only the tiles at the sinks' end, at the window's beginning and with nodes are masked.
+// 32 single tokens through a window of 4096 with 4 sinks, 4-bit rows: 46 us (all keys 121);
+// 64 requests of up to 8 nodes through 2048 with 64 sinks, 16-bit rows: 150 us, 717 MB (as
+// the row tiles of a request, two a work-group, come by its rows one after the other).
 struct Req {
     uint32_t t0, nodes, len, keys, nrt, nkt, flaw;  // flaw: WL_PAGED_E_* (its rows get NaN)
     uint32_t st, skip;
@@ -210,7 +214,7 @@ WL_DEV Place find_place(const Tree& p, uint32_t c, uint32_t min_per, uint64_t* t
     f.pieces = 0;
     uint64_t at = inc - mine;
     for (uint32_t w = 0; w < wv; w++) at += tmp[w];
-    if (share == 1 && all < GRID && (f.total >> 32) == 0) {
+    if (share == 1 && (R > 1 || rq[0][0] > 1) && all < GRID && (f.total >> 32) == 0) {
         // the least of some lengths with which the pieces are no more than the work-groups
         const uint32_t per = (uint32_t)f.per, step = (kSlack + per / 16u + kTries - 2u) / (kTries - 1u);
         for (uint32_t k = wv; k < kTries; k += NW) {

@@ -13,6 +13,38 @@ typedef __attribute__((ext_vector_type(6))) uint32_t u32x6;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(32))) float f32x32;
 
+// ---- 16-bit queries, 4-bit rows --------------------------------------------------
+// As over 16-bit rows (tree_attn.hip: a reference instead of a running maximum, weights
+// in bf16 divided by the sum of what they are then, a walk done again where weights pass
+// kMost), with 64 rows (node, head) against 32 keys at a time by eight waves:
+//   S^T[keys][rows] = K Q^T: wave w takes rows 16 (w / 2) and keys 16 (w % 2). The values
+//           meet the scaled products as they lie in the cache, 128 columns at a time with
+//           their blocks' scales; the queries, in bf16, are cut into three pieces of 6 bits
+//           each (E2M3) with scales of their own per 32 columns: a piece has 4 leading bits
+//           and takes 4 to 5 bits of what is left, so 14 below the block's largest value, all
+//           8 bits of a query that is at least a 120th of it. Their products and sums are
+//           f32. The rotary part is a product in bf16.
+//   O^T[cols][rows] += V^T P^T: the tile's values are brought to bf16 (which holds them
+//           exactly) once for all waves, in LDS, and read transposed: wave w has columns
+//           [16 LC w, + 16 LC) of all rows. (Scaled products here would need the weights in
+//           pieces too, and the values transposed in halves of bytes.)
+// A row is 400 bytes instead of 1152, so what bounds this is not memory but the CU: a
+// tile is some 2200 clocks, of which products take 760 to 1000 and LDS some 1050 (a tile
+// comes in, is read as keys, by its wave's lanes once more for conversion, written in
+// bf16, read transposed), the rest is waits at the turn's one barrier; a work-group a
+// CU has two waves a SIMD to fill them. Hence: a ring of four tiles, three on the way;
+// operands read ahead of their products, values converted between the scores' products,
+// LDS rows and chunks placed so that no access meets a bank twice, a walk's addresses
+// found 64 tiles at a time.
+// Measured (512 + 64 columns, both launches): 32 requests of one token x 64 heads over
+// up to 65536 keys (22775 on average, 296 MB) 121 to 125 us, 820 TFLOP/s or 57 % of a
+// large bf16 product's rate (over 16-bit rows 170); 64 of up to 8 nodes (279
+// in all) over up to 8192 164 us, 610 TFLOP/s (205); one token over 4096 keys 26, all of it
+// latencies (28).
+// Two pieces of the queries instead of three would be 6 % faster and lose 5 of the 14
+// bits. Without effect: the two waves of a SIMD in opposite order, wave priorities, values
+// read before the barrier.
+
 // Pieces of 32 queries that meet one scale of a key: q = sum of p_i 2^s_i, p_i of E2M3;
 // s_1 puts the largest into (3.75, 7.5], the others fall by 4 and 9 powers of two.
 constexpr uint32_t kQueryPieces = 3;  // (they are moved as three)
