@@ -41,7 +41,7 @@ namespace {
 // their weights in 32 bits 1.7e-3, which is the outputs' own rounding.)
 //
 // Measured (512 + 64 columns, first launch + join): 64 requests of up to 8 nodes, 284
-// in all, x 64 heads over up to 8192 keys, 205 + 16 us, 2326 clocks a tile of 64 rows: 1090 of
+// in all, x 64 heads over up to 8192 keys, 182 + 16 us, 2326 clocks a tile of 64 rows: 1090 of
 // the matrix cores and 1120 of LDS (265 KB at 236 bytes a clock), mostly in turn.
 // 32 requests of one token x 64 heads over up to 65536 keys,
 // 791 MB: 157 + 12 us, in the loop 6.1 TB/s, 3346 clocks a tile, the rows' way from

@@ -49,9 +49,13 @@ struct Tree {
 // are fewer); its units come chunk by chunk, in a chunk row tile by row tile:
 // the row tiles that run at the same time are at the same keys, which the L2 of
 // their XCD then holds once for all of them. (Work-group b runs on XCD b % 8:
-// c = (b % 8)(G / 8) + b / 8.) A row tile that one work-group has whole is
-// finished there; the others leave their parts in the scratch for the second
-// launch, at most two per work-group: its first walk's and its last one's.
+// c = (b % 8)(G / 8) + b / 8.) A row tile's units count from its keys' end: the next
+// work-group, which has the rest of a row tile that this one ends with, then begins at
+// the chunk's first key as this one did, and not some tiles ahead (64 requests of 8 nodes,
+// 16-bit rows: 207 us and 198; through a window 149 and 142, 717 MB fetched and 298).
+// A row tile that one work-group has whole is finished there; the others leave their
+// parts in the scratch for the second launch, at most two per work-group: its first
+// walk's and its last one's.
 // Where there are fewer row tiles than work-groups that is mostly two walks each, and
 // a walk's start, its end and its part cost as much as some kSlack tiles. So where
 // pieces of row tiles (all of a request's equally long, as many as need be) at most
@@ -71,8 +75,7 @@ constexpr uint32_t kSlack = 6;
 // key of its tile t is key_of(t). Nodes of a request see windows a few keys apart, so
 // only the tiles at the sinks' end, at the window's beginning and with nodes are masked.
 // 32 single tokens through a window of 4096 with 4 sinks, 4-bit rows: 46 us (all keys 121);
-// 64 requests of up to 8 nodes through 2048 with 64 sinks, 16-bit rows: 150 us, 717 MB (as
-// the row tiles of a request, two a work-group, come by its rows one after the other).
+// 64 requests of up to 8 nodes through 2048 with 64 sinks, 16-bit rows: 142 us.
 struct Req {
     uint32_t t0, nodes, len, keys, nrt, nkt, flaw;  // flaw: WL_PAGED_E_* (its rows get NaN)
     uint32_t st, skip;
@@ -327,10 +330,11 @@ struct Walks {
         const uint32_t ka = uni(chunk_at(w.q, nc, j)), kb = uni(chunk_at(w.q, nc, j + 1));
         const uint64_t oj = o - (uint64_t)w.q.nrt * ka;
         w.rt = uni((uint32_t)div64(oj, kb - ka));
-        w.kt0 = uni(ka + (uint32_t)(oj - (uint64_t)w.rt * (kb - ka)));
-        w.kt1 = uni(u1 - u < kb - w.kt0 ? w.kt0 + (uint32_t)(u1 - u) : kb);
+        const uint32_t k0 = (uint32_t)(oj - (uint64_t)w.rt * (kb - ka)), left = kb - ka - k0, n = uni(u1 - u < left ? (uint32_t)(u1 - u) : left);
+        w.kt1 = uni(kb - k0);  // (from the chunk's end)
+        w.kt0 = w.kt1 - n;
         w.slot = 2u * c + (u == f.u0 ? 0u : 1u);
-        u += w.kt1 - w.kt0;
+        u += n;
     }
     __device__ __forceinline__ uint32_t rows(const Walk& w) const {
         const uint32_t n = w.q.nodes * p.a.n_heads - w.rt * ROWS;
