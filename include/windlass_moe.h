@@ -899,7 +899,9 @@ wl_status wl_paged_window_attention(const wl_window_attn* w, void* stream);
  * Computed in f32 from the logits as they are. A logit of -infinity has p = 0 and
  * log p = -infinity. In a row without a finite logit, or with a NaN or +infinity, log p
  * and the entropy are NaN; ids are by order all the same, a NaN before any number. A
- * token outside [0, n_vocab) or a row outside [0, n_rows): NaN, and E_SLOT.
+ * token of -1 is passed over, d_logp[t] as it was (a step captured with room for more
+ * tokens than it has). Another one outside [0, n_vocab), or a row outside [0, n_rows):
+ * NaN, and E_SLOT.
  * n_vocab up to 2^20, n_rows and n_tokens up to 2^20. Alignment: d_logits 16 bytes
  * and stride a multiple of 8 are fastest, the elements' size is enough. d_scratch:
  * wl_token_logprobs_scratch(a) bytes (0 if `a` is invalid), 16-byte aligned; it

@@ -118,13 +118,24 @@ def test_magnitudes(gpu, shift, spread, t):
 
 def test_tokens_and_rows_outside(gpu):
     rng = np.random.default_rng(10)
-    x = Logprobs(logits(rng, 4, 300), "bf16", [5, -1, 300, 7, 299, 2 ** 31 - 1], [0, 1, 2, -1, 3, 4], n_top=2)
+    x = Logprobs(logits(rng, 4, 300), "bf16", [5, -2, 300, 7, 299, 2 ** 31 - 1], [0, 1, 2, -1, 3, 4], n_top=2)
     x.run()
     assert x.status() == paged.E_SLOT
     got = x.get("logp", 6)
     assert np.isnan(got[[1, 2, 3, 5]]).all() and np.isfinite(got[[0, 4]]).all()
     x.token, x.row = [5, 0, 0, 0, 299, 0], [0, 0, 0, 0, 3, 0]
     x.check(bad_tokens=(1, 2, 3, 5))
+
+
+def test_places_without_a_token(gpu):
+    """Token -1, whatever its row: nothing is written and nothing is wrong."""
+    rng = np.random.default_rng(11)
+    x = Logprobs(logits(rng, 3, 500), "f32", [5, -1, 7, -1, -1], [0, 1, 2, -1, 99], n_top=4).run()
+    assert x.status() == 0
+    got = x.get("logp", 5)
+    assert (got[[1, 3, 4]] == x.fill).all()
+    Logprobs(x.z, "f32", [5, 7], [0, 2], n_top=4).run().check()
+    assert np.array_equal(got[[0, 2]], Logprobs(x.z, "f32", [5, 7], [0, 2]).run().get("logp", 2))
 
 
 def test_offsets_past_32_bits(gpu):

@@ -286,6 +286,7 @@ __global__ __launch_bounds__(256) void logp_join_kernel(Logp p, uint32_t rows) {
         const uint32_t t = (blockIdx.x - rows) * 4u + wv;
         if (t >= p.a.n_tokens) return;
         const int32_t token = p.a.d_token[t], row = p.a.d_row ? p.a.d_row[t] : (int32_t)t;
+        if (token == -1) return;
         const bool ok = token >= 0 && (uint32_t)token < p.a.n_vocab && row >= 0 && (uint32_t)row < p.a.n_rows;
         float z = __builtin_nanf("");
         if (ok) {
