@@ -146,3 +146,22 @@ def test_refused_requests(gpu, q, cache):
     t = tree()
     t.upload(cu=[0, 2, 5, 6, 12]).run().check(skip=(3,))
     assert t.status() == paged.E_LEN
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("R", [300, 1500, 4096])
+def test_many_requests(gpu, R, q, cache):
+    """More requests than a work-group has threads; some without tokens, some shorter than the window."""
+    rng = np.random.default_rng(R)
+    lens, adds = [int(x) for x in rng.integers(0, 300, R)], [int(x) for x in rng.integers(0, 3, R)]
+    S.Serving(24, q, cache, 64, 8, 2, 8, lens, adds, random_trees(rng, adds), window=70, sinks=3).upload().run().check()
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("window", [0, 700])
+@pytest.mark.parametrize("H,lens,adds", [(64, [2100, 40, 900, 1500, 2100, 3], [64, 60, 64, 64, 64, 64]), (64, list(range(40, 1240, 20)), [5, 9, 1, 8] * 15),
+                                         (16, list(range(0, 3000, 100)) + [50] * 40, [1] * 30 + [0] * 40)], ids=["chunks", "rows", "singles"])
+def test_splits(gpu, H, lens, adds, window, q, cache):
+    """More row tiles than work-groups, in chunks and whole; single row tiles in pieces, among requests without tokens."""
+    rng = np.random.default_rng(31)
+    S.Serving(32, q, cache, 32, 8, H, 16, lens, adds, random_trees(rng, adds), window=window, sinks=5).upload().run().check()
