@@ -173,12 +173,15 @@ struct Stream {
     __device__ __forceinline__ void add(const float* v, uint32_t count, float most) {
         const float m = larger(x.m, most);
         x = to_reference(x, m);
+        float s[4] = {}, u[4] = {};  // (added up by themselves first, 32 values lose less)
 #pragma unroll
         for (uint32_t k = 0; k < count; k++) {
             const float d = v[k] - m, e = __builtin_amdgcn_exp2f(d * kLog2e);
-            x.s += e;
-            if (ENT) x.u = fmaf(e, fmaxf(d, -1e30f), x.u);
+            s[k % 4u] += e;
+            if (ENT) u[k % 4u] = fmaf(e, fmaxf(d, -1e30f), u[k % 4u]);
         }
+        x.s += (s[0] + s[1]) + (s[2] + s[3]);
+        if (ENT) x.u += (u[0] + u[1]) + (u[2] + u[3]);
     }
     // U vectors of a lane, 64 apart, of which those before `count` count (CUT)
     template <bool CUT>
