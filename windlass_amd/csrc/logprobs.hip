@@ -28,7 +28,7 @@ namespace {
 // Bound by the read of the logits where rows are many, by two launches where they are few.
 // 284 rows of 154880: f32 30 us (5.8 TB/s) with no n_top, 42 with 20; bf16 22 us (4.0 TB/s,
 // two exponentials' time a value) and 31. One row of them 9 us and 13. 2048 rows of 32000
-// bf16: 32 us and 47. (Lists kept in the first launch, by insertion into each lane's
+// bf16: 32 us and 47 to 49. (Lists kept in the first launch, by insertion into each lane's
 // registers: 57 us at 284 rows bf16 and n_top 20, 31 at one row.)
 constexpr uint32_t kPer = 32;             // values a lane has at a time
 constexpr uint32_t kPart = 64 * kPer;     // of a wave
@@ -173,15 +173,15 @@ struct Stream {
     __device__ __forceinline__ void add(const float* v, uint32_t count, float most) {
         const float m = larger(x.m, most);
         x = to_reference(x, m);
-        float s[4] = {}, u[4] = {};  // (added up by themselves first, 32 values lose less)
+        float s = 0.f, u = 0.f;  // (added up by themselves first, 32 values lose less)
 #pragma unroll
         for (uint32_t k = 0; k < count; k++) {
             const float d = v[k] - m, e = __builtin_amdgcn_exp2f(d * kLog2e);
-            s[k % 4u] += e;
-            if (ENT) u[k % 4u] = fmaf(e, fmaxf(d, -1e30f), u[k % 4u]);
+            s = k ? s + e : e;
+            if (ENT) u = k ? fmaf(e, fmaxf(d, -1e30f), u) : e * fmaxf(d, -1e30f);
         }
-        x.s += (s[0] + s[1]) + (s[2] + s[3]);
-        if (ENT) x.u += (u[0] + u[1]) + (u[2] + u[3]);
+        x.s += s;
+        if (ENT) x.u += u;
     }
     // U vectors of a lane, 64 apart, of which those before `count` count (CUT)
     template <bool CUT>
