@@ -905,7 +905,8 @@ wl_status wl_paged_window_attention(const wl_window_attn* w, void* stream);
  * n_vocab up to 2^20, n_rows and n_tokens up to 2^20. Alignment: d_logits 16 bytes
  * and stride a multiple of 8 are fastest, the elements' size is enough. d_scratch:
  * wl_token_logprobs_scratch(a) bytes (0 if `a` is invalid), 16-byte aligned; it
- * holds nothing between calls. Errors as the paged calls' (wl_paged_last_error). */
+ * holds nothing between calls, and what is enough for a call is enough for one of fewer
+ * or as many rows, values and alternatives. Errors as the paged calls' (wl_paged_last_error). */
 #define WL_LOGPROB_MAX_TOP 32
 typedef struct wl_logprobs {
     uint32_t dtype, n_rows, n_vocab, n_tokens, n_top;

@@ -134,3 +134,26 @@ def test_argument_blocks_are_laid_out_as_the_header_has_them(tmp_path):
         assert int(got[name]) == ctypes.sizeof(cls)
         for f in cls._fields_:
             assert int(got[f"{name}.{f[0]}"]) == getattr(cls, f[0]).offset
+
+
+@pytest.mark.parametrize("n_vocab", [1, 1000, 2049, 32000, 154880, 1 << 20])
+def test_logprobs_scratch_of_a_batch_is_enough_for_smaller_ones(n_vocab):
+    """A program takes it once, for its largest call."""
+    def need(rows, vocab, top):
+        return paged.token_logprobs_scratch(some_logits(n_rows=rows, n_vocab=vocab, stride=1 << 20, n_top=top))
+    most = {}
+    for top in {0, 1, min(32, n_vocab)}:
+        for rows in [*range(1, 300), 511, 512, 513, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8192, 8193, 20000, 1 << 20]:
+            n = need(rows, n_vocab, top)
+            for fewer in ((rows - 1, n_vocab, top), (rows, n_vocab - 1, min(top, n_vocab - 1)), (rows, n_vocab, 0)):
+                if min(fewer[:2]) > 0:
+                    assert need(*fewer) <= n, fewer
+            most[top] = max(most.get(top, 0), n)
+            assert n == most[top]  # in the order of the rows
+
+
+def test_logprobs_with_the_scratch_of_a_larger_batch():
+    """284 rows of a step, 256 of the next: not refused for its scratch (but for what is checked after it)."""
+    n = paged.token_logprobs_scratch(some_logits(n_rows=284, n_vocab=154880, stride=154880, n_top=20))
+    with pytest.raises(moe.WindlassError, match="overlap"):
+        paged.token_logprobs(some_logits(n_rows=256, n_vocab=154880, stride=154880, n_top=20, scratch_bytes=n, d_logp=at(3)))

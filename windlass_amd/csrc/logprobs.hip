@@ -405,17 +405,24 @@ __global__ __launch_bounds__(256) void logp_join_kernel(Logp p, uint32_t rows) {
 // again, which outweighs the longer join (in us at 2048, 4096 and 8192 waves, bf16 and n_top
 // 20: 284 x 154880 33.0, 31.2, 30.7, 2048 x 32000 62.9, 53.6, 46.7; without n_top 22.2, 22.8,
 // 22.9 and 32.7, 32.8, 32.4; 1024 waves 33.3 at the former).
+struct Split {
+    uint32_t waves, most;  // of the launch where rows are few; parts of a row at the most
+};
+Split split_of(const wl_logprobs& a) { return Split{a.n_top ? 8192u : 2048u, (a.n_vocab + kPart - 1u) / kPart}; }
 uint32_t parts_of(const wl_logprobs& a) {
-    const uint32_t waves = a.n_top ? 8192u : 2048u, most = (a.n_vocab + kPart - 1u) / kPart;
-    const uint32_t want = a.n_rows >= waves ? 1u : waves / (a.n_rows ? a.n_rows : 1u);
-    return want < most ? want : most;
+    const Split s = split_of(a);
+    const uint32_t want = a.n_rows >= s.waves ? 1u : s.waves / (a.n_rows ? a.n_rows : 1u);
+    return want < s.most ? want : s.most;
 }
 
 }  // namespace
 
+// Bytes for n_rows x parts_of(a) parts, rounded up to what no call of fewer rows, values or
+// alternatives exceeds: fewer rows may come in more parts in all (284 rows 28 each, 256 rows 32).
 size_t logprobs_scratch(const wl_logprobs& a) {
-    const size_t slots = (size_t)(a.n_rows ? a.n_rows : 1) * parts_of(a);
-    return slots * (16 + (a.n_top ? 256 : 0));
+    const Split s = split_of(a);
+    const size_t rows = a.n_rows ? a.n_rows : 1, all = rows * s.most, few = all < s.waves ? all : s.waves;
+    return (rows > few ? rows : few) * (16 + (a.n_top ? 256 : 0));
 }
 
 int launch_logprobs(const wl_logprobs& a, void* stream) {
