@@ -165,3 +165,15 @@ def test_splits(gpu, H, lens, adds, window, q, cache):
     """More row tiles than work-groups, in chunks and whole; single row tiles in pieces, among requests without tokens."""
     rng = np.random.default_rng(31)
     S.Serving(32, q, cache, 32, 8, H, 16, lens, adds, random_trees(rng, adds), window=window, sinks=5).upload().run().check()
+
+
+@pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("window,sinks", [(128, 0), (90, 0), (200, 40)])
+def test_chains_whose_last_node_begins_with_a_tile(gpu, window, sinks, q, cache):
+    """It sees nothing of the tile before it, with which the request's walk begins; lengths around those, too."""
+    lens, adds = [], []
+    for a in (2, 8, 33):
+        for off in (-16, -1, 0, 1, 16):
+            lens.append(32 * 11 + window - a + off)
+            adds.append(a)
+    S.Serving(33, q, cache, 128, 32, 6, 16, lens, adds, window=window, sinks=sinks).upload().run().check()

@@ -8,6 +8,7 @@
 
 #include "paged.h"
 #include "paged_dev.h"
+#include "window.h"
 
 namespace wl {
 namespace paged {
@@ -84,12 +85,11 @@ template <bool WIN>
 WL_DEV uint32_t key_of(const Req& q, uint32_t t) {
     return (WIN && t >= q.st ? t + q.skip : t) * kKT;
 }
-// Whether some node of the request may not see some of the keys [k0, k0 + n): nodes
-// are among them (or keys behind the last one), or keys that a window passes over.
+// Whether keys [k0, k0 + n) have to be masked: nodes are among them (or keys behind the
+// last one), or keys that a window passes over for some node.
 template <bool WIN>
 WL_DEV bool is_masked(const Tree& p, const Req& q, uint32_t k0, uint32_t n) {
-    if (k0 + n > q.len) return true;
-    return WIN && k0 + n > p.sinks && k0 + p.window < q.len + q.nodes;  // below the last node's first key
+    return k0 + n > q.len || (WIN && window_masks(q.len, q.nodes, p.window, p.sinks, k0, n));
 }
 // What node nd of a request sees: of the nodes those in the result (a bit each), of
 // the keys before them those from `low` on and the sinks. Its position is the number
@@ -100,8 +100,8 @@ WL_DEV uint64_t sees(const Tree& p, const Req& q, uint32_t nd, uint32_t& low) {
     low = 0;
     if (WIN) {
         const uint64_t below = bits & ((1ull << nd) - 1ull);
-        const uint32_t depth = (uint32_t)__popcll(below), pos = q.len + depth;  // below 2^31
-        low = pos >= p.window ? pos - p.window + 1u : 0u;
+        const uint32_t depth = (uint32_t)__popcll(below);
+        low = window_from(q.len + depth, p.window);
         const uint32_t drop = depth >= p.window ? depth - p.window + 1u : 0u, sunk = p.sinks > q.len ? p.sinks - q.len : 0u;
         uint64_t left = below;
         for (uint32_t i = 0; i < drop; i++) {  // at most 63
@@ -131,13 +131,11 @@ WL_DEV Req request(const Tree& p, uint32_t r, uint32_t& status) {
     q.nrt = (q.nodes * p.a.n_heads + ROWS - 1) / ROWS;
     q.nkt = q.flaw ? 1u : (q.keys + kKT - 1) / kKT;
     q.st = ~0u;
-    if (WIN && !q.flaw && q.len >= p.window) {
-        const uint32_t from = (q.len - p.window + 1u) / kKT, sunk = p.sinks / kKT + (p.sinks % kKT ? 1u : 0u);
-        if (from > sunk) {
-            q.st = sunk;
-            q.skip = from - sunk;
-            q.nkt -= q.skip;
-        }
+    if (WIN && !q.flaw) {
+        const Skip skip = window_skip(q.len, p.window, p.sinks, kKT);
+        q.st = skip.at;
+        q.skip = skip.n;
+        q.nkt -= skip.n;
     }
     return q;
 }
