@@ -162,3 +162,30 @@ def test_rows_of_few_values(gpu, V, t):
                   np.where(np.arange(V) < V // 2, 1.0, 0.0)])
     for n_top in (1, 32):
         Logprobs(z, t, rng.integers(0, V, 4), n_top=n_top).run().check()
+
+
+def fastest(x, times=12):
+    """The shortest of some calls, in ms."""
+    stream, a, b, t = hip.Stream(), hip.Event(), hip.Event(), []
+    for _ in range(times):
+        a.record(stream)
+        paged.token_logprobs(x.args, stream.handle)
+        b.record(stream)
+        b.synchronize()
+        t.append(a.elapsed_ms(b))
+    stream.destroy()
+    return min(t)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_a_list_of_equal_values_is_cut_once(gpu, t):
+    """Where a grammar leaves fewer values than are asked for, the others are equal: -infinity. The row is then read again
+    by one work-group (some 5 times the usual row's time); with a list that runs full at every step it is some 100."""
+    rng = np.random.default_rng(12)
+    V = 262144
+    z = logits(rng, 1, V)
+    usual = Logprobs(z, t, [5], n_top=20).run()
+    for few in (np.where(np.arange(V) % 30001 == 7, z, -np.inf), np.full((1, V), 0.5), np.where(np.arange(V) > V - 9, z, -1e30)):
+        x = Logprobs(few, t, [7], n_top=20).run()
+        x.check()
+        assert fastest(x) < 25 * fastest(usual)
