@@ -479,3 +479,90 @@ def test_rows_of_any_bytes(gpu, q, scale, window):
         else:
             y, far = t.want(i // 8, i % 8)
             assert np.all(np.abs(out[i] - y) <= far)
+
+
+# ---- rows of requests of very uneven lengths -------------------------------------------
+@pytest.mark.parametrize("cache,dtype", [("mxfp4", "bf16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("R", [60, 700, 4096])
+def test_read_of_uneven_requests(gpu, R, cache, dtype):
+    """A few long requests among many short and empty ones, most of their rows read by work-groups of other requests'."""
+    rng = np.random.default_rng(R)
+    lens = [int(x) for x in rng.integers(0, 4 if R < 1000 else 2, R)]
+    for r, n in ((0, 2500), (R // 2, 6100), (R - 1, 3001)):
+        lens[r] = n
+    t = S.Serving(R, "f32", cache, 128, 16, 2, 16, lens, [0] * R).upload()
+    for some in (False, True):
+        first = [n // 7 for n in lens] if some else None
+        counts = [n - n // 7 for n in lens] if some else lens
+        got, status = read(t, dtype, first, counts, pad=8)
+        assert status == 0
+        want = np.concatenate([t.rows[r][(first[r] if some else 0):][:n] for r, n in enumerate(counts)])
+        assert np.array_equal(got[:len(want), :t.W], P.as_type(want, dtype))
+        assert np.all(got[len(want):] == 7.0) and np.all(got[:, t.W:] == 7.0)
+
+
+@pytest.mark.parametrize("cache", ["mxfp4", "f32"])
+def test_read_flaws_of_uneven_requests(gpu, cache):
+    R = 600
+    rng = np.random.default_rng(3)
+    lens = [int(x) for x in rng.integers(0, 4, R)]
+    lens[100], lens[400] = 6000, 5000
+    t = S.Serving(6, "f32", cache, 64, 16, 2, 16, lens, [0] * R).upload()
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    n_rows = int(cu[-1]) + 5
+    want = np.full((n_rows, t.W), 7.0, np.float32)
+    want[:cu[-1]] = np.concatenate(t.rows)
+    table, expect = t.table.copy(), want.copy()
+    table[100, 350], table[400, 0] = -1, t.n_pages  # late and early rows
+    expect[cu[100] + 5600:cu[100] + 5616] = expect[cu[400]:cu[400] + 16] = np.nan
+    got, status = read(t, "f32", None, lens, n_rows=n_rows, table=table)
+    assert status == paged.E_PAGE and np.array_equal(got, expect, equal_nan=True)
+    first = [0] * R
+    first[100] = t.max_pages * 16 - 5999  # one row more than its table has
+    expect = want.copy()
+    expect[cu[100]:cu[101]] = 7.0
+    got, status = read(t, "f32", first, lens, n_rows=n_rows)
+    assert status == paged.E_LEN and np.array_equal(got, expect)
+    got, status = read(t, "f32", None, lens, n_rows=int(cu[400]) + 4000)  # a long one that does not fit, and those behind it
+    assert status == paged.E_LEN and np.array_equal(got, np.concatenate([want[:cu[400]], np.full((4000, t.W), 7.0)]))
+    back = cu.copy()
+    back[401:] -= 5000  # request 400 without rows
+    back[300] = cu[300] - 6000  # it falls: request 299 is left out, 300 reads from the rows of others on
+    got, status = read(t, "f32", [0] * 300 + [max(0, lens[300] - 1)] + [0] * 299, lens, n_rows=n_rows, cu=back)
+    assert status == paged.E_LEN
+    keep = np.ones(n_rows, bool)
+    keep[back[300]:back[301]] = False  # another's too, or out of its table
+    expect = want.copy()
+    expect[cu[400]:] = 7.0
+    expect[cu[400]:back[R]] = np.concatenate(t.rows[401:])
+    expect[cu[299]:cu[300]] = 7.0
+    assert np.array_equal(got[keep], expect[keep])
+
+
+def test_read_of_one_long_request_among_many(gpu):
+    """Its rows are read by more than the work-groups that one of many has (by those alone it takes 32 times as
+    long as in a call of its own, and so 2)."""
+    n, ps = 16384, 64
+    cache, out = hip.DeviceBuffer(n * 1152), hip.DeviceBuffer(n * 1152)
+    cache.zero()
+    stream, a, b = hip.Stream(), hip.Event(), hip.Event()
+
+    def fastest(lens):
+        table = np.zeros((len(lens), n // ps), np.int32)
+        table[int(np.argmax(lens))] = np.arange(n // ps)
+        held = dict(d_table=i32(table), d_cu=i32(np.concatenate([[0], np.cumsum(lens)])))
+        c = paged.Cache(d_rows=cache.ptr, dtype=1, n_pages=n // ps, page_size=ps, kv_lora_rank=512, qk_rope=64, row_stride=576)
+        args = paged.RowRead(cache=c, dtype=1, n_req=len(lens), n_rows=n, max_pages=n // ps, d_out=out.ptr, out_stride=576,
+                             **{k: v.ptr for k, v in held.items()})
+        t = []
+        for _ in range(12):
+            a.record(stream)
+            paged.read_rows(args, stream.handle)
+            b.record(stream)
+            b.synchronize()
+            t.append(a.elapsed_ms(b))
+        return min(t)
+    alone = fastest([n])
+    for r in (0, 200, 511):
+        assert fastest([0] * r + [n] + [0] * (511 - r)) < 12 * alone
+    stream.destroy()

@@ -461,24 +461,34 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowWrite a) {
 
 // ---- rows as values -----------------------------------------------------------
 // A thread has 8 values of a row, so a row's chunks, the rotary ones among them, lie in
-// a row over the threads; a request's rows are dealt out to the work-groups of its
-// column of the grid. Bound by the launch (one row 1.7 us), then by the bytes (13725 rows of
-// 4 bits to bf16, 21 MB, 7.8 us).
-template <int CT, bool OBF>
-__global__ __launch_bounds__(256) void row_read_kernel(wl_row_read p, uint32_t psh) {
+// a row over the threads; a request's are dealt out to the work-groups of its row of the
+// grid. Where a request may be much longer than the others (REST), these take `most` chunks
+// of it, and what is behind them is dealt out to the work-groups of the grid's first
+// rows, 256 chunks at a time, beginning elsewhere for each request: these look through the
+// requests for long ones. Bound by the launch (one row 2.2 us in a row of calls), then by
+// the bytes: 13725 rows of 4 bits to bf16, 21 MB, 6.8 us; of 16 bits to bf16, 32 MB, 6.4;
+// of 32 bits to 32 bits, 63 MB, 11.9; 32768 rows of these 12.4, 13.1 and 24.2 us (6.2 TB/s).
+struct RowRead {
+    wl_row_read r;
+    uint32_t psh;    // log2 page_size
+    uint32_t most;   // chunks of a request that its own work-groups read (REST)
+    uint32_t rest;   // work-groups for the others,
+    uint32_t first;  // and rows of the grid
+};
+
+template <int CT, bool OBF, bool REST>
+__global__ __launch_bounds__(256) void row_read_kernel(RowRead a) {
     constexpr bool MX = CT == WL_TYPE_MXFP4;
-    const uint32_t r = blockIdx.y, L = p.cache.kv_lora_rank, RP = p.cache.qk_rope, cl = L / 8u, per = cl + RP / 8u;
-    const int32_t c0 = p.d_cu[r], c1 = p.d_cu[r + 1], first = p.d_first ? p.d_first[r] : 0;
-    const bool head = blockIdx.x == 0 && threadIdx.x == 0;
-    if (c0 == c1) return;
-    if (c0 < 0 || c1 < c0 || (uint32_t)c1 > p.n_rows || first < 0 ||
-        (uint64_t)(uint32_t)first + (uint32_t)(c1 - c0) > ((uint64_t)p.max_pages << psh)) {
-        if (head) set_status(p.d_status, WL_PAGED_E_LEN);
-        return;
-    }
-    const uint32_t n = (uint32_t)(c1 - c0) * per;  // n_rows <= 2^24, per <= 72
-    for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < n; i += gridDim.x * 256u) {
-        const uint32_t j = i / per, k = i - j * per, key = (uint32_t)first + j;
+    const wl_row_read& p = a.r;
+    const uint32_t psh = a.psh, tid = threadIdx.x, L = p.cache.kv_lora_rank, RP = p.cache.qk_rope, cl = L / 8u, per = cl + RP / 8u;
+    // whether request r has rows that can be, in c0, c1 and first
+    auto sound = [&](int32_t c0, int32_t c1, int32_t first) {
+        return c0 >= 0 && c1 >= c0 && (uint32_t)c1 <= p.n_rows && first >= 0 &&
+               (uint64_t)(uint32_t)first + (uint32_t)(c1 - c0) <= ((uint64_t)p.max_pages << psh);
+    };
+    // chunk i of request r, whose rows begin with row c0 and token `first`
+    auto chunk = [&](uint32_t r, uint32_t c0, uint32_t first, uint32_t i) {
+        const uint32_t j = i / per, k = i - j * per, key = first + j;
         const int32_t page = p.d_table[(size_t)r * p.max_pages + (key >> psh)];
         float v[8];
         if (page < 0 || (uint32_t)page >= p.cache.n_pages) {
@@ -504,22 +514,88 @@ __global__ __launch_bounds__(256) void row_read_kernel(wl_row_read p, uint32_t p
                 load8<CT == WL_TYPE_BF16>(p.cache.d_rows, at + 8u * k, v);
             }
         }
-        store_n<8>(p.d_out, (size_t)((uint32_t)c0 + j) * p.out_stride + 8u * k, v, OBF);
+        store_n<8>(p.d_out, (size_t)(c0 + j) * p.out_stride + 8u * k, v, OBF);
+    };
+    if (!REST || blockIdx.y >= a.first) {
+        const uint32_t r = blockIdx.y - (REST ? a.first : 0u);
+        const int32_t c0 = p.d_cu[r], c1 = p.d_cu[r + 1], first = p.d_first ? p.d_first[r] : 0;
+        if (c0 == c1) return;
+        if (!sound(c0, c1, first)) {
+            if (blockIdx.x == 0 && tid == 0) set_status(p.d_status, WL_PAGED_E_LEN);
+            return;
+        }
+        const uint32_t all = (uint32_t)(c1 - c0) * per, n = !REST || all < a.most ? all : a.most;  // n_rows <= 2^24, per <= 72
+        for (uint32_t i = blockIdx.x * 256u + tid; i < n; i += gridDim.x * 256u) chunk(r, (uint32_t)c0, (uint32_t)first, i);
+        return;
+    }
+    if constexpr (REST) {
+        constexpr uint32_t EACH = WL_PAGED_MAX_REQ / 256u;  // requests of a thread
+        __shared__ uint16_t list[WL_PAGED_MAX_REQ];         // long requests with chunks for this work-group
+        __shared__ uint32_t count;
+        const uint32_t h = blockIdx.y * gridDim.x + blockIdx.x;
+        // which 256 of the rest's chunks are the work-group's first of request r
+        auto place = [&](uint32_t r) {
+            const uint32_t from = (r * 0x9E3779B1u >> 16) % a.rest;
+            return h >= from ? h - from : h + a.rest - from;
+        };
+        auto blocks = [&](uint32_t all) { return (all - a.most + 255u) / 256u; };
+        if (h >= a.rest) return;
+        if (tid == 0) count = 0;
+        int32_t c0[EACH], c1[EACH];
+#pragma unroll
+        for (uint32_t k = 0; k < EACH; k++) {
+            const uint32_t r = 256u * k + tid;
+            c0[k] = c1[k] = 0;
+            if (256u * k < p.n_req && r < p.n_req) {
+                c0[k] = p.d_cu[r];
+                c1[k] = p.d_cu[r + 1];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < EACH; k++) {
+            if (c1[k] <= c0[k] || c0[k] < 0 || (uint32_t)c1[k] > p.n_rows) continue;
+            const uint32_t r = 256u * k + tid, all = (uint32_t)(c1[k] - c0[k]) * per;
+            if (all > a.most && place(r) < blocks(all) && sound(c0[k], c1[k], p.d_first ? p.d_first[r] : 0))
+                list[atomicAdd(&count, 1u)] = (uint16_t)r;  // (their order changes no result)
+        }
+        __syncthreads();
+        for (uint32_t l = 0; l < count; l++) {
+            const uint32_t r = uni(list[l]), c = (uint32_t)p.d_cu[r], all = ((uint32_t)p.d_cu[r + 1] - c) * per;
+            const uint32_t first = p.d_first ? (uint32_t)p.d_first[r] : 0u;
+            for (uint32_t b = place(r); b < blocks(all); b += a.rest) {
+                const uint32_t i = a.most + 256u * b + tid;
+                if (i < all) chunk(r, c, first, i);
+            }
+        }
     }
 }
 
 }  // namespace
 
 int launch_read(const wl_row_read& r, void* stream) {
-    const uint32_t psh = 31u - (uint32_t)__builtin_clz(r.cache.page_size), per = (r.cache.kv_lora_rank + r.cache.qk_rope) / 8u;
-    // enough work-groups for the longest request, whichever it is, 4096 in all at the most
-    const uint32_t most = r.n_req >= 4096u ? 1u : 4096u / r.n_req, need = (uint32_t)(((uint64_t)r.n_rows * per + 255u) / 256u);
-    const dim3 grid(need < most ? need : most, r.n_req);
+    const uint32_t per = (r.cache.kv_lora_rank + r.cache.qk_rope) / 8u;
+    RowRead a{};
+    a.r = r;
+    a.psh = 31u - (uint32_t)__builtin_clz(r.cache.page_size);
+    // 4096 work-groups in all, as many for each request. One request alone may have all rows:
+    // where that would be more than 24 rounds of its work-groups (some 0.7 us each), they take
+    // twice those of an average request and four, and up to 512 others what is behind them. One
+    // request with 65536 rows among 512, 4 bits: 2156 us without them and 47, 16 bits 1477 and 35.
+    // Requests of the same length pay up to 4 % or 0.4 us: 64 x 1000 rows of 4 bits 20.5 us
+    // and 20.7, 4096 x 16 20.4 and 21.2 (with 2048 others 21.6 and 23.7), 4096 x 1 4.7 and 5.1.
+    const uint32_t need = (uint32_t)(((uint64_t)r.n_rows * per + 255u) / 256u), own = r.n_req >= 4096u ? 1u : 4096u / r.n_req;
+    const uint32_t x = need < own ? need : own, rounds = 2u * ((need + 4095u) / 4096u) + 4u;
+    a.most = x * rounds * 256u;  // below 2^32: at most 4096 x 2308 x 256
+    if (x * (rounds > 24u ? rounds : 24u) < need) a.rest = need / 8u < 512u ? need / 8u : 512u;
+    a.first = (a.rest + x - 1u) / x;
+    const dim3 grid(x, a.first + r.n_req);
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto ct) {
         constexpr int CT = decltype(ct)::value;
-        if (r.dtype == WL_TYPE_BF16) hipLaunchKernelGGL((row_read_kernel<CT, true>), grid, dim3(256), 0, st, r, psh);
-        else hipLaunchKernelGGL((row_read_kernel<CT, false>), grid, dim3(256), 0, st, r, psh);
+        auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a); };
+        if (r.dtype == WL_TYPE_BF16) a.rest ? run(row_read_kernel<CT, true, true>) : run(row_read_kernel<CT, true, false>);
+        else a.rest ? run(row_read_kernel<CT, false, true>) : run(row_read_kernel<CT, false, false>);
         return (int)hipGetLastError();
     };
     return r.cache.dtype == WL_TYPE_MXFP4  ? go(std::integral_constant<int, WL_TYPE_MXFP4>{})
