@@ -26,7 +26,7 @@ namespace {
 // values, or of -infinity where a grammar leaves fewer than n_top) the whole row is read
 // again; a list that runs full is cut down to its n best, and from then on only what is
 // before the last of them, by value or by id, comes in. (284 rows of 154880 bf16 with 8 finite
-// values, n_top 20: 93 us, one row 65; with equal values coming in whatever their ids,
+// values, n_top 20: 89 us, one row 63; with equal values coming in whatever their ids,
 // a cut at every step, 1069 and 1025.)
 //
 // Bound by the read of the logits where rows are many, by two launches where they are few.
@@ -76,22 +76,23 @@ WL_DEV Sums wave_join(Sums x) {
 // A wave's list of the values that may be among the n largest, of (ordered value, id).
 constexpr uint32_t kList = 640;
 constexpr uint32_t kLanes = 256;  // whose values are read again
-constexpr uint32_t kShare = 20, kAhead = 4;  // loads in flight
+constexpr uint32_t kAhead = 4;    // loads in flight
+// Lanes' largest values that a thread holds in registers from its first look at them to its
+// second, those behind them it reads again: 80 parts, which a row of 163840 values has where it
+// is alone. With 20 and 32 of them, bf16, n_top 20: one row of 154880 13.1 and 13.6 us, of 200003
+// 15.0 and 14.2, of 262144 18.1 and 14.7, of 2^20 61 and 57; 2048 rows of 32000, of
+// which a thread has one, 50.4 and 52.6 (registers).
+constexpr uint32_t kShare = 20;
 
 struct List {
     u32x2* const at;         // [kList] in LDS
     const uint32_t lane, n;
     uint32_t count = 0;
-    uint32_t floor = 0;      // ordered: n values are at least this,
-    uint32_t limit = ~0u;    // those that equal it having lower ids than this, or this
-    float least = -INFINITY; // the same
+    uint64_t floor = 0;      // what comes in has a place above this
     __device__ __forceinline__ List(u32x2* a, uint32_t l, uint32_t n_top) : at(a), lane(l), n(n_top) {}
+    // An ordered value and its id as one number, that of what is before others the larger one.
+    static __device__ __forceinline__ uint64_t place(uint32_t k, uint32_t i) { return (uint64_t)k << 32 | ~i; }
     static __device__ __forceinline__ bool before(uint32_t k, uint32_t i, uint32_t k2, uint32_t i2) { return k > k2 || (k == k2 && i < i2); }
-    __device__ __forceinline__ void raise(uint32_t f) {
-        if (f <= floor) return;
-        floor = f;
-        least = value_of(f);
-    }
     // From four values a lane (0: none): the n-th largest of them, to 16 bits, from below. (A
     // NaN's bound, to 16 bits, is one too.)
     __device__ __forceinline__ void bound(u32x4 mine) {
@@ -104,7 +105,7 @@ struct List {
             for (uint32_t k = 0; k < 4; k++) reach += (uint32_t)__popcll(__ballot(mine[k] >= c));
             if (reach >= n) f = c;
         }
-        raise(uni(f));
+        floor = ((uint64_t)uni(f) << 32) - (f ? 1u : 0u);
     }
     // Leaves the n best, in order.
     __device__ __forceinline__ void cut() {
@@ -144,12 +145,11 @@ struct List {
         __builtin_amdgcn_wave_barrier();
         count = m;
         if (m < n) return;
-        raise((uint32_t)__builtin_amdgcn_readlane((int)bk, (int)(n - 1u)));
-        limit = (uint32_t)__builtin_amdgcn_readlane((int)bi, (int)(n - 1u));
+        floor = place((uint32_t)__builtin_amdgcn_readlane((int)bk, (int)(n - 1u)), (uint32_t)__builtin_amdgcn_readlane((int)bi, (int)(n - 1u)));
     }
     // every lane's value o (ordered) of id i, where ok
     __device__ __forceinline__ void add(uint32_t o, uint32_t i, bool ok) {
-        ok = ok && before(o, i, floor, limit);
+        ok = ok && place(o, i) > floor;
         const uint64_t m = __ballot(ok);
         if (!m) return;
         if (ok) at[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u))] = u32x2{o, i};
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(256) void logp_join_kernel(Logp p, uint32_t rows) {
     __syncthreads();
     list.bound(highs[lane]);
     shares([&](uint32_t o, uint32_t i) {
-        if (o < list.floor) return;
+        if (List::place(o, 0u) <= list.floor) return;
         const uint32_t k = atomicAdd(&n_lanes, 1u);  // (their order changes no result)
         if (k < kLanes) lanes[k] = i;
     });
