@@ -189,3 +189,19 @@ def test_a_list_of_equal_values_is_cut_once(gpu, t):
         x = Logprobs(few, t, [7], n_top=20).run()
         x.check()
         assert fastest(x) < 25 * fastest(usual)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("R,V", [(1, 163839), (1, 163841), (2, 200003), (3, 262144), (1, 1 << 20)])
+def test_large_vocabularies(gpu, R, V, t):
+    """More lanes of a row than the second launch's threads hold the largest values of; some of the most likely in the
+    last parts, all of them, and as many as are asked for beside equal ones."""
+    rng = np.random.default_rng(V)
+    z = logits(rng, R, V)
+    late = z.copy()
+    late[:, V - 3000:] += 8.0
+    ties = np.round(2 * z) / 2
+    ties[:, V - 40:] = ties.max(1, keepdims=True)
+    for x in (z, late, ties):
+        for n_top in (1, 32):
+            Logprobs(x, t, rng.integers(0, V, R), n_top=n_top).run().check()
