@@ -29,10 +29,12 @@ namespace {
 // values, n_top 20: 89 us, one row 63; with equal values coming in whatever their ids,
 // a cut at every step, 1069 and 1025.)
 //
-// Bound by the read of the logits where rows are many, by two launches where they are few.
-// 284 rows of 154880: f32 30 us (5.8 TB/s) with no n_top, 42 with 20; bf16 22 us (4.0 TB/s,
-// two exponentials' time a value) and 31. One row of them 9 us and 13. 2048 rows of 32000
-// bf16: 32 us and 47 to 49. (Lists kept in the first launch, by insertion into each lane's
+// Where rows are many f32 is bound by the read of the logits and bf16 by vector operations:
+// 12.4 a value (8.5 million instructions of a wave counted for 44 million values), 4 clocks
+// each and an exponential 16, some 41 of the 44 thousand clocks of a CU. Where rows are few, two launches.
+// 284 rows of 154880: f32 30 us (5.8 TB/s) with no n_top, 42 with 20; bf16 22 us (4.1 TB/s)
+// and 31 to 33 (cards differ). One row of them 9 us and 13. 2048 rows of 32000
+// bf16: 30 to 32 us and 50. (Lists kept in the first launch, by insertion into each lane's
 // registers: 57 us at 284 rows bf16 and n_top 20, 31 at one row.)
 constexpr uint32_t kPer = 32;             // values a lane has at a time
 constexpr uint32_t kPart = 64 * kPer;     // of a wave

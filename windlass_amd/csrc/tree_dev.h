@@ -53,7 +53,8 @@ struct Tree {
 // c = (b % 8)(G / 8) + b / 8.) A row tile's units count from its keys' end: the next
 // work-group, which has the rest of a row tile that this one ends with, then begins at
 // the chunk's first key as this one did, and not some tiles ahead (64 requests of 8 nodes,
-// 16-bit rows: 207 us and 198; through a window 149 and 142, 717 MB fetched and 298).
+// 16-bit rows: 207 us and 198; through a window 149 and 142, 717 MB fetched and 298; 32-bit
+// queries over these rows 385 and 370, over 32-bit ones 360 and 349, 3 of 64 nodes 614 and 589).
 // A row tile that one work-group has whole is finished there; the others leave their
 // parts in the scratch for the second launch, at most two per work-group: its first
 // walk's and its last one's.
@@ -66,7 +67,8 @@ struct Tree {
 // One request of 64 nodes over 8192 keys, 32 bits: 222 us
 // without, 207 with; 5 of 7 nodes 67 and 59; 12 of 5 nodes 28 and 23; 32 contexts 191 and 179. Requests of
 // one row tile, 16-bit queries: 32 contexts of up to 65536 keys 180 and 170, of 4-bit rows 129 and 121, these
-// through a window of 4096 57 and 46; 8 of up to 3016 keys 25 and 19. (They need no chunks: their keys stand
+// through a window of 4096 57 and 46; 8 of up to 3016 keys 25 and 19; with 32-bit queries 5 of 16 heads over
+// up to 9000 keys 34 and 29, 100 of up to 9000 and one of 4096 as without. (They need no chunks: their keys stand
 // in a row; of one such request alone that makes equal pieces by itself.)
 constexpr uint32_t kSlack = 6;
 //

@@ -37,10 +37,10 @@ typedef __attribute__((ext_vector_type(32))) float f32x32;
 // LDS rows and chunks placed so that no access meets a bank twice, a walk's addresses
 // found 64 tiles at a time.
 // Measured (512 + 64 columns, both launches): 32 requests of one token x 64 heads over
-// up to 65536 keys (22775 on average, 296 MB) 121 to 125 us, 820 TFLOP/s or 57 % of a
-// large bf16 product's rate (over 16-bit rows 170); 64 of up to 8 nodes (279
-// in all) over up to 8192 164 us, 610 TFLOP/s (198); one token over 4096 keys 26, all of it
-// latencies (28).
+// up to 65536 keys (22775 on average, 296 MB) 121 to 130 us (cards differ), 780 to 840
+// TFLOP/s or 54 to 58 % of a large bf16 product's rate (over 16-bit rows 170); 64 of up to 8
+// nodes (279 in all) over up to 8192 164 to 171 us, 590 to 610 TFLOP/s (198 to 201); one token over
+// 4096 keys 26, all of it latencies (28).
 // Two pieces of the queries instead of three would be 6 % faster and lose 5 of the 14
 // bits. Without effect: the two waves of a SIMD in opposite order, wave priorities, values
 // read before the barrier.
