@@ -566,3 +566,36 @@ def test_read_of_one_long_request_among_many(gpu):
     for r in (0, 200, 511):
         assert fastest([0] * r + [n] + [0] * (511 - r)) < 12 * alone
     stream.destroy()
+
+
+def test_read_captured_with_other_lengths_later(gpu):
+    """A captured call, replayed as the requests' lengths change: long ones come and go among many."""
+    R, L, RP, ps = 500, 64, 16, 16
+    lens = [20] * R
+    for r in (0, 77, 250, 499):
+        lens[r] = 2600
+    t = S.Serving(21, "f32", "bf16", L, RP, 2, ps, lens, [0] * R).upload()
+    n_rows = 8000
+    out, cu = hip.DeviceBuffer(4 * n_rows * t.W), i32([0] * (R + 1))
+    held = dict(d_table=i32(t.table), d_status=i32([0]))
+    args = paged.RowRead(cache=t.args.cache, dtype=0, n_req=R, n_rows=n_rows, max_pages=t.max_pages, d_out=out.ptr, out_stride=t.W,
+                         d_cu=cu.ptr, **{k: v.ptr for k, v in held.items()})
+    stream = hip.Stream()
+    g = hip.Graph(stream)
+    g.begin()
+    paged.read_rows(args, stream.handle)
+    g.end()
+    rng = np.random.default_rng(4)
+    for long in ((), (77,), (0, 499), (250, 499), (), (499,)):
+        counts = [int(x) for x in rng.integers(0, 5, R)]
+        for r in long:
+            counts[r] = int(rng.integers(1500, 2600))
+        cu.upload(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
+        out.upload(np.full(n_rows * t.W, 7.0, np.float32))
+        g.launch()
+        stream.synchronize()
+        got = out.download(np.float32).reshape(n_rows, t.W)
+        want = np.concatenate([t.rows[r][:n] for r, n in enumerate(counts)])
+        assert np.array_equal(got[:len(want)], want) and np.all(got[len(want):] == 7.0)
+    assert int(held["d_status"].download(np.uint32)[0]) == 0
+    stream.destroy()
