@@ -896,7 +896,8 @@ wl_status wl_paged_window_attention(const wl_window_attn* w, void* stream);
  *                     the n_top (0 to WL_LOGPROB_MAX_TOP, at most n_vocab) largest
  *                     logits' ids, largest first, of equal ones the lowest id first,
  *                     and their log p (both may be NULL if n_top is 0)
- * Computed in f32 from the logits as they are. A logit of -infinity has p = 0 and
+ * Computed in f32 from the logits as they are; an entropy is a difference, right to about
+ * 1e-6, also where it is itself smaller. A logit of -infinity has p = 0 and
  * log p = -infinity. In a row without a finite logit, or with a NaN or +infinity, log p
  * and the entropy are NaN; ids are by order all the same, a NaN before any number. A
  * token of -1 is passed over, d_logp[t] as it was (a step captured with room for more
